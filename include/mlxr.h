@@ -298,6 +298,77 @@ int mlxr_k_sample(float* logits, int V, int32_t* hist, int32_t* status, uint64_t
 int mlxr_k_sample_noalloc(float* logits, int V, int32_t* hist, int32_t* status, uint64_t* rng, int pos,
                           const mlxr_sample_params* sp, void* stream);
 
+/* ---------------------------------------------------------------- a batch's decode step (device pointers)
+ * One new token for each of B sequences over one pool of KV-cache pages: append, attention, eviction and
+ * token selection. Like mlxr_k_sample_noalloc these calls allocate nothing, go on `stream` (a hipStream_t;
+ * NULL: the null stream) and return without waiting, so they can be captured. They have no counterpart in
+ * the reference, which decodes one sequence. Every pointer is to memory of the current device, and the
+ * stream is one of it (MLXR_E_INVALID_ARG otherwise).
+ *
+ * `work`: scratch of at least the bytes that the *_work function of the call returns, 256-byte aligned, ZERO
+ * before its first use; every call leaves it ready for the next call of the same operator, whatever the
+ * sizes. Calls that may overlap (other streams, graphs replayed side by side) need one each, and an operator
+ * does not use another one's.
+ *
+ * What lies on the device is not read on the host. A length outside [0, max_len] counts as the nearer bound,
+ * and a page number outside [0, n_pages) is never followed: its keys are left out of attention, an append
+ * there writes nothing, and eviction copies zeros from it and nothing to it. */
+typedef struct {
+    void* k; void* v;          /* the pool: [n_pages][nKV][64][D] of bf16 (st 0) or f16 (st 1), 16-byte aligned */
+    const int32_t* table;      /* [B][table_stride]: slot i of sequence b is row i % 64 of page table[b][i / 64] */
+    int32_t* len;              /* [B]: slots in use, the newest key among them; 0: an idle row */
+    float* weight;             /* [B][nKV][slot_stride] or NULL: attention each slot has drawn, one value per KV head */
+    int32_t* position;         /* [B][nKV][slot_stride] or NULL: the position whose key a slot holds */
+    int32_t n_pages, table_stride, slot_stride;
+    int32_t max_len;           /* no length is above it; at most 64 table_stride, and slot_stride with weight or position */
+    int32_t B, nKV, D, st;     /* D: 64 or 128 */
+} mlxr_paged_kv;
+
+/* Appends each sequence's newest token, at slot len[b] - 1 (an idle row: nothing). Row b of qkv holds nH query,
+ * nKV key and nKV value heads of D floats; per-head RMSNorm of queries and keys (qn / kn fp32 [D], or both
+ * NULL), RoPE over the first rot_dim values (even; half-split, or pairs of neighbours if traditional) at
+ * positions[b], or at the slot if NULL, with the angle in 64 bits; queries to q_out (row stride q_stride; may
+ * be qkv itself at its stride), keys and values to the cache, weight 0 and the position to their arrays where
+ * the cache has them. A slot's page must belong to one sequence only. */
+int mlxr_k_paged_append(const mlxr_paged_kv* kv, const float* qkv, int row_stride, const float* inv_freq, const float* qn,
+                        const float* kn, int nH, int rot_dim, int traditional, const int32_t* positions, float eps,
+                        float* q_out, int q_stride, void* stream);
+
+/* Attention of one query token per sequence over its slots, or over its last `window` ones (0: all):
+ * out[b][h] = sum_j p_j v_j with p = softmax(scale q k_j), fp32 results; an idle row, or one none of whose
+ * scores is above -infinity, gives zeros. With kv->weight:
+ * weight[b][g][j] = decay * weight_in[b][g][j] + the sum of p_j over the query heads of KV head g, for every j < len[b]
+ * (slots outside the window only decay; weight_in, with the strides of weight, may be weight itself; NULL: zeros).
+ * Pages may be shared by sequences. q, out: 16-byte aligned, strides multiples of 4. */
+int mlxr_k_paged_attention(const mlxr_paged_kv* kv, const float* q, int q_stride, int nH, int window, float scale,
+                           float* out, int out_stride, const float* weight_in, float decay, void* work, size_t work_bytes,
+                           void* stream);
+int64_t mlxr_k_paged_attention_work(const mlxr_paged_kv* kv, int nH);
+
+/* Holds each sequence at `budget` slots: copies to dst, in slot order, the first `sink` slots, the last
+ * `window`, and of those between the budget - sink - window with the largest src->weight (equal: the lower slot;
+ * NaN lowest), for each KV head on its own; a sequence of at most `budget` slots whole. Keys and values go
+ * to dst's pages, which may be in the same pool but must be pages that no sequence of src uses; weights
+ * (src->weight is required) and positions to dst's arrays where dst has them; dst->len is written. What lies
+ * behind the new length stays as it was. src and dst have the same B, nKV, D and st; their len, weight and
+ * position arrays are different ones. */
+int mlxr_k_paged_evict(const mlxr_paged_kv* src, const mlxr_paged_kv* dst, int budget, int sink, int window, void* work,
+                       size_t work_bytes, void* stream);
+int64_t mlxr_k_paged_evict_work(const mlxr_paged_kv* src, int budget);
+
+/* One token per row of logits [rows][V] (row stride `stride` floats), from the given random numbers u [rows] in
+ * [0, 1). A row's tokens are ranked by logit, equal ones by index; NaN and -infinity are never drawn. With
+ * w = exp((logit - the largest) / temperature): the first top_k ranks are kept (0 or less: all), of these
+ * those before the first with w < min_p, and the shortest prefix whose sum of w reaches top_p times that of the
+ * top_k; at least one. The token is the first rank whose running sum reaches u times the kept sum: exact over
+ * the whole vocabulary, w in 64 bits. temperature <= 0.001: the first rank. temperature [rows]; top_k, top_p,
+ * min_p [rows] or NULL (off). status (or NULL): 0, or 1 where the largest logit is infinite or there is none:
+ * the token is 0 then. V <= 1048576. The logits stay as they are. */
+int mlxr_k_sample_rows(const float* logits, int rows, int V, int64_t stride, const float* temperature, const int32_t* top_k,
+                       const float* top_p, const float* min_p, const float* u, int32_t* tokens, int32_t* status,
+                       void* work, size_t work_bytes, void* stream);
+int64_t mlxr_k_sample_rows_work(int rows, int V);
+
 #ifdef __cplusplus
 }
 #endif

@@ -51,6 +51,13 @@ class QMat(C.Structure):
     _fields_ = [("w", C.c_void_p), ("scales", C.c_void_p), ("biases", C.c_void_p), ("bias", C.c_void_p), ("O", C.c_int32)]
 
 
+class PagedKV(C.Structure):
+    """mlxr_paged_kv: a batch of sequences over one pool of KV-cache pages (device pointers)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("len", C.c_void_p), ("weight", C.c_void_p),
+                ("position", C.c_void_p), ("n_pages", C.c_int32), ("table_stride", C.c_int32), ("slot_stride", C.c_int32),
+                ("max_len", C.c_int32), ("B", C.c_int32), ("nKV", C.c_int32), ("D", C.c_int32), ("st", C.c_int32)]
+
+
 CancelFn = C.CFUNCTYPE(C.c_int, C.c_void_p)   # mlxr_cancel_fn
 
 
@@ -111,6 +118,13 @@ def _load():
         "mlxr_k_sparse_select": (I, [P, I, I, I, I, I, I, I, P, I]),
         "mlxr_k_sample": (I, [P, I, P, P, P, I, C.POINTER(SampleParams)]),
         "mlxr_k_sample_noalloc": (I, [P, I, P, P, P, I, C.POINTER(SampleParams), P]),
+        "mlxr_k_paged_append": (I, [C.POINTER(PagedKV), P, I, P, P, P, I, I, I, P, F, P, I, P]),
+        "mlxr_k_paged_attention": (I, [C.POINTER(PagedKV), P, I, I, I, F, P, I, P, F, P, C.c_size_t, P]),
+        "mlxr_k_paged_attention_work": (C.c_int64, [C.POINTER(PagedKV), I]),
+        "mlxr_k_paged_evict": (I, [C.POINTER(PagedKV), C.POINTER(PagedKV), I, I, I, P, C.c_size_t, P]),
+        "mlxr_k_paged_evict_work": (C.c_int64, [C.POINTER(PagedKV), I]),
+        "mlxr_k_sample_rows": (I, [P, I, I, C.c_int64, P, P, P, P, P, P, P, P, C.c_size_t, P]),
+        "mlxr_k_sample_rows_work": (C.c_int64, [I, I]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
