@@ -66,78 +66,438 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
 }
 
 // ---- attention ----
-// One workgroup per (KV head, sequence). A wave takes every fourth key; lane l holds dims l and l + 64. Per head:
-// running maximum m, sum and weighted values of one pass over the keys; with weights a second pass for p.
-template <int ST>
-__global__ __launch_bounds__(256) void paged_attn_simple_kernel(PagedAttnArgs a) {
-    __shared__ float ms[4], ls[4], os[4][128], stat[4096][2];   // a head's maximum and sum
-    const PagedKV& kv = a.kv;
-    const int kvh = blockIdx.x, b = blockIdx.y, D = kv.D, G = a.nH / kv.nKV;
-    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int L = paged_len(kv, b), first = a.window > 0 && L > a.window ? L - a.window : 0;
-    const uint16_t *K = static_cast<const uint16_t*>(kv.k), *V = static_cast<const uint16_t*>(kv.v);
-    float* weight = kv.weight ? kv.weight + paged_slot(kv, b, kvh, 0) : nullptr;
-    const float* win = a.weight_in ? a.weight_in + paged_slot(kv, b, kvh, 0) : nullptr;
-    int g = 0;
-    float q0, q1;
-    auto query = [&] {
-        const float* q = a.q + (int64_t)b * a.q_stride + (int64_t)(kvh * G + g) * D;
-        q0 = q[l] * a.scale;
-        q1 = D > 64 ? q[l + 64] * a.scale : 0.0f;
-    };
-    auto score = [&](int j, int64_t& row) {
-        const int page = paged_page(kv, b, j / MLXR_PAGE);
-        if (page < 0) return -INFINITY;
-        row = paged_row(kv, page, kvh, j % MLXR_PAGE);
-        return wave_sum(q0 * kv_float<ST>(K[row + l]) + (D > 64 ? q1 * kv_float<ST>(K[row + l + 64]) : 0.0f));
-    };
-    for (g = 0; g < G; g++) {
-        query();
-        float m = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-        for (int j = first + w; j < L; j += 4) {
-            int64_t row = 0;
-            const float s = score(j, row);
-            if (s == -INFINITY) continue;
-            const float mn = fmaxf(m, s), c = expf(m - mn), p = expf(s - mn);
-            o0 = o0 * c + p * kv_float<ST>(V[row + l]);
-            if (D > 64) o1 = o1 * c + p * kv_float<ST>(V[row + l + 64]);
-            sum = sum * c + p;
-            m = mn;
+//
+// out = sum_j p_j v_j, p = softmax of scale q k_j over a sequence's slots, for the G query heads of a KV head at
+// once: each key and value row is read once, 4 D bytes a slot, and that read bounds the kernel (G = 4 asks for 4
+// multiply-adds a byte, far below what the matrix cores have).
+//
+// Split. A (sequence, KV head, group of 16 query heads) is a segment of ceil(slots / 64) pages. All segments' pages,
+// laid end to end, are cut into equal runs, one per workgroup, so ragged batches keep the card as evenly busy as
+// one long sequence, and lengths may stay on the device: each workgroup finds its run by a scan over the batch's
+// page counts. A segment inside one run is written out at once; one cut by runs leaves partial results (maximum,
+// sum, unnormalised values), which the last workgroup to finish joins in run order: the same bits every time.
+//
+// Inside. A wave takes 32 keys at a time, straight from memory into the operands of 16x16x32 MFMAs, without LDS:
+//   S^T = K q^T: lane (m = l % 16, g = l / 16) holds 8 dims 32 s + 8 g .. of key m (step s); 16 rows of q are the
+//   columns. The product leaves a lane with row l % 16's scores of keys 4 g .. 4 g + 3 of both 16-key tiles.
+//   O^T = V^T P^T: those eight are what the lane has to hold of P^T as an operand, if slot e of group g stands for
+//   key 4 g + e of the first tile (e < 4) or 4 g + e - 4 of the second. So lane (m, g) loads these eight keys'
+//   dims (D / 16) m .., transposes them in registers (one byte permute per two values), and maximum, sum and rescale of
+//   a row stay within its four lanes.
+// q and p are fp32 split into parts that the matrix cores multiply exactly: three bf16 by truncation (24 bits), or
+// two f16 (22 bits, q scaled to at most 2^14 by a power of two, p by 2^14). Scores are in powers of two (log2 e is
+// in q's scale).
+constexpr int PA_MAXW = 512;       // workgroups: two a CU
+constexpr int PA_MINPER = 2;       // pages of a run at least: one for each wave pair
+constexpr int PA_ROWS = 16;
+typedef float pa_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 pa_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
+typedef uint32_t pa_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t pa_u2 __attribute__((ext_vector_type(2)));
+
+template <int ST> __device__ __forceinline__ pa_f4 pa_mfma(uint4 a, uint4 b, pa_f4 c) {
+    if constexpr (ST == 0) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_b8, a), __builtin_bit_cast(pa_b8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_h8, a), __builtin_bit_cast(pa_h8, b), c, 0, 0, 0);
+}
+constexpr int pa_parts(int ST) { return ST == 0 ? 3 : 2; }
+// The low (or high) halves of two words as one.
+__device__ __forceinline__ uint32_t pa_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t pa_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+// Eight fp32 values as parts whose sum they are (ST 0) or nearly are (ST 1).
+template <int ST> __device__ __forceinline__ void pa_split(const float* x, uint4* o) {
+    uint32_t w[pa_parts(ST)][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int t = 0; t < pa_parts(ST); t++) {
+            if constexpr (ST == 0) {
+                w[t][i] = pa_hi(__float_as_uint(a), __float_as_uint(b));
+                a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+                b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+            } else {
+                const _Float16 ha = (_Float16)a, hb = (_Float16)b;
+                w[t][i] = (uint32_t)__builtin_bit_cast(uint16_t, ha) | ((uint32_t)__builtin_bit_cast(uint16_t, hb) << 16);
+                a -= (float)ha;
+                b -= (float)hb;
+            }
         }
-        __syncthreads();
-        if (l == 0) { ms[w] = m; ls[w] = sum; }
-        os[w][l] = o0; os[w][l + 64] = o1;
-        __syncthreads();
-        const float M = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-        float total = 0.0f, o = 0.0f;
-        for (int i = 0; i < 4; i++) {
-            const float c = ms[i] == -INFINITY ? 0.0f : expf(ms[i] - M);
-            total += ls[i] * c;
-            if (threadIdx.x < D) o += os[i][threadIdx.x] * c;
-        }
-        if (threadIdx.x < D) a.out[(int64_t)b * a.out_stride + (int64_t)(kvh * G + g) * D + threadIdx.x] = total == 0.0f ? 0.0f : o / total;
-        if (threadIdx.x == 0) { stat[g][0] = M; stat[g][1] = total; }
     }
-    if (!weight) return;
-    __syncthreads();
-    for (int j = w; j < L; j += 4) {
-        int64_t row = 0;
-        float p = 0.0f;
-        for (g = 0; g < G && j >= first; g++) {
-            query();
-            const float s = score(j, row);
-            if (s != -INFINITY) p += expf(s - stat[g][0]) / stat[g][1];
+#pragma unroll
+    for (int t = 0; t < pa_parts(ST); t++) o[t] = uint4{w[t][0], w[t][1], w[t][2], w[t][3]};
+}
+
+struct PaWork {
+    unsigned* count;      // [PA_MAXW] arrivals at the segment that starts in a run and goes on behind it; zero between calls
+    float* stat;          // [B][nH][2] a row's maximum and the inverse of its sum, for the weights
+    float* part;          // [2 W] partial results: [16] maxima, [16] sums, [16][D]
+    float* score;         // [B][nH][score_stride], for the weights
+    int score_stride, W, groups;   // groups: of 16 query heads of a KV head
+};
+__host__ __device__ __forceinline__ constexpr size_t pa_part_floats(int D) { return PA_ROWS * (D + 2); }
+
+// A sequence's part of the work: keys [first, L), pages p0 .. p0 + n - 1.
+struct PaSeq { int L, first, p0, n; };
+__device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs& a, int b) {
+    PaSeq s;
+    s.L = paged_len(a.kv, b);
+    s.first = a.window > 0 && s.L > a.window ? s.L - a.window : 0;
+    s.p0 = s.first / MLXR_PAGE;
+    s.n = s.L > 0 ? (s.L - 1) / MLXR_PAGE - s.p0 + 1 : 0;
+    return s;
+}
+__device__ __forceinline__ float pa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float pa_safe(float m) { return m == -INFINITY ? 0.0f : m; }   // -inf - -inf would be NaN
+__device__ __forceinline__ void pa_store2(float* p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 pa_load2(const float* p) {
+    const uint64_t v = __hip_atomic_load(const_cast<uint64_t*>(reinterpret_cast<const uint64_t*>(p)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
+
+template <int ST, int D, bool WT>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaWork wk) {
+    constexpr int KS = D / 32, NP = pa_parts(ST), DV = D / 16, OS = D + 4;   // k steps; dims of a lane's value rows; LDS row
+    constexpr int LDS_O = 4 * PA_ROWS * OS, LDS_C = PA_MAXW * PA_ROWS;
+    __shared__ float lds[LDS_O > LDS_C ? LDS_O : LDS_C];
+    __shared__ float sm[4][PA_ROWS], sl[4][PA_ROWS];
+    __shared__ int64_t wsum[4], found_pre;
+    __shared__ int found_b, last;
+    const PagedKV& kv = a.kv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
+    const int w = blockIdx.x, G = a.nH / kv.nKV, per_seq = kv.nKV * wk.groups;
+    const uint16_t *K = static_cast<const uint16_t*>(kv.k), *V = static_cast<const uint16_t*>(kv.v);
+
+    // idle rows
+    for (int b = w; b < kv.B; b += wk.W)
+        if (paged_len(kv, b) == 0)
+            for (int i = tid; i < a.nH * D; i += 256) a.out[(int64_t)b * a.out_stride + i] = 0.0f;
+
+    // this workgroup's run of pages
+    auto scan = [&](int n, int64_t& sum) {   // exclusive over the workgroup
+        int v = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(v, o, 64); if (lane >= o) v += u; }
+        __syncthreads();
+        if (lane == 63) wsum[wave] = v;
+        __syncthreads();
+        int64_t before = v - n;
+        for (int i = 0; i < 4; i++) if (i < wave) before += wsum[i];
+        sum = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+        return before;
+    };
+    int64_t T = 0, chunk = 0, before = 0;
+    int n = 0;
+    for (int c = 0; c < kv.B; c += 256) {
+        n = c + tid < kv.B ? pa_seq(a, c + tid).n : 0;
+        before = scan(n, chunk);
+        T += chunk;
+    }
+    int64_t per = (T * per_seq + wk.W - 1) / wk.W;
+    if (per < PA_MINPER) per = PA_MINPER;
+    int64_t t = w * per;
+    const int64_t t1 = min(T * per_seq, t + per);
+    if (t >= t1) return;
+    {
+        int64_t run = 0;
+        for (int c = 0; c < kv.B; c += 256) {
+            if (kv.B > 256) {
+                n = c + tid < kv.B ? pa_seq(a, c + tid).n : 0;
+                before = scan(n, chunk);
+            }
+            const int64_t pre = run + before;
+            if (pre * per_seq <= t && t < (pre + n) * per_seq) { found_b = c + tid; found_pre = pre; }
+            run += chunk;
+            if (run * per_seq > t) break;
         }
-        if (l == 0) weight[j] = (win && a.decay != 0.0f ? a.decay * win[j] : 0.0f) + p;
+    }
+    __syncthreads();
+    int b = found_b;
+    int64_t pre = found_pre;
+    PaSeq sq = pa_seq(a, b);
+    int slot = 0;   // partial results of this workgroup: its first segment's, then its last one's
+    while (true) {
+        const int64_t local = t - pre * per_seq;
+        const int seg = (int)(local / sq.n), tile = (int)(local % sq.n), tiles = (int)min((int64_t)(sq.n - tile), t1 - t);
+        const int kvh = seg / wk.groups, h0 = (seg % wk.groups) * PA_ROWS, rows = min(PA_ROWS, G - h0);
+        // q's parts
+        uint4 q[KS][NP];
+        float unscale = 1.0f;
+        {
+            float x[KS][8];
+            const float* qr = a.q + (int64_t)b * a.q_stride + (int64_t)(kvh * G + h0 + min(r, rows - 1)) * D;
+            const float f = r < rows ? a.scale * 1.4426950408889634f : 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const float4 u = *reinterpret_cast<const float4*>(qr + 32 * s + 8 * g), v = *reinterpret_cast<const float4*>(qr + 32 * s + 8 * g + 4);
+                x[s][0] = u.x * f; x[s][1] = u.y * f; x[s][2] = u.z * f; x[s][3] = u.w * f;
+                x[s][4] = v.x * f; x[s][5] = v.y * f; x[s][6] = v.z * f; x[s][7] = v.w * f;
+            }
+            if constexpr (ST == 1) {
+                float mx = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[s][e]));
+                mx = xor32_max(xor16_max(mx));
+                int e2 = 0;
+                if (mx > 0.0f && mx < INFINITY) { frexpf(mx, &e2); e2 = 14 - e2; e2 = e2 < -126 ? -126 : (e2 > 126 ? 126 : e2); }
+                const float up = ldexpf(1.0f, e2);
+                unscale = ldexpf(1.0f, -e2);
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[s][e] *= up;
+            }
+#pragma unroll
+            for (int s = 0; s < KS; s++) pa_split<ST>(x[s], q[s]);
+        }
+        float m = -INFINITY, l = 0.0f;
+        pa_f4 o[DV];
+#pragma unroll
+        for (int j = 0; j < DV; j++) o[j] = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        int have = -1, ids = 0;   // page numbers of 64 tiles, one a lane
+        for (int u = wave; u < 2 * tiles; u += 4) {
+            const int tt = u >> 1;
+            if ((tt >> 6) != have) {
+                have = tt >> 6;
+                const int i = min(64 * have + lane, tiles - 1);
+                ids = paged_page(kv, b, sq.p0 + tile + i);
+            }
+            const int page = __builtin_amdgcn_readlane(ids, tt & 63);
+            const int key0 = (sq.p0 + tile) * MLXR_PAGE + u * 32;
+            if (key0 + 32 <= sq.first || key0 >= sq.L) continue;
+            if (page < 0) {
+                if constexpr (WT)
+                    if (r < rows)
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            wk.score[((int64_t)b * a.nH + kvh * G + h0 + r) * wk.score_stride + key0 + (e >> 2) * 16 + 4 * g + (e & 3)] = -INFINITY;
+                continue;
+            }
+            const int64_t base = paged_row(kv, page, kvh, key0 & (MLXR_PAGE - 1));
+            uint4 kr[2][KS];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int s = 0; s < KS; s++) kr[i][s] = __builtin_bit_cast(uint4, gload(reinterpret_cast<const pa_u4*>(K + base + (16 * i + r) * D + 32 * s + 8 * g)));
+            uint32_t vr[8][DV / 2];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint16_t* row = V + base + ((e >> 2) * 16 + 4 * g + (e & 3)) * D + DV * r;
+                if constexpr (DV == 8) {
+                    const pa_u4 x = gload(reinterpret_cast<const pa_u4*>(row));
+                    vr[e][0] = x.x; vr[e][1] = x.y; vr[e][2] = x.z; vr[e][3] = x.w;
+                } else {
+                    const pa_u2 x = gload(reinterpret_cast<const pa_u2*>(row));
+                    vr[e][0] = x.x; vr[e][1] = x.y;
+                }
+            }
+            pa_f4 sc[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                sc[i] = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int p = 0; p < NP; p++) sc[i] = pa_mfma<ST>(kr[i][s], q[s][p], sc[i]);
+            }
+            float sv[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) sv[e] = ST == 0 ? sc[e >> 2][e & 3] : sc[e >> 2][e & 3] * unscale;
+            if (key0 < sq.first || key0 + 32 > sq.L) {   // keys outside take no part, whatever their rows hold
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = key0 + (e >> 2) * 16 + 4 * g + (e & 3);
+                    if (key < sq.first || key >= sq.L) {
+                        sv[e] = -INFINITY;
+#pragma unroll
+                        for (int d = 0; d < DV / 2; d++) vr[e][d] = 0;
+                    }
+                }
+            }
+            if constexpr (WT)
+                if (r < rows) {
+                    float* s = wk.score + ((int64_t)b * a.nH + kvh * G + h0 + r) * wk.score_stride + key0 + 4 * g;
+                    *reinterpret_cast<float4*>(s) = float4{sv[0], sv[1], sv[2], sv[3]};
+                    *reinterpret_cast<float4*>(s + 16) = float4{sv[4], sv[5], sv[6], sv[7]};
+                }
+            float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+            mx = fmaxf(m, xor32_max(xor16_max(mx)));
+            if (__any(mx > m)) {
+                const float c = pa_exp2(m - pa_safe(mx));
+                l *= c;
+#pragma unroll
+                for (int j = 0; j < DV; j++) o[j] *= c;
+                m = mx;
+            }
+            const float ms = pa_safe(m);
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                p[e] = pa_exp2(sv[e] - ms);
+                l += p[e];
+                if constexpr (ST == 1) p[e] *= 16384.0f;
+            }
+            uint4 pp[NP];
+            pa_split<ST>(p, pp);
+#pragma unroll
+            for (int j = 0; j < DV; j++) {
+                uint4 vt;
+                if (j & 1) vt = uint4{pa_hi(vr[0][j / 2], vr[1][j / 2]), pa_hi(vr[2][j / 2], vr[3][j / 2]), pa_hi(vr[4][j / 2], vr[5][j / 2]), pa_hi(vr[6][j / 2], vr[7][j / 2])};
+                else vt = uint4{pa_lo(vr[0][j / 2], vr[1][j / 2]), pa_lo(vr[2][j / 2], vr[3][j / 2]), pa_lo(vr[4][j / 2], vr[5][j / 2]), pa_lo(vr[6][j / 2], vr[7][j / 2])};
+#pragma unroll
+                for (int i = 0; i < NP; i++) o[j] = pa_mfma<ST>(vt, pp[i], o[j]);
+            }
+        }
+        // the four waves' results: lane (r, g) has row r's dims DV (4 g + i) + j
+        l = xor32_sum(xor16_sum(l));
+        if (g == 0) { sm[wave][r] = m; sl[wave][r] = l; }
+        {
+            float* so = lds + (wave * PA_ROWS + r) * OS;
+            constexpr float down = ST == 0 ? 1.0f : 1.0f / 16384.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < DV; j += 4)
+                    *reinterpret_cast<float4*>(so + DV * (4 * g + i) + j) = float4{o[j][i] * down, o[j + 1][i] * down, o[j + 2][i] * down, o[j + 3][i] * down};
+        }
+        __syncthreads();
+        const bool whole = tiles == sq.n;
+        float* part = wk.part + (size_t)(2 * w + slot) * pa_part_floats(D);
+        for (int i = tid; i < rows * D / 2; i += 256) {
+            const int row = i / (D / 2), d = 2 * (i % (D / 2));
+            const float M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row])), Ms = pa_safe(M);
+            float sum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const float c = pa_exp2(sm[v][row] - Ms);
+                const float2 e = *reinterpret_cast<const float2*>(lds + (v * PA_ROWS + row) * OS + d);
+                sum += c * sl[v][row]; x += c * e.x; y += c * e.y;
+            }
+            if (whole) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                *reinterpret_cast<float2*>(a.out + (int64_t)b * a.out_stride + (int64_t)(kvh * G + h0 + row) * D + d) = sum == 0.0f ? float2{0.0f, 0.0f} : float2{x * inv, y * inv};
+                if (WT && d == 0) *reinterpret_cast<float2*>(wk.stat + 2 * ((int64_t)b * a.nH + kvh * G + h0 + row)) = float2{Ms, inv};
+            } else {
+                pa_store2(part + 2 * PA_ROWS + row * D + d, x, y);
+                if (d == 0) pa_store2(part + 2 * row, M, sum);
+            }
+        }
+        if (!whole) {
+            // the runs that hold the segment, from the first page's to the last one's
+            const int64_t s0 = pre * per_seq + (int64_t)seg * sq.n;
+            const int w0 = (int)(s0 / per), parts = (int)((s0 + sq.n - 1) / per) - w0 + 1;
+            const int first_slot = s0 % per == 0 ? 0 : 1;
+            parts_stored();
+            if (tid == 0) last = part_last(wk.count + w0, parts);
+            __syncthreads();
+            if (last) {
+                auto of = [&](int i) { return wk.part + (size_t)(2 * (w0 + i) + (i == 0 ? first_slot : 0)) * pa_part_floats(D); };
+                // the parts' maxima into LDS, the rows' maximum, then the parts' factors in their place
+                for (int i = tid; i < parts * PA_ROWS; i += 256) {
+                    const int row = i % PA_ROWS;
+                    const float2 x = row < rows ? pa_load2(of(i / PA_ROWS) + 2 * row) : float2{-INFINITY, 0.0f};
+                    lds[i] = x.x;
+                }
+                __syncthreads();
+                if (wave == 0) {   // lane (r, g): every fourth part
+                    float M = -INFINITY;
+                    for (int i = g; i < parts; i += 4) M = fmaxf(M, lds[i * PA_ROWS + r]);
+                    M = xor32_max(xor16_max(M));
+                    if (g == 0) sm[0][r] = pa_safe(M);
+                }
+                __syncthreads();
+                for (int i = tid; i < parts * PA_ROWS; i += 256) lds[i] = pa_exp2(lds[i] - sm[0][i % PA_ROWS]);
+                __syncthreads();
+                for (int i = tid; i < rows * D / 2; i += 256) {
+                    const int row = i / (D / 2), d = 2 * (i % (D / 2));
+                    float sum = 0.0f, x = 0.0f, y = 0.0f;
+                    constexpr int CB = 8;
+                    int k = 0;
+                    for (; k + CB <= parts; k += CB) {
+                        float2 e[CB], s[CB];
+#pragma unroll
+                        for (int c = 0; c < CB; c++) { e[c] = pa_load2(of(k + c) + 2 * PA_ROWS + row * D + d); s[c] = pa_load2(of(k + c) + 2 * row); }
+#pragma unroll
+                        for (int c = 0; c < CB; c++) { const float f = lds[(k + c) * PA_ROWS + row]; sum += f * s[c].y; x += f * e[c].x; y += f * e[c].y; }
+                    }
+                    for (; k < parts; k++) {
+                        const float2 e = pa_load2(of(k) + 2 * PA_ROWS + row * D + d), s = pa_load2(of(k) + 2 * row);
+                        const float f = lds[k * PA_ROWS + row];
+                        sum += f * s.y; x += f * e.x; y += f * e.y;
+                    }
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    *reinterpret_cast<float2*>(a.out + (int64_t)b * a.out_stride + (int64_t)(kvh * G + h0 + row) * D + d) = sum == 0.0f ? float2{0.0f, 0.0f} : float2{x * inv, y * inv};
+                    if (WT && d == 0) *reinterpret_cast<float2*>(wk.stat + 2 * ((int64_t)b * a.nH + kvh * G + h0 + row)) = float2{sm[0][row], inv};
+                }
+                if (tid == 0) part_rearm(wk.count + w0);
+            }
+        }
+        slot = 1;
+        t += tiles;
+        if (t >= t1) return;
+        while (t >= (pre + sq.n) * per_seq) { pre += sq.n; sq = pa_seq(a, ++b); }   // t < t1: another sequence has pages
+        __syncthreads();   // the LDS is written again
     }
 }
 
-size_t paged_attention_work(const PagedKV&, int) { return 256; }
+// weight = decay * weight_in + the sum of p over the query heads of a KV head, from the scores and the rows' statistics.
+__global__ __launch_bounds__(256) void paged_weight_kernel(PagedAttnArgs a, PaWork wk) {
+    const PagedKV& kv = a.kv;
+    const int kvh = blockIdx.y, b = blockIdx.z, G = a.nH / kv.nKV, j = blockIdx.x * 256 + threadIdx.x;
+    const PaSeq s = pa_seq(a, b);
+    if (j >= s.L) return;
+    float p = 0.0f;
+    if (j >= s.first) {
+        const int64_t row = (int64_t)b * a.nH + kvh * G;
+        const float2* stat = reinterpret_cast<const float2*>(wk.stat) + row;
+        const float* sc = wk.score + row * wk.score_stride + j;
+        for (int h = 0; h < G; h++) { const float2 st = stat[h]; p += pa_exp2(sc[(int64_t)h * wk.score_stride] - st.x) * st.y; }
+    }
+    const int64_t at = paged_slot(kv, b, kvh, j);
+    kv.weight[at] = (a.weight_in && a.decay != 0.0f ? a.decay * a.weight_in[at] : 0.0f) + p;
+}
+
+static size_t pa_layout(const PagedKV& kv, int nH, void* base, PaWork& wk) {
+    const int G = nH / kv.nKV;
+    wk.groups = (G + PA_ROWS - 1) / PA_ROWS;
+    const int64_t most = (int64_t)kv.B * kv.nKV * wk.groups * ((kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE), runs = (most + PA_MINPER - 1) / PA_MINPER;
+    wk.W = (int)(runs < PA_MAXW ? runs : PA_MAXW);
+    wk.score_stride = (kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE * MLXR_PAGE;
+    uint8_t* p = static_cast<uint8_t*>(base);
+    size_t at = 0;
+    auto take = [&](size_t bytes) { uint8_t* q = p ? p + at : nullptr; at += (bytes + 255) / 256 * 256; return q; };
+    wk.count = reinterpret_cast<unsigned*>(take(PA_MAXW * sizeof(unsigned)));   // first: where it is for every size
+    wk.part = reinterpret_cast<float*>(take((size_t)2 * wk.W * pa_part_floats(kv.D) * sizeof(float)));
+    wk.stat = wk.score = nullptr;
+    if (kv.weight) {
+        wk.stat = reinterpret_cast<float*>(take((size_t)kv.B * nH * 2 * sizeof(float)));
+        wk.score = reinterpret_cast<float*>(take((size_t)kv.B * nH * wk.score_stride * sizeof(float)));
+    }
+    return at;
+}
+
+size_t paged_attention_work(const PagedKV& kv, int nH) {
+    PaWork wk;
+    return pa_layout(kv, nH, nullptr, wk);
+}
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
-    const dim3 grid(a.kv.nKV, a.kv.B);
-    if (a.kv.st == 0) hipLaunchKernelGGL(paged_attn_simple_kernel<0>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(paged_attn_simple_kernel<1>, grid, dim3(256), 0, s, a);
+    PaWork wk;
+    pa_layout(a.kv, a.nH, a.work, wk);
+#define PA_GO(ST, D, WT) hipLaunchKernelGGL((paged_attn_kernel<ST, D, WT>), dim3(wk.W), dim3(256), 0, s, a, wk)
+#define PA_D(ST, WT) do { if (a.kv.D == 64) PA_GO(ST, 64, WT); else PA_GO(ST, 128, WT); } while (0)
+    if (a.kv.weight) { if (a.kv.st == 0) PA_D(0, true); else PA_D(1, true); }
+    else { if (a.kv.st == 0) PA_D(0, false); else PA_D(1, false); }
+#undef PA_D
+#undef PA_GO
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !a.kv.weight) return e;
+    hipLaunchKernelGGL(paged_weight_kernel, dim3((a.kv.max_len + 255) / 256, a.kv.nKV, a.kv.B), dim3(256), 0, s, a, wk);
     return hipGetLastError();
 }
 
