@@ -23,7 +23,8 @@
 namespace mlxr {
 
 constexpr double SR_ONE = 8796093022208.0;   // 2^43: the weight of the largest logit
-constexpr int SR_T = 1024, SR_BINS = 2048;
+constexpr int SR_T = 1024, SR_W = SR_T / 64;   // threads and waves of a workgroup
+constexpr int SR_BINS = 2048, SR_PER = SR_BINS / SR_T;
 constexpr uint32_t SR_MINUS_INF = 0x007fffffu;   // the order key of -infinity; NaN has 0
 
 __device__ __forceinline__ uint32_t sr_key(float v) {
@@ -35,11 +36,23 @@ __device__ __forceinline__ float sr_value(uint32_t k) { return __uint_as_float((
 
 struct SrRow {
     const float* v; int V;
+    bool vec;           // 16-byte loads of four neighbours from indices divisible by four
     float top;          // the largest logit
     double inv;         // 1 / T
     __device__ __forceinline__ double weight(float x) const { return exp(((double)x - (double)top) * inv); }
     __device__ __forceinline__ uint64_t fixed(float x) const { return (uint64_t)(weight(x) * SR_ONE + 0.5); }
 };
+
+// Four neighbours from index i (divisible by four); -infinity behind the row.
+__device__ __forceinline__ void sr_load4(const SrRow& r, int i, float* o) {
+    if (r.vec && i + 4 <= r.V) {
+        const float4 x = gload4(r.v + i);
+        o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = i + e < r.V ? gload(r.v + i + e) : -INFINITY;
+}
 
 // The tokens with a key above `key`, and `n` of those that have it (lowest indices first).
 struct SrCut { uint32_t key; uint32_t n; };
@@ -51,8 +64,8 @@ __device__ __forceinline__ SrCut sr_min(SrCut a, SrCut b) {   // the shorter of 
 struct SrShared {
     uint64_t mass[SR_BINS];
     uint32_t count[SR_BINS];
-    uint64_t wmass[16], sum;
-    uint32_t wcount[16], pick;
+    uint64_t wmass[SR_W];
+    uint32_t wcount[SR_W], pick;
     uint64_t above_mass; uint32_t above_count;
 };
 
@@ -63,7 +76,7 @@ __device__ uint64_t sr_sum(uint64_t v, SrShared& sh) {
     if ((threadIdx.x & 63) == 0) sh.wmass[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t t = 0;
-    for (int i = 0; i < SR_T / 64; i++) t += sh.wmass[i];
+    for (int i = 0; i < SR_W; i++) t += sh.wmass[i];
     return t;
 }
 __device__ uint64_t sr_max(uint64_t v, SrShared& sh) {
@@ -72,7 +85,7 @@ __device__ uint64_t sr_max(uint64_t v, SrShared& sh) {
     if ((threadIdx.x & 63) == 0) sh.wmass[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t t = 0;
-    for (int i = 0; i < SR_T / 64; i++) t = sh.wmass[i] > t ? sh.wmass[i] : t;
+    for (int i = 0; i < SR_W; i++) t = sh.wmass[i] > t ? sh.wmass[i] : t;
     return t;
 }
 // The sum of the weights within a cut.
@@ -114,12 +127,14 @@ __device__ SrCut sr_descend(const SrRow& r, SrCut cut, bool by_mass, uint64_t ta
         }
         if (tid == 0) { sh.pick = 0xffffffffu; }
         __syncthreads();
-        // thread t has bins - 1 - 2t and the one below it: sums of everything above by scans
-        const int b1 = (int)bins - 1 - 2 * tid, b0 = b1 - 1;
-        const uint32_t c1 = b1 >= 0 ? sh.count[b1] : 0, c0 = b0 >= 0 ? sh.count[b0] : 0;
-        const uint64_t m1 = b1 >= 0 ? sh.mass[b1] : 0, m0 = b0 >= 0 ? sh.mass[b0] : 0;
-        uint32_t c = c1 + c0;
-        uint64_t m = m1 + m0;
+        // thread t has SR_PER bins from bins - 1 - SR_PER t down: sums of everything above by scans
+        const int b1 = (int)bins - 1 - SR_PER * tid;
+        uint32_t c = 0;
+        uint64_t m = 0;
+#pragma unroll
+        for (int h = 0; h < SR_PER; h++) if (b1 - h >= 0) { c += sh.count[b1 - h]; m += sh.mass[b1 - h]; }
+        const uint32_t own_c = c;
+        const uint64_t own_m = m;
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t c2 = __shfl_up(c, o, 64);
             const uint64_t m2 = __shfl_up(m, o, 64);
@@ -127,20 +142,18 @@ __device__ SrCut sr_descend(const SrRow& r, SrCut cut, bool by_mass, uint64_t ta
         }
         if (lane == 63) { sh.wcount[wave] = c; sh.wmass[wave] = m; }
         __syncthreads();
-        uint32_t ca = above_count, call = above_count;
-        uint64_t ma = above_mass, mall = above_mass;
-        for (int i = 0; i < SR_T / 64; i++) {
+        uint32_t ca = above_count + c - own_c, call = above_count;
+        uint64_t ma = above_mass + m - own_m, mall = above_mass;
+        for (int i = 0; i < SR_W; i++) {
             if (i < wave) { ca += sh.wcount[i]; ma += sh.wmass[i]; }
             call += sh.wcount[i]; mall += sh.wmass[i];
         }
         if (level == 0 && (by_mass ? mall : (uint64_t)call) < target) { *mass = mall; return cut; }
-        ca += c - c1 - c0; ma += m - m1 - m0;   // above this thread's bins
-        const uint64_t s0 = by_mass ? ma : ca, s1 = s0 + (by_mass ? m1 : c1), s2 = s1 + (by_mass ? m0 : c0);
-        if (s0 < target && s2 >= target) {   // one thread: sums only grow
-            const bool upper = s1 >= target;
-            sh.pick = (uint32_t)(upper ? b1 : b0);
-            sh.above_count = ca + (upper ? 0 : c1);
-            sh.above_mass = ma + (upper ? 0 : m1);
+        for (int h = 0; h < SR_PER && b1 - h >= 0; h++) {   // one bin of one thread: sums only grow
+            const uint32_t cb = sh.count[b1 - h];
+            const uint64_t mb = sh.mass[b1 - h], s0 = by_mass ? ma : ca, s1 = s0 + (by_mass ? mb : cb);
+            if (s0 < target && s1 >= target) { sh.pick = (uint32_t)(b1 - h); sh.above_count = ca; sh.above_mass = ma; }
+            ca += cb; ma += mb;
         }
         __syncthreads();
         prefix |= sh.pick << shift; mask |= (bins - 1) << shift;
@@ -155,7 +168,7 @@ __device__ SrCut sr_descend(const SrRow& r, SrCut cut, bool by_mass, uint64_t ta
 
 // The index of the n-th (from 1) token with this key.
 __device__ int sr_nth(const SrRow& r, uint32_t key, uint32_t n, SrShared& sh) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = ((r.V + 15) / 16 + 63) & ~63;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = ((r.V + SR_W - 1) / SR_W + 63) & ~63;
     const int i0 = min(r.V, wave * per), i1 = min(r.V, i0 + per);
     uint32_t c = 0;
     for (int i = i0; i < i1; i += 64) c += (uint32_t)__popcll(__ballot(i + lane < i1 && sr_key(r.v[min(i + lane, r.V - 1)]) == key));
@@ -186,19 +199,18 @@ __device__ __forceinline__ uint64_t sr_target(double share, uint64_t sum) {
     return t >= (double)sum ? sum : (uint64_t)t;
 }
 
-// The radix descent over a whole row: any parameters, one workgroup.
-__device__ int sr_descent_token(const SampleRowsArgs& a, int row, const SrRow& r, uint32_t top, SrShared& sh) {
+// The radix descent over a whole row: any parameters, one workgroup. A call of its own: its code is as long as all the rest.
+__device__ __noinline__ int sr_descent_token(const float* v, int V, float largest, double inv, int k, float p, float low, float given, SrShared& sh) {
     const int tid = threadIdx.x;
+    const SrRow r{v, V, false, largest, inv};
+    const uint32_t top = sr_key(largest);
     uint64_t mass = 0, kept_mass = 0;
     SrCut cut{SR_MINUS_INF, 0};
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0 && k < r.V) cut = sr_descend(r, cut, false, (uint64_t)k, sh, &mass);
+    if (k < r.V) cut = sr_descend(r, cut, false, (uint64_t)k, sh, &mass);
     else mass = sr_mass(r, cut, sh);
     SrCut end = cut;
     kept_mass = mass;
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
     if (p < 1.0f) end = sr_descend(r, cut, true, sr_target((double)p, mass), sh, &kept_mass);
-    const float low = a.min_p ? a.min_p[row] : 0.0f;
     if (low > 0.0f) {
         uint64_t least = 0;   // the complement of the smallest key that stays
         for (int i = tid; i < r.V; i += SR_T) {
@@ -219,19 +231,24 @@ __device__ int sr_descent_token(const SampleRowsArgs& a, int row, const SrRow& r
         }
     }
     uint64_t unused;
-    const SrCut at = sr_descend(r, end, true, sr_target((double)a.u[row], kept_mass), sh, &unused);
+    const SrCut at = sr_descend(r, end, true, sr_target((double)given, kept_mass), sh, &unused);
     return sr_nth(r, at.key, at.n, sh);
 }
 
 // ---- bins, gathered tokens and their order ----
 constexpr int SR_GROUP = 64, SR_LIST = 2048;
 constexpr double SR_WIDTH = 64.0;   // bins per unit of x
+typedef uint32_t sr_w4 __attribute__((ext_vector_type(4)));
+typedef uint16_t sr_h2 __attribute__((ext_vector_type(2)));
 
 struct SrWork {
     float* gmax;        // [rows][groups]
+    uint16_t* bin;      // [rows][groups][64]: the tokens' bins (65535: none), written where sums over the row are needed
     uint64_t* mass;     // [rows][SR_BINS]: sums of f, cleared by the first launch where the second adds to them
     unsigned* count;    // [rows]: the workgroups that have added theirs
-    int groups, spans, per;   // groups of a row; workgroups of a row and the groups of each
+    int groups;               // of a row
+    int spans, per;           // the first launch's workgroups of a row, and the groups of each
+    int sum_spans, sum_per;   // the second's, where it adds up bins
 };
 
 // What a row asks for.
@@ -253,12 +270,14 @@ struct SrBins {
     double top, inv;   // the largest logit, bins per unit of logit
     __device__ __forceinline__ double x(float v) const { return (top - (double)v) * inv; }   // in bins; NaN or infinite outside
 };
-// exp(-y / 64) for y in [0, 1): the Taylor sum to the fifth power is off by 2^-45.
-__device__ __forceinline__ double sr_small_exp(double y) {
-    y *= 1.0 / SR_WIDTH;
-    return 1.0 - y * (1.0 - y * (0.5 - y * (1.0 / 6 - y * (1.0 / 24 - y * (1.0 / 120)))));
+// 2^43 exp(-y / 64) for y = x - bin in [0, 1), rounded to a whole number: the Taylor sum to the fifth power is off by
+// 2^-45; added to 2^52 it is rounded into the mantissa's low bits.
+__device__ __forceinline__ uint64_t sr_fixed(double x, int bin) {
+    constexpr double c1 = SR_ONE / SR_WIDTH, c2 = c1 / SR_WIDTH / 2, c3 = c2 / SR_WIDTH / 3, c4 = c3 / SR_WIDTH / 4, c5 = c4 / SR_WIDTH / 5;
+    const double y = x - (double)bin;
+    const double e = fma(y, fma(y, fma(y, fma(y, fma(y, -c5, c4), -c3), c2), -c1), SR_ONE);
+    return __builtin_bit_cast(uint64_t, e + 0x1p52) & 0xfffffffffffffull;
 }
-__device__ __forceinline__ uint64_t sr_fixed(double x, int bin) { return (uint64_t)(sr_small_exp(x - (double)bin) * SR_ONE + 0.5); }
 
 // Per 64 logits the maximum (NaN ignored). A lane has four neighbours, 16 lanes a group.
 template <bool VEC>
@@ -295,188 +314,387 @@ __global__ __launch_bounds__(256) void sample_groups_kernel(SampleRowsArgs a, Sr
     }
 }
 
+// What one workgroup keeps of its row. Code that runs once is paid for by its size (instructions come from memory
+// like data), so loops here stay rolled and exponentials are looked up.
+constexpr int SR_MAXGROUPS = (1 << 20) / SR_GROUP, SR_NEAR = 4096;   // groups of the longest row; of these kept in LDS
 struct SrPick {
-    uint64_t list[SR_LIST], ranked[SR_LIST];
-    double run[SR_LIST], wave_sum[16];
-    int ids[SR_T];
-    int n, nids, first;
+    uint64_t list[SR_LIST];
+    union {
+        struct { uint64_t ranked[SR_LIST]; double run[SR_LIST]; };
+        uint16_t ids[SR_MAXGROUPS];   // while tokens are gathered, before they are ranked
+    };
+    float gmax[SR_NEAR];
+    double exp_whole[32], exp_part[64];   // exp(-i), exp(-i / 64)
+    double wave_sum[2][SR_W];
+    int wave_count[2][4][SR_W];
+    float wave_top[SR_W];
+    int n, nids, found;
     uint32_t best;
-    float wave_top[16];
 };
+static_assert(SR_LIST == SR_BINS && SR_BINS == 32 * 64, "run holds the bins' sums and the gathered tokens'");
 
-// Running sums (inclusive) of two values a thread, 2 tid and 2 tid + 1, over the workgroup: into run.
-__device__ void sr_scan(double a0, double a1, SrPick& s) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    double v = a0 + a1;
-    for (int o = 1; o < 64; o <<= 1) { const double u = __shfl_up(v, o, 64); if (lane >= o) v += u; }
-    __syncthreads();
-    if (lane == 63) s.wave_sum[wave] = v;
-    __syncthreads();
-    double before = 0.0;
-    for (int i = 0; i < wave; i++) before += s.wave_sum[i];
-    const double up = __shfl_up(v, 1, 64);
-    if (lane) before += up;
-    s.run[2 * tid] = before + a0;
-    s.run[2 * tid + 1] = (before + a0) + a1;
-    __syncthreads();
+// Inclusive sums over a wave: within rows of 16 lanes, then the rows' last lanes on to the rows behind.
+template <int CTRL, int ROWS> __device__ __forceinline__ int sr_dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS> __device__ __forceinline__ double sr_dpp(double v) {   // 0 where there is no lane before
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)sr_dpp<CTRL, ROWS>((int)(uint32_t)u), hi = (uint32_t)sr_dpp<CTRL, ROWS>((int)(uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
 }
-// The first i < n with run[i] + base >= target; n if there is none.
-__device__ int sr_first(double target, double base, int n, SrPick& s) {
-    __syncthreads();
-    if (threadIdx.x == 0) s.first = n;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += SR_T)
-        if (s.run[i] + base >= target && (i == 0 || !(s.run[i - 1] + base >= target))) atomicMin(&s.first, i);
-    __syncthreads();
-    return s.first;
-}
-// The first i < n whose weight is below `low` (in [.., n]); the ranked tokens' weights fall.
-__device__ int sr_first_below(double low, int n, const SrBins& bins, SrPick& s) {
-    __syncthreads();
-    if (threadIdx.x == 0) s.first = n;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += SR_T)
-        if (exp(-bins.x(sr_value((uint32_t)(s.ranked[i] >> 32))) / SR_WIDTH) < low) atomicMin(&s.first, i);
-    __syncthreads();
-    return s.first;
+template <typename T> __device__ __forceinline__ T sr_wave_scan(T v) {
+    v += sr_dpp<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8
+    v += sr_dpp<0x112, 0xF>(v);
+    v += sr_dpp<0x114, 0xF>(v);
+    v += sr_dpp<0x118, 0xF>(v);
+    v += sr_dpp<0x142, 0xA>(v);   // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+    v += sr_dpp<0x143, 0xC>(v);
+    return v;
 }
 
-// Gathers the tokens of bins b0 .. b1, ranked, with running sums of their weights in run. Returns how many there
-// are; more than SR_LIST: nothing else is done.
-__device__ int sr_gather(const SrRow& r, const SrBins& bins, const float* gmax, int groups, int b0, int b1, SrPick& s) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    __syncthreads();
-    if (tid == 0) s.n = 0;
-    for (int base = 0; base < groups; base += SR_T) {
-        if (tid == 0) s.nids = 0;
-        __syncthreads();
-        const int g = base + tid;
-        const bool has = g < groups && bins.x(gmax[g]) < (double)(b1 + 1);
-        const uint64_t m = __ballot(has);
-        int at = 0;
-        if (lane == 0 && m) at = atomicAdd(&s.nids, (int)__popcll(m));
-        at = __shfl(at, 0, 64) + (int)__popcll(m & (lane ? ~0ull >> (64 - lane) : 0ull));
-        if (has) s.ids[at] = g;
-        __syncthreads();
-        const int n = s.nids;
-        constexpr int UN = 4;
-        for (int i = wave; i < n; i += 16 * UN) {
-            float v[UN];
-            int idx[UN];
+// The logits within [lo, hi] or [lo2, hi2] of the given groups, as keys, to the list (as many as it holds; n counts all).
+// A wave reads four groups at a time, four neighbours a lane, UN such loads in flight.
+template <int UN>
+__device__ __forceinline__ void sr_collect(const float* v, int V, bool vec, const uint16_t* ids, int count, float lo, float hi, float lo2, float hi2,
+                                           uint64_t* list, int* n) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t before = lane ? ~0ull >> (64 - lane) : 0ull;
+    const SrRow r{v, V, vec, 0.0f, 0.0};
+#pragma unroll 1
+    for (int i = 4 * wave; i < count; i += 4 * SR_W * UN) {
+        float x[UN][4];
+        int idx[UN];
 #pragma unroll
-            for (int u = 0; u < UN; u++) {
-                idx[u] = i + 16 * u < n ? s.ids[i + 16 * u] * SR_GROUP + lane : r.V;
-                v[u] = idx[u] < r.V ? r.v[idx[u]] : -INFINITY;
+        for (int u = 0; u < UN; u++) {
+            const int q = i + 4 * SR_W * u + (lane >> 4);
+            idx[u] = q < count ? ids[q] * SR_GROUP + 4 * (lane & 15) : V;
+            sr_load4(r, idx[u], x[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            uint64_t in[4];
+            int total = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                in[e] = __ballot((x[u][e] >= lo && x[u][e] <= hi) || (x[u][e] >= lo2 && x[u][e] <= hi2));
+                total += (int)__popcll(in[e]);
             }
+            if (!total) continue;
+            int to = 0;
+            if (lane == 0) to = atomicAdd(n, total);
+            to = __builtin_amdgcn_readfirstlane(to);
 #pragma unroll
-            for (int u = 0; u < UN; u++) {
-                const double x = bins.x(v[u]);
-                const bool in = x >= (double)b0 && x < (double)(b1 + 1);
-                const uint64_t mi = __ballot(in);
-                if (!mi) continue;
-                int to = 0;
-                if (lane == 0) to = atomicAdd(&s.n, (int)__popcll(mi));
-                to = __shfl(to, 0, 64) + (int)__popcll(mi & (lane ? ~0ull >> (64 - lane) : 0ull));
-                if (in && to < SR_LIST) s.list[to] = ((uint64_t)sr_key(v[u]) << 32) | (uint32_t)~(uint32_t)idx[u];
+            for (int e = 0; e < 4; e++) {
+                const int at = to + (int)__popcll(in[e] & before);
+                if (((in[e] >> lane) & 1) && at < SR_LIST) list[at] = ((uint64_t)sr_key(x[u][e]) << 32) | (uint32_t)~(uint32_t)(idx[u] + e);
+                to += (int)__popcll(in[e]);
             }
         }
-        __syncthreads();
     }
-    const int n = s.n;
-    if (n > SR_LIST) return n;
-    // each wave sorts its runs of 64 in registers; a key's rank is its place in its run and, for every other run, how
-    // many of that run's keys are larger
-    const int runs = (n + 63) / 64;
-    uint64_t mine[2];
+}
+// The same over a row's bin numbers, as the first pass over it has left them: the logits of bins b0 and `also`. Eight
+// numbers a lane and load, found by packed minima of their differences; a lane with a hit goes on by itself.
+__device__ __noinline__ void sr_collect_bins(const float* v, const uint16_t* bin, int V, int b0, int also, uint64_t* list, int* n) {
+    const uint32_t t0 = (uint32_t)b0 * 0x10001u, t1 = (uint32_t)(also < 0 ? b0 : also) * 0x10001u;
+    auto least = [](uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(sr_h2, a), __builtin_bit_cast(sr_h2, b))); };
+    constexpr int UN = 4;
+#pragma unroll 1
+    for (int i = 8 * (int)threadIdx.x; i < V; i += 8 * SR_T * UN) {
+        sr_w4 x[UN];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int q = wave + 16 * h;
-        mine[h] = 0;
-        if (q < runs) {
-            mine[h] = 64 * q + lane < n ? s.list[64 * q + lane] : 0;
-            uint64_t k = mine[h];
+        for (int u = 0; u < UN; u++) {
+            const int at = i + 8 * SR_T * u;   // rows of numbers are padded to eight
+            x[u] = sr_w4{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            if (at < V) {   // other workgroups' stores of this launch: past the caches
+                const uint64_t* p = reinterpret_cast<const uint64_t*>(bin + at);
+                const uint64_t a = __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                const uint64_t b = __hip_atomic_load(const_cast<uint64_t*>(p + 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                x[u] = sr_w4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
+            }
+        }
+#pragma unroll 1
+        for (int u = 0; u < UN; u++) {
+            const sr_w4 w = x[0];
 #pragma unroll
-            for (int size = 2; size <= 64; size <<= 1)
+            for (int k = 0; k + 1 < UN; k++) x[k] = x[k + 1];
+            uint32_t m[4];
 #pragma unroll
-                for (int d = size >> 1; d > 0; d >>= 1) {
-                    const uint64_t p = __shfl_xor(k, d, 64);
-                    const bool lower = (lane & d) == 0, desc = size == 64 || (lane & size) == 0;
-                    k = (lower == desc) ? (p > k ? p : k) : (p < k ? p : k);
-                }
-            mine[h] = k;
+            for (int k = 0; k < 4; k++) m[k] = least(w[k] ^ t0, w[k] ^ t1);
+            const uint32_t all = least(least(m[0], m[1]), least(m[2], m[3]));
+            if ((all & 0xffffu) && (all >> 16)) continue;
+            uint32_t hits = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) hits |= (m[k] & 0xffffu ? 0u : 1u << (2 * k)) | (m[k] >> 16 ? 0u : 2u << (2 * k));
+            while (hits) {
+                const int at = i + 8 * SR_T * u + __builtin_ctz(hits);
+                hits &= hits - 1;
+                if (at >= V) break;   // the last eight may reach behind the row, where nothing was written
+                const int to = atomicAdd(n, 1);
+                if (to < SR_LIST) list[to] = ((uint64_t)sr_key(gload(v + at)) << 32) | (uint32_t)~(uint32_t)at;
+            }
         }
     }
+}
+
+// The n > 256 gathered tokens, ranked: each wave sorts runs of 64 in registers; a key's rank is its place in its run
+// and, for every other run, how many of that run's keys are larger.
+__device__ __noinline__ void sr_rank_many(uint64_t* list, uint64_t* ranked, int n) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), runs = (n + 63) / 64;
+    for (int q = wave; q < runs; q += SR_W) {
+        uint64_t k = 64 * q + lane < n ? list[64 * q + lane] : 0;
+#pragma unroll 1
+        for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll 1
+            for (int d = size >> 1; d > 0; d >>= 1) {
+                const uint64_t p = __shfl_xor(k, d, 64);
+                const bool lower = (lane & d) == 0, desc = size == 64 || (lane & size) == 0;
+                k = (lower == desc) ? (p > k ? p : k) : (p < k ? p : k);
+            }
+        list[64 * q + lane] = k;
+    }
     __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; h++) if (wave + 16 * h < runs) s.list[64 * (wave + 16 * h) + lane] = mine[h];
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int q = wave + 16 * h;
-        if (q >= runs) continue;
-        int rank = lane;
+    for (int q = wave; q < runs; q += SR_W) {
+        const uint64_t k = list[64 * q + lane];
+        int at = lane;
+#pragma unroll 1
         for (int o = 0; o < runs; o++) {
             if (o == q) continue;
-            const uint64_t* run = s.list + 64 * o;
+            const uint64_t* run = list + 64 * o;
             int lo = 0;
 #pragma unroll
-            for (int step = 32; step > 0; step >>= 1) lo += run[lo + step - 1] > mine[h] ? step : 0;
-            lo += run[lo] > mine[h] ? 1 : 0;
-            rank += lo;
+            for (int step = 32; step > 0; step >>= 1) lo += run[lo + step - 1] > k ? step : 0;
+            at += lo + (run[lo] > k ? 1 : 0);
         }
-        if (mine[h]) s.ranked[rank] = mine[h];
+        if (k) ranked[at] = k;
+    }
+}
+
+// One workgroup at work on a row. The helpers alternate between two places for what waves tell each other, so that
+// each needs one barrier: a place is written again only behind the next one's.
+struct SrTeam {
+    SrPick& s;
+    const SrRow& r;
+    SrBins bins;
+    const float* gmax; int groups;
+    const uint16_t* bin;   // the bins of the row's tokens, where they were written down
+    int tid, lane, wave, flip;
+
+    __device__ __forceinline__ float group(int g) const { return g < SR_NEAR ? s.gmax[g] : gmax[g]; }
+    // A bin's constant, and a logit's weight in units of 2^-43, as the bins' sums have it (0 behind the bins).
+    __device__ __forceinline__ double constant(int bin) const { return s.exp_whole[bin >> 6] * s.exp_part[bin & 63]; }
+    __device__ __forceinline__ double weight(float v) const {
+        const double x = bins.x(v);
+        if (!(x < (double)SR_BINS)) return 0.0;
+        const int bin = (int)x;
+        return constant(bin) * (double)sr_fixed(x, bin);
+    }
+    __device__ __forceinline__ float ranked(int i) const { return sr_value((uint32_t)(s.ranked[i] >> 32)); }
+    __device__ __forceinline__ int token(int i) const { return (int)~(uint32_t)s.ranked[i]; }
+
+    // Running sums (inclusive) of SR_PER values a thread, SR_PER tid .., over the workgroup: into run.
+    __device__ __forceinline__ void scan(const double* a) {
+        double v = 0.0;
+#pragma unroll
+        for (int h = 0; h < SR_PER; h++) v += a[h];
+        v = sr_wave_scan(v);
+        double* sums = s.wave_sum[flip ^= 1];
+        if (lane == 63) sums[wave] = v;
+        __syncthreads();
+        double before = sr_dpp<0x138, 0xF>(v);   // the lane before
+        for (int i = 0; i < wave; i++) before += sums[i];
+#pragma unroll
+        for (int h = 0; h < SR_PER; h++) s.run[SR_PER * tid + h] = before += a[h];
+        __syncthreads();
+    }
+    // Over the workgroup, how often each of up to four conditions holds for an i < n.
+    template <int C, typename F> __device__ __forceinline__ void counts(int n, F yes, int* c) {
+        for (int q = 0; q < C; q++) c[q] = 0;
+        for (int i = tid; i - lane < n; i += SR_T) {
+            bool b[C];
+            for (int q = 0; q < C; q++) b[q] = false;
+            if (i < n) yes(i, b);
+#pragma unroll
+            for (int q = 0; q < C; q++) c[q] += (int)__popcll(__ballot(b[q]));
+        }
+        flip ^= 1;
+        if (lane == 0)
+#pragma unroll
+            for (int q = 0; q < C; q++) s.wave_count[flip][q][wave] = c[q];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < C; q++) {
+            c[q] = 0;
+#pragma unroll
+            for (int i = 0; i < SR_W; i++) c[q] += s.wave_count[flip][q][i];
+        }
+    }
+    // The first i < n with run[i] + base >= target (n if there is none): the sums only grow.
+    __device__ __forceinline__ int first(double target, double base, int n) {
+        int c;
+        counts<1>(n, [&](int i, bool* b) { b[0] = s.run[i] + base < target; }, &c);
+        return c;
+    }
+    // The first i < n whose weight is below `low`: the ranked tokens' weights only fall.
+    __device__ __forceinline__ int first_below(double low, int n) {
+        int c;
+        counts<1>(n, [&](int i, bool* b) { b[0] = weight(ranked(i)) >= low * SR_ONE; }, &c);
+        return c;
+    }
+
+    // Ranks the n gathered tokens.
+    __device__ __forceinline__ void rank(int n) {
+        if (n <= 256) {   // each against all
+            for (int i = tid; i - lane < n; i += SR_T) {
+                const uint64_t k = i < n ? s.list[i] : 0;
+                int above = 0;
+#pragma unroll 4
+                for (int o = 0; o < n; o++) above += s.list[o] > k;
+                if (i < n) s.ranked[above] = k;
+            }
+        } else {
+            sr_rank_many(s.list, s.ranked, n);
+        }
+        __syncthreads();
+    }
+    // The logits of bins b0 .. b1 lie in [lo, hi]; a few of the neighbouring bins may too.
+    __device__ __forceinline__ void range(int b0, int b1, float& lo, float& hi) const {
+        const double top = bins.top, slack = fabs(top) * 0x1p-22 + 0x1p-120;
+        const double l = top - (double)(b1 + 1) / bins.inv, h = top - (double)b0 / bins.inv;
+        lo = fmaxf((float)(l - fabs(l) * 0x1p-22 - slack), -3.402823466e38f);
+        hi = (float)fmin(h + fabs(h) * 0x1p-22 + slack, top);
+        if (!(hi <= (float)top)) hi = (float)top;   // T infinite: 0 / 0
+    }
+    // Gathers the tokens of bins b0 .. b1 and of bin `also` (before them, or -1), and perhaps a few of the bins next to
+    // them, ranked, with the running sums of their weights in run. Returns how many; above SR_LIST nothing else is done.
+    __device__ __forceinline__ int gather(int also, int b0, int b1) {
+        const uint64_t before = lane ? ~0ull >> (64 - lane) : 0ull;
+        float lo, hi, lo2 = 1.0f, hi2 = 0.0f;
+        range(b0, b1, lo, hi);
+        if (also >= 0) range(also, also, lo2, hi2);
+        __syncthreads();
+        if (tid == 0) { s.n = 0; s.nids = 0; }
+        __syncthreads();
+        for (int g = tid; g - lane < groups; g += SR_T) {
+            const uint64_t has = __ballot(g < groups && group(g) >= lo);
+            if (!has) continue;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&s.nids, (int)__popcll(has));
+            at = __builtin_amdgcn_readfirstlane(at) + (int)__popcll(has & before);
+            if ((has >> lane) & 1) s.ids[at] = (uint16_t)g;
+        }
+        __syncthreads();
+        const int ids = s.nids;
+        if (ids <= 8 * SR_W || !bin) sr_collect<1>(r.v, r.V, r.vec, s.ids, ids, lo, hi, lo2, hi2, s.list, &s.n);
+        else sr_collect_bins(r.v, bin, r.V, b0, also, s.list, &s.n);
+        __syncthreads();
+        const int n = s.n;
+        if (n > SR_LIST) return n;
+        rank(n);
+        double w[SR_PER];
+#pragma unroll 1
+        for (int h = 0; h < SR_PER; h++) w[h] = SR_PER * tid + h < n ? weight(ranked(SR_PER * tid + h)) : 0.0;
+        scan(w);
+        return n;
+    }
+};
+
+// The bin down to which there are `want` groups, by their maxima (the last one if there are fewer).
+__device__ __forceinline__ int sr_bin_of(SrTeam& t, int want) {
+    SrPick& s = t.s;
+    int* cnt = reinterpret_cast<int*>(s.list);
+    for (int i = t.tid; i < SR_BINS; i += SR_T) cnt[i] = 0;
+    if (t.tid == 0) s.found = SR_BINS - 1;
+    __syncthreads();
+    for (int g = t.tid; g < t.groups; g += SR_T) {
+        const double x = t.bins.x(t.group(g));
+        if (x < (double)SR_BINS) atomicAdd(&cnt[(int)x], 1);
     }
     __syncthreads();
-    double w[2];
+    int c[SR_PER], v = 0;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        w[h] = 0.0;
-        if (2 * tid + h < n) {
-            const double x = bins.x(sr_value((uint32_t)(s.ranked[2 * tid + h] >> 32)));
-            const int bin = (int)x;
-            w[h] = exp((double)-bin / SR_WIDTH) * (double)sr_fixed(x, bin);   // as the bins' sums have it
-        }
+    for (int h = 0; h < SR_PER; h++) v += c[h] = cnt[SR_PER * t.tid + h];
+    const int own = v;
+    v = sr_wave_scan(v);
+    int* sums = s.wave_count[t.flip ^= 1][0];
+    if (t.lane == 63) sums[t.wave] = v;
+    __syncthreads();
+    v -= own;
+    for (int i = 0; i < t.wave; i++) v += sums[i];
+#pragma unroll
+    for (int h = 0; h < SR_PER; h++) {
+        if (v < want && v + c[h] >= want) s.found = SR_PER * t.tid + h;
+        v += c[h];
     }
-    sr_scan(w[0], w[1], s);
-    return n;
+    __syncthreads();
+    return s.found;
 }
 
 __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrWork wk) {
     __shared__ union { SrShared sh; SrPick pick; } u;
     __shared__ int go;
     SrPick& s = u.pick;
-    const int row = blockIdx.y, span = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.y, span = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float* gmax = wk.gmax + (int64_t)row * wk.groups;
+    constexpr int GU = SR_NEAR / SR_T;
+    float near[GU];
+#pragma unroll
+    for (int k = 0; k < GU; k++) near[k] = gload(gmax + min(tid + k * SR_T, wk.groups - 1));   // in flight while the rest is looked up
     const SrAsk ask = sr_ask(a, row);
     if (span && ask.kind != SR_SUM) return;
+    const float T = a.temperature[row], given = a.u[row];
     SrRow r;
     r.v = a.logits + (int64_t)row * a.stride;
     r.V = a.V;
-    const float* gmax = wk.gmax + (int64_t)row * wk.groups;
+    r.vec = a.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
+    SrTeam t{s, r, SrBins{}, gmax, wk.groups, ask.kind == SR_SUM ? wk.bin + (int64_t)row * wk.groups * SR_GROUP : nullptr, tid, lane, wave, 0};
+    if (wave < 2) {
+        const double e = exp(wave ? (double)-(lane & 31) : (double)-lane / 64.0);
+        if (!wave) s.exp_part[lane] = e;
+        else if (lane < 32) s.exp_whole[lane] = e;
+    }
     float top = -INFINITY;
-    for (int g = tid; g < wk.groups; g += SR_T) top = fmaxf(top, gmax[g]);
+#pragma unroll
+    for (int k = 0; k < GU; k++) { s.gmax[tid + k * SR_T] = near[k]; top = fmaxf(top, near[k]); }
+    for (int g = SR_NEAR + tid; g < wk.groups; g += SR_T) top = fmaxf(top, gload(gmax + g));
     top = wave_max(top);
     if (lane == 0) s.wave_top[wave] = top;
+    if (tid == 0) s.best = 0xffffffffu;
     __syncthreads();
-    for (int i = 0; i < 16; i++) top = fmaxf(top, s.wave_top[i]);
+#pragma unroll
+    for (int i = 0; i < SR_W; i++) top = fmaxf(top, s.wave_top[i]);
     if (!isfinite(top)) {   // none, or infinite
         if (span == 0 && tid == 0) { a.tokens[row] = 0; if (a.status) a.status[row] = 1; }
         return;
     }
     r.top = top;
-    const float T = a.temperature[row];
     r.inv = 1.0 / (double)T;
-    const SrBins bins{(double)top, SR_WIDTH / (double)T};
+    t.bins = SrBins{(double)top, SR_WIDTH * r.inv};
     if (ask.kind == SR_SUM) {
         // the span's share of the bins' sums
         uint64_t* hist = s.list;
         for (int i = tid; i < SR_BINS; i += SR_T) hist[i] = 0;
         __syncthreads();
-        const int i1 = min(r.V, (span + 1) * wk.per * SR_GROUP);
-        for (int i = span * wk.per * SR_GROUP + tid; i < i1; i += SR_T) {
-            const double x = bins.x(r.v[i]);
-            if (x < (double)SR_BINS) {   // not NaN, not -infinity
-                const int bin = (int)x;
-                atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin]), (unsigned long long)sr_fixed(x, bin));
+        const int i1 = min(r.V, (span + 1) * wk.sum_per * SR_GROUP);
+        constexpr int UN = 2;
+#pragma unroll 1
+        for (int i = span * wk.sum_per * SR_GROUP + 4 * tid; i < i1; i += 4 * SR_T * UN) {
+            float v[UN][4];
+#pragma unroll
+            for (int k = 0; k < UN; k++) sr_load4(r, i + 4 * SR_T * k < i1 ? i + 4 * SR_T * k : r.V, v[k]);
+#pragma unroll
+            for (int k = 0; k < UN; k++) {
+                uint32_t bin[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const double x = t.bins.x(v[k][e]);
+                    bin[e] = 0xffffu;
+                    if (x < (double)SR_BINS) {   // not NaN, not -infinity
+                        bin[e] = (uint32_t)(int)x;
+                        atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin[e]]), (unsigned long long)sr_fixed(x, (int)bin[e]));
+                    }
+                }
+                const int at = i + 4 * SR_T * k;
+                if (at < i1)   // read by the row's last workgroup: past the caches, like its other parts
+                    __hip_atomic_store(reinterpret_cast<uint64_t*>(const_cast<uint16_t*>(t.bin) + at),
+                                       (uint64_t)(bin[0] | (bin[1] << 16)) | ((uint64_t)(bin[2] | (bin[3] << 16)) << 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
         __syncthreads();
@@ -484,117 +702,122 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
         for (int i = tid; i < SR_BINS; i += SR_T)
             if (hist[i]) __hip_atomic_fetch_add(&all[i], hist[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         parts_stored();
-        if (tid == 0) go = part_last(wk.count + row, wk.spans);
+        if (tid == 0) go = part_last(wk.count + row, wk.sum_spans);
         __syncthreads();
         if (!go) return;
     }
-    if (tid == 0 && a.status) a.status[row] = 0;
-    if (ask.kind == SR_GREEDY || (ask.low > 1.0f)) {   // no weight is above 1
-        if (tid == 0) s.best = 0xffffffffu;
-        __syncthreads();
-        for (int g = tid; g < wk.groups; g += SR_T) if (gmax[g] == top) atomicMin(&s.best, (uint32_t)g);
-        __syncthreads();
-        const int i = (int)s.best * SR_GROUP + lane;
-        const uint64_t m = __ballot(wave == 0 && i < r.V && r.v[min(i, r.V - 1)] == top);
-        if (tid == 0) a.tokens[row] = (int)s.best * SR_GROUP + (int)__builtin_ctzll(m);
-        return;
-    }
-    double goal = (double)a.u[row];
+    double goal = (double)given;
     goal = goal > 0.0 ? (goal < 1.0 ? goal : 1.0) : 0.0;
     int token = -1;
-    if (ask.kind == SR_TOP) {
-        int b1 = SR_BINS - 1;
-        if (r.V > SR_LIST) {
-            // the bin down to which there are k tokens: that of the k-th largest group maximum; with min-p no further than its own
-            if (ask.k < r.V) {
-                uint32_t* cnt = reinterpret_cast<uint32_t*>(s.list);
-                for (int i = tid; i < SR_BINS; i += SR_T) cnt[i] = 0;
-                __syncthreads();
-                for (int g = tid; g < wk.groups; g += SR_T) {
-                    const double x = bins.x(gmax[g]);
-                    if (x < (double)SR_BINS) atomicAdd(&cnt[(int)x], 1u);
-                }
-                __syncthreads();
-                sr_scan((double)cnt[2 * tid], (double)cnt[2 * tid + 1], s);
-                b1 = min(b1, sr_first((double)ask.k, 0.0, SR_BINS, s));
-            }
-            if (ask.low > 0.0f && ask.p >= 1.0f) b1 = min(b1, (int)(-log((double)ask.low) * SR_WIDTH) + 1);
-        }
-        const int n = sr_gather(r, bins, gmax, wk.groups, 0, b1, s);
-        if (n <= SR_LIST) {
-            const int k = min(ask.k, n);
-            int end = k;
-            if (ask.p < 1.0f) end = min(end, sr_first((double)ask.p * s.run[k - 1], 0.0, k, s) + 1);
-            if (ask.low > 0.0f) end = min(end, sr_first_below((double)ask.low, k, bins, s));
-            end = max(end, 1);
-            const int at = min(sr_first(goal * s.run[end - 1], 0.0, end, s), end - 1);
-            token = (int)~(uint32_t)s.ranked[at];
-        }
+    if (ask.kind == SR_GREEDY || ask.low > 1.0f) {   // no weight is above 1
+        for (int g = tid; g < wk.groups; g += SR_T) if (t.group(g) == top) atomicMin(&s.best, (uint32_t)g);
+        __syncthreads();
+        const int i = (int)s.best * SR_GROUP + lane;
+        const uint64_t m = __ballot(i < r.V && r.v[min(i, r.V - 1)] == top);
+        token = (int)s.best * SR_GROUP + (int)__builtin_ctzll(m);
     } else {
-        const uint64_t* all = wk.mass + (int64_t)row * SR_BINS;
-        double w[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-            w[h] = exp((double)-(2 * tid + h) / SR_WIDTH) * (double)__hip_atomic_load(const_cast<uint64_t*>(&all[2 * tid + h]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sr_scan(w[0], w[1], s);
-        const double sum = s.run[SR_BINS - 1], p_goal = (double)ask.p * sum;
-        int bp = SR_BINS, bm = SR_BINS;
-        if (ask.p < 1.0f) bp = min(sr_first(p_goal, 0.0, SR_BINS, s), SR_BINS - 1);
-        if (ask.low > 0.0f) { const double x = -log((double)ask.low) * SR_WIDTH; if (x < (double)SR_BINS) bm = (int)x; }
-        const int be = min(bp, bm);   // the bin in which the kept tokens end
-        double kept = sum, before = 0.0;
-        int draw = -1;
-        double draw_before = 0.0;
-        if (be == SR_BINS) draw = min(sr_first(goal * kept, 0.0, SR_BINS, s), SR_BINS - 1);
-        else {
-            before = be ? s.run[be - 1] : 0.0;
-            // where the draw falls if it falls before that bin: looked up now, while the bins' sums are there
-        }
-        int n = 0, end = 0;
-        if (be < SR_BINS) {
-            const double keep_run0 = s.run[2 * tid], keep_run1 = s.run[2 * tid + 1];
-            n = sr_gather(r, bins, gmax, wk.groups, be, be, s);
-            if (n <= SR_LIST) {
-                end = n;
-                if (bp == be) end = min(end, sr_first(p_goal, before, n, s) + 1);
-                if (bm == be) end = min(end, sr_first_below((double)ask.low, n, bins, s));
-                kept = before + (end ? s.run[end - 1] : 0.0);
-                if (before == 0.0) end = max(end, 1);
-                if (end && (goal * kept > before || before == 0.0)) {
-                    const int at = min(sr_first(goal * kept, before, end, s), end - 1);
-                    token = (int)~(uint32_t)s.ranked[at];
-                } else {
-                    __syncthreads();
-                    s.run[2 * tid] = keep_run0; s.run[2 * tid + 1] = keep_run1;
-                    draw = min(sr_first(goal * kept, 0.0, be, s), be - 1);
-                }
+        // Where the kept tokens end and the draw falls among them. One gather does for most rows, and a second one if
+        // the draw falls in another bin than was guessed.
+        int also = -1, b0 = 0, b1 = SR_BINS - 1;
+        int bp = SR_BINS, bm = SR_BINS;      // the bins in which top-p and min-p cut
+        double p_goal = 0.0, kept = 0.0, before = 0.0, also_before = 0.0;
+        double sums[SR_PER];                 // the bins' running sums, which the gathered tokens' take the place of
+        bool drawing = false;                // the gathered bin is the draw's
+        if (ask.kind == SR_TOP) {
+            // all tokens down to a bin: that of the k-th largest group maximum, with min-p no further than its own
+            if (r.V > SR_LIST) {
+                if (ask.k < r.V) b1 = sr_bin_of(t, ask.k);
+                if (ask.low > 0.0f && ask.p >= 1.0f) b1 = min(b1, (int)(-log((double)ask.low) * SR_WIDTH) + 1);
             }
+        } else {
+            const uint64_t* all = wk.mass + (int64_t)row * SR_BINS;
+#pragma unroll
+            for (int h = 0; h < SR_PER; h++)
+                sums[h] = t.constant(SR_PER * tid + h) * (double)__hip_atomic_load(const_cast<uint64_t*>(&all[SR_PER * tid + h]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            t.scan(sums);
+#pragma unroll
+            for (int h = 0; h < SR_PER; h++) sums[h] = s.run[SR_PER * tid + h];
+            kept = s.run[SR_BINS - 1];
+            p_goal = (double)ask.p * kept;
+            if (ask.p < 1.0f) bp = min(t.first(p_goal, 0.0, SR_BINS), SR_BINS - 1);
+            if (ask.low > 0.0f) { const double x = -log((double)ask.low) * SR_WIDTH; if (x < (double)SR_BINS) bm = (int)x; }
+            b0 = min(bp, bm);
+            drawing = b0 == SR_BINS;         // nothing is cut
+            // the draw's bin, if all tokens of the bin that the kept ones end in were kept: most often that is it
+            const int last = min(b0, SR_BINS - 1), guess = min(t.first(goal * s.run[last], 0.0, last + 1), last);
+            if (drawing || guess == b0) b0 = guess;
+            else also = guess;
+            b1 = b0;
+            before = b0 ? s.run[b0 - 1] : 0.0;
+            also_before = also > 0 ? s.run[also - 1] : 0.0;
         }
-        if (draw >= 0) {
-            draw_before = draw ? s.run[draw - 1] : 0.0;
-            n = sr_gather(r, bins, gmax, wk.groups, draw, draw, s);
-            if (n > 0 && n <= SR_LIST) token = (int)~(uint32_t)s.ranked[min(sr_first(goal * kept, draw_before, n, s), n - 1)];
+#pragma unroll 1
+        while (true) {
+            const int n = t.gather(also, b0, b1);
+            if (n > SR_LIST) break;
+            if (ask.kind == SR_TOP) {
+                const int k = min(ask.k, n);
+                int end = k;
+                if (ask.p < 1.0f) end = min(end, t.first((double)ask.p * s.run[k - 1], 0.0, k) + 1);
+                if (ask.low > 0.0f) end = min(end, t.first_below((double)ask.low, k));
+                end = max(end, 1);
+                token = t.token(min(t.first(goal * s.run[end - 1], 0.0, end), end - 1));
+                break;
+            }
+            int c[4];   // the list holds bin b0's tokens at c[0] .. c[1] - 1, those of `also` at c[2] .. c[3] - 1
+            t.counts<4>(n, [&](int i, bool* b) {
+                const double x = t.bins.x(t.ranked(i));
+                b[0] = x < (double)b0; b[1] = x < (double)(b0 + 1); b[2] = x < (double)also; b[3] = x < (double)(also + 1);
+            }, c);
+            const double base = before - (c[0] ? s.run[c[0] - 1] : 0.0);
+            int end = c[1];
+            if (!drawing) {
+                if (bp == b0) end = min(end, max(c[0], t.first(p_goal, base, c[1])) + 1);
+                if (bm == b0) end = min(end, max(c[0], t.first_below((double)ask.low, c[1])));
+                if (b0 == 0) end = max(end, 1);
+                kept = end > c[0] ? base + s.run[end - 1] : before;
+            }
+            if (drawing || goal * kept > before || b0 == 0) {
+                if (end > c[0]) token = t.token(min(max(c[0], t.first(goal * kept, base, end)), end - 1));
+                break;
+            }
+            if (also >= 0 && goal * kept > also_before) {
+                if (c[3] > c[2]) token = t.token(min(max(c[2], t.first(goal * kept, also_before - (c[2] ? s.run[c[2] - 1] : 0.0), c[3])), c[3] - 1));
+                break;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < SR_PER; h++) s.run[SR_PER * tid + h] = sums[h];
+            __syncthreads();
+            b1 = b0 = min(t.first(goal * kept, 0.0, b0), b0 - 1);
+            before = b0 ? s.run[b0 - 1] : 0.0;
+            also = -1;
+            drawing = true;
         }
     }
     if (token < 0) {
         __syncthreads();
-        token = sr_descent_token(a, row, r, sr_key(top), u.sh);
+        token = sr_descent_token(r.v, r.V, r.top, r.inv, ask.k, ask.p, ask.low, given, u.sh);
     }
-    if (tid == 0) a.tokens[row] = token;
+    if (tid == 0) { a.tokens[row] = token; if (a.status) a.status[row] = 0; }
 }
 
+constexpr int SR_SUM_WGS = 512;
 static size_t sr_layout(int rows, int V, void* base, SrWork& wk) {
     wk.groups = (V + SR_GROUP - 1) / SR_GROUP;
-    // about a thousand workgroups, of 64 groups each at least
-    const int most = (wk.groups + 63) / 64, want = (1024 + rows - 1) / rows;
-    wk.spans = want < most ? want : most;
-    wk.per = (wk.groups + wk.spans - 1) / wk.spans;
-    wk.spans = (wk.groups + wk.per - 1) / wk.per;
+    auto cut = [&](int wgs, int& spans, int& per) {   // about wgs workgroups in all, of 64 groups each at least
+        const int most = (wk.groups + 63) / 64, want = (wgs + rows - 1) / rows;
+        per = (wk.groups + (want < most ? want : most) - 1) / (want < most ? want : most);
+        spans = (wk.groups + per - 1) / per;
+    };
+    cut(1024, wk.spans, wk.per);
+    cut(SR_SUM_WGS, wk.sum_spans, wk.sum_per);
     uint8_t* p = static_cast<uint8_t*>(base);
     size_t at = 0;
     auto take = [&](size_t bytes) { uint8_t* q = p ? p + at : nullptr; at += (bytes + 255) / 256 * 256; return q; };
     wk.count = reinterpret_cast<unsigned*>(take((size_t)rows * 4));
     wk.gmax = reinterpret_cast<float*>(take((size_t)rows * wk.groups * 4));
+    wk.bin = reinterpret_cast<uint16_t*>(take((size_t)rows * wk.groups * SR_GROUP * 2));
     wk.mass = reinterpret_cast<uint64_t*>(take((size_t)rows * SR_BINS * 8));
     return at;
 }
@@ -611,7 +834,7 @@ hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s) {
     const bool vec = a.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
     if (vec) hipLaunchKernelGGL(sample_groups_kernel<true>, grid, dim3(256), 0, s, a, wk);
     else hipLaunchKernelGGL(sample_groups_kernel<false>, grid, dim3(256), 0, s, a, wk);
-    hipLaunchKernelGGL(sample_pick_kernel, grid, dim3(SR_T), 0, s, a, wk);
+    hipLaunchKernelGGL(sample_pick_kernel, dim3(wk.sum_spans, a.rows), dim3(SR_T), 0, s, a, wk);
     return hipGetLastError();
 }
 
