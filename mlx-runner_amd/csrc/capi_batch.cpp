@@ -18,6 +18,7 @@ int check_kv(const mlxr_paged_kv* kv) {
     if (kv->st != 0 && kv->st != 1) return bad("paged cache: st must be 0 (bf16) or 1 (f16)");
     if (kv->B < 1 || kv->nKV < 1 || kv->n_pages < 1 || kv->table_stride < 1 || kv->max_len < 1) return bad("paged cache: sizes");
     if (kv->nKV > 1024 || kv->B > 65535) return set_error(MLXR_E_UNSUPPORTED, "paged cache: at most 1024 KV heads and 65535 sequences");
+    if (kv->max_len > (1 << 24)) return set_error(MLXR_E_UNSUPPORTED, "paged cache: at most 16777216 slots a sequence");
     if (kv->max_len > (int64_t)kv->table_stride * MLXR_PAGE) return bad("paged cache: max_len is more than the table holds");
     if ((kv->weight || kv->position) && kv->slot_stride < kv->max_len) return bad("paged cache: slot_stride is less than max_len");
     if (!aligned(kv->k, 16) || !aligned(kv->v, 16)) return bad("paged cache: k and v must be 16-byte aligned");

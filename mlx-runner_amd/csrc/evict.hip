@@ -11,68 +11,101 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // ---- selection: one workgroup of 1024 threads per (KV head, sequence) ----
-// Of the middle slots (behind the sink, before the window) the `want` heaviest: an 8-bit radix select of the
-// want-th largest key, then one ordered pass that keeps every larger key and the first of the equal ones. The
-// kept slots go to the list in order, weights and positions straight to dst.
-__global__ __launch_bounds__(1024) void evict_select_kernel(PagedEvictArgs a, int* list, int list_stride) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t pick[2];
-    __shared__ uint32_t wsum[2][16];
-    const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Of the middle slots (behind the sink, before the window) the `want` heaviest. The weights are read once, as keys
+// into LDS (of sequences longer than that holds, the rest is read again from memory each time). A radix select finds
+// the want-th largest key, 11, 11 and 10 bits at a time, and stops as soon as a bin is kept whole. Then each wave
+// counts in a range of slots of its own, and after one barrier writes what is kept of it in order: every larger key,
+// and the first of the equal ones.
+constexpr int EV_T = 1024, EV_W = EV_T / 64, EV_BINS = 2048, EV_NEAR = 32768;   // keys in LDS at most
+constexpr int EV_DEFAULT = 13000;   // of these, as many as a launch may have without asking for more LDS
+
+__global__ __launch_bounds__(EV_T) void evict_select_kernel(PagedEvictArgs a, int* list, int list_stride, int near) {
+    extern __shared__ uint32_t keys[];   // [near]
+    __shared__ int hist[EV_BINS];
+    __shared__ int sums[EV_W], kept_of[EV_W], equal_of[EV_W], pick[3];
+    const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float* w = a.src.weight + paged_slot(a.src, b, kvh, 0);
     const int n = paged_len(a.src, b), kept = min(n, a.budget);
     if (kvh == 0 && tid == 0) a.dst.len[b] = kept;
-    const float* w = a.src.weight + paged_slot(a.src, b, kvh, 0);
     int* out = list + ((int64_t)b * a.src.nKV + kvh) * list_stride;
-    const int lo = min(a.sink, n), hi = n - a.window;
-    uint32_t prefix = 0, want = 0;
-    if (n > kept) {
-        want = (uint32_t)(kept - a.sink - a.window);
-        uint32_t mask = 0;
-        for (int shift = 24; shift >= 0 && want; shift -= 8) {
-            for (int i = tid; i < 256; i += 1024) hist[i] = 0;
-            __syncthreads();
-            for (int j = lo + tid; j < hi; j += 1024) {
-                const uint32_t k = weight_key(w[j]);
-                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                uint32_t run = 0;
-                int bin = 255;
-                while (bin > 0 && run + hist[bin] < want) run += hist[bin--];
-                pick[0] = (uint32_t)bin; pick[1] = want - run;
-            }
-            __syncthreads();
-            prefix |= pick[0] << shift; mask |= 255u << shift; want = pick[1];
-            __syncthreads();
-        }
-        if (a.budget == a.sink + a.window) prefix = 0xffffffffu;   // no middle slot stays (no key is that large)
+    const int lo = min(a.sink, n), hi = n - a.window;   // the middle slots, where any goes
+    const bool cut = n > kept;
+    uint32_t least = 0xffffffffu;   // kept: keys above it, and of the equal ones the first `want`
+    int want = 0;
+    if (cut) {
+#pragma unroll 4
+        for (int j = tid; j < min(n, near); j += EV_T) keys[j] = weight_key(gload(w + j));
     }
-    // ordered pass: per 1024 slots the kept ones before each, among the equal keys the first `want`
-    uint32_t base = 0, equal = 0;
-    for (int j0 = 0; j0 < n; j0 += 1024) {
-        const int j = j0 + tid;
-        uint32_t k = 0;
-        bool mid = false, eq = false;
-        if (j < n && n > kept && j >= lo && j < hi) { mid = true; k = weight_key(w[j]); eq = k == prefix; }
-        const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
-        const uint64_t be = __ballot(eq);
-        if (lane == 0) wsum[0][wave] = (uint32_t)__popcll(be);
-        __syncthreads();
-        uint32_t e = equal + (uint32_t)__popcll(be & below);
-        for (int i = 0; i < 16; i++) { if (i < wave) e += wsum[0][i]; equal += wsum[0][i]; }
-        const bool keep = j < n && (!mid || k > prefix || (eq && e < want));
-        const uint64_t bk = __ballot(keep);
-        if (lane == 0) wsum[1][wave] = (uint32_t)__popcll(bk);
-        __syncthreads();
-        uint32_t at = base + (uint32_t)__popcll(bk & below);
-        for (int i = 0; i < 16; i++) { if (i < wave) at += wsum[1][i]; base += wsum[1][i]; }
-        if (keep && at < (uint32_t)kept) {
-            out[at] = j;
-            if (a.dst.weight) a.dst.weight[paged_slot(a.dst, b, kvh, (int)at)] = w[j];
-            if (a.dst.position) a.dst.position[paged_slot(a.dst, b, kvh, (int)at)] = a.src.position[paged_slot(a.src, b, kvh, j)];
+    auto key = [&](int j) { return j < near ? keys[j] : weight_key(w[j]); };
+    if (cut && kept > a.sink + a.window) {
+        want = kept - a.sink - a.window;
+        uint32_t prefix = 0, mask = 0;
+        for (int level = 0; level < 3; level++) {
+            const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bins = level == 2 ? 1024 : 2048;
+            for (int i = tid; i < EV_BINS; i += EV_T) hist[i] = 0;
+            __syncthreads();
+            for (int j = lo + tid; j < hi; j += EV_T) {
+                const uint32_t k = key(j);
+                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+            }
+            __syncthreads();
+            // thread t has bins 2047 - 2 t and 2046 - 2 t: the sums above them by a scan
+            const int b1 = EV_BINS - 1 - 2 * tid, c1 = hist[b1], c0 = hist[b1 - 1];
+            int v = wave_scan(c1 + c0);
+            if (lane == 63) sums[wave] = v;
+            __syncthreads();
+            v -= c1 + c0;
+            for (int i = 0; i < wave; i++) v += sums[i];
+            if (v < want && v + c1 + c0 >= want) {
+                const bool upper = v + c1 >= want;
+                pick[0] = upper ? b1 : b1 - 1;
+                pick[1] = want - (upper ? v : v + c1);           // of this bin's
+                pick[2] = pick[1] == (upper ? c1 : c0);          // all of them
+            }
+            __syncthreads();
+            prefix |= (uint32_t)pick[0] << shift; mask |= (uint32_t)(bins - 1) << shift;
+            want = pick[1];
+            least = prefix;
+            if (pick[2] && prefix) { least = prefix - 1; want = 0; break; }
         }
+    } else if (cut) {
         __syncthreads();
+    }
+    // each wave's range: how much of it stays for sure, how much is equal to `least`
+    const int per = ((n + EV_W - 1) / EV_W + 63) & ~63, j0 = min(n, wave * per), j1 = min(n, j0 + per);
+    auto look = [&](int j, bool& sure, bool& equal) {
+        const bool mid = cut && j >= lo && j < hi;
+        const uint32_t k = mid && j < j1 ? key(j) : 0;
+        sure = j < j1 && (!mid || k > least);
+        equal = j < j1 && mid && k == least;
+    };
+    int ks = 0, es = 0;
+    for (int j = j0 + lane; j - lane < j1; j += 64) {
+        bool sure, equal;
+        look(j, sure, equal);
+        ks += (int)__popcll(__ballot(sure));
+        es += (int)__popcll(__ballot(equal));
+    }
+    if (lane == 0) { kept_of[wave] = ks; equal_of[wave] = es; }
+    __syncthreads();
+    int at = 0, seen = 0;
+    for (int i = 0; i < wave; i++) { at += kept_of[i]; seen += equal_of[i]; }
+    at += min(seen, want);
+    const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
+    for (int j = j0 + lane; j - lane < j1; j += 64) {
+        bool sure, equal;
+        look(j, sure, equal);
+        const uint64_t be = __ballot(equal);
+        const bool keep = sure || (equal && seen + (int)__popcll(be & below) < want);
+        const uint64_t bk = __ballot(keep);
+        const int to = at + (int)__popcll(bk & below);
+        if (keep && to < kept) {
+            out[to] = j;
+            if (a.dst.weight) a.dst.weight[paged_slot(a.dst, b, kvh, to)] = w[j];
+            if (a.dst.position) a.dst.position[paged_slot(a.dst, b, kvh, to)] = a.src.position[paged_slot(a.src, b, kvh, j)];
+        }
+        seen += (int)__popcll(be);
+        at += (int)__popcll(bk);
     }
 }
 
@@ -104,7 +137,11 @@ size_t paged_evict_work(const PagedKV& src, int budget) {
 hipError_t launch_paged_evict(const PagedEvictArgs& a, hipStream_t s) {
     const int room = evict_room(a.src, a.budget);
     int* list = static_cast<int*>(a.work);
-    hipLaunchKernelGGL(evict_select_kernel, dim3(a.src.nKV, a.src.B), dim3(1024), 0, s, a, list, room);
+    const int near = a.src.max_len < EV_NEAR ? a.src.max_len : EV_NEAR;
+    if (near > EV_DEFAULT)   // asked for each time: it holds for the current device only
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(evict_select_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, EV_NEAR * 4)) return e;
+    hipLaunchKernelGGL(evict_select_kernel, dim3(a.src.nKV, a.src.B), dim3(EV_T), (size_t)near * 4, s, a, list, room, near);
+    if (hipError_t e = hipGetLastError()) return e;
     const int64_t threads = (int64_t)room * (a.src.D / 8);
     hipLaunchKernelGGL(evict_copy_kernel, dim3((unsigned)((threads + 255) / 256), a.src.nKV, a.src.B), dim3(256), 0, s, a, list, room);
     return hipGetLastError();

@@ -245,7 +245,6 @@ struct SrWork {
     float* gmax;        // [rows][groups]
     uint16_t* bin;      // [rows][groups][64]: the tokens' bins (65535: none), written where sums over the row are needed
     uint64_t* mass;     // [rows][SR_BINS]: sums of f, cleared by the first launch where the second adds to them
-    unsigned* count;    // [rows]: the workgroups that have added theirs
     int groups;               // of a row
     int spans, per;           // the first launch's workgroups of a row, and the groups of each
     int sum_spans, sum_per;   // the second's, where it adds up bins
@@ -266,8 +265,10 @@ __device__ __forceinline__ SrAsk sr_ask(const SampleRowsArgs& a, int row) {
     return q;
 }
 
+__host__ __device__ __forceinline__ bool sr_vec(const SampleRowsArgs& a) { return a.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0; }
+
 struct SrBins {
-    double top, inv;   // the largest logit, bins per unit of logit
+    double top, inv, width;   // the largest logit; bins per unit of logit, and the other way round
     __device__ __forceinline__ double x(float v) const { return (top - (double)v) * inv; }   // in bins; NaN or infinite outside
 };
 // 2^43 exp(-y / 64) for y = x - bin in [0, 1), rounded to a whole number: the Taylor sum to the fifth power is off by
@@ -284,7 +285,6 @@ template <bool VEC>
 __global__ __launch_bounds__(256) void sample_groups_kernel(SampleRowsArgs a, SrWork wk) {
     const int row = blockIdx.y, span = blockIdx.x, tid = threadIdx.x;
     const float* v = a.logits + (int64_t)row * a.stride;
-    if (tid == 0 && span == 0) wk.count[row] = 0;
     if (sr_ask(a, row).kind == SR_SUM)
         for (int i = span * 256 + tid; i < SR_BINS; i += wk.spans * 256) wk.mass[(int64_t)row * SR_BINS + i] = 0;
     const int g1 = min(wk.groups, (span + 1) * wk.per);
@@ -314,6 +314,55 @@ __global__ __launch_bounds__(256) void sample_groups_kernel(SampleRowsArgs a, Sr
     }
 }
 
+// The bins' sums of the rows that need them, several workgroups a row, and each token's bin.
+constexpr int SR_SUM_T = 512;
+__global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a, SrWork wk) {
+    __shared__ uint64_t hist[SR_BINS];
+    __shared__ float wave_top[SR_SUM_T / 64];
+    const int row = blockIdx.y, tid = threadIdx.x;
+    if (sr_ask(a, row).kind != SR_SUM) return;
+    const float* gmax = wk.gmax + (int64_t)row * wk.groups;
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int g = tid; g < wk.groups; g += SR_SUM_T) top = fmaxf(top, gload(gmax + g));
+    for (int i = tid; i < SR_BINS; i += SR_SUM_T) hist[i] = 0;
+    top = wave_max(top);
+    if ((tid & 63) == 0) wave_top[tid >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SR_SUM_T / 64; i++) top = fmaxf(top, wave_top[i]);
+    if (!isfinite(top)) return;
+    const SrRow r{a.logits + (int64_t)row * a.stride, a.V, sr_vec(a), top, 0.0};
+    const SrBins bins{(double)top, SR_WIDTH * (1.0 / (double)a.temperature[row]), 0.0};
+    uint16_t* out = wk.bin + (int64_t)row * wk.groups * SR_GROUP;
+    const int i1 = min(a.V, ((int)blockIdx.x + 1) * wk.sum_per * SR_GROUP);
+    constexpr int UN = 4;
+#pragma unroll 1
+    for (int i = blockIdx.x * wk.sum_per * SR_GROUP + 4 * tid; i < i1; i += 4 * SR_SUM_T * UN) {
+        float v[UN][4];
+#pragma unroll
+        for (int k = 0; k < UN; k++) sr_load4(r, i + 4 * SR_SUM_T * k < i1 ? i + 4 * SR_SUM_T * k : a.V, v[k]);
+#pragma unroll
+        for (int k = 0; k < UN; k++) {
+            uint32_t bin[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double x = bins.x(v[k][e]);
+                bin[e] = 0xffffu;
+                if (x < (double)SR_BINS) {   // not NaN, not -infinity
+                    bin[e] = (uint32_t)(int)x;
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin[e]]), (unsigned long long)sr_fixed(x, (int)bin[e]));
+                }
+            }
+            const int at = i + 4 * SR_SUM_T * k;
+            if (at < i1) *reinterpret_cast<uint2*>(out + at) = uint2{bin[0] | (bin[1] << 16), bin[2] | (bin[3] << 16)};
+        }
+    }
+    __syncthreads();
+    unsigned long long* all = reinterpret_cast<unsigned long long*>(wk.mass + (int64_t)row * SR_BINS);
+    for (int i = tid; i < SR_BINS; i += SR_SUM_T) if (hist[i]) atomicAdd(all + i, (unsigned long long)hist[i]);
+}
+
 // What one workgroup keeps of its row. Code that runs once is paid for by its size (instructions come from memory
 // like data), so loops here stay rolled and exponentials are looked up.
 constexpr int SR_MAXGROUPS = (1 << 20) / SR_GROUP, SR_NEAR = 4096;   // groups of the longest row; of these kept in LDS
@@ -332,23 +381,6 @@ struct SrPick {
     uint32_t best;
 };
 static_assert(SR_LIST == SR_BINS && SR_BINS == 32 * 64, "run holds the bins' sums and the gathered tokens'");
-
-// Inclusive sums over a wave: within rows of 16 lanes, then the rows' last lanes on to the rows behind.
-template <int CTRL, int ROWS> __device__ __forceinline__ int sr_dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
-template <int CTRL, int ROWS> __device__ __forceinline__ double sr_dpp(double v) {   // 0 where there is no lane before
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)sr_dpp<CTRL, ROWS>((int)(uint32_t)u), hi = (uint32_t)sr_dpp<CTRL, ROWS>((int)(uint32_t)(u >> 32));
-    return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
-}
-template <typename T> __device__ __forceinline__ T sr_wave_scan(T v) {
-    v += sr_dpp<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8
-    v += sr_dpp<0x112, 0xF>(v);
-    v += sr_dpp<0x114, 0xF>(v);
-    v += sr_dpp<0x118, 0xF>(v);
-    v += sr_dpp<0x142, 0xA>(v);   // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
-    v += sr_dpp<0x143, 0xC>(v);
-    return v;
-}
 
 // The logits within [lo, hi] or [lo2, hi2] of the given groups, as keys, to the list (as many as it holds; n counts all).
 // A wave reads four groups at a time, four neighbours a lane, UN such loads in flight.
@@ -403,12 +435,7 @@ __device__ __noinline__ void sr_collect_bins(const float* v, const uint16_t* bin
         for (int u = 0; u < UN; u++) {
             const int at = i + 8 * SR_T * u;   // rows of numbers are padded to eight
             x[u] = sr_w4{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-            if (at < V) {   // other workgroups' stores of this launch: past the caches
-                const uint64_t* p = reinterpret_cast<const uint64_t*>(bin + at);
-                const uint64_t a = __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                const uint64_t b = __hip_atomic_load(const_cast<uint64_t*>(p + 1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                x[u] = sr_w4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
-            }
+            if (at < V) x[u] = gload(reinterpret_cast<const sr_w4*>(bin + at));
         }
 #pragma unroll 1
         for (int u = 0; u < UN; u++) {
@@ -428,10 +455,12 @@ __device__ __noinline__ void sr_collect_bins(const float* v, const uint16_t* bin
                 hits &= hits - 1;
                 if (at >= V) break;   // the last eight may reach behind the row, where nothing was written
                 const int to = atomicAdd(n, 1);
-                if (to < SR_LIST) list[to] = ((uint64_t)sr_key(gload(v + at)) << 32) | (uint32_t)~(uint32_t)at;
+                if (to < SR_LIST) list[to] = (uint32_t)~(uint32_t)at;
             }
         }
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(*n, SR_LIST); i += SR_T) list[i] |= (uint64_t)sr_key(gload(v + (int)~(uint32_t)list[i])) << 32;
 }
 
 // The n > 256 gathered tokens, ranked: each wave sorts runs of 64 in registers; a key's rank is its place in its run
@@ -494,11 +523,11 @@ struct SrTeam {
         double v = 0.0;
 #pragma unroll
         for (int h = 0; h < SR_PER; h++) v += a[h];
-        v = sr_wave_scan(v);
+        v = wave_scan(v);
         double* sums = s.wave_sum[flip ^= 1];
         if (lane == 63) sums[wave] = v;
         __syncthreads();
-        double before = sr_dpp<0x138, 0xF>(v);   // the lane before
+        double before = lane_before<0x138, 0xF>(v);   // the lane before
         for (int i = 0; i < wave; i++) before += sums[i];
 #pragma unroll
         for (int h = 0; h < SR_PER; h++) s.run[SR_PER * tid + h] = before += a[h];
@@ -557,10 +586,10 @@ struct SrTeam {
     // The logits of bins b0 .. b1 lie in [lo, hi]; a few of the neighbouring bins may too.
     __device__ __forceinline__ void range(int b0, int b1, float& lo, float& hi) const {
         const double top = bins.top, slack = fabs(top) * 0x1p-22 + 0x1p-120;
-        const double l = top - (double)(b1 + 1) / bins.inv, h = top - (double)b0 / bins.inv;
+        const double l = top - (double)(b1 + 1) * bins.width, h = top - (double)b0 * bins.width;
         lo = fmaxf((float)(l - fabs(l) * 0x1p-22 - slack), -3.402823466e38f);
         hi = (float)fmin(h + fabs(h) * 0x1p-22 + slack, top);
-        if (!(hi <= (float)top)) hi = (float)top;   // T infinite: 0 / 0
+        if (!(hi <= (float)top)) hi = (float)top;   // T infinite: 0 times infinity
     }
     // Gathers the tokens of bins b0 .. b1 and of bin `also` (before them, or -1), and perhaps a few of the bins next to
     // them, ranked, with the running sums of their weights in run. Returns how many; above SR_LIST nothing else is done.
@@ -569,8 +598,6 @@ struct SrTeam {
         float lo, hi, lo2 = 1.0f, hi2 = 0.0f;
         range(b0, b1, lo, hi);
         if (also >= 0) range(also, also, lo2, hi2);
-        __syncthreads();
-        if (tid == 0) { s.n = 0; s.nids = 0; }
         __syncthreads();
         for (int g = tid; g - lane < groups; g += SR_T) {
             const uint64_t has = __ballot(g < groups && group(g) >= lo);
@@ -612,7 +639,7 @@ __device__ __forceinline__ int sr_bin_of(SrTeam& t, int want) {
 #pragma unroll
     for (int h = 0; h < SR_PER; h++) v += c[h] = cnt[SR_PER * t.tid + h];
     const int own = v;
-    v = sr_wave_scan(v);
+    v = wave_scan(v);
     int* sums = s.wave_count[t.flip ^= 1][0];
     if (t.lane == 63) sums[t.wave] = v;
     __syncthreads();
@@ -629,21 +656,19 @@ __device__ __forceinline__ int sr_bin_of(SrTeam& t, int want) {
 
 __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrWork wk) {
     __shared__ union { SrShared sh; SrPick pick; } u;
-    __shared__ int go;
     SrPick& s = u.pick;
-    const int row = blockIdx.y, span = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* gmax = wk.gmax + (int64_t)row * wk.groups;
     constexpr int GU = SR_NEAR / SR_T;
     float near[GU];
 #pragma unroll
     for (int k = 0; k < GU; k++) near[k] = gload(gmax + min(tid + k * SR_T, wk.groups - 1));   // in flight while the rest is looked up
     const SrAsk ask = sr_ask(a, row);
-    if (span && ask.kind != SR_SUM) return;
     const float T = a.temperature[row], given = a.u[row];
     SrRow r;
     r.v = a.logits + (int64_t)row * a.stride;
     r.V = a.V;
-    r.vec = a.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
+    r.vec = sr_vec(a);
     SrTeam t{s, r, SrBins{}, gmax, wk.groups, ask.kind == SR_SUM ? wk.bin + (int64_t)row * wk.groups * SR_GROUP : nullptr, tid, lane, wave, 0};
     if (wave < 2) {
         const double e = exp(wave ? (double)-(lane & 31) : (double)-lane / 64.0);
@@ -656,56 +681,17 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
     for (int g = SR_NEAR + tid; g < wk.groups; g += SR_T) top = fmaxf(top, gload(gmax + g));
     top = wave_max(top);
     if (lane == 0) s.wave_top[wave] = top;
-    if (tid == 0) s.best = 0xffffffffu;
+    if (tid == 0) { s.best = 0xffffffffu; s.n = 0; s.nids = 0; }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < SR_W; i++) top = fmaxf(top, s.wave_top[i]);
     if (!isfinite(top)) {   // none, or infinite
-        if (span == 0 && tid == 0) { a.tokens[row] = 0; if (a.status) a.status[row] = 1; }
+        if (tid == 0) { a.tokens[row] = 0; if (a.status) a.status[row] = 1; }
         return;
     }
     r.top = top;
     r.inv = 1.0 / (double)T;
-    t.bins = SrBins{(double)top, SR_WIDTH * r.inv};
-    if (ask.kind == SR_SUM) {
-        // the span's share of the bins' sums
-        uint64_t* hist = s.list;
-        for (int i = tid; i < SR_BINS; i += SR_T) hist[i] = 0;
-        __syncthreads();
-        const int i1 = min(r.V, (span + 1) * wk.sum_per * SR_GROUP);
-        constexpr int UN = 2;
-#pragma unroll 1
-        for (int i = span * wk.sum_per * SR_GROUP + 4 * tid; i < i1; i += 4 * SR_T * UN) {
-            float v[UN][4];
-#pragma unroll
-            for (int k = 0; k < UN; k++) sr_load4(r, i + 4 * SR_T * k < i1 ? i + 4 * SR_T * k : r.V, v[k]);
-#pragma unroll
-            for (int k = 0; k < UN; k++) {
-                uint32_t bin[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const double x = t.bins.x(v[k][e]);
-                    bin[e] = 0xffffu;
-                    if (x < (double)SR_BINS) {   // not NaN, not -infinity
-                        bin[e] = (uint32_t)(int)x;
-                        atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin[e]]), (unsigned long long)sr_fixed(x, (int)bin[e]));
-                    }
-                }
-                const int at = i + 4 * SR_T * k;
-                if (at < i1)   // read by the row's last workgroup: past the caches, like its other parts
-                    __hip_atomic_store(reinterpret_cast<uint64_t*>(const_cast<uint16_t*>(t.bin) + at),
-                                       (uint64_t)(bin[0] | (bin[1] << 16)) | ((uint64_t)(bin[2] | (bin[3] << 16)) << 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        }
-        __syncthreads();
-        uint64_t* all = wk.mass + (int64_t)row * SR_BINS;
-        for (int i = tid; i < SR_BINS; i += SR_T)
-            if (hist[i]) __hip_atomic_fetch_add(&all[i], hist[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        parts_stored();
-        if (tid == 0) go = part_last(wk.count + row, wk.sum_spans);
-        __syncthreads();
-        if (!go) return;
-    }
+    t.bins = SrBins{(double)top, SR_WIDTH * r.inv, (double)T / SR_WIDTH};
     double goal = (double)given;
     goal = goal > 0.0 ? (goal < 1.0 ? goal : 1.0) : 0.0;
     int token = -1;
@@ -733,7 +719,7 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
             const uint64_t* all = wk.mass + (int64_t)row * SR_BINS;
 #pragma unroll
             for (int h = 0; h < SR_PER; h++)
-                sums[h] = t.constant(SR_PER * tid + h) * (double)__hip_atomic_load(const_cast<uint64_t*>(&all[SR_PER * tid + h]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                sums[h] = t.constant(SR_PER * tid + h) * (double)all[SR_PER * tid + h];
             t.scan(sums);
 #pragma unroll
             for (int h = 0; h < SR_PER; h++) sums[h] = s.run[SR_PER * tid + h];
@@ -788,6 +774,7 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
             __syncthreads();
 #pragma unroll
             for (int h = 0; h < SR_PER; h++) s.run[SR_PER * tid + h] = sums[h];
+            if (tid == 0) { s.n = 0; s.nids = 0; }
             __syncthreads();
             b1 = b0 = min(t.first(goal * kept, 0.0, b0), b0 - 1);
             before = b0 ? s.run[b0 - 1] : 0.0;
@@ -802,20 +789,19 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
     if (tid == 0) { a.tokens[row] = token; if (a.status) a.status[row] = 0; }
 }
 
-constexpr int SR_SUM_WGS = 512;
+constexpr int SR_SUM_LEAST = 256;
 static size_t sr_layout(int rows, int V, void* base, SrWork& wk) {
     wk.groups = (V + SR_GROUP - 1) / SR_GROUP;
-    auto cut = [&](int wgs, int& spans, int& per) {   // about wgs workgroups in all, of 64 groups each at least
-        const int most = (wk.groups + 63) / 64, want = (wgs + rows - 1) / rows;
+    auto cut = [&](int wgs, int least, int& spans, int& per) {   // about wgs workgroups in all, of `least` groups each or more
+        const int most = (wk.groups + least - 1) / least, want = (wgs + rows - 1) / rows;
         per = (wk.groups + (want < most ? want : most) - 1) / (want < most ? want : most);
         spans = (wk.groups + per - 1) / per;
     };
-    cut(1024, wk.spans, wk.per);
-    cut(SR_SUM_WGS, wk.sum_spans, wk.sum_per);
+    cut(1024, 64, wk.spans, wk.per);
+    cut(2048, SR_SUM_LEAST, wk.sum_spans, wk.sum_per);   // each adds all of its bins to the row's in the end
     uint8_t* p = static_cast<uint8_t*>(base);
     size_t at = 0;
     auto take = [&](size_t bytes) { uint8_t* q = p ? p + at : nullptr; at += (bytes + 255) / 256 * 256; return q; };
-    wk.count = reinterpret_cast<unsigned*>(take((size_t)rows * 4));
     wk.gmax = reinterpret_cast<float*>(take((size_t)rows * wk.groups * 4));
     wk.bin = reinterpret_cast<uint16_t*>(take((size_t)rows * wk.groups * SR_GROUP * 2));
     wk.mass = reinterpret_cast<uint64_t*>(take((size_t)rows * SR_BINS * 8));
@@ -831,10 +817,11 @@ hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s) {
     SrWork wk;
     sr_layout(a.rows, a.V, a.work, wk);
     const dim3 grid(wk.spans, a.rows);
-    const bool vec = a.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
-    if (vec) hipLaunchKernelGGL(sample_groups_kernel<true>, grid, dim3(256), 0, s, a, wk);
+    if (sr_vec(a)) hipLaunchKernelGGL(sample_groups_kernel<true>, grid, dim3(256), 0, s, a, wk);
     else hipLaunchKernelGGL(sample_groups_kernel<false>, grid, dim3(256), 0, s, a, wk);
-    hipLaunchKernelGGL(sample_pick_kernel, dim3(wk.sum_spans, a.rows), dim3(SR_T), 0, s, a, wk);
+    // a row needs sums over all of it only without a top-k; who gives none may still have them off, row by row
+    hipLaunchKernelGGL(sample_sums_kernel, dim3(wk.sum_spans, a.rows), dim3(SR_SUM_T), 0, s, a, wk);
+    hipLaunchKernelGGL(sample_pick_kernel, dim3(a.rows), dim3(SR_T), 0, s, a, wk);
     return hipGetLastError();
 }
 
