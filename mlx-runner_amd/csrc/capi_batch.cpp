@@ -29,6 +29,12 @@ int check_heads(const mlxr_paged_kv* kv, int nH) {
     if (nH < 1 || nH > 4096 || nH % kv->nKV) return bad("query heads: a multiple of the KV heads, at most 4096");
     return MLXR_OK;
 }
+// Attention counts the pages of every sequence, KV head and group of 16 query heads in 32 bits.
+int check_pages(const mlxr_paged_kv* kv, int nH) {
+    const double groups = (nH / kv->nKV + 15) / 16, pages = (kv->max_len + MLXR_PAGE - 1) / MLXR_PAGE + 4;
+    if (groups * pages * kv->B * kv->nKV >= 2147483648.0) return set_error(MLXR_E_UNSUPPORTED, "paged_attention: the batch could hold 2^31 pages");
+    return MLXR_OK;
+}
 int check_work(const void* work, size_t have, int64_t need) {
     if (!work || !aligned(work, 256)) return bad("work: null or not 256-byte aligned");
     if (have < (size_t)need) return set_error(MLXR_E_INVALID_ARG, "work: " + std::to_string(have) + " bytes, " + std::to_string(need) + " needed");
@@ -86,7 +92,7 @@ int mlxr_k_paged_append(const mlxr_paged_kv* kv, const float* qkv, int row_strid
 }
 
 int64_t mlxr_k_paged_attention_work(const mlxr_paged_kv* kv, int nH) {
-    return guarded([&]() -> int { if (int rc = check_kv(kv)) return rc; return check_heads(kv, nH); }) == MLXR_OK ? (int64_t)paged_attention_work(*kv, nH)
+    return guarded([&]() -> int { if (int rc = check_kv(kv)) return rc; if (int rc = check_heads(kv, nH)) return rc; return check_pages(kv, nH); }) == MLXR_OK ? (int64_t)paged_attention_work(*kv, nH)
                                                                                                                 : MLXR_E_INVALID_ARG;
 }
 int mlxr_k_paged_attention(const mlxr_paged_kv* kv, const float* q, int q_stride, int nH, int window, float scale, float* out, int out_stride,
@@ -94,6 +100,7 @@ int mlxr_k_paged_attention(const mlxr_paged_kv* kv, const float* q, int q_stride
     return guarded([&]() -> int {
         if (int rc = check_kv(kv)) return rc;
         if (int rc = check_heads(kv, nH)) return rc;
+        if (int rc = check_pages(kv, nH)) return rc;
         if (!q || !out) return bad("paged_attention: null pointer");
         if (q_stride < (int64_t)nH * kv->D || out_stride < (int64_t)nH * kv->D || q_stride % 4 || out_stride % 4 || !aligned(q, 16) || !aligned(out, 16))
             return bad("paged_attention: q and out 16-byte aligned, strides multiples of 4 and at least nH * D");

@@ -72,9 +72,9 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
 // multiply-adds a byte, far below what the matrix cores have).
 //
 // Split. A (sequence, KV head, group of 16 query heads) is a segment of ceil(slots / 64) pages. All segments' pages,
-// laid end to end, are cut into equal runs, one per workgroup, so ragged batches keep the card as evenly busy as
-// one long sequence, and lengths may stay on the device: each workgroup finds its run by a scan over the batch's
-// page counts. A segment inside one run is written out at once; one cut by runs leaves partial results (maximum,
+// laid end to end with PA_GAP places behind each segment (what beginning and ending one costs, in pages), are cut into
+// equal runs, one per workgroup, so ragged batches keep the card as evenly busy as one long sequence, and lengths may
+// stay on the device: each workgroup finds its run by a scan over the batch's page counts. A segment inside one run is written out at once; one cut by runs leaves partial results (maximum,
 // sum, unnormalised values), which the last workgroup to finish joins in run order: the same bits every time.
 //
 // Inside. A wave takes 32 keys at a time, straight from memory into the operands of 16x16x32 MFMAs, without LDS:
@@ -87,8 +87,10 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
 // q and p are fp32 split into parts that the matrix cores multiply exactly: three bf16 by truncation (24 bits), or
 // two f16 (22 bits, q scaled to at most 2^14 by a power of two, p by 2^14). Scores are in powers of two (log2 e is
 // in q's scale).
-constexpr int PA_MAXW = 512;       // workgroups: two a CU
-constexpr int PA_MINPER = 2;       // pages of a run at least: one for each wave pair
+constexpr int PA_WV = 8, PA_T = 64 * PA_WV;   // waves and threads of a workgroup
+constexpr int PA_MAXW = 256;       // workgroups: one a CU
+constexpr int PA_GAP = 4;
+constexpr int PA_MINPER = 4;       // places of a run at least
 constexpr int PA_ROWS = 16;
 typedef float pa_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 pa_b8 __attribute__((ext_vector_type(8)));
@@ -139,14 +141,16 @@ __host__ __device__ __forceinline__ constexpr size_t pa_part_floats(int D) { ret
 
 // A sequence's part of the work: keys [first, L), pages p0 .. p0 + n - 1.
 struct PaSeq { int L, first, p0, n; };
-__device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs& a, int b) {
+__device__ __forceinline__ PaSeq pa_seq_of(const PagedAttnArgs& a, int L) {
     PaSeq s;
-    s.L = paged_len(a.kv, b);
+    s.L = L;
     s.first = a.window > 0 && s.L > a.window ? s.L - a.window : 0;
     s.p0 = s.first / MLXR_PAGE;
     s.n = s.L > 0 ? (s.L - 1) / MLXR_PAGE - s.p0 + 1 : 0;
     return s;
 }
+__device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs& a, int b) { return pa_seq_of(a, paged_len(a.kv, b)); }
+__device__ __forceinline__ int pa_places(int pages) { return pages ? pages + PA_GAP : 0; }
 __device__ __forceinline__ float pa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float pa_safe(float m) { return m == -INFINITY ? 0.0f : m; }   // -inf - -inf would be NaN
 __device__ __forceinline__ void pa_store2(float* p, float a, float b) {
@@ -159,89 +163,98 @@ __device__ __forceinline__ float2 pa_load2(const float* p) {
 }
 
 template <int ST, int D, bool WT>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaWork wk) {
+__global__ __launch_bounds__(PA_T, 2) void paged_attn_kernel(PagedAttnArgs a, PaWork wk) {
     constexpr int KS = D / 32, NP = pa_parts(ST), DV = D / 16, OS = D + 4;   // k steps; dims of a lane's value rows; LDS row
-    constexpr int LDS_O = 4 * PA_ROWS * OS, LDS_C = PA_MAXW * PA_ROWS;
+    constexpr int LDS_O = PA_WV * PA_ROWS * OS, LDS_C = 2 * PA_MAXW * PA_ROWS + 5 * PA_T;
     __shared__ float lds[LDS_O > LDS_C ? LDS_O : LDS_C];
-    __shared__ float sm[4][PA_ROWS], sl[4][PA_ROWS];
-    __shared__ int64_t wsum[4], found_pre;
-    __shared__ int found_b, last;
+    __shared__ float sm[PA_WV][PA_ROWS], sl[PA_WV][PA_ROWS];
+    __shared__ uint32_t wsum[2][PA_WV], found_pre;
+    __shared__ int found_b, found_len, last;
     const PagedKV& kv = a.kv;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
-    const int w = blockIdx.x, G = a.nH / kv.nKV, per_seq = kv.nKV * wk.groups;
+    const uint32_t w = blockIdx.x;
+    const int G = a.nH / kv.nKV;
+    const uint32_t per_seq = (uint32_t)(kv.nKV * wk.groups);   // segments of a sequence
     const uint16_t *K = static_cast<const uint16_t*>(kv.k), *V = static_cast<const uint16_t*>(kv.v);
 
-    // idle rows
-    for (int b = w; b < kv.B; b += wk.W)
-        if (paged_len(kv, b) == 0)
-            for (int i = tid; i < a.nH * D; i += 256) a.out[(int64_t)b * a.out_stride + i] = 0.0f;
-
-    // this workgroup's run of pages
-    auto scan = [&](int n, int64_t& sum) {   // exclusive over the workgroup
-        int v = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(v, o, 64); if (lane >= o) v += u; }
-        __syncthreads();
-        if (lane == 63) wsum[wave] = v;
-        __syncthreads();
-        int64_t before = v - n;
-        for (int i = 0; i < 4; i++) if (i < wave) before += wsum[i];
-        sum = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-        return before;
-    };
-    int64_t T = 0, chunk = 0, before = 0;
-    int n = 0;
-    for (int c = 0; c < kv.B; c += 256) {
-        n = c + tid < kv.B ? pa_seq(a, c + tid).n : 0;
-        before = scan(n, chunk);
-        T += chunk;
-    }
-    int64_t per = (T * per_seq + wk.W - 1) / wk.W;
-    if (per < PA_MINPER) per = PA_MINPER;
-    int64_t t = w * per;
-    const int64_t t1 = min(T * per_seq, t + per);
-    if (t >= t1) return;
-    {
-        int64_t run = 0;
-        for (int c = 0; c < kv.B; c += 256) {
-            if (kv.B > 256) {
-                n = c + tid < kv.B ? pa_seq(a, c + tid).n : 0;
-                before = scan(n, chunk);
+    // This workgroup's run of pages: the sequences' page counts, PA_T at a time, summed for the total and again for the
+    // sequence in which the run begins (the host has checked that all pages of all segments number less than 2^31).
+    uint32_t T = 0, before = 0, chunk = 0;
+    int n = 0, len = 0;
+    auto scan = [&](int c, bool zero) {
+        len = c + tid < kv.B ? paged_len(kv, c + tid) : -1;
+        n = len < 0 ? -1 : pa_places(pa_seq_of(a, len).n);
+        if (zero) {   // idle rows: zeros, from one workgroup each
+            for (uint64_t idle = __ballot(n == 0 && (uint32_t)(c + tid) % (uint32_t)wk.W == w); idle; idle &= idle - 1) {
+                float* o = a.out + (int64_t)(c + 64 * wave + (int)__builtin_ctzll(idle)) * a.out_stride;
+                for (int i = 4 * lane; i < a.nH * D; i += 256) *reinterpret_cast<float4*>(o + i) = float4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            const int64_t pre = run + before;
-            if (pre * per_seq <= t && t < (pre + n) * per_seq) { found_b = c + tid; found_pre = pre; }
+        }
+        n = n < 0 ? 0 : n;
+        const uint32_t v = (uint32_t)wave_scan(n);
+        uint32_t* sums = wsum[(c / PA_T) & 1];
+        if (lane == 63) sums[wave] = v;
+        __syncthreads();
+        before = v - n;
+        chunk = 0;
+#pragma unroll
+        for (int i = 0; i < PA_WV; i++) { before += i < wave ? sums[i] : 0; chunk += sums[i]; }
+    };
+    for (int c = 0; c < kv.B; c += PA_T) { scan(c, true); T += chunk; }
+    const uint32_t all = T * per_seq;
+    const uint32_t per = max((uint32_t)PA_MINPER, (all + wk.W - 1) / (uint32_t)wk.W);
+    uint32_t t = w * per;
+    if (t >= all) return;
+    const uint32_t t1 = min(all, t + per);
+    {
+        uint32_t run = 0;
+        for (int c = 0; c < kv.B; c += PA_T) {
+            if (kv.B > PA_T) { __syncthreads(); scan(c, false); }
+            const uint32_t pre = run + before;
+            if (pre * per_seq <= t && t < (pre + n) * per_seq) { found_b = c + tid; found_pre = pre; found_len = len; }
             run += chunk;
             if (run * per_seq > t) break;
         }
     }
     __syncthreads();
-    int b = found_b;
-    int64_t pre = found_pre;
-    PaSeq sq = pa_seq(a, b);
+    int b = __builtin_amdgcn_readfirstlane(found_b);
+    uint32_t pre = __builtin_amdgcn_readfirstlane(found_pre);
+    PaSeq sq = pa_seq_of(a, __builtin_amdgcn_readfirstlane(found_len));
     int slot = 0;   // partial results of this workgroup: its first segment's, then its last one's
     while (true) {
-        const int64_t local = t - pre * per_seq;
-        const int seg = (int)(local / sq.n), tile = (int)(local % sq.n), tiles = (int)min((int64_t)(sq.n - tile), t1 - t);
-        const int kvh = seg / wk.groups, h0 = (seg % wk.groups) * PA_ROWS, rows = min(PA_ROWS, G - h0);
-        // q's parts
+        const uint32_t places = (uint32_t)pa_places(sq.n), local = t - pre * per_seq, seg = local / places;
+        const int tile = (int)(local - seg * places), tiles = min(sq.n - tile, (int)(t1 - t));
+        // on to the run's next segment: places left of this one, then the sequences behind it
+        auto ahead = [&] {
+            t += places - (uint32_t)tile;
+            if (t >= t1) return false;
+            while (t >= (pre + (uint32_t)pa_places(sq.n)) * per_seq) { pre += (uint32_t)pa_places(sq.n); sq = pa_seq(a, ++b); }   // t < t1: another one has pages
+            return true;
+        };
+        if (tiles <= 0) {   // the run begins behind a segment's pages
+            if (!ahead()) return;
+            slot = 1;            // a segment's first part is in the second place unless the run begins with it
+            continue;
+        }
+        const int kvh = (int)(seg / (uint32_t)wk.groups), h0 = (int)(seg - kvh * wk.groups) * PA_ROWS, rows = min(PA_ROWS, G - h0);
+        // page numbers, one a lane, and q's parts
+        int have = 0, ids = paged_page(kv, b, sq.p0 + tile + min(lane, tiles - 1));
         uint4 q[KS][NP];
-        float unscale = 1.0f;
-        {
-            float x[KS][8];
-            const float* qr = a.q + (int64_t)b * a.q_stride + (int64_t)(kvh * G + h0 + min(r, rows - 1)) * D;
-            const float f = r < rows ? a.scale * 1.4426950408889634f : 0.0f;
+        float x[KS][8], unscale = 1.0f;
+        const float* qr = a.q + (int64_t)b * a.q_stride + (int64_t)(kvh * G + h0 + min(r, rows - 1)) * D;
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const float4 u = *reinterpret_cast<const float4*>(qr + 32 * s + 8 * g), v = *reinterpret_cast<const float4*>(qr + 32 * s + 8 * g + 4);
-                x[s][0] = u.x * f; x[s][1] = u.y * f; x[s][2] = u.z * f; x[s][3] = u.w * f;
-                x[s][4] = v.x * f; x[s][5] = v.y * f; x[s][6] = v.z * f; x[s][7] = v.w * f;
-            }
+        for (int s = 0; s < KS; s++) {
+            const float4 u = gload4(qr + 32 * s + 8 * g), v = gload4(qr + 32 * s + 8 * g + 4);
+            x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w; x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
+        }
+        {
+            float f = r < rows ? a.scale * 1.4426950408889634f : 0.0f;
             if constexpr (ST == 1) {
                 float mx = 0.0f;
 #pragma unroll
                 for (int s = 0; s < KS; s++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[s][e]));
+                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[s][e] * f));
                 mx = xor32_max(xor16_max(mx));
                 int e2 = 0;
                 if (mx > 0.0f && mx < INFINITY) { frexpf(mx, &e2); e2 = 14 - e2; e2 = e2 < -126 ? -126 : (e2 > 126 ? 126 : e2); }
@@ -250,7 +263,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaW
 #pragma unroll
                 for (int s = 0; s < KS; s++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[s][e] *= up;
+                    for (int e = 0; e < 8; e++) x[s][e] = x[s][e] * f * up;
+            } else {
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[s][e] *= f;
             }
 #pragma unroll
             for (int s = 0; s < KS; s++) pa_split<ST>(x[s], q[s]);
@@ -259,32 +277,40 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaW
         pa_f4 o[DV];
 #pragma unroll
         for (int j = 0; j < DV; j++) o[j] = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        int have = -1, ids = 0;   // page numbers of 64 tiles, one a lane
-        for (int u = wave; u < 2 * tiles; u += 4) {
-            const int tt = u >> 1;
-            if ((tt >> 6) != have) {
-                have = tt >> 6;
-                const int i = min(64 * have + lane, tiles - 1);
-                ids = paged_page(kv, b, sq.p0 + tile + i);
-            }
-            const int page = __builtin_amdgcn_readlane(ids, tt & 63);
-            const int key0 = (sq.p0 + tile) * MLXR_PAGE + u * 32;
-            if (key0 + 32 <= sq.first || key0 >= sq.L) continue;
-            if (page < 0) {
+        float* score = WT ? wk.score + ((int64_t)b * a.nH + kvh * G + h0 + min(r, rows - 1)) * wk.score_stride : nullptr;
+        // the wave's next 32 keys from half page u on (every PA_WV-th is its own): where they are, whether there are any
+        int u = wave, key0 = 0;
+        int64_t base = 0;
+        auto seek = [&] {
+            for (; u < 2 * tiles; u += PA_WV) {
+                const int tt = u >> 1;
+                if ((tt >> 6) != have) {
+                    have = tt >> 6;
+                    ids = paged_page(kv, b, sq.p0 + tile + min(64 * have + lane, tiles - 1));
+                }
+                const int page = __builtin_amdgcn_readlane(ids, tt & 63);
+                key0 = (sq.p0 + tile) * MLXR_PAGE + u * 32;
+                if (key0 + 32 <= sq.first || key0 >= sq.L) continue;
+                if (page >= 0) {
+                    base = paged_row(kv, page, kvh, key0 & (MLXR_PAGE - 1));
+                    return true;
+                }
                 if constexpr (WT)
                     if (r < rows)
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            wk.score[((int64_t)b * a.nH + kvh * G + h0 + r) * wk.score_stride + key0 + (e >> 2) * 16 + 4 * g + (e & 3)] = -INFINITY;
-                continue;
+                        for (int e = 0; e < 8; e++) score[key0 + (e >> 2) * 16 + 4 * g + (e & 3)] = -INFINITY;
             }
-            const int64_t base = paged_row(kv, page, kvh, key0 & (MLXR_PAGE - 1));
-            uint4 kr[2][KS];
+            return false;
+        };
+        uint4 kr[2][KS];
+        uint32_t vr[8][DV / 2];
+        auto load_k = [&] {
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int s = 0; s < KS; s++) kr[i][s] = __builtin_bit_cast(uint4, gload(reinterpret_cast<const pa_u4*>(K + base + (16 * i + r) * D + 32 * s + 8 * g)));
-            uint32_t vr[8][DV / 2];
+        };
+        auto load_v = [&] {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const uint16_t* row = V + base + ((e >> 2) * 16 + 4 * g + (e & 3)) * D + DV * r;
@@ -296,6 +322,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaW
                     vr[e][0] = x.x; vr[e][1] = x.y;
                 }
             }
+        };
+        for (; seek(); u += PA_WV) {
+            load_k();
+            load_v();
+            const int key = key0;
             pa_f4 sc[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -308,11 +339,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaW
             float sv[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) sv[e] = ST == 0 ? sc[e >> 2][e & 3] : sc[e >> 2][e & 3] * unscale;
-            if (key0 < sq.first || key0 + 32 > sq.L) {   // keys outside take no part, whatever their rows hold
+            if (key < sq.first || key + 32 > sq.L) {   // keys outside take no part, whatever their rows hold
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const int key = key0 + (e >> 2) * 16 + 4 * g + (e & 3);
-                    if (key < sq.first || key >= sq.L) {
+                    const int k = key + (e >> 2) * 16 + 4 * g + (e & 3);
+                    if (k < sq.first || k >= sq.L) {
                         sv[e] = -INFINITY;
 #pragma unroll
                         for (int d = 0; d < DV / 2; d++) vr[e][d] = 0;
@@ -321,7 +352,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaW
             }
             if constexpr (WT)
                 if (r < rows) {
-                    float* s = wk.score + ((int64_t)b * a.nH + kvh * G + h0 + r) * wk.score_stride + key0 + 4 * g;
+                    float* s = score + key + 4 * g;
                     *reinterpret_cast<float4*>(s) = float4{sv[0], sv[1], sv[2], sv[3]};
                     *reinterpret_cast<float4*>(s + 16) = float4{sv[4], sv[5], sv[6], sv[7]};
                 }
@@ -353,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaW
                 for (int i = 0; i < NP; i++) o[j] = pa_mfma<ST>(vt, pp[i], o[j]);
             }
         }
-        // the four waves' results: lane (r, g) has row r's dims DV (4 g + i) + j
+        // the waves' results: lane (r, g) has row r's dims DV (4 g + i) + j
         l = xor32_sum(xor16_sum(l));
         if (g == 0) { sm[wave][r] = m; sl[wave][r] = l; }
         {
@@ -367,80 +398,111 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttnArgs a, PaW
         }
         __syncthreads();
         const bool whole = tiles == sq.n;
+        auto most = [&](int row) {   // of the waves' maxima
+            float M = sm[0][row];
+#pragma unroll
+            for (int v = 1; v < PA_WV; v++) M = fmaxf(M, sm[v][row]);
+            return M;
+        };
         float* part = wk.part + (size_t)(2 * w + slot) * pa_part_floats(D);
-        for (int i = tid; i < rows * D / 2; i += 256) {
+        float* out = a.out + (int64_t)b * a.out_stride + (int64_t)(kvh * G + h0) * D;
+        float* stat = WT ? wk.stat + 2 * ((int64_t)b * a.nH + kvh * G + h0) : nullptr;
+        auto finish = [&](int row, int d, float M, float sum, float x, float y) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            *reinterpret_cast<float2*>(out + row * D + d) = sum == 0.0f ? float2{0.0f, 0.0f} : float2{x * inv, y * inv};
+            if (WT && d == 0) *reinterpret_cast<float2*>(stat + 2 * row) = float2{M, inv};
+        };
+        for (int i = tid; i < rows * D / 2; i += PA_T) {
             const int row = i / (D / 2), d = 2 * (i % (D / 2));
-            const float M = fmaxf(fmaxf(sm[0][row], sm[1][row]), fmaxf(sm[2][row], sm[3][row])), Ms = pa_safe(M);
+            const float M = most(row), Ms = pa_safe(M);
             float sum = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
-            for (int v = 0; v < 4; v++) {
+            for (int v = 0; v < PA_WV; v++) {
                 const float c = pa_exp2(sm[v][row] - Ms);
                 const float2 e = *reinterpret_cast<const float2*>(lds + (v * PA_ROWS + row) * OS + d);
                 sum += c * sl[v][row]; x += c * e.x; y += c * e.y;
             }
-            if (whole) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                *reinterpret_cast<float2*>(a.out + (int64_t)b * a.out_stride + (int64_t)(kvh * G + h0 + row) * D + d) = sum == 0.0f ? float2{0.0f, 0.0f} : float2{x * inv, y * inv};
-                if (WT && d == 0) *reinterpret_cast<float2*>(wk.stat + 2 * ((int64_t)b * a.nH + kvh * G + h0 + row)) = float2{Ms, inv};
-            } else {
+            if (whole) finish(row, d, Ms, sum, x, y);
+            else {
                 pa_store2(part + 2 * PA_ROWS + row * D + d, x, y);
                 if (d == 0) pa_store2(part + 2 * row, M, sum);
             }
         }
         if (!whole) {
             // the runs that hold the segment, from the first page's to the last one's
-            const int64_t s0 = pre * per_seq + (int64_t)seg * sq.n;
-            const int w0 = (int)(s0 / per), parts = (int)((s0 + sq.n - 1) / per) - w0 + 1;
-            const int first_slot = s0 % per == 0 ? 0 : 1;
+            const uint32_t s0 = pre * per_seq + seg * places, w0 = s0 / per;
+            const int parts = (int)((s0 + sq.n - 1) / per - w0) + 1, first_slot = s0 == w0 * per ? 0 : 1;
             parts_stored();
             if (tid == 0) last = part_last(wk.count + w0, parts);
             __syncthreads();
             if (last) {
                 auto of = [&](int i) { return wk.part + (size_t)(2 * (w0 + i) + (i == 0 ? first_slot : 0)) * pa_part_floats(D); };
-                // the parts' maxima into LDS, the rows' maximum, then the parts' factors in their place
-                for (int i = tid; i < parts * PA_ROWS; i += 256) {
-                    const int row = i % PA_ROWS;
-                    const float2 x = row < rows ? pa_load2(of(i / PA_ROWS) + 2 * row) : float2{-INFINITY, 0.0f};
-                    lds[i] = x.x;
-                }
-                __syncthreads();
-                if (wave == 0) {   // lane (r, g): every fourth part
-                    float M = -INFINITY;
-                    for (int i = g; i < parts; i += 4) M = fmaxf(M, lds[i * PA_ROWS + r]);
-                    M = xor32_max(xor16_max(M));
-                    if (g == 0) sm[0][r] = pa_safe(M);
-                }
-                __syncthreads();
-                for (int i = tid; i < parts * PA_ROWS; i += 256) lds[i] = pa_exp2(lds[i] - sm[0][i % PA_ROWS]);
-                __syncthreads();
-                for (int i = tid; i < rows * D / 2; i += 256) {
-                    const int row = i / (D / 2), d = 2 * (i % (D / 2));
-                    float sum = 0.0f, x = 0.0f, y = 0.0f;
-                    constexpr int CB = 8;
-                    int k = 0;
-                    for (; k + CB <= parts; k += CB) {
-                        float2 e[CB], s[CB];
+                // a thread has four dims of a row and every ways-th part: all threads have some, most parts are in flight at once
+                const int items = rows * D / 4, ways = items >= PA_T ? 1 : PA_T / items;
+                constexpr int CB = 8;
+                float2* ml = reinterpret_cast<float2*>(lds);
+                for (int e0 = 0; e0 < items; e0 += PA_T) {
+                    const int at = e0 + tid, way = ways == 1 ? 0 : min(at / items, ways), item = ways == 1 ? min(at, items - 1) : at % items;
+                    const int row = item / (D / 4), d = 4 * (item % (D / 4));
+                    float2 e[CB][2];
+                    auto load = [&](int k) {
 #pragma unroll
-                        for (int c = 0; c < CB; c++) { e[c] = pa_load2(of(k + c) + 2 * PA_ROWS + row * D + d); s[c] = pa_load2(of(k + c) + 2 * row); }
+                        for (int c = 0; c < CB; c++) {
+                            const float* p = of(min(k + ways * c, parts - 1)) + 2 * PA_ROWS + row * D + d;
+                            e[c][0] = pa_load2(p); e[c][1] = pa_load2(p + 2);
+                        }
+                    };
+                    load(way);
+                    if (e0 == 0) {   // all parts' maxima and sums, and the rows' maximum
+                        for (int k = tid; k < parts * PA_ROWS; k += 4 * PA_T) {
+                            float2 v[4];
 #pragma unroll
-                        for (int c = 0; c < CB; c++) { const float f = lds[(k + c) * PA_ROWS + row]; sum += f * s[c].y; x += f * e[c].x; y += f * e[c].y; }
+                            for (int c = 0; c < 4; c++) {
+                                const int q = min(k + PA_T * c, parts * PA_ROWS - 1);
+                                v[c] = pa_load2(of(q / PA_ROWS) + 2 * min(q % PA_ROWS, rows - 1));
+                            }
+#pragma unroll
+                            for (int c = 0; c < 4; c++) if (k + PA_T * c < parts * PA_ROWS) ml[k + PA_T * c] = v[c];
+                        }
+                        __syncthreads();
+                        float M = -INFINITY;
+                        for (int k = 4 * wave + g; k < parts; k += 4 * PA_WV) M = fmaxf(M, ml[k * PA_ROWS + r].x);
+                        M = xor32_max(xor16_max(M));
+                        if (g == 0) sm[wave][r] = M;
+                        __syncthreads();
                     }
-                    for (; k < parts; k++) {
-                        const float2 e = pa_load2(of(k) + 2 * PA_ROWS + row * D + d), s = pa_load2(of(k) + 2 * row);
-                        const float f = lds[k * PA_ROWS + row];
-                        sum += f * s.y; x += f * e.x; y += f * e.y;
+                    const float M = pa_safe(most(row));
+                    float sum = 0.0f;
+                    float4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int k = way; k < parts && way < ways; k += ways * CB) {
+#pragma unroll
+                        for (int c = 0; c < CB; c++) {
+                            const float2 s = ml[min(k + ways * c, parts - 1) * PA_ROWS + row];
+                            const float f = k + ways * c < parts ? pa_exp2(s.x - M) : 0.0f;
+                            if (f != 0.0f) { sum += f * s.y; x.x += f * e[c][0].x; x.y += f * e[c][0].y; x.z += f * e[c][1].x; x.w += f * e[c][1].y; }
+                        }
+                        if (k + ways * CB < parts) load(k + ways * CB);
                     }
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    *reinterpret_cast<float2*>(a.out + (int64_t)b * a.out_stride + (int64_t)(kvh * G + h0 + row) * D + d) = sum == 0.0f ? float2{0.0f, 0.0f} : float2{x * inv, y * inv};
-                    if (WT && d == 0) *reinterpret_cast<float2*>(wk.stat + 2 * ((int64_t)b * a.nH + kvh * G + h0 + row)) = float2{sm[0][row], inv};
+                    if (ways > 1) {   // the ways' sums, in their order
+                        float* all_sums = lds + 2 * PA_ROWS * parts;
+                        float* mine = all_sums + 5 * tid;
+                        mine[0] = sum; mine[1] = x.x; mine[2] = x.y; mine[3] = x.z; mine[4] = x.w;
+                        __syncthreads();
+                        for (int v = 1; v < ways && way == 0; v++) {
+                            const float* p = all_sums + 5 * (tid + v * items);
+                            sum += p[0]; x.x += p[1]; x.y += p[2]; x.z += p[3]; x.w += p[4];
+                        }
+                    }
+                    if (way == 0 && at < items) {
+                        finish(row, d, M, sum, x.x, x.y);
+                        finish(row, d + 2, M, sum, x.z, x.w);
+                    }
                 }
                 if (tid == 0) part_rearm(wk.count + w0);
             }
         }
         slot = 1;
-        t += tiles;
-        if (t >= t1) return;
-        while (t >= (pre + sq.n) * per_seq) { pre += sq.n; sq = pa_seq(a, ++b); }   // t < t1: another sequence has pages
+        if (!ahead()) return;
         __syncthreads();   // the LDS is written again
     }
 }
@@ -465,7 +527,7 @@ __global__ __launch_bounds__(256) void paged_weight_kernel(PagedAttnArgs a, PaWo
 static size_t pa_layout(const PagedKV& kv, int nH, void* base, PaWork& wk) {
     const int G = nH / kv.nKV;
     wk.groups = (G + PA_ROWS - 1) / PA_ROWS;
-    const int64_t most = (int64_t)kv.B * kv.nKV * wk.groups * ((kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE), runs = (most + PA_MINPER - 1) / PA_MINPER;
+    const int64_t places = (kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE + 1 + PA_GAP, runs = ((int64_t)kv.B * kv.nKV * wk.groups * places + PA_MINPER - 1) / PA_MINPER;
     wk.W = (int)(runs < PA_MAXW ? runs : PA_MAXW);
     wk.score_stride = (kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE * MLXR_PAGE;
     uint8_t* p = static_cast<uint8_t*>(base);
@@ -489,7 +551,7 @@ size_t paged_attention_work(const PagedKV& kv, int nH) {
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t s) {
     PaWork wk;
     pa_layout(a.kv, a.nH, a.work, wk);
-#define PA_GO(ST, D, WT) hipLaunchKernelGGL((paged_attn_kernel<ST, D, WT>), dim3(wk.W), dim3(256), 0, s, a, wk)
+#define PA_GO(ST, D, WT) hipLaunchKernelGGL((paged_attn_kernel<ST, D, WT>), dim3(wk.W), dim3(PA_T), 0, s, a, wk)
 #define PA_D(ST, WT) do { if (a.kv.D == 64) PA_GO(ST, 64, WT); else PA_GO(ST, 128, WT); } while (0)
     if (a.kv.weight) { if (a.kv.st == 0) PA_D(0, true); else PA_D(1, true); }
     else { if (a.kv.st == 0) PA_D(0, false); else PA_D(1, false); }
