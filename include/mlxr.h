@@ -339,7 +339,8 @@ int mlxr_k_paged_append(const mlxr_paged_kv* kv, const float* qkv, int row_strid
  * scores is above -infinity, gives zeros. With kv->weight:
  * weight[b][g][j] = decay * weight_in[b][g][j] + the sum of p_j over the query heads of KV head g, for every j < len[b]
  * (slots outside the window only decay; weight_in, with the strides of weight, may be weight itself; NULL: zeros).
- * Pages may be shared by sequences. q, out: 16-byte aligned, strides multiples of 4. */
+ * Pages may be shared by sequences. q, out: 16-byte aligned, strides multiples of 4; out may be q itself at its
+ * stride. The same call gives the same bits; another batch around a sequence may cut its sums elsewhere. */
 int mlxr_k_paged_attention(const mlxr_paged_kv* kv, const float* q, int q_stride, int nH, int window, float scale,
                            float* out, int out_stride, const float* weight_in, float decay, void* work, size_t work_bytes,
                            void* stream);

@@ -80,6 +80,7 @@ int mlxr_k_paged_append(const mlxr_paged_kv* kv, const float* qkv, int row_strid
         if (int rc = check_heads(kv, nH)) return rc;
         const int D = kv->D;
         if (!qkv || !q_out || (rot_dim && !inv_freq) || (qn == nullptr) != (kn == nullptr)) return bad("paged_append: null pointer (qn and kn go together)");
+        if ((int64_t)(nH + 2 * kv->nKV) * kv->B >= (1 << 26)) return set_error(MLXR_E_UNSUPPORTED, "paged_append: 2^26 heads or more in one call");
         if (rot_dim < 0 || rot_dim > D || rot_dim % 2) return bad("paged_append: rot_dim even, 0 .. D");
         if (row_stride < (int64_t)(nH + 2 * kv->nKV) * D || q_stride < (int64_t)nH * D) return bad("paged_append: strides");
         if (q_out == qkv && q_stride != row_stride) return bad("paged_append: q_out over qkv needs its stride");
@@ -104,6 +105,7 @@ int mlxr_k_paged_attention(const mlxr_paged_kv* kv, const float* q, int q_stride
         if (!q || !out) return bad("paged_attention: null pointer");
         if (q_stride < (int64_t)nH * kv->D || out_stride < (int64_t)nH * kv->D || q_stride % 4 || out_stride % 4 || !aligned(q, 16) || !aligned(out, 16))
             return bad("paged_attention: q and out 16-byte aligned, strides multiples of 4 and at least nH * D");
+        if (out == q && out_stride != q_stride) return bad("paged_attention: out over q needs its stride");
         if (window < 0) return bad("paged_attention: window");
         if (!(scale == scale) || !(decay == decay)) return bad("paged_attention: scale or decay is NaN");
         if (weight_in && !kv->weight) return bad("paged_attention: weight_in without the cache's weight");

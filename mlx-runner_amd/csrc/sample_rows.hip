@@ -3,21 +3,25 @@
 //
 // Every cut and the draw itself are one question, asked of the tokens in rank order (logit descending, equal
 // ones by index): where does a running sum of weights w = exp((v - max) / T) (top-k: of ones) reach a target? The
-// answer needs the order only where the sum crosses. Two launches:
-//   1. sample_groups_kernel, several workgroups a row: the maximum of every 64 logits. One read of the logits, and
-//      that read bounds the operator: 0.6 MB a row of 152 thousand.
-//   2. sample_pick_kernel. With the row's maximum known, tokens fall into bins of 1/64 of x = (max - v) / T, 2048 of
-//      them (what lies behind x = 32 has no weight that counts). Where the sum of a whole row matters (top-p or
-//      nothing over all tokens) its workgroups first add up the bins' weights, and the last one goes on alone: it
-//      finds the bins in which the sums cross, gathers just their tokens (the groups' maxima say where none are),
-//      sorts them and walks. For top-k and min-p alone no sum over the row is needed: the groups' maxima give a
-//      bin down to which there are k tokens or more, and these are gathered and sorted at once.
+// answer needs the order only where the sum crosses. Three launches:
+//   1. sample_groups_kernel, about a thousand workgroups: the maximum of every 64 logits. The one read of the logits that
+//      every row needs: 0.6 MB a row of 152 thousand, 37 us for 256 of them (4.2 TB/s), 3 us for one.
+//   2. sample_sums_kernel, for rows that ask for a sum over all their tokens (top-p, or nothing, without top-k). With the
+//      row's maximum known, tokens fall into bins of 1/64 of x = (max - v) / T, 2048 of them: what lies behind x = 32 has
+//      no weight that counts. Each bin's weights are added up, and each token's bin is written down. Bound by the 64-bit
+//      arithmetic and the adds in LDS: 25 us for 102 rows of 152 thousand; other rows leave at once (2 us).
+//   3. sample_pick_kernel, one workgroup a row. A row with sums: the bins in which the sums cross are found, just their
+//      tokens are gathered (through the groups' maxima, or by the bin numbers where most groups qualify), ranked and
+//      walked. A row without: the groups' maxima give a bin down to which there are k tokens or more, or min-p does, and
+//      these are gathered. Bound by what waits for what in one workgroup: 9 us for a top-k of 40, about 20 us where a cut lies
+//      among the bulk of the tokens (13 us to look through 152 thousand bin numbers).
 // A bin's weights are a constant times f in (exp(-1/64), 1], added as multiples of 2^-43: no order of the atomic adds
-// changes a result, and 2^20 of them stay below 2^63. Everything else is 64-bit floating point: a draw lies next to
-// a border only if it is within about 2^-43 of it.
-// Rows whose crossing bins hold too many tokens for that (thousands of equal logits, top-k of thousands) take the
-// radix descent instead, which asks for no room: a histogram of the order keys' leading bits, the bin in which the
-// sum crosses, and again within that bin, until one key is left, whose tokens have one weight.
+// changes a result, and 2^20 of them stay below 2^63. Everything else is 64-bit floating point, so a token differs from
+// the exact sums' only if the draw is within about 2^-43 of a border.
+// Rows whose crossing bins hold too many tokens for the list (thousands of equal logits, top-k of thousands, a
+// temperature of 5 and more over a large vocabulary) take the radix descent instead, which asks for no room: a histogram
+// of the order keys' leading bits, the bin in which the sum crosses, and again within that bin, until one key is left,
+// whose tokens have one weight. Up to 15 passes of one workgroup over the row: about 350 us for 152 thousand.
 #include "batch.h"
 
 namespace mlxr {
@@ -244,7 +248,7 @@ typedef uint16_t sr_h2 __attribute__((ext_vector_type(2)));
 struct SrWork {
     float* gmax;        // [rows][groups]
     uint16_t* bin;      // [rows][groups][64]: the tokens' bins (65535: none), written where sums over the row are needed
-    uint64_t* mass;     // [rows][SR_BINS]: sums of f, cleared by the first launch where the second adds to them
+    uint64_t* mass;     // [rows][sum_spans][SR_BINS]: sums of f
     int groups;               // of a row
     int spans, per;           // the first launch's workgroups of a row, and the groups of each
     int sum_spans, sum_per;   // the second's, where it adds up bins
@@ -285,8 +289,6 @@ template <bool VEC>
 __global__ __launch_bounds__(256) void sample_groups_kernel(SampleRowsArgs a, SrWork wk) {
     const int row = blockIdx.y, span = blockIdx.x, tid = threadIdx.x;
     const float* v = a.logits + (int64_t)row * a.stride;
-    if (sr_ask(a, row).kind == SR_SUM)
-        for (int i = span * 256 + tid; i < SR_BINS; i += wk.spans * 256) wk.mass[(int64_t)row * SR_BINS + i] = 0;
     const int g1 = min(wk.groups, (span + 1) * wk.per);
     constexpr int UN = 4;   // loads in flight
     for (int g = span * wk.per + (tid >> 4); g < g1; g += 16 * UN) {
@@ -359,12 +361,13 @@ __global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a,
         }
     }
     __syncthreads();
-    unsigned long long* all = reinterpret_cast<unsigned long long*>(wk.mass + (int64_t)row * SR_BINS);
-    for (int i = tid; i < SR_BINS; i += SR_SUM_T) if (hist[i]) atomicAdd(all + i, (unsigned long long)hist[i]);
+    uint64_t* mine = wk.mass + ((int64_t)row * wk.sum_spans + blockIdx.x) * SR_BINS;
+    for (int i = tid; i < SR_BINS; i += SR_SUM_T) mine[i] = hist[i];
 }
 
 // What one workgroup keeps of its row. Code that runs once is paid for by its size (instructions come from memory
-// like data), so loops here stay rolled and exponentials are looked up.
+// like data: the same steps unrolled, in 76 KB, took 21 us for one row where these 22 KB take 14), so loops here stay
+// rolled and exponentials are looked up.
 constexpr int SR_MAXGROUPS = (1 << 20) / SR_GROUP, SR_NEAR = 4096;   // groups of the longest row; of these kept in LDS
 struct SrPick {
     uint64_t list[SR_LIST];
@@ -570,7 +573,7 @@ struct SrTeam {
 
     // Ranks the n gathered tokens.
     __device__ __forceinline__ void rank(int n) {
-        if (n <= 256) {   // each against all
+        if (n <= 256) {   // each against all (256 mixed rows: 89 us; only up to 64: 94, up to 1024: 101)
             for (int i = tid; i - lane < n; i += SR_T) {
                 const uint64_t k = i < n ? s.list[i] : 0;
                 int above = 0;
@@ -609,6 +612,8 @@ struct SrTeam {
         }
         __syncthreads();
         const int ids = s.nids;
+        // few groups: theirs (2 or 8 loads a wave for 128 or 512 of them); most groups, in the bulk: all bin numbers at once,
+        // half the bytes and a quarter of the work a token (2374 groups of 64: 13 us, 29 us by groups)
         if (ids <= 8 * SR_W || !bin) sr_collect<1>(r.v, r.V, r.vec, s.ids, ids, lo, hi, lo2, hi2, s.list, &s.n);
         else sr_collect_bins(r.v, bin, r.V, b0, also, s.list, &s.n);
         __syncthreads();
@@ -716,10 +721,14 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
                 if (ask.low > 0.0f && ask.p >= 1.0f) b1 = min(b1, (int)(-log((double)ask.low) * SR_WIDTH) + 1);
             }
         } else {
-            const uint64_t* all = wk.mass + (int64_t)row * SR_BINS;
+            const uint64_t* all = wk.mass + (int64_t)row * wk.sum_spans * SR_BINS + SR_PER * tid;
+            uint64_t mass[SR_PER] = {};
+#pragma unroll 4
+            for (int k = 0; k < wk.sum_spans; k++)
 #pragma unroll
-            for (int h = 0; h < SR_PER; h++)
-                sums[h] = t.constant(SR_PER * tid + h) * (double)all[SR_PER * tid + h];
+                for (int h = 0; h < SR_PER; h++) mass[h] += gload(all + (int64_t)k * SR_BINS + h);
+#pragma unroll
+            for (int h = 0; h < SR_PER; h++) sums[h] = t.constant(SR_PER * tid + h) * (double)mass[h];
             t.scan(sums);
 #pragma unroll
             for (int h = 0; h < SR_PER; h++) sums[h] = s.run[SR_PER * tid + h];
@@ -789,6 +798,7 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
     if (tid == 0) { a.tokens[row] = token; if (a.status) a.status[row] = 0; }
 }
 
+// Groups of a workgroup that adds up bins, at least: it also clears and stores 2048 of them (33 rows: 34 us, with 64 39 us).
 constexpr int SR_SUM_LEAST = 256;
 static size_t sr_layout(int rows, int V, void* base, SrWork& wk) {
     wk.groups = (V + SR_GROUP - 1) / SR_GROUP;
@@ -804,7 +814,7 @@ static size_t sr_layout(int rows, int V, void* base, SrWork& wk) {
     auto take = [&](size_t bytes) { uint8_t* q = p ? p + at : nullptr; at += (bytes + 255) / 256 * 256; return q; };
     wk.gmax = reinterpret_cast<float*>(take((size_t)rows * wk.groups * 4));
     wk.bin = reinterpret_cast<uint16_t*>(take((size_t)rows * wk.groups * SR_GROUP * 2));
-    wk.mass = reinterpret_cast<uint64_t*>(take((size_t)rows * SR_BINS * 8));
+    wk.mass = reinterpret_cast<uint64_t*>(take((size_t)rows * wk.sum_spans * SR_BINS * 8));
     return at;
 }
 
@@ -819,7 +829,7 @@ hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s) {
     const dim3 grid(wk.spans, a.rows);
     if (sr_vec(a)) hipLaunchKernelGGL(sample_groups_kernel<true>, grid, dim3(256), 0, s, a, wk);
     else hipLaunchKernelGGL(sample_groups_kernel<false>, grid, dim3(256), 0, s, a, wk);
-    // a row needs sums over all of it only without a top-k; who gives none may still have them off, row by row
+    // which rows need sums is on the device: the others' workgroups leave at once
     hipLaunchKernelGGL(sample_sums_kernel, dim3(wk.sum_spans, a.rows), dim3(SR_SUM_T), 0, s, a, wk);
     hipLaunchKernelGGL(sample_pick_kernel, dim3(a.rows), dim3(SR_T), 0, s, a, wk);
     return hipGetLastError();

@@ -44,7 +44,7 @@ def sample(**over):
 
 
 KV_BAD = [("k", None), ("v", None), ("table", None), ("len", None), ("D", 96), ("D", 256), ("st", 2), ("st", -1), ("B", 0), ("B", 65536), ("nKV", 0),
-          ("nKV", 2048), ("n_pages", 0), ("table_stride", 0), ("max_len", 0), ("max_len", 129), ("k", P + 8), ("v", P + 2), ("len", P + 2), ("table", P + 1)]
+          ("nKV", 2048), ("n_pages", 0), ("table_stride", 0), ("max_len", 0), ("max_len", 129), ("max_len", 1 << 25), ("k", P + 8), ("v", P + 2), ("len", P + 2), ("table", P + 1)]
 
 
 @pytest.mark.parametrize("field,value", KV_BAD)
@@ -80,7 +80,7 @@ def test_append_refuses(over):
 
 @pytest.mark.parametrize("over", [dict(q=None), dict(out=None), dict(nH=0), dict(nH=5), dict(window=-1), dict(scale=float("nan")), dict(decay=float("nan")),
                                   dict(weight_in=P), dict(q_stride=508), dict(q_stride=514), dict(out_stride=510), dict(q=P + 4), dict(out=P + 8),
-                                  dict(work=None), dict(work=P + 16), dict(work_bytes=16)])
+                                  dict(work=None), dict(work=P + 16), dict(work_bytes=16), dict(q=P, out=P, q_stride=512, out_stride=516)])
 def test_attention_refuses(over):
     assert attention(**over) == INVALID
 
@@ -117,6 +117,15 @@ def test_work_sizes():
     big = kv(B=4096, nKV=8, max_len=131072, table_stride=2048, slot_stride=131072, weight=P)
     assert lib.mlxr_k_paged_evict_work(ctypes.byref(big), 131072) >= 4096 * 8 * 131072 * 4
     assert lib.mlxr_k_paged_attention_work(ctypes.byref(big), 32) > 0
+
+
+def test_batches_too_large_to_count():
+    """More pages or heads than the kernels count in 32 bits are refused, whatever the workspace."""
+    c = kv(B=60000, nKV=8, max_len=1 << 24, table_stride=1 << 18, slot_stride=1 << 24)
+    assert attention(c, nH=8, q_stride=1024, out_stride=1024) == UNSUPPORTED
+    assert mlxr.lib.mlxr_k_paged_attention_work(ctypes.byref(c), 8) < 0
+    c = kv(B=65535, nKV=1024, table_stride=1, slot_stride=64, max_len=64)
+    assert append(c, nH=1024, row_stride=3 * 1024 * 128, q_stride=1024 * 128) == UNSUPPORTED
 
 
 @pytest.mark.skipif(mlxr.device_count() > 0, reason="what a call without a device says")

@@ -271,6 +271,89 @@ def test_attention_same_bits_again(gpu):
         assert same(attend(gpu, small, qs, 4, work=work).view(np.uint32), s.view(np.uint32))
 
 
+def test_attention_many_sequences(gpu):
+    """More sequences than a workgroup scans at once, most of them short, idle ones among them."""
+    rs = np.random.default_rng(13)
+    lens = rs.integers(0, 70, 1300)
+    lens[::9] = 0
+    lens[[5, 700, 1299]] = [700, 1, 333]
+    c = Cache(gpu, lens, 1, 64, 0, seed=14).up()
+    q = queries(c, 2)
+    out, tol, _, _ = attention_reference(c, q, 2, 0, 0.09)
+    check_out(attend(gpu, c, q, 2), c, 2, out, tol)
+
+
+def test_attention_in_place(gpu):
+    """The output over the queries, at their stride."""
+    c = Cache(gpu, [500, 0, 2000, 64], 2, 128, 0, seed=15).up()
+    q = queries(c, 8, pad=0)
+    out, tol, _, _ = attention_reference(c, q, 8, 0, 0.09)
+    kv, dq = c.desc(), gpu.DeviceArray.from_numpy(q)
+    work = workspace(gpu, gpu.lib.mlxr_k_paged_attention_work(ctypes.byref(kv), 8))
+    gpu.check(gpu.lib.mlxr_k_paged_attention(ctypes.byref(kv), dq.ptr, 1024, 8, 0, 0.09, dq.ptr, 1024, None, 1.0, work.ptr, work.nbytes, None))
+    gpu.synchronize()
+    assert within(np.abs(dq.numpy() - out), tol) <= 1
+
+
+def far_pool(gpu, c, page_bytes):
+    """The cache's pages at the far end of pools whose offsets pass 2^32 elements and more; the table goes with them."""
+    pages = (1 << 32) // (page_bytes // 2) + 64 + c.k.shape[0]
+    pools = [gpu.DeviceArray(pages * page_bytes, np.uint8) for _ in range(2)]
+    shift = pages - c.k.shape[0]
+    for pool, a in zip(pools, (c.k, c.v)):
+        gpu.check(gpu.lib.mlxr_memcpy_h2d(pool.ptr + shift * page_bytes, a.ctypes.data, a.nbytes))
+    return pools, pages, shift
+
+
+def fetch(gpu, pool, at, like):
+    a = np.empty_like(like)
+    gpu.check(gpu.lib.mlxr_memcpy_d2h(a.ctypes.data, pool.ptr + at, a.nbytes))
+    return a
+
+
+def test_offsets_past_32_bits(gpu):
+    """The same step with its pages behind 2^32 elements of the pools: the same bits from append, attention and eviction."""
+    nKV, D, nH = 8, 128, 32
+    page_bytes = nKV * PAGE * D * 2
+    src, dst = pair(gpu, [200, 64, 300], nKV, D, 0, 100, seed=51)
+    src.up(), dst.up()
+    rs = np.random.default_rng(52)
+    qkv, inv = rs.standard_normal((3, (nH + 2 * nKV) * D)).astype(np.float32), (1e6 ** (-np.arange(0, D, 2) / D)).astype(np.float32)
+    pools, pages, shift = far_pool(gpu, src, page_bytes)
+    tables = [gpu.DeviceArray.from_numpy(np.where(t < 0, -1, t + shift).astype(np.int32)) for t in (src.table, dst.table)]
+    near = run_append(gpu, src, qkv, nH, inv, None, None, D, 0, None, 1e-6, False, q_pad=0)[0]
+    got = [attend(gpu, src, near, nH)]
+    evict(gpu, src, dst, 100, 4, 16)
+    k_near, v_near = src.dk.numpy(), src.dv.numpy()
+    far = dict(k=pools[0].ptr, v=pools[1].ptr, n_pages=pages)
+    a, b = src.desc(table=tables[0].ptr, **far), dst.desc(table=tables[1].ptr, **far)
+    dx, df, dq = gpu.DeviceArray.from_numpy(qkv), gpu.DeviceArray.from_numpy(inv), gpu.DeviceArray.zeros((3, nH * D), np.float32)
+    gpu.check(gpu.lib.mlxr_k_paged_append(ctypes.byref(a), dx.ptr, qkv.shape[1], df.ptr, None, None, nH, D, 0, None, 1e-6, dq.ptr, nH * D, None))
+    assert same(dq.numpy(), near)
+    got.append(attend(gpu, src, near, nH, desc=a))
+    assert same(got[0], got[1])
+    work = workspace(gpu, gpu.lib.mlxr_k_paged_evict_work(ctypes.byref(a), 100))
+    # the attention above kept weights: eviction reads them as they are now in both runs' arrays
+    gpu.check(gpu.lib.mlxr_k_paged_evict(ctypes.byref(a), ctypes.byref(b), 100, 4, 16, work.ptr, work.nbytes, None))
+    gpu.synchronize()
+    assert same(fetch(gpu, pools[0], shift * page_bytes, src.k), k_near) and same(fetch(gpu, pools[1], shift * page_bytes, src.v), v_near)
+
+
+def test_sample_far_rows(gpu):
+    """Rows of logits 2^30 and more floats apart."""
+    V, stride, R = 40000, (1 << 30) + 3, 4
+    x = model_logits(np.random.default_rng(53), R, V)
+    buf = gpu.DeviceArray((R - 1) * stride + V, np.float32)
+    for r in range(R):
+        gpu.check(gpu.lib.mlxr_memcpy_h2d(buf.ptr + 4 * r * stride, x[r].ctypes.data, x[r].nbytes))
+    d = gpu.DeviceArray.from_numpy
+    t, p, u, tok = d(np.full(R, 0.8, np.float32)), d(np.full(R, 0.9, np.float32)), d(np.array([0.1, 0.5, 0.9, 0.99], np.float32)), gpu.DeviceArray.zeros(R, np.int32)
+    work = workspace(gpu, gpu.lib.mlxr_k_sample_rows_work(R, V))
+    gpu.check(gpu.lib.mlxr_k_sample_rows(buf.ptr, R, V, stride, t.ptr, None, p.ptr, None, u.ptr, tok.ptr, None, work.ptr, work.nbytes, None))
+    gpu.synchronize()
+    assert same(tok.numpy(), sample(gpu, x, 0.8, p=0.9, u=[0.1, 0.5, 0.9, 0.99])[0])
+
+
 # ------------------------------------------------------------------------------------------- append
 def run_append(mlxr, c, qkv, nH, inv_freq, qn, kn, rot, traditional, positions, eps, in_place, q_pad=2):
     d = mlxr.DeviceArray.from_numpy
@@ -568,6 +651,16 @@ def test_sample_mixed_rows(gpu, V, stride):
     check_tokens(gpu, x, t, k, p, low, rs.random(R).astype(np.float32), stride=stride)
 
 
+@pytest.mark.parametrize("V", [262145, 300001, 1 << 20])
+def test_sample_large_vocabularies(gpu, V):
+    print(f"[case] V={V}", flush=True)
+    rs = np.random.default_rng(V)
+    x = model_logits(rs, 4, V, 300)
+    x[3] = rs.integers(0, 3, V)
+    for t, k, p, low in [(0.7, 40, 0.95, 0.0), (1.0, None, 0.9, None), (1.0, None, None, None), (0.0, None, None, None), (1.0, None, None, 0.02), (1.0, 5000, 0.9, None)]:
+        check_tokens(gpu, x, t, k, p, low, rs.random(4).astype(np.float32))
+
+
 def test_sample_ties(gpu):
     """Equal logits are ranked by index, at every cut: rows of one value, of three, and of +0 and -0."""
     rs = np.random.default_rng(3)
@@ -786,6 +879,26 @@ def test_step_captured(gpu):
         hip.wait(st)
         for x, y in zip(a.state(), b.state()):
             assert same(x, y), n
+    hip("hipGraphExecDestroy", graph)
+    hip("hipStreamDestroy", st)
+
+
+def test_eviction_of_long_sequences_captured(gpu):
+    """Lengths for which a launch asks for more LDS than it has by itself, in a HIP graph: every replay is the eager result."""
+    hip = Hip(gpu)
+    src, dst = pair(gpu, [20000, 31000, 40000], 1, 64, 0, 3000, seed=61)
+    src.up(), dst.up()
+    st, a = hip.stream(), src.desc()
+    b = dst.desc(k=src.dk.ptr, v=src.dv.ptr, n_pages=src.k.shape[0])
+    work = workspace(gpu, gpu.lib.mlxr_k_paged_evict_work(ctypes.byref(a), 3000))
+    run = lambda: gpu.check(gpu.lib.mlxr_k_paged_evict(ctypes.byref(a), ctypes.byref(b), 3000, 4, 512, work.ptr, work.nbytes, st))  # noqa: E731
+    graph = hip.capture(st, run)
+    for n in range(3):
+        src.weight = np.random.default_rng(62 + n).exponential(1.0, src.weight.shape).astype(np.float32)
+        src.dw.upload(src.weight)
+        hip("hipGraphLaunch", graph, st)
+        hip.wait(st)
+        check_evicted(src, dst, 3000, 4, 512, src.k.copy(), src.v.copy(), dst.weight, dst.position)
     hip("hipGraphExecDestroy", graph)
     hip("hipStreamDestroy", st)
 
