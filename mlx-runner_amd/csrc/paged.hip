@@ -89,16 +89,17 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
 // two f16 (22 bits, q scaled to at most 2^14 by a power of two, p by 2^14). Scores are in powers of two (log2 e is
 // in q's scale).
 //
-// Measured (bf16, D 128): 4 sequences of 99 to 131 thousand slots, 40 / 8 heads 317 us (5.9 TB/s; a copy of 4 GiB reaches
-// 4.7); 32 of 0 to 8191, 32 / 8 heads 101 us (5.3 TB/s); one of 4096 12 us, of which 2 go by until the first keys are asked
-// for, 3 until they are multiplied and 5 to hand over and join. One workgroup a CU of eight waves: two of four take 102, 322,
-// 12.7 us, and 512 of eight 109, 322, 13. No place behind a segment: 106 us for the 32, 22 us instead of 17 for
-// a window of 1024 over 24 sequences of 5 to 16000 (short ones cost their ends, not their pages). Asking for the next
-// keys ahead of these ones' softmax takes more registers and a second copy of the step, and was slower (121, 340, 15 us).
+// Measured (bf16, D 128): 4 sequences of 99 to 131 thousand slots, 40 / 8 heads 315 us (6.0 TB/s; a copy of 4 GiB reaches
+// 4.7); 32 of 0 to 8191, 32 / 8 heads 100 us (5.4 TB/s); one of 4096 11.5 us, of which 2 go by until the first keys are
+// asked for, 3 until they are multiplied and 5 to hand over and join. Beside that, each change alone, in us for the three:
+// two workgroups of four waves a CU 322, 102, 12.7; 512 workgroups of eight 322, 109, 13.1; no places behind a segment
+// 322, 106, and 22 instead of 17.4 for a window of 1024 over 24 sequences of 5 to 16000 slots (short ones cost their ends,
+// not their pages); the next keys asked for ahead of these ones' softmax, for more registers and a second copy of the
+// step, 340, 121, 15.0; runs found by barriers for up to 64 sequences too 316, 101, 12.1.
 constexpr int PA_WV = 8, PA_T = 64 * PA_WV;   // waves and threads of a workgroup
 constexpr int PA_MAXW = 256;       // workgroups: one a CU
 constexpr int PA_GAP = 4;          // places behind a segment
-constexpr int PA_MINPER = 4;       // places of a run at least (one sequence of 4096: 12 us; 6: 13, 8: 15.5)
+constexpr int PA_MINPER = 4;       // places of a run at least (one sequence of 4096: 12.1 us; with 6 13.1, with 8 15.5)
 constexpr int PA_ROWS = 16;
 typedef float pa_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 pa_b8 __attribute__((ext_vector_type(8)));
@@ -185,49 +186,65 @@ __global__ __launch_bounds__(PA_T, 2) void paged_attn_kernel(PagedAttnArgs a, Pa
     const uint32_t per_seq = (uint32_t)(kv.nKV * wk.groups);   // segments of a sequence
     const uint16_t *K = static_cast<const uint16_t*>(kv.k), *V = static_cast<const uint16_t*>(kv.v);
 
-    // This workgroup's run of pages: the sequences' page counts, PA_T at a time, summed for the total and again for the
-    // sequence in which the run begins (the host has checked that all pages of all segments number less than 2^31).
-    uint32_t T = 0, before = 0, chunk = 0;
-    int n = 0, len = 0;
-    auto scan = [&](int c, bool zero) {
-        len = c + tid < kv.B ? paged_len(kv, c + tid) : -1;
-        n = len < 0 ? -1 : pa_places(pa_seq_of(a, len).n);
-        if (zero) {   // idle rows: zeros, from one workgroup each
-            for (uint64_t idle = __ballot(n == 0 && (uint32_t)(c + tid) % (uint32_t)wk.W == w); idle; idle &= idle - 1) {
-                float* o = a.out + (int64_t)(c + 64 * wave + (int)__builtin_ctzll(idle)) * a.out_stride;
-                for (int i = 4 * lane; i < a.nH * D; i += 256) *reinterpret_cast<float4*>(o + i) = float4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
+    // This workgroup's run of pages. Up to 64 sequences each wave finds by itself; more are summed 512 at a time, for
+    // the total and again for the sequence in which the run begins (the host has checked that all pages of all segments
+    // number less than 2^31). Idle rows get their zeros here, from one workgroup each.
+    auto zero = [&](uint64_t idle, int b0) {
+        for (; idle; idle &= idle - 1) {
+            float* o = a.out + (int64_t)(b0 + (int)__builtin_ctzll(idle)) * a.out_stride;
+            for (int i = 4 * lane; i < a.nH * D; i += 256) *reinterpret_cast<float4*>(o + i) = float4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        n = n < 0 ? 0 : n;
-        const uint32_t v = (uint32_t)wave_scan(n);
-        uint32_t* sums = wsum[(c / PA_T) & 1];
-        if (lane == 63) sums[wave] = v;
-        __syncthreads();
-        before = v - n;
-        chunk = 0;
-#pragma unroll
-        for (int i = 0; i < PA_WV; i++) { before += i < wave ? sums[i] : 0; chunk += sums[i]; }
     };
-    for (int c = 0; c < kv.B; c += PA_T) { scan(c, true); T += chunk; }
-    const uint32_t all = T * per_seq;
-    const uint32_t per = max((uint32_t)PA_MINPER, (all + wk.W - 1) / (uint32_t)wk.W);
-    uint32_t t = w * per;
-    if (t >= all) return;
-    const uint32_t t1 = min(all, t + per);
-    {
+    auto run_of = [&](uint32_t places, uint32_t& per, uint32_t& t, uint32_t& t1) {   // false: there are fewer runs than workgroups
+        const uint32_t all = places * per_seq;
+        per = max((uint32_t)PA_MINPER, (all + wk.W - 1) / (uint32_t)wk.W);
+        t = w * per;
+        t1 = min(all, t + per);
+        return t < all;
+    };
+    uint32_t per, t, t1, pre;
+    int b, L;
+    if (kv.B <= 64) {
+        const int len = lane < kv.B ? paged_len(kv, lane) : -1, n = len < 0 ? 0 : pa_places(pa_seq_of(a, len).n);
+        const uint64_t idle = __ballot(len == 0 && (uint32_t)lane % (uint32_t)wk.W == w);
+        if (wave == 0) zero(idle, 0);
+        const uint32_t upto = (uint32_t)wave_scan(n), before = upto - n;
+        if (!run_of((uint32_t)__builtin_amdgcn_readlane((int)upto, 63), per, t, t1)) return;
+        b = (int)__builtin_ctzll(__ballot(before * per_seq <= t && t < upto * per_seq));
+        pre = (uint32_t)__builtin_amdgcn_readlane((int)before, b);
+        L = __builtin_amdgcn_readlane(len, b);
+    } else {
+        uint32_t T = 0, before = 0, chunk = 0;
+        int n = 0, len = 0;
+        auto scan = [&](int c, bool first) {
+            len = c + tid < kv.B ? paged_len(kv, c + tid) : -1;
+            n = len < 0 ? 0 : pa_places(pa_seq_of(a, len).n);
+            if (first) zero(__ballot(len == 0 && (uint32_t)(c + tid) % (uint32_t)wk.W == w), c + 64 * wave);
+            const uint32_t v = (uint32_t)wave_scan(n);
+            uint32_t* sums = wsum[(c / PA_T) & 1];
+            if (lane == 63) sums[wave] = v;
+            __syncthreads();
+            before = v - n;
+            chunk = 0;
+#pragma unroll
+            for (int i = 0; i < PA_WV; i++) { before += i < wave ? sums[i] : 0; chunk += sums[i]; }
+        };
+        for (int c = 0; c < kv.B; c += PA_T) { scan(c, true); T += chunk; }
+        if (!run_of(T, per, t, t1)) return;
         uint32_t run = 0;
         for (int c = 0; c < kv.B; c += PA_T) {
             if (kv.B > PA_T) { __syncthreads(); scan(c, false); }
-            const uint32_t pre = run + before;
-            if (pre * per_seq <= t && t < (pre + n) * per_seq) { found_b = c + tid; found_pre = pre; found_len = len; }
+            const uint32_t p = run + before;
+            if (p * per_seq <= t && t < (p + n) * per_seq) { found_b = c + tid; found_pre = p; found_len = len; }
             run += chunk;
             if (run * per_seq > t) break;
         }
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(found_b);
+        pre = __builtin_amdgcn_readfirstlane(found_pre);
+        L = __builtin_amdgcn_readfirstlane(found_len);
     }
-    __syncthreads();
-    int b = __builtin_amdgcn_readfirstlane(found_b);
-    uint32_t pre = __builtin_amdgcn_readfirstlane(found_pre);
-    PaSeq sq = pa_seq_of(a, __builtin_amdgcn_readfirstlane(found_len));
+    PaSeq sq = pa_seq_of(a, L);
     int slot = 0;   // partial results of this workgroup: its first segment's, then its last one's
     while (true) {
         const uint32_t places = (uint32_t)pa_places(sq.n), local = t - pre * per_seq, seg = local / places;
@@ -395,7 +412,7 @@ __global__ __launch_bounds__(PA_T, 2) void paged_attn_kernel(PagedAttnArgs a, Pa
         // the waves' results: lane (r, g) has row r's dims DV (4 g + i) + j
         l = xor32_sum(xor16_sum(l));
         if (g == 0) { sm[wave][r] = m; sl[wave][r] = l; }
-        {
+        if (r < rows) {
             float* so = lds + (wave * PA_ROWS + r) * OS;
             constexpr float down = ST == 0 ? 1.0f : 1.0f / 16384.0f;
 #pragma unroll
