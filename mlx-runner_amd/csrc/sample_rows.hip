@@ -7,8 +7,8 @@
 //   1. sample_groups_kernel, about a thousand workgroups: the maximum of every 64 logits. The one read of the logits that
 //      every row needs: 0.6 MB a row of 152 thousand, 37 us for 256 of them (4.2 TB/s), 3 us for one.
 //   2. sample_sums_kernel, for rows that ask for a sum over all their tokens (top-p, or nothing, without top-k). With the
-//      row's maximum known, tokens fall into bins of 1/64 of x = (max - v) / T, 2048 of them: what lies behind x = 32 has
-//      no weight that counts. Each bin's weights are added up, and each token's bin is written down. Bound by the 64-bit
+//      row's maximum known, tokens fall into 2048 bins of x = (max - v) / T, 64 to a unit: what lies behind x = 32 has
+//      no weight that counts (finer ones above a temperature of 1). Each bin's weights are added up, and each token's bin is written down. Bound by the 64-bit
 //      arithmetic and the adds in LDS: 25 us for 102 rows of 152 thousand; other rows leave at once (2 us).
 //   3. sample_pick_kernel, one workgroup a row. A row with sums: the bins in which the sums cross are found, just their
 //      tokens are gathered (through the groups' maxima, or by the bin numbers where most groups qualify), ranked and
@@ -18,10 +18,10 @@
 // A bin's weights are a constant times f in (exp(-1/64), 1], added as multiples of 2^-43: no order of the atomic adds
 // changes a result, and 2^20 of them stay below 2^63. Everything else is 64-bit floating point, so a token differs from
 // the exact sums' only if the draw is within about 2^-43 of a border.
-// Rows whose crossing bins hold too many tokens for the list (thousands of equal logits, top-k of thousands, a
-// temperature of 5 and more over a large vocabulary) take the radix descent instead, which asks for no room: a histogram
-// of the order keys' leading bits, the bin in which the sum crosses, and again within that bin, until one key is left,
-// whose tokens have one weight. Up to 15 passes of one workgroup over the row: about 350 us for 152 thousand.
+// Rows whose crossing bins hold too many tokens for the list (thousands of equal logits, top-k of thousands) take the
+// radix descent instead, which asks for no room: a histogram of the order keys' leading bits, the bin in which the sum
+// crosses, and again within that bin, until one key is left, whose tokens have one weight. Up to 15 passes of one
+// workgroup over the row: about 500 us for 152 thousand.
 #include "batch.h"
 
 namespace mlxr {
@@ -119,8 +119,14 @@ __device__ SrCut sr_descend(const SrRow& r, SrCut cut, bool by_mass, uint64_t ta
             const uint32_t k = sr_key(x);
             if (k > cut.key && (k & mask) == prefix) {
                 const uint32_t bin = (k >> shift) & (bins - 1);
-                atomicAdd(&sh.count[bin], 1u);
-                atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[bin]), (unsigned long long)r.fixed(x));
+                // lanes with one key (ties by the thousand) add once: as many adds to one place would wait for each other
+                const uint64_t lanes = __ballot(true), equal = __ballot(k == (uint32_t)__builtin_amdgcn_readfirstlane((int)k));
+                const bool one = equal == lanes;
+                const uint32_t times = one ? (uint32_t)__popcll(lanes) : 1u;
+                if (!one || lane == (int)__builtin_ctzll(lanes)) {
+                    atomicAdd(&sh.count[bin], times);
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[bin]), (unsigned long long)(times * r.fixed(x)));
+                }
             }
         }
         __syncthreads();
@@ -241,7 +247,6 @@ __device__ __noinline__ int sr_descent_token(const float* v, int V, float larges
 
 // ---- bins, gathered tokens and their order ----
 constexpr int SR_GROUP = 64, SR_LIST = 2048;
-constexpr double SR_WIDTH = 64.0;   // bins per unit of x
 typedef uint32_t sr_w4 __attribute__((ext_vector_type(4)));
 typedef uint16_t sr_h2 __attribute__((ext_vector_type(2)));
 
@@ -271,16 +276,27 @@ __device__ __forceinline__ SrAsk sr_ask(const SampleRowsArgs& a, int row) {
 
 __host__ __device__ __forceinline__ bool sr_vec(const SampleRowsArgs& a) { return a.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0; }
 
+// Bins: 64 to a unit of x at temperatures up to 1, and as many to a unit of the logits at those up to 8, where the bulk's
+// logits lie closer in x (at 3, two bins of 64 a unit may hold 3000 of 152 thousand tokens; one row with a top-p of 0.9 then
+// took 475 us through the radix descent, and takes 44). They end at x = 32 or, above 1,
+// at 32 of the logits, behind which tokens may have weight: `edge`.
 struct SrBins {
     double top, inv, width;   // the largest logit; bins per unit of logit, and the other way round
+    double per, inv_per;      // bins per unit of x
+    bool edge;
     __device__ __forceinline__ double x(float v) const { return (top - (double)v) * inv; }   // in bins; NaN or infinite outside
 };
-// 2^43 exp(-y / 64) for y = x - bin in [0, 1), rounded to a whole number: the Taylor sum to the fifth power is off by
-// 2^-45; added to 2^52 it is rounded into the mantissa's low bits.
-__device__ __forceinline__ uint64_t sr_fixed(double x, int bin) {
-    constexpr double c1 = SR_ONE / SR_WIDTH, c2 = c1 / SR_WIDTH / 2, c3 = c2 / SR_WIDTH / 3, c4 = c3 / SR_WIDTH / 4, c5 = c4 / SR_WIDTH / 5;
-    const double y = x - (double)bin;
-    const double e = fma(y, fma(y, fma(y, fma(y, fma(y, -c5, c4), -c3), c2), -c1), SR_ONE);
+__device__ __forceinline__ SrBins sr_bins(float top, float T, double inv_T) {
+    const double per = T > 1.0f ? 64.0 * fmin((double)T, 8.0) : 64.0, inv_per = T > 1.0f ? fmax(inv_T, 0.125) / 64.0 : 1.0 / 64.0;
+    return SrBins{(double)top, per * inv_T, (double)T * inv_per, per, inv_per, T > 1.0f};
+}
+// exp(-x), where the bins' tables end: a call of its own, for the length of its code.
+__device__ __noinline__ double sr_far_exp(double x) { return exp(-x); }
+// 2^43 exp(-y / per) for y = x - bin in [0, 1), rounded to a whole number: the Taylor sum to the fifth power is off by
+// 2^-45 at most; added to 2^52 it is rounded into the mantissa's low bits.
+__device__ __forceinline__ uint64_t sr_fixed(double x, int bin, double inv_per) {
+    const double y = (x - (double)bin) * inv_per;
+    const double e = fma(y, fma(y, fma(y, fma(y, fma(y, -SR_ONE / 120, SR_ONE / 24), -SR_ONE / 6), SR_ONE / 2), -SR_ONE), SR_ONE);
     return __builtin_bit_cast(uint64_t, e + 0x1p52) & 0xfffffffffffffull;
 }
 
@@ -335,7 +351,9 @@ __global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a,
     for (int i = 0; i < SR_SUM_T / 64; i++) top = fmaxf(top, wave_top[i]);
     if (!isfinite(top)) return;
     const SrRow r{a.logits + (int64_t)row * a.stride, a.V, sr_vec(a), top, 0.0};
-    const SrBins bins{(double)top, SR_WIDTH * (1.0 / (double)a.temperature[row]), 0.0};
+    const SrBins bins = sr_bins(top, a.temperature[row], 1.0 / (double)a.temperature[row]);
+    const double inv_per = bins.inv_per;
+    bool far = false;
     uint16_t* out = wk.bin + (int64_t)row * wk.groups * SR_GROUP;
     const int i1 = min(a.V, ((int)blockIdx.x + 1) * wk.sum_per * SR_GROUP);
     constexpr int UN = 4;
@@ -353,13 +371,23 @@ __global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a,
                 bin[e] = 0xffffu;
                 if (x < (double)SR_BINS) {   // not NaN, not -infinity
                     bin[e] = (uint32_t)(int)x;
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin[e]]), (unsigned long long)sr_fixed(x, (int)bin[e]));
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin[e]]), (unsigned long long)sr_fixed(x, (int)bin[e], inv_per));
+                } else if (x < INFINITY) {
+                    far = bins.edge;
                 }
             }
             const int at = i + 4 * SR_SUM_T * k;
             if (at < i1) *reinterpret_cast<uint2*>(out + at) = uint2{bin[0] | (bin[1] << 16), bin[2] | (bin[3] << 16)};
         }
     }
+    // what lies behind the bins goes to the last one (in which no sum may cross then)
+    if (far)
+        for (int i = blockIdx.x * wk.sum_per * SR_GROUP + 4 * tid; i < i1; i += 4 * SR_SUM_T)
+            for (int e = i; e < min(i + 4, i1); e++) {
+                const double x = bins.x(r.v[e]);
+                if (x >= (double)SR_BINS && x < INFINITY)
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&hist[SR_BINS - 1]), (unsigned long long)(sr_far_exp((x - (SR_BINS - 1)) * inv_per) * SR_ONE + 0.5));
+            }
     __syncthreads();
     uint64_t* mine = wk.mass + ((int64_t)row * wk.sum_spans + blockIdx.x) * SR_BINS;
     for (int i = tid; i < SR_BINS; i += SR_SUM_T) mine[i] = hist[i];
@@ -376,7 +404,7 @@ struct SrPick {
         uint16_t ids[SR_MAXGROUPS];   // while tokens are gathered, before they are ranked
     };
     float gmax[SR_NEAR];
-    double exp_whole[32], exp_part[64];   // exp(-i), exp(-i / 64)
+    double exp_whole[32], exp_part[64];   // exp(-64 i / per), exp(-i / per)
     double wave_sum[2][SR_W];
     int wave_count[2][4][SR_W];
     float wave_top[SR_W];
@@ -510,13 +538,13 @@ struct SrTeam {
     int tid, lane, wave, flip;
 
     __device__ __forceinline__ float group(int g) const { return g < SR_NEAR ? s.gmax[g] : gmax[g]; }
-    // A bin's constant, and a logit's weight in units of 2^-43, as the bins' sums have it (0 behind the bins).
+    // A bin's constant, and a logit's weight in units of 2^-43, as the bins' sums have it.
     __device__ __forceinline__ double constant(int bin) const { return s.exp_whole[bin >> 6] * s.exp_part[bin & 63]; }
     __device__ __forceinline__ double weight(float v) const {
         const double x = bins.x(v);
-        if (!(x < (double)SR_BINS)) return 0.0;
+        if (!(x < (double)SR_BINS)) return bins.edge && x < INFINITY ? sr_far_exp(x * bins.inv_per) * SR_ONE : 0.0;
         const int bin = (int)x;
-        return constant(bin) * (double)sr_fixed(x, bin);
+        return constant(bin) * (double)sr_fixed(x, bin, bins.inv_per);
     }
     __device__ __forceinline__ float ranked(int i) const { return sr_value((uint32_t)(s.ranked[i] >> 32)); }
     __device__ __forceinline__ int token(int i) const { return (int)~(uint32_t)s.ranked[i]; }
@@ -586,11 +614,11 @@ struct SrTeam {
         }
         __syncthreads();
     }
-    // The logits of bins b0 .. b1 lie in [lo, hi]; a few of the neighbouring bins may too.
+    // The logits of bins b0 .. b1 lie in [lo, hi]; a few of the neighbouring bins may too. b1 SR_BINS: those behind the bins too.
     __device__ __forceinline__ void range(int b0, int b1, float& lo, float& hi) const {
         const double top = bins.top, slack = fabs(top) * 0x1p-22 + 0x1p-120;
         const double l = top - (double)(b1 + 1) * bins.width, h = top - (double)b0 * bins.width;
-        lo = fmaxf((float)(l - fabs(l) * 0x1p-22 - slack), -3.402823466e38f);
+        lo = b1 == SR_BINS ? -3.402823466e38f : fmaxf((float)(l - fabs(l) * 0x1p-22 - slack), -3.402823466e38f);
         hi = (float)fmin(h + fabs(h) * 0x1p-22 + slack, top);
         if (!(hi <= (float)top)) hi = (float)top;   // T infinite: 0 times infinity
     }
@@ -628,12 +656,13 @@ struct SrTeam {
     }
 };
 
-// The bin down to which there are `want` groups, by their maxima (the last one if there are fewer).
+// The bin down to which there are `want` groups, by their maxima; if there are fewer, the last one, or all tokens where
+// weight may lie behind it.
 __device__ __forceinline__ int sr_bin_of(SrTeam& t, int want) {
     SrPick& s = t.s;
     int* cnt = reinterpret_cast<int*>(s.list);
     for (int i = t.tid; i < SR_BINS; i += SR_T) cnt[i] = 0;
-    if (t.tid == 0) s.found = SR_BINS - 1;
+    if (t.tid == 0) s.found = t.bins.edge ? SR_BINS : SR_BINS - 1;
     __syncthreads();
     for (int g = t.tid; g < t.groups; g += SR_T) {
         const double x = t.bins.x(t.group(g));
@@ -674,9 +703,10 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
     r.v = a.logits + (int64_t)row * a.stride;
     r.V = a.V;
     r.vec = sr_vec(a);
-    SrTeam t{s, r, SrBins{}, gmax, wk.groups, ask.kind == SR_SUM ? wk.bin + (int64_t)row * wk.groups * SR_GROUP : nullptr, tid, lane, wave, 0};
+    r.inv = 1.0 / (double)T;
+    SrTeam t{s, r, sr_bins(0.0f, T, r.inv), gmax, wk.groups, ask.kind == SR_SUM ? wk.bin + (int64_t)row * wk.groups * SR_GROUP : nullptr, tid, lane, wave, 0};
     if (wave < 2) {
-        const double e = exp(wave ? (double)-(lane & 31) : (double)-lane / 64.0);
+        const double e = exp((wave ? -64.0 * (double)(lane & 31) : (double)-lane) * t.bins.inv_per);
         if (!wave) s.exp_part[lane] = e;
         else if (lane < 32) s.exp_whole[lane] = e;
     }
@@ -695,8 +725,7 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
         return;
     }
     r.top = top;
-    r.inv = 1.0 / (double)T;
-    t.bins = SrBins{(double)top, SR_WIDTH * r.inv, (double)T / SR_WIDTH};
+    t.bins.top = (double)top;
     double goal = (double)given;
     goal = goal > 0.0 ? (goal < 1.0 ? goal : 1.0) : 0.0;
     int token = -1;
@@ -716,9 +745,10 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
         bool drawing = false;                // the gathered bin is the draw's
         if (ask.kind == SR_TOP) {
             // all tokens down to a bin: that of the k-th largest group maximum, with min-p no further than its own
+            if (t.bins.edge) b1 = SR_BINS;
             if (r.V > SR_LIST) {
                 if (ask.k < r.V) b1 = sr_bin_of(t, ask.k);
-                if (ask.low > 0.0f && ask.p >= 1.0f) b1 = min(b1, (int)(-log((double)ask.low) * SR_WIDTH) + 1);
+                if (ask.low > 0.0f && ask.p >= 1.0f) b1 = min(b1, (int)(-log((double)ask.low) * t.bins.per) + 1);
             }
         } else {
             const uint64_t* all = wk.mass + (int64_t)row * wk.sum_spans * SR_BINS + SR_PER * tid;
@@ -735,7 +765,7 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
             kept = s.run[SR_BINS - 1];
             p_goal = (double)ask.p * kept;
             if (ask.p < 1.0f) bp = min(t.first(p_goal, 0.0, SR_BINS), SR_BINS - 1);
-            if (ask.low > 0.0f) { const double x = -log((double)ask.low) * SR_WIDTH; if (x < (double)SR_BINS) bm = (int)x; }
+            if (ask.low > 0.0f) { const double x = -log((double)ask.low) * t.bins.per; if (x < (double)SR_BINS) bm = (int)x; }
             b0 = min(bp, bm);
             drawing = b0 == SR_BINS;         // nothing is cut
             // the draw's bin, if all tokens of the bin that the kept ones end in were kept: most often that is it
@@ -747,9 +777,16 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
             also_before = also > 0 ? s.run[also - 1] : 0.0;
         }
 #pragma unroll 1
-        while (true) {
+        while (!(t.bins.edge && b0 == SR_BINS - 1)) {   // a sum that crosses behind the bins
             const int n = t.gather(also, b0, b1);
-            if (n > SR_LIST) break;
+            if (n > SR_LIST) {
+                if (also < 0) break;
+                also = -1;   // without the guessed bin there may be room
+                __syncthreads();
+                if (tid == 0) { s.n = 0; s.nids = 0; }
+                __syncthreads();
+                continue;
+            }
             if (ask.kind == SR_TOP) {
                 const int k = min(ask.k, n);
                 int end = k;

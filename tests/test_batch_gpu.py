@@ -574,7 +574,7 @@ def sample(mlxr, logits, t, k=None, p=None, low=None, u=None, stride=None, statu
 
 
 def reference_token(v, t, k, p, low, u):
-    """(tokens that may come, status): one token, or the two next to a border that the goal lies on. The kernel's weights
+    """(tokens that may come, status): one token, or those next to a border that the goal lies on. The kernel's weights
     are multiples of 2^-43 (off by 2^-44 each), its sums exact: a border may be off by V 2^-44."""
     v = np.asarray(v, np.float64)
     ok = ~np.isnan(v) & (v != -np.inf)
@@ -599,8 +599,8 @@ def reference_token(v, t, k, p, low, u):
     may = set()
     for e in set(ends):
         goal = (float(np.float32(u)) if u == u else 0.0) * run[e - 1]
-        for d in (-slack, 0, slack):
-            may.add(int(order[min(e - 1, int(np.searchsorted(run[:e], goal + d)))]))
+        first, last = (min(e - 1, int(np.searchsorted(run[:e], goal + d))) for d in (-slack, slack))
+        may.update(int(i) for i in order[first:last + 1])   # every token whose border lies within the slack
     return may, 0
 
 
@@ -637,6 +637,23 @@ def test_sample_parameters(gpu, V):
                          (1.0, 10 ** 9, 1.0, 0.0), (1.0, -3, 0.0, None), (1.0, None, 1e-9, None), (1.0, None, None, 1.0), (1.0, None, None, 7.0), (100.0, 700, 0.5, 0.9)]:
         doubtful += check_tokens(gpu, x, t, k, p, low, u)[1]
     assert doubtful < 17   # the reference decides nearly all
+
+
+@pytest.mark.parametrize("V", [1500, 30000, 151936])
+def test_sample_temperatures(gpu, V):
+    """Temperatures around and above 1 over logits that reach far down (to -200, where weight may lie far behind the bins)."""
+    print(f"[case] V={V}", flush=True)
+    rs = np.random.default_rng(V)
+    x = model_logits(rs, 12, V)
+    x[4:8] = rs.uniform(-200, 0, (4, V))
+    x[8:] -= rs.exponential(15, (4, V)).astype(np.float32)
+    u = rs.random(12).astype(np.float32)
+    u[[0, 5, 9]] = 1 - 2.0 ** -24
+    doubtful = 0
+    for t in (0.05, 0.999, 1.0, 1.001, 1.7, 3.0, 5.0, 8.0, 9.5, 40.0, 1e4):
+        for k, p, low in [(None, 0.9, None), (None, None, None), (40, 0.95, None), (None, None, 0.03), (700, 0.99, 1e-6), (None, 0.999, 1e-5), (None, None, 1e-20)]:
+            doubtful += check_tokens(gpu, x, t, k, p, low, u)[1]
+    assert doubtful < 80   # of 924: the three rows drawn at 1 - 2^-24 end among tokens lighter than the slack
 
 
 @pytest.mark.parametrize("V,stride", [(151936, 151936), (50257, 50258), (777, 779)])
