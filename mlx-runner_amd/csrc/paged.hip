@@ -75,8 +75,9 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
 // Split. A (sequence, KV head, group of 16 query heads) is a segment of ceil(slots / 64) pages. All segments' pages,
 // laid end to end with PA_GAP places behind each segment (what beginning and ending one costs, in pages), are cut into
 // equal runs, one per workgroup, so ragged batches keep the card as evenly busy as one long sequence, and lengths may
-// stay on the device: each workgroup finds its run by a scan over the batch's page counts. A segment inside one run is written out at once; one cut by runs leaves partial results (maximum,
-// sum, unnormalised values), which the last workgroup to finish joins in run order: the same bits every time.
+// stay on the device: each workgroup finds its run by a scan over the batch's page counts. A segment inside one run is
+// written out at once; one cut by runs leaves partial results (maximum, sum, unnormalised values), which the last
+// workgroup to finish joins in run order: the same bits every time.
 //
 // Inside. A wave takes 32 keys at a time, straight from memory into the operands of 16x16x32 MFMAs, without LDS:
 //   S^T = K q^T: lane (m = l % 16, g = l / 16) holds 8 dims 32 s + 8 g .. of key m (step s); 16 rows of q are the

@@ -8,8 +8,9 @@
 //      every row needs: 0.6 MB a row of 152 thousand, 37 us for 256 of them (4.2 TB/s), 3 us for one.
 //   2. sample_sums_kernel, for rows that ask for a sum over all their tokens (top-p, or nothing, without top-k). With the
 //      row's maximum known, tokens fall into 2048 bins of x = (max - v) / T, 64 to a unit: what lies behind x = 32 has
-//      no weight that counts (finer ones above a temperature of 1). Each bin's weights are added up, and each token's bin is written down. Bound by the 64-bit
-//      arithmetic and the adds in LDS: 25 us for 102 rows of 152 thousand; other rows leave at once (2 us).
+//      no weight that counts (finer ones above a temperature of 1). Each bin's weights are added up, and each token's bin
+//      is written down. Bound by the 64-bit arithmetic and the adds in LDS: 27 us for 102 rows of 152 thousand; other rows
+//      leave at once (2 us).
 //   3. sample_pick_kernel, one workgroup a row. A row with sums: the bins in which the sums cross are found, just their
 //      tokens are gathered (through the groups' maxima, or by the bin numbers where most groups qualify), ranked and
 //      walked. A row without: the groups' maxima give a bin down to which there are k tokens or more, or min-p does, and
@@ -278,20 +279,25 @@ __host__ __device__ __forceinline__ bool sr_vec(const SampleRowsArgs& a) { retur
 
 // Bins: 64 to a unit of x at temperatures up to 1, and as many to a unit of the logits at those up to 8, where the bulk's
 // logits lie closer in x (at 3, two bins of 64 a unit may hold 3000 of 152 thousand tokens; one row with a top-p of 0.9 then
-// took 475 us through the radix descent, and takes 44). They end at x = 32 or, above 1,
-// at 32 of the logits, behind which tokens may have weight: `edge`.
+// took 475 us through the radix descent, and takes 44). They end at x = 32 or, above 1, at 32 of the logits, behind which
+// tokens may have weight: `edge`. The row's numbers are in scalar registers: the last launch has no others to spare (14
+// vector registers spilled without; 38.7 and 38.1 us for 256 mixed rows).
 struct SrBins {
     double top, inv, width;   // the largest logit; bins per unit of logit, and the other way round
     double per, inv_per;      // bins per unit of x
     bool edge;
     __device__ __forceinline__ double x(float v) const { return (top - (double)v) * inv; }   // in bins; NaN or infinite outside
 };
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ double sr_uniform(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
 __device__ __forceinline__ SrBins sr_bins(float top, float T, double inv_T) {
     const double per = T > 1.0f ? 64.0 * fmin((double)T, 8.0) : 64.0, inv_per = T > 1.0f ? fmax(inv_T, 0.125) / 64.0 : 1.0 / 64.0;
-    return SrBins{(double)top, per * inv_T, (double)T * inv_per, per, inv_per, T > 1.0f};
+    return SrBins{(double)top, sr_uniform(per * inv_T), sr_uniform((double)T * inv_per), sr_uniform(per), sr_uniform(inv_per), T > 1.0f};
 }
-// exp(-x), where the bins' tables end: a call of its own, for the length of its code.
-__device__ __noinline__ double sr_far_exp(double x) { return exp(-x); }
 // 2^43 exp(-y / per) for y = x - bin in [0, 1), rounded to a whole number: the Taylor sum to the fifth power is off by
 // 2^-45 at most; added to 2^52 it is rounded into the mantissa's low bits.
 __device__ __forceinline__ uint64_t sr_fixed(double x, int bin, double inv_per) {
@@ -386,7 +392,7 @@ __global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a,
             for (int e = i; e < min(i + 4, i1); e++) {
                 const double x = bins.x(r.v[e]);
                 if (x >= (double)SR_BINS && x < INFINITY)
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&hist[SR_BINS - 1]), (unsigned long long)(sr_far_exp((x - (SR_BINS - 1)) * inv_per) * SR_ONE + 0.5));
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&hist[SR_BINS - 1]), (unsigned long long)(exp(-(x - (SR_BINS - 1)) * inv_per) * SR_ONE + 0.5));
             }
     __syncthreads();
     uint64_t* mine = wk.mass + ((int64_t)row * wk.sum_spans + blockIdx.x) * SR_BINS;
@@ -541,10 +547,14 @@ struct SrTeam {
     // A bin's constant, and a logit's weight in units of 2^-43, as the bins' sums have it.
     __device__ __forceinline__ double constant(int bin) const { return s.exp_whole[bin >> 6] * s.exp_part[bin & 63]; }
     __device__ __forceinline__ double weight(float v) const {
-        const double x = bins.x(v);
-        if (!(x < (double)SR_BINS)) return bins.edge && x < INFINITY ? sr_far_exp(x * bins.inv_per) * SR_ONE : 0.0;
+        double x = bins.x(v), c = 1.0;
+        // behind the bins: powers of the tables' last entry, until it is near enough or nothing is left
+        for (; !(x < (double)SR_BINS); x -= 64.0 * 31) {
+            if (!(bins.edge && c > 0.0)) return 0.0;
+            c *= s.exp_whole[31];
+        }
         const int bin = (int)x;
-        return constant(bin) * (double)sr_fixed(x, bin, bins.inv_per);
+        return c * constant(bin) * (double)sr_fixed(x, bin, bins.inv_per);
     }
     __device__ __forceinline__ float ranked(int i) const { return sr_value((uint32_t)(s.ranked[i] >> 32)); }
     __device__ __forceinline__ int token(int i) const { return (int)~(uint32_t)s.ranked[i]; }
@@ -725,7 +735,7 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
         return;
     }
     r.top = top;
-    t.bins.top = (double)top;
+    t.bins.top = sr_uniform((double)top);
     double goal = (double)given;
     goal = goal > 0.0 ? (goal < 1.0 ? goal : 1.0) : 0.0;
     int token = -1;
