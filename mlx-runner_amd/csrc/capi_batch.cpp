@@ -93,8 +93,12 @@ int mlxr_k_paged_append(const mlxr_paged_kv* kv, const float* qkv, int row_strid
 }
 
 int64_t mlxr_k_paged_attention_work(const mlxr_paged_kv* kv, int nH) {
-    return guarded([&]() -> int { if (int rc = check_kv(kv)) return rc; if (int rc = check_heads(kv, nH)) return rc; return check_pages(kv, nH); }) == MLXR_OK ? (int64_t)paged_attention_work(*kv, nH)
-                                                                                                                : MLXR_E_INVALID_ARG;
+    const int rc = guarded([&]() -> int {
+        if (int bad_kv = check_kv(kv)) return bad_kv;
+        if (int bad_heads = check_heads(kv, nH)) return bad_heads;
+        return check_pages(kv, nH);
+    });
+    return rc == MLXR_OK ? (int64_t)paged_attention_work(*kv, nH) : MLXR_E_INVALID_ARG;
 }
 int mlxr_k_paged_attention(const mlxr_paged_kv* kv, const float* q, int q_stride, int nH, int window, float scale, float* out, int out_stride,
                            const float* weight_in, float decay, void* work, size_t work_bytes, void* stream) {
