@@ -48,11 +48,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
         return;
     }
     const int page = paged_page(kv, b, slot / MLXR_PAGE), kvh = (h - a.nH) % kv.nKV;
+    if (page < 0) return;   // the slot holds no key: its weight and position stay too
     if (!isV && l == 0) {
         if (kv.weight) kv.weight[paged_slot(kv, b, kvh, slot)] = 0.0f;
         if (kv.position) kv.position[paged_slot(kv, b, kvh, slot)] = pos;
     }
-    if (page < 0 || !on) return;
+    if (!on) return;
     uint16_t* row = static_cast<uint16_t*>(isV ? kv.v : kv.k) + paged_row(kv, page, kvh, slot % MLXR_PAGE);
     row[d0] = kv_round<ST>(v0);
     row[d1] = kv_round<ST>(v1);
