@@ -505,8 +505,8 @@ __global__ __launch_bounds__(PA_T, 2) void paged_attn_kernel(PagedAttnArgs a, Pa
 #pragma unroll
                         for (int c = 0; c < CB; c++) {
                             const float2 s = ml[min(k + ways * c, parts - 1) * PA_ROWS + row];
-                            const float f = k + ways * c < parts ? pa_exp2(s.x - M) : 0.0f;
-                            if (f != 0.0f) { sum += f * s.y; x.x += f * e[c][0].x; x.y += f * e[c][0].y; x.z += f * e[c][1].x; x.w += f * e[c][1].y; }
+                            const float f = pa_exp2(s.x - M);   // a part of NaN counts, whatever its maximum: 0 times NaN is NaN
+                            if (k + ways * c < parts) { sum += f * s.y; x.x += f * e[c][0].x; x.y += f * e[c][0].y; x.z += f * e[c][1].x; x.w += f * e[c][1].y; }
                         }
                         if (k + ways * CB < parts) load(k + ways * CB);
                     }
