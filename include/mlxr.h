@@ -335,8 +335,10 @@ int mlxr_k_paged_append(const mlxr_paged_kv* kv, const float* qkv, int row_strid
                         float* q_out, int q_stride, void* stream);
 
 /* Attention of one query token per sequence over its slots, or over its last `window` ones (0: all):
- * out[b][h] = sum_j p_j v_j with p = softmax(scale q k_j), fp32 results; an idle row, or one none of whose
- * scores is above -infinity, gives zeros. With kv->weight:
+ * out[b][h] = sum_j p_j v_j with p = softmax(scale q k_j), fp32 results; a key whose score is -infinity takes no
+ * part, and an idle row, or one none of whose scores is above -infinity, gives zeros. Infinite keys and values and
+ * NaN count as the formula has them (a value's infinity stays, however small its p; waves that meet them take their
+ * keys again in a slower way). With kv->weight:
  * weight[b][g][j] = decay * weight_in[b][g][j] + the sum of p_j over the query heads of KV head g, for every j < len[b]
  * (slots outside the window only decay; weight_in, with the strides of weight, may be weight itself; NULL: zeros).
  * Pages may be shared by sequences. q, out: 16-byte aligned, strides multiples of 4; out may be q itself at its

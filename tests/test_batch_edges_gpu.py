@@ -1,18 +1,138 @@
-"""The batch's decode step at its edges: NaN in cache and queries, appends to pages outside the pool. Helpers and
+"""The batch's decode step at its edges: infinities and NaN in cache and queries, appends to pages outside the pool. Helpers and
 tolerances are those of test_batch_gpu."""
 import numpy as np
 import pytest
 
-from test_batch_gpu import PAGE, Cache, attend, attention_reference, queries, run_append, same, to_half, within
+from test_batch_gpu import PAGE, Cache, attend, attention_reference, check_out, queries, run_append, same, to_half, within
 
 pytestmark = pytest.mark.gpu
+INF = np.float32(np.inf)
+EIGHTH = next(x for x in (np.float32(0.125 / np.log2(np.e)) + np.float32(i * 2.0 ** -28) for i in range(-9, 9))
+              if np.float32(x * np.float32(np.log2(np.e))) == 0.125)   # a scale that is 2^-3 in powers of two: no bits of its own
+
+
+class Without:
+    """A cache seen without some of its slots: `gone` [B][nKV][slot] take no part."""
+
+    def __init__(self, c, gone):
+        self.c, self.gone = c, gone
+
+    def __getattr__(self, name):
+        return getattr(self.c, name)
+
+    def rows(self, pool, b, h, n):
+        x, there = self.c.rows(pool, b, h, n)
+        there = there & ~self.gone[b, h, :n]
+        return np.where(there[:, None], x, 0), there
 
 
 def put(c, pool, b, h, j, dims, value):
-    pool[c.table[b, j // PAGE], h, j % PAGE, dims] = to_half(np.float32(value), c.st)
+    pool[c.table[b, j // PAGE], h, j % PAGE, dims] = to_half(np.full(1, value, np.float32), c.st)[0]
+
+
+def plain_weights(c, given, p, p_tol, G):
+    want = given[:, :, :c.max_len] + p
+    return want, p_tol + 2.0 ** -23 * (np.abs(given[:, :, :c.max_len]) + np.abs(want)) + (G + 2) * 2.0 ** -24 * p
 
 
 # ------------------------------------------------------------------------------------------- infinities and NaN
+@pytest.mark.parametrize("D,st", [(128, 0), (64, 0), (128, 1), (64, 1)])
+@pytest.mark.parametrize("nKV,G,window", [(2, 4, 0), (1, 17, 0), (2, 1, 150)])
+@pytest.mark.parametrize("exact", [True, False])
+def test_attention_infinite_keys(gpu, D, st, nKV, G, window, exact):
+    """Keys with infinite elements whose scores are -infinity take no part, whatever parts a query is split into: queries of
+    few bits (parts of zero) and of many."""
+    print(f"[case] {D} {st} {nKV} {G} {window} {exact}", flush=True)
+    nH = nKV * G
+    c = Cache(gpu, [1, 65, 700, 0, 2600, 64], nKV, D, st, seed=71, weight=True)
+    q = queries(c, nH)
+    heads = q[:, :nH * D].reshape(c.B, nH, D)
+    heads[:, :, 3], heads[:, :, 5] = np.abs(heads[:, :, 3]) + 1, -np.abs(heads[:, :, 5]) - 1
+    if exact:
+        heads[:] = few_bits(heads)
+    gone = np.zeros((c.B, nKV, c.max_len), bool)
+    rs = np.random.default_rng(72)
+    for b, L in enumerate(c.lens):
+        for h in range(nKV):
+            for j in rs.choice(L, min(L, 9), replace=False) if b != 5 else range(64):
+                gone[b, h, j] = True
+                put(c, c.k, b, h, j, 3, -INF)
+                if j % 2:
+                    put(c, c.k, b, h, j, 5, INF)
+                if j % 3 == 0:
+                    put(c, c.v, b, h, j, slice(None), INF if j % 2 else np.nan)   # of no account
+    given = c.weight.copy()
+    c.up()
+    scale = float(EIGHTH) if exact else 0.09
+    out, tol, p, p_tol = attention_reference(Without(c, gone), q, nH, window, scale)
+    assert not out[[0, 3, 5]].any()
+    check_out(attend(gpu, c, q, nH, window=window, scale=scale, weight_in=c.dw), c, nH, out, tol)
+    want, w_tol = plain_weights(c, given.astype(np.float64), p, p_tol, G)
+    got = c.dw.numpy()
+    for b, L in enumerate(c.lens):
+        assert within(np.abs(got[b, :, :L] - want[b, :, :L]), w_tol[b, :, :L]) <= 1
+        assert same(got[b, :, L:], given[b, :, L:])
+
+
+def few_bits(x):
+    """A value of at most eight bits, which both cache types hold exactly."""
+    return np.round(x * 16).astype(np.float32) / 16
+
+
+@pytest.mark.parametrize("D,st", [(128, 0), (64, 1)])
+@pytest.mark.parametrize("weight", [False, True])
+def test_attention_infinite_values(gpu, D, st, weight):
+    """An infinite value of a key that takes part gives that infinity, however small the key's share is, and two of
+    different signs NaN; all other dims are as without."""
+    c = Cache(gpu, [300, 64, 3000, 40, 129], 2, D, st, seed=73, weight=weight)
+    q = queries(c, 8)
+    plain = attention_reference(c, q, 8, 0, 0.09)
+    put(c, c.v, 0, 0, 299, 7, INF)
+    put(c, c.v, 1, 1, 0, 0, -INF)
+    for j in (5, 1500, 2999):
+        put(c, c.v, 2, 0, j, D - 1, INF)
+    put(c, c.v, 2, 1, 10, 2, INF)
+    put(c, c.v, 2, 1, 2900, 2, -INF)
+    put(c, c.v, 3, 1, 39, slice(None), -INF)
+    out, tol = (x.reshape(c.B, 8, D).copy() for x in plain[:2])
+    for b, h, d, x in [(0, 0, 7, INF), (1, 1, 0, -INF), (2, 0, D - 1, INF), (2, 1, 2, np.nan), (3, 1, slice(None), -INF)]:
+        out[b, 4 * h:4 * h + 4, d] = x
+    c.up()
+    given = c.weight.copy() if weight else None
+    got = attend(gpu, c, q, 8, weight_in=c.dw)[:, :8 * D].reshape(c.B, 8, D)
+    odd = ~np.isfinite(out)
+    assert np.array_equal(got[odd], out[odd].astype(np.float32), equal_nan=True)
+    assert within(np.abs(got[~odd] - out[~odd]), tol[~odd]) <= 1
+    if weight:
+        want, w_tol = plain_weights(c, given.astype(np.float64), plain[2], plain[3], 4)
+        for b, L in enumerate(c.lens):
+            assert within(np.abs(c.dw.numpy()[b, :, :L] - want[b, :, :L]), w_tol[b, :, :L]) <= 1
+
+
+@pytest.mark.parametrize("st", [0, 1])
+def test_attention_infinite_value_of_a_tiny_share(gpu, st):
+    """Shares below what 32 bits hold (e^-200) are not nothing: an infinite value there is the result, in keys before and
+    behind the heaviest one, in its run and in others."""
+    c = Cache(gpu, [2000] * 5, 1, 128, st, seed=74)
+    q = queries(c, 2)
+    q[:, :256] = 0
+    q[:, [0, 128]] = 20.0
+    for b in range(5):
+        for i in range(0, 2000, PAGE):
+            c.k[c.table[b, i // PAGE], 0, :, 0] = to_half(np.float32(-10.0), st)
+        put(c, c.k, b, 0, 1000, 0, 10.0)                      # scores 200 and -200 at a scale of 1
+    for b, j in enumerate([999, 1001, 0, 1999]):
+        put(c, c.v, b, 0, j, 9, INF)
+    c.up()
+    got = attend(gpu, c, q, 2, scale=1.0)[:, :256].reshape(5, 2, 128)
+    assert (got[:4, :, 9] == INF).all()
+    keep = np.arange(128) != 9
+    for b in range(5):
+        v = c.rows(c.v, b, 0, 2000)[0][1000]
+        assert np.abs(got[b][:, keep] - v[keep]).max() <= 2.0 ** -22 * np.abs(v).max()   # one p of 1: products and a quotient
+    assert np.isfinite(got[4]).all()
+
+
 @pytest.mark.parametrize("st", [0, 1])
 @pytest.mark.parametrize("length", [1, 64, 5000])
 def test_attention_nan(gpu, st, length):
@@ -31,6 +151,22 @@ def test_attention_nan(gpu, st, length):
     nan[0, 2] = nan[1, 4:] = True
     assert np.isnan(got[nan]).all()
     assert within(np.abs(got[~nan] - out[~nan]), tol[~nan]) <= 1
+
+
+def test_append_past_f16_and_attention(gpu):
+    """What passes f16's largest number is infinite in its cache: a key that scores -infinity then takes no part."""
+    c = Cache(gpu, [200, 65], 1, 64, 1, seed=76, weight=True).up()
+    qkv = np.random.default_rng(77).standard_normal((2, 4 * 64)).astype(np.float32)
+    qkv[:, 128] = -1e5
+    qkv[:, [0, 64]] = [0.75, 1.5]          # both query heads: positive, of few bits
+    q, _ = run_append(gpu, c, qkv, 2, np.zeros(0, np.float32), None, None, 0, 0, None, 1e-6, False, q_pad=0)
+    c.k, c.v = c.dk.numpy(), c.dv.numpy()
+    gone = np.zeros((2, 1, c.max_len), bool)
+    gone[0, 0, 199] = gone[1, 0, 64] = True
+    out, tol, _, _ = attention_reference(Without(c, gone), q, 2, 0, float(EIGHTH))
+    got = attend(gpu, c, q, 2, scale=float(EIGHTH))
+    assert within(np.abs(got - out), tol) <= 1
+    assert c.dw.numpy()[0, 0, 199] == 0 and c.dw.numpy()[1, 0, 64] == 0
 
 
 # ------------------------------------------------------------------------------------------- append
