@@ -1,9 +1,11 @@
-"""The batch's decode step at its edges: infinities and NaN in cache and queries, appends to pages outside the pool. Helpers and
-tolerances are those of test_batch_gpu."""
+"""The batch's decode step at its edges: infinities and NaN in cache and queries, appends to pages outside the pool,
+host memory in place of the device's. Helpers and tolerances are those of test_batch_gpu."""
+import ctypes
+
 import numpy as np
 import pytest
 
-from test_batch_gpu import PAGE, Cache, attend, attention_reference, check_out, queries, run_append, same, to_half, within
+from test_batch_gpu import PAGE, Cache, Hip, attend, attention_reference, check_out, model_logits, queries, run_append, same, to_half, within
 
 pytestmark = pytest.mark.gpu
 INF = np.float32(np.inf)
@@ -181,3 +183,102 @@ def test_append_bad_pages_leave_everything(gpu):
     w, p = c.weight.copy(), c.position.copy()
     w[2, :, 2], p[2, :, 2] = 0, 2
     assert same(c.dw.numpy(), w) and same(c.dp.numpy(), p)
+
+
+# ------------------------------------------------------------------------------------------- memory
+class Calls:
+    """The four calls over device memory, any one of whose pointers can be given another address."""
+
+    def __init__(self, gpu):
+        d = lambda x: gpu.DeviceArray.from_numpy(np.ascontiguousarray(x))  # noqa: E731
+        rs = np.random.default_rng(91)
+        pool, floats, table = rs.standard_normal((8, 2, PAGE, 128)), rs.random((2, 2, 128)).astype(np.float32), np.arange(8, dtype=np.int32).reshape(4, 2)
+        a = dict(k=d(to_half(pool, 0)), v=d(to_half(pool, 0)), table=d(table[:2]), len=d(np.array([70, 128], np.int32)), weight=d(floats),
+                 position=d(np.zeros((2, 2, 128), np.int32)))
+        b = dict(a, table=d(table[2:]), len=d(np.zeros(2, np.int32)), weight=d(floats), position=d(np.zeros((2, 2, 128), np.int32)))
+        x = dict(qkv=d(rs.standard_normal((2, 1024)).astype(np.float32)), inv=d(np.ones(64, np.float32)), qn=d(np.ones(128, np.float32)),
+                 kn=d(np.ones(128, np.float32)), pos=d(np.array([69, 127], np.int32)), q=gpu.DeviceArray.zeros((2, 512), np.float32),
+                 out=gpu.DeviceArray.zeros((2, 512), np.float32), work=gpu.DeviceArray.zeros(1 << 22, np.uint8))
+        y = dict(logits=d(model_logits(rs, 3, 5000)), t=d(np.full(3, 0.8, np.float32)), k=d(np.full(3, 50, np.int32)), p=d(np.full(3, 0.9, np.float32)),
+                 low=d(np.zeros(3, np.float32)), u=d(np.array([0.2, 0.5, 0.9], np.float32)), tokens=gpu.DeviceArray.zeros(3, np.int32),
+                 status=gpu.DeviceArray.zeros(3, np.int32), work=gpu.DeviceArray.zeros(1 << 22, np.uint8))
+        self.gpu, self.src, self.dst, self.x, self.y = gpu, a, b, x, y
+
+    def cache(self, arrays, over):
+        n = {k: over.get(k, v.ptr) for k, v in arrays.items()}
+        return self.gpu.PagedKV(n_pages=8, table_stride=2, slot_stride=128, max_len=128, B=2, nKV=2, D=128, st=0, **n)
+
+    def append(self, s=None, **over):
+        o, kv = {k: over.get(k, v.ptr) for k, v in self.x.items()}, self.cache(self.src, over)
+        return self.gpu.lib.mlxr_k_paged_append(ctypes.byref(kv), o["qkv"], 1024, o["inv"], o["qn"], o["kn"], 4, 128, 0, o["pos"], 1e-6, o["q"], 512, s)
+
+    def attention(self, s=None, **over):
+        o, kv = {k: over.get(k, v.ptr) for k, v in self.x.items()}, self.cache(self.src, over)
+        return self.gpu.lib.mlxr_k_paged_attention(ctypes.byref(kv), o["q"], 512, 4, 0, 0.1, o["out"], 512, over.get("weight_in", kv.weight), 1.0, o["work"],
+                                                   1 << 22, s)
+
+    def evict(self, s=None, **over):
+        to = {k[3:]: v for k, v in over.items() if k.startswith("to_")}
+        a, b = self.cache(self.src, over), self.cache(self.dst, to)
+        return self.gpu.lib.mlxr_k_paged_evict(ctypes.byref(a), ctypes.byref(b), 64, 4, 16, over.get("work", self.x["work"].ptr), 1 << 22, s)
+
+    def sample(self, s=None, **over):
+        o = {k: over.get(k, v.ptr) for k, v in self.y.items()}
+        return self.gpu.lib.mlxr_k_sample_rows(o["logits"], 3, 5000, 5000, o["t"], o["k"], o["p"], o["low"], o["u"], o["tokens"], o["status"], o["work"], 1 << 22, s)
+
+
+CACHE = ["k", "v", "table", "len", "weight", "position"]
+
+
+@pytest.mark.parametrize("call,names", [
+    ("append", CACHE + ["qkv", "inv", "qn", "kn", "pos", "q"]), ("attention", CACHE[:5] + ["q", "out", "weight_in", "work"]),
+    ("evict", CACHE + ["to_" + x for x in CACHE] + ["work"]), ("sample", ["logits", "t", "k", "p", "low", "u", "tokens", "status", "work"])])
+def test_host_memory_is_refused_everywhere(gpu, call, names):
+    """Pageable host memory as any one of a call's pointers: refused, and nothing is launched."""
+    c, host = Calls(gpu), np.zeros(1 << 20, np.uint8)
+    at = (host.ctypes.data + 255) & ~255
+    for name in names:
+        print(f"[case] {call} {name}", flush=True)
+        assert getattr(c, call)(**{name: at}) == -10, name
+    assert not host.any()
+    assert getattr(c, call)() == 0
+    gpu.synchronize()
+
+
+def test_pinned_memory_is_taken(gpu):
+    """Random numbers in pinned host memory give the tokens that they give on the device."""
+    c, hip = Calls(gpu), Hip(gpu)
+    gpu.check(c.sample())
+    gpu.synchronize()
+    want = c.y["tokens"].numpy()
+    p = ctypes.c_void_p()
+    hip("hipHostMalloc", ctypes.byref(p), ctypes.c_size_t(4096), 0)
+    u = c.y["u"].numpy()
+    ctypes.memmove(p, u.ctypes.data, u.nbytes)
+    c.y["tokens"].upload(np.full(3, -1, np.int32))
+    gpu.check(c.sample(u=p.value))
+    gpu.synchronize()
+    assert same(c.y["tokens"].numpy(), want)
+    hip("hipHostFree", p)
+
+
+def test_calls_captured_in_the_strictest_mode(gpu):
+    """Nothing that the calls ask of the runtime is forbidden in a capture of mode 'global'."""
+    c, hip = Calls(gpu), Hip(gpu)
+    s, graph, ex = hip.stream(), ctypes.c_void_p(), ctypes.c_void_p()
+    hip("hipStreamBeginCapture", s, 0)
+    rc = [getattr(c, n)(s=s) for n in ("append", "attention", "evict", "sample")]
+    hip("hipStreamEndCapture", s, ctypes.byref(graph))
+    assert rc == [0, 0, 0, 0]
+    hip("hipGraphInstantiate", ctypes.byref(ex), graph, None, None, ctypes.c_size_t(0))
+    for _ in range(3):
+        hip("hipGraphLaunch", ex, s)
+        hip.wait(s)
+    out, tokens = c.x["out"].numpy(), c.y["tokens"].numpy()
+    e = Calls(gpu)
+    for n in ("append", "attention", "evict", "sample"):
+        gpu.check(getattr(e, n)())
+    gpu.synchronize()
+    assert same(out, e.x["out"].numpy()) and same(tokens, e.y["tokens"].numpy())
+    hip("hipGraphExecDestroy", ex)
+    hip("hipStreamDestroy", s)
