@@ -7,9 +7,9 @@
 //   1. sample_groups_kernel, about a thousand workgroups: the maximum of every 64 logits. The one read of the logits that
 //      every row needs: 0.6 MB a row of 152 thousand, 37 us for 256 of them (4.2 TB/s), 3 us for one.
 //   2. sample_sums_kernel, for rows that ask for a sum over all their tokens (top-p, or nothing, without top-k). With the
-//      row's maximum known, tokens fall into 2048 bins of x = (max - v) / T, 64 to a unit: what lies behind x = 32 has
-//      no weight that counts (finer ones above a temperature of 1). Each bin's weights are added up, and each token's bin
-//      is written down. Bound by the 64-bit arithmetic and the adds in LDS: 27 us for 102 rows of 152 thousand; other rows
+//      row's maximum known, tokens fall into 2048 bins of x = (max - v) / T, 64 to a unit (finer ones above a temperature
+//      of 1), and what lies behind x = 32 into the last one. Each bin's weights are added up, and each token's bin is
+//      written down. Bound by the 64-bit arithmetic and the adds in LDS: 27 us for 102 rows of 152 thousand; other rows
 //      leave at once (2 us).
 //   3. sample_pick_kernel, one workgroup a row. A row with sums: the bins in which the sums cross are found, just their
 //      tokens are gathered (through the groups' maxima, or by the bin numbers where most groups qualify), ranked and
@@ -279,13 +279,14 @@ __host__ __device__ __forceinline__ bool sr_vec(const SampleRowsArgs& a) { retur
 
 // Bins: 64 to a unit of x at temperatures up to 1, and as many to a unit of the logits at those up to 8, where the bulk's
 // logits lie closer in x (at 3, two bins of 64 a unit may hold 3000 of 152 thousand tokens; one row with a top-p of 0.9 then
-// took 475 us through the radix descent, and takes 44). They end at x = 32 or, above 1, at 32 of the logits, behind which
-// tokens may have weight: `edge`. The row's numbers are in scalar registers: the last launch has no others to spare (14
-// vector registers spilled without; 38.7 and 38.1 us for 256 mixed rows).
+// took 475 us through the radix descent, and takes 44). Sums are kept of those up to x = 32 or, above 1, of the logits. Tokens
+// behind them have weight, up to x = 52 (`reach`): 2^20 tokens of e^-52 are less than 2^-54 of the sum. The row's numbers are
+// in scalar registers: the last launch has no others to spare (14 vector registers spilled without; 38.7 and 38.1 us for
+// 256 mixed rows).
 struct SrBins {
     double top, inv, width;   // the largest logit; bins per unit of logit, and the other way round
     double per, inv_per;      // bins per unit of x
-    bool edge;
+    int reach;                // the first bin whose tokens have no weight that counts
     __device__ __forceinline__ double x(float v) const { return (top - (double)v) * inv; }   // in bins; NaN or infinite outside
 };
 // A value that all lanes hold, in scalar registers.
@@ -296,7 +297,8 @@ __device__ __forceinline__ double sr_uniform(double v) {
 }
 __device__ __forceinline__ SrBins sr_bins(float top, float T, double inv_T) {
     const double per = T > 1.0f ? 64.0 * fmin((double)T, 8.0) : 64.0, inv_per = T > 1.0f ? fmax(inv_T, 0.125) / 64.0 : 1.0 / 64.0;
-    return SrBins{(double)top, sr_uniform(per * inv_T), sr_uniform((double)T * inv_per), sr_uniform(per), sr_uniform(inv_per), T > 1.0f};
+    return SrBins{(double)top, sr_uniform(per * inv_T), sr_uniform((double)T * inv_per), sr_uniform(per), sr_uniform(inv_per),
+                  __builtin_amdgcn_readfirstlane((int)(52.0 * per))};
 }
 // 2^43 exp(-y / per) for y = x - bin in [0, 1), rounded to a whole number: the Taylor sum to the fifth power is off by
 // 2^-45 at most; added to 2^52 it is rounded into the mantissa's low bits.
@@ -338,10 +340,13 @@ __global__ __launch_bounds__(256) void sample_groups_kernel(SampleRowsArgs a, Sr
     }
 }
 
-// The bins' sums of the rows that need them, several workgroups a row, and each token's bin.
-constexpr int SR_SUM_T = 512;
+// The bins' sums of the rows that need them, several workgroups a row, and each token's bin. What lies behind the last bin
+// goes to it (no sum may cross in it then): up to SR_WIDE bins are added up like the others (all that have weight, at
+// temperatures up to 1) and then as multiples of the last one's constant, tokens behind those one by one.
+constexpr int SR_SUM_T = 512, SR_WIDE = 52 * 64;
 __global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a, SrWork wk) {
-    __shared__ uint64_t hist[SR_BINS];
+    __shared__ uint64_t hist[SR_WIDE];
+    __shared__ double wave_tail[SR_SUM_T / 64];
     __shared__ float wave_top[SR_SUM_T / 64];
     const int row = blockIdx.y, tid = threadIdx.x;
     if (sr_ask(a, row).kind != SR_SUM) return;
@@ -349,7 +354,7 @@ __global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a,
     float top = -INFINITY;
 #pragma unroll 4
     for (int g = tid; g < wk.groups; g += SR_SUM_T) top = fmaxf(top, gload(gmax + g));
-    for (int i = tid; i < SR_BINS; i += SR_SUM_T) hist[i] = 0;
+    for (int i = tid; i < SR_WIDE; i += SR_SUM_T) hist[i] = 0;
     top = wave_max(top);
     if ((tid & 63) == 0) wave_top[tid >> 6] = top;
     __syncthreads();
@@ -375,25 +380,35 @@ __global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a,
             for (int e = 0; e < 4; e++) {
                 const double x = bins.x(v[k][e]);
                 bin[e] = 0xffffu;
-                if (x < (double)SR_BINS) {   // not NaN, not -infinity
+                if (x < (double)SR_WIDE) {   // not NaN, not -infinity
                     bin[e] = (uint32_t)(int)x;
                     atomicAdd(reinterpret_cast<unsigned long long*>(&hist[bin[e]]), (unsigned long long)sr_fixed(x, (int)bin[e], inv_per));
-                } else if (x < INFINITY) {
-                    far = bins.edge;
+                } else if (x < (double)bins.reach) {
+                    far = true;
                 }
             }
             const int at = i + 4 * SR_SUM_T * k;
             if (at < i1) *reinterpret_cast<uint2*>(out + at) = uint2{bin[0] | (bin[1] << 16), bin[2] | (bin[3] << 16)};
         }
     }
-    // what lies behind the bins goes to the last one (in which no sum may cross then)
+    __syncthreads();
+    double tail = 0.0;
+    for (int i = SR_BINS + tid; i < SR_WIDE; i += SR_SUM_T)
+        if (hist[i]) tail += exp((double)(SR_BINS - 1 - i) * inv_per) * (double)hist[i];
     if (far)
         for (int i = blockIdx.x * wk.sum_per * SR_GROUP + 4 * tid; i < i1; i += 4 * SR_SUM_T)
             for (int e = i; e < min(i + 4, i1); e++) {
                 const double x = bins.x(r.v[e]);
-                if (x >= (double)SR_BINS && x < INFINITY)
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&hist[SR_BINS - 1]), (unsigned long long)(exp(-(x - (SR_BINS - 1)) * inv_per) * SR_ONE + 0.5));
+                if (x >= (double)SR_WIDE && x < (double)bins.reach) tail += exp(((double)(SR_BINS - 1) - x) * inv_per) * SR_ONE;
             }
+    tail = wave_scan(tail);
+    if ((tid & 63) == 63) wave_tail[tid >> 6] = tail;
+    __syncthreads();
+    if (tid == 0) {
+        tail = 0.0;
+        for (int i = 0; i < SR_SUM_T / 64; i++) tail += wave_tail[i];
+        hist[SR_BINS - 1] += (uint64_t)(tail + 0.5);
+    }
     __syncthreads();
     uint64_t* mine = wk.mass + ((int64_t)row * wk.sum_spans + blockIdx.x) * SR_BINS;
     for (int i = tid; i < SR_BINS; i += SR_SUM_T) mine[i] = hist[i];
@@ -550,7 +565,7 @@ struct SrTeam {
         double x = bins.x(v), c = 1.0;
         // behind the bins: powers of the tables' last entry, until it is near enough or nothing is left
         for (; !(x < (double)SR_BINS); x -= 64.0 * 31) {
-            if (!(bins.edge && c > 0.0)) return 0.0;
+            if (!(c > 0.0)) return 0.0;
             c *= s.exp_whole[31];
         }
         const int bin = (int)x;
@@ -624,11 +639,11 @@ struct SrTeam {
         }
         __syncthreads();
     }
-    // The logits of bins b0 .. b1 lie in [lo, hi]; a few of the neighbouring bins may too. b1 SR_BINS: those behind the bins too.
+    // The logits of bins b0 .. b1 lie in [lo, hi]; a few of the neighbouring bins may too.
     __device__ __forceinline__ void range(int b0, int b1, float& lo, float& hi) const {
         const double top = bins.top, slack = fabs(top) * 0x1p-22 + 0x1p-120;
         const double l = top - (double)(b1 + 1) * bins.width, h = top - (double)b0 * bins.width;
-        lo = b1 == SR_BINS ? -3.402823466e38f : fmaxf((float)(l - fabs(l) * 0x1p-22 - slack), -3.402823466e38f);
+        lo = fmaxf((float)(l - fabs(l) * 0x1p-22 - slack), -3.402823466e38f);
         hi = (float)fmin(h + fabs(h) * 0x1p-22 + slack, top);
         if (!(hi <= (float)top)) hi = (float)top;   // T infinite: 0 times infinity
     }
@@ -666,36 +681,44 @@ struct SrTeam {
     }
 };
 
-// The bin down to which there are `want` groups, by their maxima; if there are fewer, the last one, or all tokens where
-// weight may lie behind it.
+// The bin down to which there are `want` groups, by their maxima. Where the bins of the tables hold fewer it is looked for
+// once more in wider ones, up to where no token has weight that counts: that is the answer if there are fewer still.
 __device__ __forceinline__ int sr_bin_of(SrTeam& t, int want) {
     SrPick& s = t.s;
     int* cnt = reinterpret_cast<int*>(s.list);
-    for (int i = t.tid; i < SR_BINS; i += SR_T) cnt[i] = 0;
-    if (t.tid == 0) s.found = t.bins.edge ? SR_BINS : SR_BINS - 1;
-    __syncthreads();
-    for (int g = t.tid; g < t.groups; g += SR_T) {
-        const double x = t.bins.x(t.group(g));
-        if (x < (double)SR_BINS) atomicAdd(&cnt[(int)x], 1);
-    }
-    __syncthreads();
-    int c[SR_PER], v = 0;
+    int shift = 0;
+#pragma unroll 1
+    while (true) {
+        for (int i = t.tid; i < SR_BINS; i += SR_T) cnt[i] = 0;
+        if (t.tid == 0) s.found = -1;
+        __syncthreads();
+        for (int g = t.tid; g < t.groups; g += SR_T) {
+            const double x = t.bins.x(t.group(g));
+            if (x < (double)t.bins.reach && ((int)x >> shift) < SR_BINS) atomicAdd(&cnt[(int)x >> shift], 1);
+        }
+        __syncthreads();
+        int c[SR_PER], v = 0;
 #pragma unroll
-    for (int h = 0; h < SR_PER; h++) v += c[h] = cnt[SR_PER * t.tid + h];
-    const int own = v;
-    v = wave_scan(v);
-    int* sums = s.wave_count[t.flip ^= 1][0];
-    if (t.lane == 63) sums[t.wave] = v;
-    __syncthreads();
-    v -= own;
-    for (int i = 0; i < t.wave; i++) v += sums[i];
+        for (int h = 0; h < SR_PER; h++) v += c[h] = cnt[SR_PER * t.tid + h];
+        const int own = v;
+        v = wave_scan(v);
+        int* sums = s.wave_count[t.flip ^= 1][0];
+        if (t.lane == 63) sums[t.wave] = v;
+        __syncthreads();
+        v -= own;
+        for (int i = 0; i < t.wave; i++) v += sums[i];
 #pragma unroll
-    for (int h = 0; h < SR_PER; h++) {
-        if (v < want && v + c[h] >= want) s.found = SR_PER * t.tid + h;
-        v += c[h];
+        for (int h = 0; h < SR_PER; h++) {
+            if (v < want && v + c[h] >= want) s.found = SR_PER * t.tid + h;
+            v += c[h];
+        }
+        __syncthreads();
+        const int found = s.found;
+        if (found >= 0) return ((found + 1) << shift) - 1;
+        if (shift) return t.bins.reach;
+        while ((t.bins.reach >> shift) >= SR_BINS) shift++;
+        __syncthreads();   // all have read what is written again
     }
-    __syncthreads();
-    return s.found;
 }
 
 __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrWork wk) {
@@ -748,14 +771,13 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
     } else {
         // Where the kept tokens end and the draw falls among them. One gather does for most rows, and a second one if
         // the draw falls in another bin than was guessed.
-        int also = -1, b0 = 0, b1 = SR_BINS - 1;
+        int also = -1, b0 = 0, b1 = t.bins.reach;
         int bp = SR_BINS, bm = SR_BINS;      // the bins in which top-p and min-p cut
         double p_goal = 0.0, kept = 0.0, before = 0.0, also_before = 0.0;
         double sums[SR_PER];                 // the bins' running sums, which the gathered tokens' take the place of
         bool drawing = false;                // the gathered bin is the draw's
         if (ask.kind == SR_TOP) {
             // all tokens down to a bin: that of the k-th largest group maximum, with min-p no further than its own
-            if (t.bins.edge) b1 = SR_BINS;
             if (r.V > SR_LIST) {
                 if (ask.k < r.V) b1 = sr_bin_of(t, ask.k);
                 if (ask.low > 0.0f && ask.p >= 1.0f) b1 = min(b1, (int)(-log((double)ask.low) * t.bins.per) + 1);
@@ -787,7 +809,7 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
             also_before = also > 0 ? s.run[also - 1] : 0.0;
         }
 #pragma unroll 1
-        while (!(t.bins.edge && b0 == SR_BINS - 1)) {   // a sum that crosses behind the bins
+        while (b0 < SR_BINS - 1) {   // else a sum crosses behind the bins
             const int n = t.gather(also, b0, b1);
             if (n > SR_LIST) {
                 if (also < 0) break;

@@ -1,11 +1,12 @@
 """The batch's decode step at its edges: infinities and NaN in cache and queries, appends to pages outside the pool,
-host memory in place of the device's. Helpers and tolerances are those of test_batch_gpu."""
+draws next to a border, host memory in place of the device's. Helpers and tolerances are those of test_batch_gpu."""
 import ctypes
 
 import numpy as np
 import pytest
 
-from test_batch_gpu import PAGE, Cache, Hip, attend, attention_reference, check_out, model_logits, queries, run_append, same, to_half, within
+from test_batch_gpu import (PAGE, Cache, Hip, attend, attention_reference, check_out, model_logits, queries, run_append, same, sample,
+                            to_half, within)
 
 pytestmark = pytest.mark.gpu
 INF = np.float32(np.inf)
@@ -183,6 +184,36 @@ def test_append_bad_pages_leave_everything(gpu):
     w, p = c.weight.copy(), c.position.copy()
     w[2, :, 2], p[2, :, 2] = 0, 2
     assert same(c.dw.numpy(), w) and same(c.dp.numpy(), p)
+
+
+# ------------------------------------------------------------------------------------------- sampling
+@pytest.mark.parametrize("V,t,far,k", [
+    (151936, 1.0, -33.0, None), (151936, 0.5, -17.5, None), (1 << 20, 1.0, -34.0, None), (151936, 1.0, -40.0, None),
+    (151936, 0.1, -3.5, None), (1 << 20, 3.0, -110.0, None), (1 << 20, 8.0, -280.0, None), (2000, 1.0, -33.0, None), (2000, 0.7, -23.0, 1500)])
+def test_sample_tail_counts(gpu, V, t, far, k):
+    """Two equal logits above a tail that weighs less than 2^-24 in all: half of the sum is more than the first's weight,
+    so a draw at 0.5 takes the second one. (The two weights are exact, and the tail's share is hundreds of steps of a
+    64-bit sum at least.)"""
+    print(f"[case] {V} {t} {far} {k}", flush=True)
+    tail = (min(k or V, V) - 2) * np.exp(far / float(np.float32(t)))
+    assert 2.0 ** -44 < tail < 2.0 ** -25
+    x = np.full((2, V), np.float32(far))
+    x[0, [7, V - 3]] = 0.0
+    x[1] = np.float32(far) - np.random.default_rng(V).random(V).astype(np.float32) * np.float32(0.5 * t)   # no two alike, most of them
+    x[1, [V // 2, V // 2 + 1]] = 0.0
+    assert list(sample(gpu, x, t, k, u=0.5)[0]) == [V - 3, V // 2 + 1]
+
+
+def test_sample_kept_tail_of_few_ranks(gpu):
+    """The same with 48 ranks of about e^-33 behind the two: their share, 2^-42, is more than a 64-bit sum's steps."""
+    V = 151936
+    for t, scale in ((1.0, 1.0), (0.1, 0.1), (0.02, 0.02)):
+        x = np.full((1, V), -2000.0, np.float32)
+        x[0, 100:148] = -np.float32(33 * scale) - np.arange(48, dtype=np.float32) * np.float32(0.01 * scale)
+        x[0, [5, 90000]] = 0.0
+        for k in (50, 40, 3, None):
+            assert list(sample(gpu, x, t, k, u=0.5)[0]) == [90000], (t, k)
+        assert list(sample(gpu, x, t, 2, u=0.5)[0]) == [5]
 
 
 # ------------------------------------------------------------------------------------------- memory
