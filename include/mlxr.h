@@ -363,8 +363,9 @@ int64_t mlxr_k_paged_evict_work(const mlxr_paged_kv* src, int budget);
  * [0, 1). A row's tokens are ranked by logit, equal ones by index; NaN and -infinity are never drawn. With
  * w = exp((logit - the largest) / temperature): the first top_k ranks are kept (0 or less: all), of these
  * those before the first with w < min_p, and the shortest prefix whose sum of w reaches top_p times that of the
- * top_k; at least one. The token is the first rank whose running sum reaches u times the kept sum: exact over
- * the whole vocabulary, w in 64 bits. temperature <= 0.001: the first rank. temperature [rows]; top_k, top_p,
+ * top_k; at least one. The token is the first rank whose running sum reaches u times the kept sum, over the whole
+ * vocabulary: each w is right to 2^-43 of itself (the largest is exact), their sums and targets to less, and what lies
+ * below e^-52 counts as nothing. temperature <= 0.001: the first rank. temperature [rows]; top_k, top_p,
  * min_p [rows] or NULL (off). status (or NULL): 0, or 1 where the largest logit is infinite or there is none:
  * the token is 0 then. V <= 1048576. The logits stay as they are. */
 int mlxr_k_sample_rows(const float* logits, int rows, int V, int64_t stride, const float* temperature, const int32_t* top_k,

@@ -29,10 +29,12 @@ __device__ __forceinline__ int64_t paged_slot(const PagedKV& kv, int b, int kvh,
 
 // Inclusive sums over a wave: within rows of 16 lanes, then the rows' last lanes on to the rows behind.
 template <int CTRL, int ROWS> __device__ __forceinline__ int lane_before(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
-template <int CTRL, int ROWS> __device__ __forceinline__ double lane_before(double v) {   // 0 where there is no lane before
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)lane_before<CTRL, ROWS>((int)(uint32_t)u), hi = (uint32_t)lane_before<CTRL, ROWS>((int)(uint32_t)(u >> 32));
-    return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t lane_before(uint64_t v) {   // 0 where there is no lane before
+    const uint32_t lo = (uint32_t)lane_before<CTRL, ROWS>((int)(uint32_t)v), hi = (uint32_t)lane_before<CTRL, ROWS>((int)(uint32_t)(v >> 32));
+    return (uint64_t)lo | ((uint64_t)hi << 32);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double lane_before(double v) {
+    return __builtin_bit_cast(double, lane_before<CTRL, ROWS>(__builtin_bit_cast(uint64_t, v)));
 }
 template <typename T> __device__ __forceinline__ T wave_scan(T v) {
     v += lane_before<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8

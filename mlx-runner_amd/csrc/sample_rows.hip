@@ -17,12 +17,16 @@
 //      these are gathered. Bound by what waits for what in one workgroup: 9 us for a top-k of 40, about 20 us where a cut lies
 //      among the bulk of the tokens (13 us to look through 152 thousand bin numbers).
 // A bin's weights are a constant times f in (exp(-1/64), 1], added as multiples of 2^-43: no order of the atomic adds
-// changes a result, and 2^20 of them stay below 2^63. Everything else is 64-bit floating point, so a token differs from
-// the exact sums' only if the draw is within about 2^-43 of a border.
-// Rows whose crossing bins hold too many tokens for the list (thousands of equal logits, top-k of thousands) take the
-// radix descent instead, which asks for no room: a histogram of the order keys' leading bits, the bin in which the sum
-// crosses, and again within that bin, until one key is left, whose tokens have one weight. Up to 15 passes of one
-// workgroup over the row: about 500 us for 152 thousand.
+// changes a result, and 2^20 of them stay below 2^63. So a weight is off by 2^-43 of itself at most (the largest logit's is
+// exact), and everything else is 64-bit floating point: a token differs from the exact sums' only if the draw, or a cut, is
+// within about 2^-42 of a border, as a share of the sum.
+// Rows whose tokens to be ranked are more than the list holds (2048) take the radix descent instead, which asks for no room: a
+// histogram of the order keys' leading bits, the bin in which the sum crosses, and again within that bin, until one key is
+// left, whose tokens have one weight. These are rows with a top-k of more than about one token in 64 (from 125 at a vocabulary
+// of 8000, 490 at 32000 and 1400 at 152 thousand with normally spread logits: the groups' maxima cannot tell the k-th), with
+// thousands of equal logits where a sum crosses, of a bulk so flat that a bin holds thousands (2^20 logits of deviation 2 at a
+// temperature of 1, 152 thousand from about 35), and sums that cross behind the bins. Up to 16 passes of one workgroup over
+// the row: 42 us for a top-k of 100 of 4097, 410 for 5000 of 152 thousand (580 with every cut), 2.7 ms for 40000 of 2^20.
 #include "batch.h"
 
 namespace mlxr {
@@ -39,13 +43,71 @@ __device__ __forceinline__ uint32_t sr_key(float v) {
 }
 __device__ __forceinline__ float sr_value(uint32_t k) { return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k); }
 
+// Bins: 64 to a unit of x at temperatures up to 1, and as many to a unit of the logits at those up to 8, where the bulk's
+// logits lie closer in x (at 3, two bins of 64 a unit may hold 3000 of 152 thousand tokens; one row with a top-p of 0.9 then
+// took 475 us through the radix descent, and takes 44). Sums are kept of those up to x = 32 or, above 1, of the logits. Tokens
+// behind them have weight, up to x = 52 (`reach`): 2^20 tokens of e^-52 are less than 2^-54 of the sum. The row's numbers are
+// in scalar registers: the last launch has no others to spare (14 vector registers spilled without; 38.7 and 38.1 us for
+// 256 mixed rows).
+struct SrBins {
+    double top, inv, width;   // the largest logit; bins per unit of logit, and the other way round
+    double per, inv_per;      // bins per unit of x
+    int reach;                // the first bin whose tokens have no weight that counts
+    __device__ __forceinline__ double x(float v) const { return (top - (double)v) * inv; }   // in bins; NaN or infinite outside
+};
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ double sr_uniform(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ SrBins sr_bins(float top, float T, double inv_T) {
+    const double per = T > 1.0f ? 64.0 * fmin((double)T, 8.0) : 64.0, inv_per = T > 1.0f ? fmax(inv_T, 0.125) / 64.0 : 1.0 / 64.0;
+    return SrBins{(double)top, sr_uniform(per * inv_T), sr_uniform((double)T * inv_per), sr_uniform(per), sr_uniform(inv_per),
+                  __builtin_amdgcn_readfirstlane((int)(52.0 * per))};
+}
+// 2^43 exp(-y / per) for y = x - bin in [0, 1), rounded to a whole number: the Taylor sum to the fifth power is off by
+// 2^-45 at most; added to 2^52 it is rounded into the mantissa's low bits.
+__device__ __forceinline__ uint64_t sr_fixed(double x, int bin, double inv_per) {
+    const double y = (x - (double)bin) * inv_per;
+    const double e = fma(y, fma(y, fma(y, fma(y, fma(y, -SR_ONE / 120, SR_ONE / 24), -SR_ONE / 6), SR_ONE / 2), -SR_ONE), SR_ONE);
+    return __builtin_bit_cast(uint64_t, e + 0x1p52) & 0xfffffffffffffull;
+}
+// exp(-64 i / per) and exp(-i / per): a bin's constant is one of each.
+struct SrTables { double whole[32], part[64]; };
+__device__ __forceinline__ double sr_constant(const SrTables& t, int bin) { return t.whole[bin >> 6] * t.part[bin & 63]; }
+// A logit's weight in units of 2^-43, as the bins' sums have it.
+__device__ __forceinline__ double sr_weight(const SrBins& bins, const SrTables& t, float v) {
+    double x = bins.x(v), c = 1.0;
+    if (!(x < (double)bins.reach)) return 0.0;
+    for (; x >= (double)SR_BINS; x -= 64.0 * 31) c *= t.whole[31];   // behind the bins: powers of the tables' last entry
+    const int bin = (int)x;
+    return c * sr_constant(t, bin) * (double)sr_fixed(x, bin, bins.inv_per);
+}
+
+// A sum of weights in the radix descent: multiples of 2^-43 and, beside them, of 2^-76. So no order of the atomic adds
+// changes it, and of 2^20 weights, at most 1 each, it loses 2^-56 at most.
+typedef unsigned __int128 sr_u128;
+constexpr double SR_LOW = 8589934592.0;   // 2^33
+struct SrMass {
+    uint64_t high, low;
+    __device__ __forceinline__ void add(SrMass m, uint32_t times = 1) { high += times * m.high; low += times * m.low; }
+    __device__ __forceinline__ sr_u128 sum() const { return ((sr_u128)high << 33) + low; }
+};
+
 struct SrRow {
     const float* v; int V;
     bool vec;           // 16-byte loads of four neighbours from indices divisible by four
-    float top;          // the largest logit
-    double inv;         // 1 / T
-    __device__ __forceinline__ double weight(float x) const { return exp(((double)x - (double)top) * inv); }
-    __device__ __forceinline__ uint64_t fixed(float x) const { return (uint64_t)(weight(x) * SR_ONE + 0.5); }
+};
+// Weights in the radix descent.
+struct SrScale {
+    SrBins bins;
+    const SrTables& t;
+    __device__ __forceinline__ double weight(float v) const { return sr_weight(bins, t, v); }
+    __device__ __forceinline__ SrMass fixed(float v) const {
+        const double w = weight(v), whole = floor(w);
+        return SrMass{(uint64_t)whole, (uint64_t)((w - whole) * SR_LOW)};
+    }
 };
 
 // Four neighbours from index i (divisible by four); -infinity behind the row.
@@ -67,114 +129,170 @@ __device__ __forceinline__ SrCut sr_min(SrCut a, SrCut b) {   // the shorter of 
 }
 
 struct SrShared {
-    uint64_t mass[SR_BINS];
+    uint64_t high[SR_BINS], low[SR_BINS];
     uint32_t count[SR_BINS];
-    uint64_t wmass[SR_W];
-    uint32_t wcount[SR_W], pick;
-    uint64_t above_mass; uint32_t above_count;
+    SrMass wmass[SR_W], above_mass;
+    uint64_t wsum[SR_W];
+    uint32_t wcount[SR_W], pick, above_count;
 };
 
 // Sum over the workgroup, to every thread.
 __device__ uint64_t sr_sum(uint64_t v, SrShared& sh) {
     for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.wmass[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) sh.wsum[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t t = 0;
-    for (int i = 0; i < SR_W; i++) t += sh.wmass[i];
+    for (int i = 0; i < SR_W; i++) t += sh.wsum[i];
     return t;
 }
 __device__ uint64_t sr_max(uint64_t v, SrShared& sh) {
     for (int o = 1; o < 64; o <<= 1) { const uint64_t p = __shfl_xor(v, o, 64); v = p > v ? p : v; }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.wmass[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) sh.wsum[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t t = 0;
-    for (int i = 0; i < SR_W; i++) t = sh.wmass[i] > t ? sh.wmass[i] : t;
+    for (int i = 0; i < SR_W; i++) t = sh.wsum[i] > t ? sh.wsum[i] : t;
     return t;
 }
 // The sum of the weights within a cut.
-__device__ uint64_t sr_mass(const SrRow& r, SrCut cut, SrShared& sh) {
-    uint64_t t = 0;
-    for (int i = threadIdx.x; i < r.V; i += SR_T) if (sr_key(r.v[i]) > cut.key) t += r.fixed(r.v[i]);
-    if (threadIdx.x == 0 && cut.n) t += cut.n * r.fixed(sr_value(cut.key));
-    return sr_sum(t, sh);
+__device__ sr_u128 sr_mass(const SrRow& r, const SrScale& sc, SrCut cut, SrShared& sh) {
+    SrMass t = {0, 0};
+    for (int i = threadIdx.x; i < r.V; i += SR_T) if (sr_key(r.v[i]) > cut.key) t.add(sc.fixed(r.v[i]));
+    if (threadIdx.x == 0 && cut.n) t.add(sc.fixed(sr_value(cut.key)), cut.n);
+    t.high = sr_sum(t.high, sh);
+    t.low = sr_sum(t.low, sh);
+    return t.sum();
 }
 
-// The shortest prefix of the cut's tokens whose count (by_mass false) or sum of weights reaches `target` (>= 1):
-// the whole cut if none does. *mass: its sum of weights.
-__device__ SrCut sr_descend(const SrRow& r, SrCut cut, bool by_mass, uint64_t target, SrShared& sh, uint64_t* mass) {
+// How many weights w reach `need`: the quotient rounded up, at least 1. The quotient of doubles is off by one at most.
+__device__ uint32_t sr_times(sr_u128 need, sr_u128 w) {
+    if (w == 0) return 1;
+    auto real = [](sr_u128 v) { return (double)(uint64_t)(v >> 64) * 0x1p64 + (double)(uint64_t)v; };
+    uint32_t n = (uint32_t)(real(need) / real(w));
+    while (n * w < need) n++;
+    while (n > 1 && (n - 1) * w >= need) n--;
+    return n ? n : 1;
+}
+
+// The order keys' bits that a level of the descent takes.
+struct SrLevel {
+    int shift; uint32_t bins;
+    __device__ __forceinline__ SrLevel(int level) : shift(level == 0 ? 21 : level == 1 ? 10 : 0), bins(level == 2 ? 1024 : 2048) {}
+    __device__ __forceinline__ uint32_t bin(uint32_t key) const { return (key >> shift) & (bins - 1); }
+};
+// What a wave's lanes at work on one key each add to its bin: lanes with one key (ties by the thousand) add once, as many adds
+// to one place would wait for each other. Calls add(times) in the lanes that do.
+template <typename F> __device__ __forceinline__ void sr_add(uint32_t k, F add) {
+    const uint64_t lanes = __ballot(true), equal = __ballot(k == (uint32_t)__builtin_amdgcn_readfirstlane((int)k));
+    const bool one = equal == lanes;
+    if (!one || (threadIdx.x & 63) == (unsigned)__builtin_ctzll(lanes)) add(one ? (uint32_t)__popcll(lanes) : 1u);
+}
+
+// The first k tokens (1 .. V - 1 of them), all of those above -infinity where there are fewer.
+__device__ SrCut sr_first(const SrRow& r, uint32_t k, SrShared& sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint32_t prefix = 0, mask = 0, above_count = 0;
-    uint64_t above_mass = 0;
-    const uint64_t edge = cut.n ? r.fixed(sr_value(cut.key)) : 0;   // the weight of the tokens at the cut's key
-    const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
-    for (int level = 0; level < 3; level++) {
-        const int shift = shifts[level];
-        const uint32_t bins = 1u << bits[level];
+    uint32_t prefix = 0, mask = 0, above = 0;
+#pragma unroll 1
+    for (int l = 0; l < 3; l++) {
+        const SrLevel level(l);
         __syncthreads();
-        for (int i = tid; i < SR_BINS; i += SR_T) { sh.mass[i] = 0; sh.count[i] = 0; }
+        for (int i = tid; i < SR_BINS; i += SR_T) sh.count[i] = 0;
         __syncthreads();
         for (int i = tid; i < r.V; i += SR_T) {
-            const float x = r.v[i];
-            const uint32_t k = sr_key(x);
-            if (k > cut.key && (k & mask) == prefix) {
-                const uint32_t bin = (k >> shift) & (bins - 1);
-                // lanes with one key (ties by the thousand) add once: as many adds to one place would wait for each other
-                const uint64_t lanes = __ballot(true), equal = __ballot(k == (uint32_t)__builtin_amdgcn_readfirstlane((int)k));
-                const bool one = equal == lanes;
-                const uint32_t times = one ? (uint32_t)__popcll(lanes) : 1u;
-                if (!one || lane == (int)__builtin_ctzll(lanes)) {
-                    atomicAdd(&sh.count[bin], times);
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[bin]), (unsigned long long)(times * r.fixed(x)));
-                }
-            }
+            const uint32_t key = sr_key(gload(r.v + i));
+            if (key > SR_MINUS_INF && (key & mask) == prefix) sr_add(key, [&](uint32_t times) { atomicAdd(&sh.count[level.bin(key)], times); });
+        }
+        __syncthreads();
+        // thread t has SR_PER bins from bins - 1 - SR_PER t down: sums of everything above by scans
+        const int b1 = (int)level.bins - 1 - SR_PER * tid;
+        int own = 0;
+#pragma unroll
+        for (int h = 0; h < SR_PER; h++) if (b1 - h >= 0) own += (int)sh.count[b1 - h];
+        const int c = wave_scan(own);
+        if (lane == 63) sh.wcount[wave] = (uint32_t)c;
+        __syncthreads();
+        uint32_t before = above + (uint32_t)(c - own), all = above;
+        for (int i = 0; i < SR_W; i++) {
+            if (i < wave) before += sh.wcount[i];
+            all += sh.wcount[i];
+        }
+        if (all < k) return SrCut{SR_MINUS_INF, 0};   // the first level's only
+        for (int h = 0; h < SR_PER && b1 - h >= 0; h++) {
+            const uint32_t with = before + sh.count[b1 - h];
+            if (before < k && with >= k) { sh.pick = (uint32_t)(b1 - h); sh.above_count = before; }
+            before = with;
+        }
+        __syncthreads();
+        prefix |= sh.pick << level.shift; mask |= (level.bins - 1) << level.shift;
+        above = sh.above_count;
+    }
+    return SrCut{prefix, k - above};
+}
+
+// The shortest prefix of the cut's tokens whose sum of weights reaches `target` (>= 1): the whole cut if none does. *mass: its
+// sum of weights.
+__device__ SrCut sr_descend(const SrRow& r, const SrScale& sc, SrCut cut, sr_u128 target, SrShared& sh, sr_u128* mass) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t prefix = 0, mask = 0;
+    SrMass above = {0, 0};
+    const SrMass edge = cut.n ? sc.fixed(sr_value(cut.key)) : SrMass{0, 0};   // the weight of the tokens at the cut's key
+    auto bin_mass = [&](int i) { return SrMass{sh.high[i], sh.low[i]}; };
+#pragma unroll 1
+    for (int l = 0; l < 3; l++) {
+        const SrLevel level(l);
+        __syncthreads();
+        for (int i = tid; i < SR_BINS; i += SR_T) { sh.high[i] = 0; sh.low[i] = 0; }
+        __syncthreads();
+        for (int i = tid; i < r.V; i += SR_T) {
+            const float x = gload(r.v + i);
+            const uint32_t key = sr_key(x);
+            if (key > cut.key && (key & mask) == prefix)
+                sr_add(key, [&](uint32_t times) {
+                    const SrMass m = sc.fixed(x);
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.high[level.bin(key)]), (unsigned long long)(times * m.high));
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&sh.low[level.bin(key)]), (unsigned long long)(times * m.low));
+                });
         }
         __syncthreads();
         if (tid == 0 && cut.n && (cut.key & mask) == prefix) {
-            const uint32_t bin = (cut.key >> shift) & (bins - 1);
-            sh.count[bin] += cut.n;
-            sh.mass[bin] += cut.n * edge;
+            const uint32_t bin = level.bin(cut.key);
+            sh.high[bin] += cut.n * edge.high;
+            sh.low[bin] += cut.n * edge.low;
         }
         if (tid == 0) { sh.pick = 0xffffffffu; }
         __syncthreads();
-        // thread t has SR_PER bins from bins - 1 - SR_PER t down: sums of everything above by scans
-        const int b1 = (int)bins - 1 - SR_PER * tid;
-        uint32_t c = 0;
-        uint64_t m = 0;
+        const int b1 = (int)level.bins - 1 - SR_PER * tid;
+        SrMass own = {0, 0};
 #pragma unroll
-        for (int h = 0; h < SR_PER; h++) if (b1 - h >= 0) { c += sh.count[b1 - h]; m += sh.mass[b1 - h]; }
-        const uint32_t own_c = c;
-        const uint64_t own_m = m;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t c2 = __shfl_up(c, o, 64);
-            const uint64_t m2 = __shfl_up(m, o, 64);
-            if (lane >= o) { c += c2; m += m2; }
-        }
-        if (lane == 63) { sh.wcount[wave] = c; sh.wmass[wave] = m; }
+        for (int h = 0; h < SR_PER; h++) if (b1 - h >= 0) own.add(bin_mass(b1 - h));
+        const SrMass m = {wave_scan(own.high), wave_scan(own.low)};
+        if (lane == 63) sh.wmass[wave] = m;
         __syncthreads();
-        uint32_t ca = above_count + c - own_c, call = above_count;
-        uint64_t ma = above_mass + m - own_m, mall = above_mass;
+        SrMass before = above, all = above;
+        before.add(m);
+        before.high -= own.high; before.low -= own.low;
+#pragma unroll 4
         for (int i = 0; i < SR_W; i++) {
-            if (i < wave) { ca += sh.wcount[i]; ma += sh.wmass[i]; }
-            call += sh.wcount[i]; mall += sh.wmass[i];
+            if (i < wave) before.add(sh.wmass[i]);
+            all.add(sh.wmass[i]);
         }
-        if (level == 0 && (by_mass ? mall : (uint64_t)call) < target) { *mass = mall; return cut; }
+        if (l == 0 && all.sum() < target) { *mass = all.sum(); return cut; }
+#pragma unroll 1
         for (int h = 0; h < SR_PER && b1 - h >= 0; h++) {   // one bin of one thread: sums only grow
-            const uint32_t cb = sh.count[b1 - h];
-            const uint64_t mb = sh.mass[b1 - h], s0 = by_mass ? ma : ca, s1 = s0 + (by_mass ? mb : cb);
-            if (s0 < target && s1 >= target) { sh.pick = (uint32_t)(b1 - h); sh.above_count = ca; sh.above_mass = ma; }
-            ca += cb; ma += mb;
+            SrMass with = before;
+            with.add(bin_mass(b1 - h));
+            if (before.sum() < target && with.sum() >= target) { sh.pick = (uint32_t)(b1 - h); sh.above_mass = before; }
+            before = with;
         }
         __syncthreads();
-        prefix |= sh.pick << shift; mask |= (bins - 1) << shift;
-        above_count = sh.above_count; above_mass = sh.above_mass;
+        prefix |= sh.pick << level.shift; mask |= (level.bins - 1) << level.shift;
+        above = sh.above_mass;
     }
-    const uint64_t w = r.fixed(sr_value(prefix));
-    uint64_t need = target - (by_mass ? above_mass : (uint64_t)above_count);
-    if (by_mass) need = w ? (need + w - 1) / w : 1;
-    *mass = above_mass + need * w;
-    return SrCut{prefix, (uint32_t)need};
+    const sr_u128 w = sc.fixed(sr_value(prefix)).sum();
+    const uint32_t need = sr_times(target - above.sum(), w);
+    *mass = above.sum() + need * w;
+    return SrCut{prefix, need};
 }
 
 // The index of the n-th (from 1) token with this key.
@@ -203,30 +321,38 @@ __device__ int sr_nth(const SrRow& r, uint32_t key, uint32_t n, SrShared& sh) {
     return (int)sh.pick;
 }
 
-// A target a fraction of a sum: the least whole number not below it, at least 1.
-__device__ __forceinline__ uint64_t sr_target(double share, uint64_t sum) {
-    const double t = ceil(share * (double)sum);
-    if (!(t >= 1.0)) return 1;
-    return t >= (double)sum ? sum : (uint64_t)t;
+// A target a fraction of a sum: the least whole number not below it, at least 1. The fraction is 24 bits over a power of two,
+// a sum less than 2^97.
+__device__ __forceinline__ sr_u128 sr_target(float share, sr_u128 sum) {
+    if (!(share > 0.0f)) return 1;
+    if (share >= 1.0f) return sum;
+    int e;
+    const uint32_t bits = (uint32_t)(frexpf(share, &e) * 16777216.0f);
+    const int down = 24 - e;
+    if (down > 126) return 1;
+    const sr_u128 t = (sum * bits + (((sr_u128)1 << down) - 1)) >> down;
+    return t > 0 ? t : 1;
 }
 
 // The radix descent over a whole row: any parameters, one workgroup. A call of its own: its code is as long as all the rest.
-__device__ __noinline__ int sr_descent_token(const float* v, int V, float largest, double inv, int k, float p, float low, float given, SrShared& sh) {
+__device__ __noinline__ int sr_descent_token(const float* v, int V, float largest, float T, const SrTables& tables, int k, float p, float low,
+                                             float given, SrShared& sh) {
     const int tid = threadIdx.x;
-    const SrRow r{v, V, false, largest, inv};
+    const SrRow r{v, V, false};
+    const SrScale sc{sr_bins(largest, T, 1.0 / (double)T), tables};
     const uint32_t top = sr_key(largest);
-    uint64_t mass = 0, kept_mass = 0;
+    sr_u128 mass = 0, kept_mass = 0;
     SrCut cut{SR_MINUS_INF, 0};
-    if (k < r.V) cut = sr_descend(r, cut, false, (uint64_t)k, sh, &mass);
-    else mass = sr_mass(r, cut, sh);
+    if (k < r.V) cut = sr_first(r, (uint32_t)k, sh);
+    mass = sr_mass(r, sc, cut, sh);
     SrCut end = cut;
     kept_mass = mass;
-    if (p < 1.0f) end = sr_descend(r, cut, true, sr_target((double)p, mass), sh, &kept_mass);
+    if (p < 1.0f) end = sr_descend(r, sc, cut, sr_target(p, mass), sh, &kept_mass);
     if (low > 0.0f) {
         uint64_t least = 0;   // the complement of the smallest key that stays
         for (int i = tid; i < r.V; i += SR_T) {
             const uint32_t key = sr_key(r.v[i]);
-            if (key > SR_MINUS_INF && r.weight(r.v[i]) >= (double)low) { const uint64_t c = (uint32_t)~key; least = c > least ? c : least; }
+            if (key > SR_MINUS_INF && sc.weight(r.v[i]) >= (double)low * SR_ONE) { const uint64_t c = (uint32_t)~key; least = c > least ? c : least; }
         }
         least = sr_max(least, sh);
         const SrCut by = least ? SrCut{~(uint32_t)least, 0xffffffffu} : SrCut{top, 1u};
@@ -238,11 +364,11 @@ __device__ __noinline__ int sr_descent_token(const float* v, int V, float larges
                 for (int i = tid; i < r.V; i += SR_T) c += sr_key(r.v[i]) == end.key;
                 end.n = (uint32_t)sr_sum(c, sh);
             }
-            kept_mass = sr_mass(r, end, sh);
+            kept_mass = sr_mass(r, sc, end, sh);
         }
     }
-    uint64_t unused;
-    const SrCut at = sr_descend(r, end, true, sr_target((double)given, kept_mass), sh, &unused);
+    sr_u128 unused;
+    const SrCut at = sr_descend(r, sc, end, sr_target(given, kept_mass), sh, &unused);
     return sr_nth(r, at.key, at.n, sh);
 }
 
@@ -276,37 +402,6 @@ __device__ __forceinline__ SrAsk sr_ask(const SampleRowsArgs& a, int row) {
 }
 
 __host__ __device__ __forceinline__ bool sr_vec(const SampleRowsArgs& a) { return a.stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0; }
-
-// Bins: 64 to a unit of x at temperatures up to 1, and as many to a unit of the logits at those up to 8, where the bulk's
-// logits lie closer in x (at 3, two bins of 64 a unit may hold 3000 of 152 thousand tokens; one row with a top-p of 0.9 then
-// took 475 us through the radix descent, and takes 44). Sums are kept of those up to x = 32 or, above 1, of the logits. Tokens
-// behind them have weight, up to x = 52 (`reach`): 2^20 tokens of e^-52 are less than 2^-54 of the sum. The row's numbers are
-// in scalar registers: the last launch has no others to spare (14 vector registers spilled without; 38.7 and 38.1 us for
-// 256 mixed rows).
-struct SrBins {
-    double top, inv, width;   // the largest logit; bins per unit of logit, and the other way round
-    double per, inv_per;      // bins per unit of x
-    int reach;                // the first bin whose tokens have no weight that counts
-    __device__ __forceinline__ double x(float v) const { return (top - (double)v) * inv; }   // in bins; NaN or infinite outside
-};
-// A value that all lanes hold, in scalar registers.
-__device__ __forceinline__ double sr_uniform(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
-    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-}
-__device__ __forceinline__ SrBins sr_bins(float top, float T, double inv_T) {
-    const double per = T > 1.0f ? 64.0 * fmin((double)T, 8.0) : 64.0, inv_per = T > 1.0f ? fmax(inv_T, 0.125) / 64.0 : 1.0 / 64.0;
-    return SrBins{(double)top, sr_uniform(per * inv_T), sr_uniform((double)T * inv_per), sr_uniform(per), sr_uniform(inv_per),
-                  __builtin_amdgcn_readfirstlane((int)(52.0 * per))};
-}
-// 2^43 exp(-y / per) for y = x - bin in [0, 1), rounded to a whole number: the Taylor sum to the fifth power is off by
-// 2^-45 at most; added to 2^52 it is rounded into the mantissa's low bits.
-__device__ __forceinline__ uint64_t sr_fixed(double x, int bin, double inv_per) {
-    const double y = (x - (double)bin) * inv_per;
-    const double e = fma(y, fma(y, fma(y, fma(y, fma(y, -SR_ONE / 120, SR_ONE / 24), -SR_ONE / 6), SR_ONE / 2), -SR_ONE), SR_ONE);
-    return __builtin_bit_cast(uint64_t, e + 0x1p52) & 0xfffffffffffffull;
-}
 
 // Per 64 logits the maximum (NaN ignored). A lane has four neighbours, 16 lanes a group.
 template <bool VEC>
@@ -361,7 +456,7 @@ __global__ __launch_bounds__(SR_SUM_T) void sample_sums_kernel(SampleRowsArgs a,
 #pragma unroll
     for (int i = 0; i < SR_SUM_T / 64; i++) top = fmaxf(top, wave_top[i]);
     if (!isfinite(top)) return;
-    const SrRow r{a.logits + (int64_t)row * a.stride, a.V, sr_vec(a), top, 0.0};
+    const SrRow r{a.logits + (int64_t)row * a.stride, a.V, sr_vec(a)};
     const SrBins bins = sr_bins(top, a.temperature[row], 1.0 / (double)a.temperature[row]);
     const double inv_per = bins.inv_per;
     bool far = false;
@@ -425,7 +520,6 @@ struct SrPick {
         uint16_t ids[SR_MAXGROUPS];   // while tokens are gathered, before they are ranked
     };
     float gmax[SR_NEAR];
-    double exp_whole[32], exp_part[64];   // exp(-64 i / per), exp(-i / per)
     double wave_sum[2][SR_W];
     int wave_count[2][4][SR_W];
     float wave_top[SR_W];
@@ -441,7 +535,7 @@ __device__ __forceinline__ void sr_collect(const float* v, int V, bool vec, cons
                                            uint64_t* list, int* n) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t before = lane ? ~0ull >> (64 - lane) : 0ull;
-    const SrRow r{v, V, vec, 0.0f, 0.0};
+    const SrRow r{v, V, vec};
 #pragma unroll 1
     for (int i = 4 * wave; i < count; i += 4 * SR_W * UN) {
         float x[UN][4];
@@ -552,6 +646,7 @@ __device__ __noinline__ void sr_rank_many(uint64_t* list, uint64_t* ranked, int 
 // each needs one barrier: a place is written again only behind the next one's.
 struct SrTeam {
     SrPick& s;
+    const SrTables& tables;
     const SrRow& r;
     SrBins bins;
     const float* gmax; int groups;
@@ -559,18 +654,8 @@ struct SrTeam {
     int tid, lane, wave, flip;
 
     __device__ __forceinline__ float group(int g) const { return g < SR_NEAR ? s.gmax[g] : gmax[g]; }
-    // A bin's constant, and a logit's weight in units of 2^-43, as the bins' sums have it.
-    __device__ __forceinline__ double constant(int bin) const { return s.exp_whole[bin >> 6] * s.exp_part[bin & 63]; }
-    __device__ __forceinline__ double weight(float v) const {
-        double x = bins.x(v), c = 1.0;
-        // behind the bins: powers of the tables' last entry, until it is near enough or nothing is left
-        for (; !(x < (double)SR_BINS); x -= 64.0 * 31) {
-            if (!(c > 0.0)) return 0.0;
-            c *= s.exp_whole[31];
-        }
-        const int bin = (int)x;
-        return c * constant(bin) * (double)sr_fixed(x, bin, bins.inv_per);
-    }
+    __device__ __forceinline__ double constant(int bin) const { return sr_constant(tables, bin); }
+    __device__ __forceinline__ double weight(float v) const { return sr_weight(bins, tables, v); }
     __device__ __forceinline__ float ranked(int i) const { return sr_value((uint32_t)(s.ranked[i] >> 32)); }
     __device__ __forceinline__ int token(int i) const { return (int)~(uint32_t)s.ranked[i]; }
 
@@ -723,6 +808,7 @@ __device__ __forceinline__ int sr_bin_of(SrTeam& t, int want) {
 
 __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrWork wk) {
     __shared__ union { SrShared sh; SrPick pick; } u;
+    __shared__ SrTables tables;
     SrPick& s = u.pick;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* gmax = wk.gmax + (int64_t)row * wk.groups;
@@ -736,12 +822,11 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
     r.v = a.logits + (int64_t)row * a.stride;
     r.V = a.V;
     r.vec = sr_vec(a);
-    r.inv = 1.0 / (double)T;
-    SrTeam t{s, r, sr_bins(0.0f, T, r.inv), gmax, wk.groups, ask.kind == SR_SUM ? wk.bin + (int64_t)row * wk.groups * SR_GROUP : nullptr, tid, lane, wave, 0};
+    SrTeam t{s, tables, r, sr_bins(0.0f, T, 1.0 / (double)T), gmax, wk.groups, ask.kind == SR_SUM ? wk.bin + (int64_t)row * wk.groups * SR_GROUP : nullptr, tid, lane, wave, 0};
     if (wave < 2) {
         const double e = exp((wave ? -64.0 * (double)(lane & 31) : (double)-lane) * t.bins.inv_per);
-        if (!wave) s.exp_part[lane] = e;
-        else if (lane < 32) s.exp_whole[lane] = e;
+        if (!wave) tables.part[lane] = e;
+        else if (lane < 32) tables.whole[lane] = e;
     }
     float top = -INFINITY;
 #pragma unroll
@@ -757,7 +842,6 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
         if (tid == 0) { a.tokens[row] = 0; if (a.status) a.status[row] = 1; }
         return;
     }
-    r.top = top;
     t.bins.top = sr_uniform((double)top);
     double goal = (double)given;
     goal = goal > 0.0 ? (goal < 1.0 ? goal : 1.0) : 0.0;
@@ -862,7 +946,7 @@ __global__ __launch_bounds__(SR_T) void sample_pick_kernel(SampleRowsArgs a, SrW
     }
     if (token < 0) {
         __syncthreads();
-        token = sr_descent_token(r.v, r.V, r.top, r.inv, ask.k, ask.p, ask.low, given, u.sh);
+        token = sr_descent_token(r.v, r.V, top, T, tables, ask.k, ask.p, ask.low, given, u.sh);
     }
     if (tid == 0) { a.tokens[row] = token; if (a.status) a.status[row] = 0; }
 }

@@ -187,9 +187,50 @@ def test_append_bad_pages_leave_everything(gpu):
 
 
 # ------------------------------------------------------------------------------------------- sampling
+STEP = 2.0 ** -43   # what a weight may be off by, of itself; the largest logit's is exact
+
+
+def tokens_next_to(v, t, k, p, low, u):
+    """The tokens that may come where every sum may be off by 2^-42 of itself (twice what the weights in it are)."""
+    v = np.asarray(v, np.float64)
+    idx = np.nonzero(~np.isnan(v) & (v != -np.inf))[0]
+    order = idx[np.lexsort((idx, -v[idx]))]
+    if not t > 0.001:
+        return {int(order[0])}
+    if k is not None and k > 0:
+        order = order[:k]
+    w = np.exp((v[order] - v[order[0]]) / float(np.float32(t))) if np.isfinite(t) else np.ones(len(order))
+    run = np.cumsum(w.astype(np.longdouble))
+    ends = {len(w)}
+    if p is not None and p < 1:
+        goal = np.longdouble(float(np.float32(p))) * run[-1]
+        ends = {max(1, min(len(w), int(np.searchsorted(run, goal * (1 + e))) + 1)) for e in (-2 * STEP, 0, 2 * STEP)}
+    if low is not None and low > 0:
+        ends = {max(1, min(e, int((w >= float(np.float32(low)) * (1 + d)).sum()))) for e in ends for d in (-2 * STEP, 0, 2 * STEP)}
+    may = set()
+    for e in ends:
+        goal = np.longdouble(float(np.float32(u))) * run[e - 1]
+        first, last = (min(e - 1, int(np.searchsorted(run[:e], goal * (1 + d)))) for d in (-2 * STEP, 2 * STEP))
+        may.update(int(i) for i in order[first:last + 1])
+    return may
+
+
+def check_near(gpu, x, t, k=None, p=None, low=None, u=None):
+    tok, st = sample(gpu, x, t, k, p, low, u)
+    at = lambda y, r: None if y is None else (y[r] if np.ndim(y) else y)  # noqa: E731
+    doubtful = 0
+    for r in range(x.shape[0]):
+        may = tokens_next_to(x[r], at(t, r), at(k, r), at(p, r), at(low, r), at(u, r))
+        assert int(tok[r]) in may, (r, int(tok[r]), sorted(may)[:9], t, k, p, low, at(u, r))
+        doubtful += len(may) > 1
+    assert not st.any()
+    return doubtful
+
+
 @pytest.mark.parametrize("V,t,far,k", [
     (151936, 1.0, -33.0, None), (151936, 0.5, -17.5, None), (1 << 20, 1.0, -34.0, None), (151936, 1.0, -40.0, None),
-    (151936, 0.1, -3.5, None), (1 << 20, 3.0, -110.0, None), (1 << 20, 8.0, -280.0, None), (2000, 1.0, -33.0, None), (2000, 0.7, -23.0, 1500)])
+    (151936, 0.1, -3.5, None), (1 << 20, 3.0, -110.0, None), (1 << 20, 8.0, -280.0, None), (2000, 1.0, -33.0, None), (2000, 0.7, -23.0, 1500),
+    (151936, 1.0, -33.0, 2000), (151936, 1.0, -33.0, 100000), (151936, 1.0, -36.0, 100000), (30000, 0.25, -8.25, 400)])
 def test_sample_tail_counts(gpu, V, t, far, k):
     """Two equal logits above a tail that weighs less than 2^-24 in all: half of the sum is more than the first's weight,
     so a draw at 0.5 takes the second one. (The two weights are exact, and the tail's share is hundreds of steps of a
@@ -214,6 +255,36 @@ def test_sample_kept_tail_of_few_ranks(gpu):
         for k in (50, 40, 3, None):
             assert list(sample(gpu, x, t, k, u=0.5)[0]) == [90000], (t, k)
         assert list(sample(gpu, x, t, 2, u=0.5)[0]) == [5]
+
+
+@pytest.mark.parametrize("V", [4097, 151936, 1 << 20])
+def test_sample_next_to_a_border(gpu, V):
+    """Tokens against sums that may be off by 2^-42 of themselves only, at temperatures from 0.02 to 20."""
+    print(f"[case] V={V}", flush=True)
+    rs = np.random.default_rng(V + 1)
+    x = model_logits(rs, 4, V)
+    x[3] = np.round(x[3] * 4) / 4                     # thousands of equal ones
+    doubtful = 0
+    for t in (0.02, 0.1, 0.3, 0.7, 1.0, 1.9, 6.0, 20.0):
+        u = rs.random(4).astype(np.float32)
+        for k, p, low in [(40, 0.95, None), (None, None, None), (None, 0.9, None), (3000, None, None), (None, 0.999, 1e-6), (None, None, 1e-9)]:
+            doubtful += check_near(gpu, x, t, k, p, low, u)
+    assert doubtful <= 2
+
+
+def test_sample_ties_of_little_weight(gpu):
+    """Half a million equal logits of 1e-9 of the largest's weight each and as many of 7e-10: the draw next to 1 falls among
+    the last 100 of them, on a token that the sums to 2^-42 decide."""
+    V = 1 << 20
+    x = np.full((2, V), np.float32(-20.7))
+    x[:, ::2] = np.float32(-21.1)
+    x[0, 12345] = 0.0
+    x[1, [3, 777, 5000]] = 0.0
+    assert check_near(gpu, x, 1.0, u=1 - 2.0 ** -24) == 0
+    for u in (0.9996, 0.99925):                       # among the others: their weights' own error would count thousandfold
+        assert check_near(gpu, x, 1.0, u=u) == 0
+    assert check_near(gpu, x * np.float32(2), 2.0, k=1000000, u=1 - 2.0 ** -24) == 0
+    assert check_near(gpu, x, 1.0, p=1 - 2.0 ** -23, u=1 - 2.0 ** -22) == 0
 
 
 # ------------------------------------------------------------------------------------------- memory
