@@ -1,11 +1,11 @@
 """The batch's decode step at its edges: infinities and NaN in cache and queries, appends to pages outside the pool,
-draws next to a border, host memory in place of the device's. Helpers and tolerances are those of test_batch_gpu."""
+the order of NaN weights, draws next to a border, host memory in place of the device's. Helpers and tolerances are those of test_batch_gpu."""
 import ctypes
 
 import numpy as np
 import pytest
 
-from test_batch_gpu import (PAGE, Cache, Hip, attend, attention_reference, check_out, model_logits, queries, run_append, same, sample,
+from test_batch_gpu import (PAGE, Cache, Hip, attend, attention_reference, check_out, evict, model_logits, pair, queries, run_append, same, sample,
                             to_half, within)
 
 pytestmark = pytest.mark.gpu
@@ -184,6 +184,48 @@ def test_append_bad_pages_leave_everything(gpu):
     w, p = c.weight.copy(), c.position.copy()
     w[2, :, 2], p[2, :, 2] = 0, 2
     assert same(c.dw.numpy(), w) and same(c.dp.numpy(), p)
+
+
+# ------------------------------------------------------------------------------------------- eviction
+def heaviest(w, n, budget, sink, window):
+    """The kept slots: NaN below -infinity, equal ones by slot."""
+    if n <= budget:
+        return np.arange(n)
+    mid = np.arange(sink, n - window)
+    nan = np.isnan(w[mid])
+    mid = mid[np.lexsort((mid, -np.where(nan, 0, w[mid]).astype(np.float64), nan))][:budget - sink - window]
+    return np.sort(np.concatenate([np.arange(sink), mid, np.arange(n - window, n)])).astype(int)
+
+
+@pytest.mark.parametrize("budget,sink,window", [(100, 4, 32), (64, 0, 0), (260, 1, 9)])
+def test_evict_nan_and_minus_infinity(gpu, budget, sink, window):
+    """Cuts that fall among NaN weights (the lower slot stays), among those of -infinity, and between the two."""
+    lens = [500, 500, 500, 300]
+    src, dst = pair(gpu, lens, 2, 64, 0, budget, seed=81)
+    room = budget - sink - window
+    rs = np.random.default_rng(82)
+    src.weight[0] = np.nan                                              # nothing else
+    src.weight[1] = np.where(rs.random(src.weight[1].shape) < 0.5, np.nan, -INF)
+    for h in range(2):                                                  # so many numbers above -infinity and NaN
+        for b, above in ((2, room // 2), (3, 0)):
+            n = lens[b]
+            w = np.full(src.stride, np.nan, np.float32)
+            order = rs.permutation(np.arange(sink, n - window))
+            w[order[:above]] = rs.standard_normal(above)
+            w[order[above:room]] = -INF                                 # the cut lies between these and NaN
+            if h:
+                w[order[above + 1:above + 2]] = np.nan                  # one too few: a NaN stays
+            src.weight[b, h] = w
+    src.up(), dst.up()
+    k0 = src.k.copy()
+    evict(gpu, src, dst, budget, sink, window)
+    pos = dst.dp.numpy()
+    for b, n in enumerate(lens):
+        for h in range(2):
+            kept = heaviest(src.weight[b, h, :n], n, budget, sink, window)
+            assert same(pos[b, h, :len(kept)], src.position[b, h, kept]), (b, h)
+            j = np.arange(len(kept))
+            assert same(src.dk.numpy()[dst.table[b, j // PAGE], h, j % PAGE], k0[src.table[b, kept // PAGE], h, kept % PAGE])
 
 
 # ------------------------------------------------------------------------------------------- sampling
