@@ -352,9 +352,9 @@ int64_t mlxr_k_paged_attention_work(const mlxr_paged_kv* kv, int nH);
  * `window`, and of those between the budget - sink - window with the largest src->weight (equal: the lower slot;
  * NaN lowest), for each KV head on its own; a sequence of at most `budget` slots whole. Keys and values go
  * to dst's pages, which may be in the same pool but must be pages that no sequence of src uses; weights
- * (src->weight is required) and positions to dst's arrays where dst has them; dst->len is written. What lies
- * behind the new length stays as it was. src and dst have the same B, nKV, D and st; their len, weight and
- * position arrays are different ones. */
+ * (src->weight is required) and positions to dst's arrays where dst has them, whatever page their slot lies in;
+ * dst->len is written. What lies behind the new length stays as it was. src and dst have the same B, nKV, D and
+ * st; their len, weight and position arrays are different ones. */
 int mlxr_k_paged_evict(const mlxr_paged_kv* src, const mlxr_paged_kv* dst, int budget, int sink, int window, void* work,
                        size_t work_bytes, void* stream);
 int64_t mlxr_k_paged_evict_work(const mlxr_paged_kv* src, int budget);

@@ -9,8 +9,9 @@
 //   2. sample_sums_kernel, for rows that ask for a sum over all their tokens (top-p, or nothing, without top-k). With the
 //      row's maximum known, tokens fall into 2048 bins of x = (max - v) / T, 64 to a unit (finer ones above a temperature
 //      of 1), and what lies behind x = 32 into the last one. Each bin's weights are added up, and each token's bin is
-//      written down. Bound by the 64-bit arithmetic and the adds in LDS: 27 us for 102 rows of 152 thousand; other rows
-//      leave at once (2 us).
+//      written down. 27 us for 102 rows of 152 thousand, in which no unit is busy: of the waves' cycles half go by waiting
+//      for memory or a barrier and a quarter waiting to issue, LDS is in use a sixth of the time, most of it for bank
+//      conflicts; there are three workgroups a CU and each is a chain of two dependent reads. Other rows leave at once (2 us).
 //   3. sample_pick_kernel, one workgroup a row. A row with sums: the bins in which the sums cross are found, just their
 //      tokens are gathered (through the groups' maxima, or by the bin numbers where most groups qualify), ranked and
 //      walked. A row without: the groups' maxima give a bin down to which there are k tokens or more, or min-p does, and
@@ -26,7 +27,7 @@
 // of 8000, 490 at 32000 and 1400 at 152 thousand with normally spread logits: the groups' maxima cannot tell the k-th), with
 // thousands of equal logits where a sum crosses, of a bulk so flat that a bin holds thousands (2^20 logits of deviation 2 at a
 // temperature of 1, 152 thousand from about 35), and sums that cross behind the bins. Up to 16 passes of one workgroup over
-// the row: 42 us for a top-k of 100 of 4097, 410 for 5000 of 152 thousand (580 with every cut), 2.7 ms for 40000 of 2^20.
+// the row: 38 us for a top-k of 100 of 4097, 415 for 5000 of 152 thousand (570 with every cut), 2.7 ms for 40000 of 2^20.
 #include "batch.h"
 
 namespace mlxr {
@@ -47,8 +48,8 @@ __device__ __forceinline__ float sr_value(uint32_t k) { return __uint_as_float((
 // logits lie closer in x (at 3, two bins of 64 a unit may hold 3000 of 152 thousand tokens; one row with a top-p of 0.9 then
 // took 475 us through the radix descent, and takes 44). Sums are kept of those up to x = 32 or, above 1, of the logits. Tokens
 // behind them have weight, up to x = 52 (`reach`): 2^20 tokens of e^-52 are less than 2^-54 of the sum. The row's numbers are
-// in scalar registers: the last launch has no others to spare (14 vector registers spilled without; 38.7 and 38.1 us for
-// 256 mixed rows).
+// in scalar registers: the last launch has no others to spare (14 vector registers spilled without, 28 scalar ones are kept
+// in lanes of vector registers with; 38.7 and 38.1 us for 256 mixed rows).
 struct SrBins {
     double top, inv, width;   // the largest logit; bins per unit of logit, and the other way round
     double per, inv_per;      // bins per unit of x
@@ -155,14 +156,29 @@ __device__ uint64_t sr_max(uint64_t v, SrShared& sh) {
     for (int i = 0; i < SR_W; i++) t = sh.wsum[i] > t ? sh.wsum[i] : t;
     return t;
 }
+// What the waves before this one and all of them have, from one value a wave in LDS.
+__device__ __forceinline__ uint64_t sr_lane(uint64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+    return (uint64_t)lo | ((uint64_t)hi << 32);
+}
+__device__ __forceinline__ void sr_waves(const SrMass* w, SrMass& before, SrMass& all) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const SrMass m = lane < SR_W ? w[lane] : SrMass{0, 0}, upto = {wave_scan(m.high), wave_scan(m.low)};
+    before.add(SrMass{sr_lane(upto.high - m.high, wave), sr_lane(upto.low - m.low, wave)});
+    all.add(SrMass{sr_lane(upto.high, SR_W - 1), sr_lane(upto.low, SR_W - 1)});
+}
 // The sum of the weights within a cut.
 __device__ sr_u128 sr_mass(const SrRow& r, const SrScale& sc, SrCut cut, SrShared& sh) {
     SrMass t = {0, 0};
     for (int i = threadIdx.x; i < r.V; i += SR_T) if (sr_key(r.v[i]) > cut.key) t.add(sc.fixed(r.v[i]));
     if (threadIdx.x == 0 && cut.n) t.add(sc.fixed(sr_value(cut.key)), cut.n);
-    t.high = sr_sum(t.high, sh);
-    t.low = sr_sum(t.low, sh);
-    return t.sum();
+    t = SrMass{wave_scan(t.high), wave_scan(t.low)};
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sh.wmass[threadIdx.x >> 6] = t;
+    __syncthreads();
+    SrMass before = {0, 0}, all = {0, 0};
+    sr_waves(sh.wmass, before, all);
+    return all.sum();
 }
 
 // How many weights w reach `need`: the quotient rounded up, at least 1. The quotient of doubles is off by one at most.
@@ -272,11 +288,7 @@ __device__ SrCut sr_descend(const SrRow& r, const SrScale& sc, SrCut cut, sr_u12
         SrMass before = above, all = above;
         before.add(m);
         before.high -= own.high; before.low -= own.low;
-#pragma unroll 4
-        for (int i = 0; i < SR_W; i++) {
-            if (i < wave) before.add(sh.wmass[i]);
-            all.add(sh.wmass[i]);
-        }
+        sr_waves(sh.wmass, before, all);
         if (l == 0 && all.sum() < target) { *mass = all.sum(); return cut; }
 #pragma unroll 1
         for (int h = 0; h < SR_PER && b1 - h >= 0; h++) {   // one bin of one thread: sums only grow
