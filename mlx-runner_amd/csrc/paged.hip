@@ -301,10 +301,8 @@ __global__ __launch_bounds__(PA_T, 2) void paged_attn_kernel(PagedAttnArgs a, Pa
 #pragma unroll
             for (int s = 0; s < KS; s++) pa_split<ST>(x[s], q[s]);
         }
-        float m = -INFINITY, l = 0.0f;
+        float m, l;
         pa_f4 o[DV];
-#pragma unroll
-        for (int j = 0; j < DV; j++) o[j] = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
         float* score = WT ? wk.score + ((int64_t)b * a.nH + kvh * G + h0 + min(r, rows - 1)) * wk.score_stride : nullptr;
         // the wave's next 32 keys from half page u on (every PA_WV-th is its own): where they are, whether there are any
         int u = wave, key0 = 0;
@@ -351,120 +349,162 @@ __global__ __launch_bounds__(PA_T, 2) void paged_attn_kernel(PagedAttnArgs a, Pa
                 }
             }
         };
-        for (; seek(); u += PA_WV) {
-            load_k();
-            load_v();
-            const int key = key0;
-            pa_f4 sc[2];
+        // Products in parts are not what infinite keys and values ask for (a part of 0 times infinity, parts of two signs). A
+        // wave with a row that is not finite takes its keys again, with care: tiles that hold something infinite or NaN key by
+        // key in fp32, lane (r, g) with row r's dims D / 4 g ... A score of -infinity is a key that takes no part; an infinite
+        // value stays, however small its p is. A NaN in a row's query is NaN in its result, whatever the keys are. With one
+        // infinite value in each cache, 32 sequences of 0 to 8191 take 185 us in place of 99, 4 of 99 to 131 thousand 515 in
+        // place of 315 (900 and 2900 with all of such a wave's keys one by one). Tiles are loaded in a place of their own for
+        // the look at them: a branch between loading and multiplying costs every call 2 % (102 and 320 us).
+        bool careful = false, odd_q = false;
+        auto odd_tile = [&] {
+            uint32_t odd = 0;
+            constexpr uint32_t EXP = ST == 0 ? 0x7f80u : 0x7c00u;
+            auto look = [&](uint32_t w) { odd |= (uint32_t)((w & EXP) == EXP) | (uint32_t)((w >> 16 & EXP) == EXP); };
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                sc[i] = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int s = 0; s < KS; s++)
+                for (int s = 0; s < KS; s++) { look(kr[i][s].x); look(kr[i][s].y); look(kr[i][s].z); look(kr[i][s].w); }
 #pragma unroll
-                    for (int p = 0; p < NP; p++) sc[i] = pa_mfma<ST>(kr[i][s], q[s][p], sc[i]);
-            }
-            float sv[8];
+            for (int e = 0; e < 8; e++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) sv[e] = ST == 0 ? sc[e >> 2][e & 3] : sc[e >> 2][e & 3] * unscale;
-            if (key < sq.first || key + 32 > sq.L) {   // keys outside take no part, whatever their rows hold
+                for (int d = 0; d < DV / 2; d++) look(vr[e][d]);
+            return (bool)__any(odd);
+        };
+        auto slow_step = [&] {
+            const float f = a.scale * 1.4426950408889634f;
+#pragma unroll 1
+            for (int e = 0; e < 32; e++) {
+                const int key = key0 + e;
+                if (key < sq.first || key >= sq.L) continue;   // its score in the workspace is -infinity or unread
+                const int64_t at = base + e * D + D / 4 * g;
+                float sc = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < D / 4; d += 8) {
+                    const pa_u4 k = gload(reinterpret_cast<const pa_u4*>(K + at + d));
+                    const float4 y = gload4(qr + D / 4 * g + d), z = gload4(qr + D / 4 * g + d + 4);
+                    const float x8[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int k = key + (e >> 2) * 16 + 4 * g + (e & 3);
-                    if (k < sq.first || k >= sq.L) {
-                        sv[e] = -INFINITY;
-#pragma unroll
-                        for (int d = 0; d < DV / 2; d++) vr[e][d] = 0;
-                    }
+                    for (int c = 0; c < 8; c++) sc = fmaf(x8[c] * f, kv_float<ST>((uint16_t)(k[c / 2] >> 16 * (c & 1))), sc);
                 }
-            }
-            if constexpr (WT)
-                if (r < rows) {
-                    float* s = score + key + 4 * g;
-                    *reinterpret_cast<float4*>(s) = float4{sv[0], sv[1], sv[2], sv[3]};
-                    *reinterpret_cast<float4*>(s + 16) = float4{sv[4], sv[5], sv[6], sv[7]};
-                }
-            float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
-            mx = fmaxf(m, xor32_max(xor16_max(mx)));
-            if (__any(mx > m)) {
-                const float c = pa_exp2(m - pa_safe(mx));
-                l *= c;
-#pragma unroll
-                for (int j = 0; j < DV; j++) o[j] *= c;
+                sc = xor32_sum(xor16_sum(sc));
+                if constexpr (WT) if (g == ((e >> 2) & 3) && r < rows) score[key] = sc;   // the lane that wrote it before
+                if (sc == -INFINITY) continue;
+                const float mx = fmaxf(m, sc), c = pa_exp2(m - pa_safe(mx)), p = pa_exp2(sc - mx);
                 m = mx;
+                l = l * c + (g == 0 ? p : 0.0f);   // the four lanes' sums are added in the end
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < DV; j += 2) {
+                        const uint32_t v = gload(reinterpret_cast<const uint32_t*>(V + at + DV * i + j));
+                        constexpr float up = ST == 0 ? 1.0f : 16384.0f;
+                        o[j][i] = pa_times(c, o[j][i]) + pa_times(p * up, kv_float<ST>((uint16_t)v));
+                        o[j + 1][i] = pa_times(c, o[j + 1][i]) + pa_times(p * up, kv_float<ST>((uint16_t)(v >> 16)));
+                    }
             }
-            const float ms = pa_safe(m);
-            float p[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                p[e] = pa_exp2(sv[e] - ms);
-                l += p[e];
-                if constexpr (ST == 1) p[e] *= 16384.0f;
-            }
-            uint4 pp[NP];
-            pa_split<ST>(p, pp);
-#pragma unroll
-            for (int j = 0; j < DV; j++) {
-                uint4 vt;
-                if (j & 1) vt = uint4{pa_hi(vr[0][j / 2], vr[1][j / 2]), pa_hi(vr[2][j / 2], vr[3][j / 2]), pa_hi(vr[4][j / 2], vr[5][j / 2]), pa_hi(vr[6][j / 2], vr[7][j / 2])};
-                else vt = uint4{pa_lo(vr[0][j / 2], vr[1][j / 2]), pa_lo(vr[2][j / 2], vr[3][j / 2]), pa_lo(vr[4][j / 2], vr[5][j / 2]), pa_lo(vr[6][j / 2], vr[7][j / 2])};
-#pragma unroll
-                for (int i = 0; i < NP; i++) o[j] = pa_mfma<ST>(vt, pp[i], o[j]);
-            }
-        }
-        // Products in parts are not what infinite keys and values ask for (a part of 0 times infinity, parts of two signs): a
-        // wave with a row that is not finite takes its keys again, one by one in fp32, lane (r, g) with row r's dims D / 4 g ...
-        // A score of -infinity is a key that takes no part; an infinite value stays, however small its p is. The look itself
-        // and those where results meet cost 0.4 us of one sequence of 4096 (0.8 with the exact product for every factor there).
-        float odd[4] = {0.0f * l, 0.0f, 0.0f, 0.0f};   // NaN where one of them is not finite
-#pragma unroll
-        for (int j = 0; j < DV; j++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) odd[i] = fmaf(0.0f, o[j][i], odd[i]);
-        const float any_odd = (odd[0] + odd[1]) + (odd[2] + odd[3]);
-        if (__any(any_odd != any_odd && r < rows)) {
-            float y[D / 4], acc[D / 4];
-#pragma unroll
-            for (int d = 0; d < D / 4; d += 4) {
-                const float4 v = gload4(qr + D / 4 * g + d);
-                const float f = a.scale * 1.4426950408889634f;
-                y[d] = v.x * f; y[d + 1] = v.y * f; y[d + 2] = v.z * f; y[d + 3] = v.w * f;
-                acc[d] = acc[d + 1] = acc[d + 2] = acc[d + 3] = 0.0f;
-            }
+        };
+        while (true) {
             m = -INFINITY;
             l = 0.0f;
-            have = -1;
+#pragma unroll
+            for (int j = 0; j < DV; j++) o[j] = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
             for (u = wave; seek(); u += PA_WV) {
-#pragma unroll 1
-                for (int e = 0; e < 32; e++) {
-                    const int key = key0 + e;
-                    if (key < sq.first || key >= sq.L) continue;   // its score in the workspace is -infinity or unread
-                    uint16_t kx[D / 4], vx[D / 4];
-                    const int64_t at = base + e * D + D / 4 * g;
+                if (__builtin_expect(careful, 0)) {   // loaded again below
+                    load_k();
+                    load_v();
+                    if (odd_q || odd_tile()) { slow_step(); continue; }
+                }
+                load_k();
+                load_v();
+                const int key = key0;
+                pa_f4 sc[2];
 #pragma unroll
-                    for (int d = 0; d < D / 4; d += 8) {
-                        *reinterpret_cast<pa_u4*>(kx + d) = gload(reinterpret_cast<const pa_u4*>(K + at + d));
-                        *reinterpret_cast<pa_u4*>(vx + d) = gload(reinterpret_cast<const pa_u4*>(V + at + d));
+                for (int i = 0; i < 2; i++) {
+                    sc[i] = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int s = 0; s < KS; s++)
+#pragma unroll
+                        for (int p = 0; p < NP; p++) sc[i] = pa_mfma<ST>(kr[i][s], q[s][p], sc[i]);
+                }
+                float sv[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) sv[e] = ST == 0 ? sc[e >> 2][e & 3] : sc[e >> 2][e & 3] * unscale;
+                if (key < sq.first || key + 32 > sq.L) {   // keys outside take no part, whatever their rows hold
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int k = key + (e >> 2) * 16 + 4 * g + (e & 3);
+                        if (k < sq.first || k >= sq.L) {
+                            sv[e] = -INFINITY;
+#pragma unroll
+                            for (int d = 0; d < DV / 2; d++) vr[e][d] = 0;
+                        }
                     }
-                    float sc = 0.0f;
+                }
+                if constexpr (WT)
+                    if (r < rows) {
+                        float* s = score + key + 4 * g;
+                        *reinterpret_cast<float4*>(s) = float4{sv[0], sv[1], sv[2], sv[3]};
+                        *reinterpret_cast<float4*>(s + 16) = float4{sv[4], sv[5], sv[6], sv[7]};
+                    }
+                float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+                mx = fmaxf(m, xor32_max(xor16_max(mx)));
+                if (__any(mx > m)) {
+                    const float c = pa_exp2(m - pa_safe(mx));
+                    l *= c;
+                    if (__builtin_expect(careful, 0)) {
 #pragma unroll
-                    for (int d = 0; d < D / 4; d++) sc = fmaf(y[d], kv_float<ST>(kx[d]), sc);
-                    sc = xor32_sum(xor16_sum(sc));
-                    if constexpr (WT) if (g == ((e >> 2) & 3) && r < rows) score[key] = sc;   // the lane that wrote it before
-                    if (sc == -INFINITY) continue;
-                    const float mx = fmaxf(m, sc), c = pa_exp2(m - pa_safe(mx)), p = pa_exp2(sc - mx);
+                        for (int j = 0; j < DV; j++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[j][i] = pa_times(c, o[j][i]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < DV; j++) o[j] *= c;
+                    }
                     m = mx;
-                    l = l * c + p;
+                }
+                const float ms = pa_safe(m);
+                float p[8];
 #pragma unroll
-                    for (int d = 0; d < D / 4; d++) acc[d] = pa_times(c, acc[d]) + pa_times(p, kv_float<ST>(vx[d]));
+                for (int e = 0; e < 8; e++) {
+                    p[e] = pa_exp2(sv[e] - ms);
+                    l += p[e];
+                    if constexpr (ST == 1) p[e] *= 16384.0f;
+                }
+                uint4 pp[NP];
+                pa_split<ST>(p, pp);
+#pragma unroll
+                for (int j = 0; j < DV; j++) {
+                    uint4 vt;
+                    if (j & 1) vt = uint4{pa_hi(vr[0][j / 2], vr[1][j / 2]), pa_hi(vr[2][j / 2], vr[3][j / 2]), pa_hi(vr[4][j / 2], vr[5][j / 2]), pa_hi(vr[6][j / 2], vr[7][j / 2])};
+                    else vt = uint4{pa_lo(vr[0][j / 2], vr[1][j / 2]), pa_lo(vr[2][j / 2], vr[3][j / 2]), pa_lo(vr[4][j / 2], vr[5][j / 2]), pa_lo(vr[6][j / 2], vr[7][j / 2])};
+#pragma unroll
+                    for (int i = 0; i < NP; i++) o[j] = pa_mfma<ST>(vt, pp[i], o[j]);
                 }
             }
-            if (g != 0) l = 0.0f;   // the four lanes' sums are added below
-            constexpr float up = ST == 0 ? 1.0f : 16384.0f;
+            float odd[4] = {0.0f * l, 0.0f, 0.0f, 0.0f};   // NaN where one of them is not finite
 #pragma unroll
             for (int j = 0; j < DV; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[j][i] = acc[DV * i + j] * up;
+                for (int i = 0; i < 4; i++) odd[i] = fmaf(0.0f, o[j][i], odd[i]);
+            const float any_odd = (odd[0] + odd[1]) + (odd[2] + odd[3]);
+            if (careful || !__any(any_odd != any_odd && r < rows)) break;
+            // rows whose query holds NaN are what they are; one that holds infinities has no tile in parts
+            bool nan_q = false, inf_q = false;
+#pragma unroll 1
+            for (int d = 0; d < D / 4; d++) {
+                const float y = gload(qr + D / 4 * g + d);
+                nan_q |= y != y;
+                inf_q |= __builtin_isinf(y);
+            }
+            uint64_t nan_rows = __ballot(nan_q);
+            nan_rows |= nan_rows >> 32;
+            nan_rows |= nan_rows >> 16;
+            const bool mine = r < rows && !((nan_rows >> r) & 1);
+            if (!__any(any_odd != any_odd && mine)) break;
+            odd_q = __any(inf_q && mine);
+            careful = true;
+            have = -1;
         }
         // the waves' results: lane (r, g) has row r's dims DV (4 g + i) + j
         l = xor32_sum(xor16_sum(l));

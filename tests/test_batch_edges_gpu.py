@@ -156,6 +156,44 @@ def test_attention_nan(gpu, st, length):
     assert within(np.abs(got[~nan] - out[~nan]), tol[~nan]) <= 1
 
 
+@pytest.mark.parametrize("st", [0, 1])
+@pytest.mark.parametrize("length", [1, 100, 5000])
+def test_attention_infinite_queries(gpu, st, length):
+    """A query's infinity against keys of the other sign scores -infinity at every one: zeros, and no weight. Against keys of
+    both signs the row is NaN, as the formula is; the other rows are as they were."""
+    c = Cache(gpu, [length, length, 70], 1, 64, st, seed=78, weight=True)
+    q = queries(c, 3)
+    for b in range(2):
+        for i in range(0, length, PAGE):
+            page = c.table[b, i // PAGE]
+            n = min(PAGE, length - i)
+            c.k[page, 0, :n, 11] = to_half(-1 - np.arange(n, dtype=np.float32), st)
+    q2 = q.copy()
+    q2[0, 64 + 11] = INF                                       # head 1 of sequence 0: all scores -infinity
+    q2[1, 128 + 11] = -INF                                     # head 2 of sequence 1: all +infinity
+    clean = q2.copy()
+    clean[~np.isfinite(q2) & ~np.isnan(q2)] = 0
+    out, tol, p, p_tol = attention_reference(c, clean, 3, 0, 0.09)
+    c.up()
+    given = c.weight.copy()
+    got = attend(gpu, c, q2, 3, weight_in=c.dw)[:, :192].reshape(3, 3, 64)
+    out, tol = out.reshape(3, 3, 64), tol.reshape(3, 3, 64)
+    assert not got[0, 1].any() and np.isnan(got[1, 2]).all()
+    rest = np.ones((3, 3), bool)
+    rest[0, 1] = rest[1, 2] = False
+    assert within(np.abs(got[rest] - out[rest]), tol[rest]) <= 1
+    w = c.dw.numpy()
+    assert np.isnan(w[1, 0, :length]).all()
+    # sequence 0: heads 0 and 2 only
+    kk = c.rows(c.k, 0, 0, length)[0]
+    want = given[0, 0, :length].astype(np.float64)
+    for h in (0, 2):
+        s = float(np.float32(0.09)) * (kk @ q2[0, 64 * h:64 * h + 64].astype(np.float64))
+        e = np.exp(s - s.max())
+        want += e / e.sum()
+    assert within(np.abs(w[0, 0, :length] - want), p_tol[0, 0, :length] + 2.0 ** -22 * want) <= 1
+
+
 def test_append_past_f16_and_attention(gpu):
     """What passes f16's largest number is infinite in its cache: a key that scores -infinity then takes no part."""
     c = Cache(gpu, [200, 65], 1, 64, 1, seed=76, weight=True).up()
