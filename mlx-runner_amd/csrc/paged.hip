@@ -9,8 +9,8 @@ template <int ST> __device__ __forceinline__ float kv_float(uint16_t v) { return
 // ---- append ----
 // One wave per (head, sequence). Lane l holds one pair of a head's dims: of the rotated ones those that rotate
 // into each other (half-split: l and l + rot / 2; neighbours: 2l and 2l + 1), of the rest two neighbours. So the
-// norm is one wave sum and the rotation needs no exchange. Bound by the launch: 4.5 us for one sequence and for 200
-// (10 MB) alike, as launches follow each other. The angle is position * frequency: 32 bits would
+// norm is one wave sum and the rotation needs no exchange. Bound by the launch: 4.4 us for one sequence, 4.9 for
+// 200 (10 MB), as launches follow each other. The angle is position * frequency: 32 bits would
 // leave it 2^-24 of up to 131072 radians off (0.008), so turns are counted in 64 bits, and what is left after
 // whole turns goes on in 32. Keys and values are rounded once, to nearest.
 template <int ST>
@@ -91,8 +91,8 @@ hipError_t launch_paged_append(const PagedAppendArgs& a, hipStream_t s) {
 // two f16 (22 bits, q scaled to at most 2^14 by a power of two, p by 2^14). Scores are in powers of two (log2 e is
 // in q's scale).
 //
-// Measured (bf16, D 128): 4 sequences of 99 to 131 thousand slots, 40 / 8 heads 315 us (6.0 TB/s; a copy of 4 GiB reaches
-// 4.7); 32 of 0 to 8191, 32 / 8 heads 100 us (5.4 TB/s); one of 4096 11.5 us, of which 2 go by until the first keys are
+// Measured (bf16, D 128): 4 sequences of 99 to 131 thousand slots, 40 / 8 heads 314 us (6.0 TB/s; a copy of 4 GiB reaches
+// 4.7); 32 of 0 to 8191, 32 / 8 heads 99 us (5.4 TB/s); one of 4096 11.4 us, of which 2 go by until the first keys are
 // asked for, 3 until they are multiplied and 5 to hand over and join. Beside that, each change alone, in us for the three:
 // two workgroups of four waves a CU 322, 102, 12.7; 512 workgroups of eight 322, 109, 13.1; no places behind a segment
 // 322, 106, and 22 instead of 17.4 for a window of 1024 over 24 sequences of 5 to 16000 slots (short ones cost their ends,
