@@ -302,8 +302,9 @@ int mlxr_k_sample_noalloc(float* logits, int V, int32_t* hist, int32_t* status, 
  * One new token for each of B sequences over one pool of KV-cache pages: append, attention, eviction and
  * token selection. Like mlxr_k_sample_noalloc these calls allocate nothing, go on `stream` (a hipStream_t;
  * NULL: the null stream) and return without waiting, so they can be captured. They have no counterpart in
- * the reference, which decodes one sequence. Every pointer is to memory of the current device (pinned host memory
- * counts), and the stream is one of it: other host memory, and another device's, are MLXR_E_INVALID_ARG.
+ * the reference, which decodes one sequence. Every pointer that a call reads or writes through is to memory of the
+ * current device (pinned host memory counts), and the stream is one of it: other host memory, and another device's,
+ * are MLXR_E_INVALID_ARG.
  *
  * `work`: scratch of at least the bytes that the *_work function of the call returns, 256-byte aligned, ZERO
  * before its first use; every call leaves it ready for the next call of the same operator, whatever the
