@@ -194,6 +194,39 @@ def test_attention_infinite_queries(gpu, st, length):
     assert within(np.abs(w[0, 0, :length] - want), p_tol[0, 0, :length] + 2.0 ** -22 * want) <= 1
 
 
+@pytest.mark.parametrize("st", [0, 1])
+def test_attention_infinite_keys_in_long_runs(gpu, st):
+    """More pages a run than a wave holds numbers of at once, some of them with a key that takes no part: 17003 pages, of 40
+    in turn."""
+    n, L, D = 40, 64 * 17003 - 5, 64
+    c = Cache(gpu, [64 * n], 1, D, st, seed=79)
+    table = np.resize(c.table[0, :n], 17003).astype(np.int32)
+    q = queries(c, 2)
+    q[0, [3, 64 + 3]] = 0.5
+    for page in (2, 17, 39):
+        put(c, c.k, 0, 0, 64 * page + 20, 3, -INF)
+    gone = np.zeros(64 * n, bool)
+    gone[[64 * 2 + 20, 64 * 17 + 20, 64 * 39 + 20]] = True
+    c.up()
+    dt, dl = gpu.DeviceArray.from_numpy(table.reshape(1, -1)), gpu.DeviceArray.from_numpy(np.array([L], np.int32))
+    kv = c.desc(table=dt.ptr, len=dl.ptr, table_stride=17003, max_len=64 * 17003)
+    got = attend(gpu, c, q, 2, desc=kv)[0, :2 * D].reshape(2, D)
+    (k, _), (v, _) = c.rows(c.k, 0, 0, 64 * n), c.rows(c.v, 0, 0, 64 * n)
+    times = np.bincount(np.arange(L) % (64 * n), minlength=64 * n)[~gone]
+    k, v = k[~gone], v[~gone]
+    U = 2.0 ** -24
+    for h in range(2):
+        x = q[0, h * D:(h + 1) * D].astype(np.float64)
+        s = float(np.float32(0.09)) * (k @ x)
+        p = np.exp(s - s.max())
+        p /= (times * p).sum()
+        # the terms of attention_reference's bound, each slot's share counted as often as it is there
+        ds = 4 * np.sqrt(D) * U * 0.09 * np.sqrt((k ** 2) @ (x ** 2)) + 4 * U * np.abs(s) + 2 * U * np.abs(s).max()
+        want, rel = (times * p) @ v, 2 * ds.max() + 8 * U
+        tol = rel * ((times * p) @ np.abs(v)) + 4 * np.sqrt(L) * U * np.sqrt((times * p ** 2) @ (v ** 2)) + np.abs(want) * (4 * np.sqrt(L) * U * np.sqrt((times * p ** 2).sum()) + 2 * U)
+        assert within(np.abs(got[h] - want), tol) <= 1
+
+
 def test_append_past_f16_and_attention(gpu):
     """What passes f16's largest number is infinite in its cache: a key that scores -infinity then takes no part."""
     c = Cache(gpu, [200, 65], 1, 64, 1, seed=76, weight=True).up()
