@@ -374,6 +374,53 @@ int mlxr_k_sample_rows(const float* logits, int rows, int V, int64_t stride, con
                        void* work, size_t work_bytes, void* stream);
 int64_t mlxr_k_sample_rows_work(int rows, int V);
 
+/* ---------------------------------------------------------------- a batch's steps with any number of new tokens
+ * Prompts whole or in chunks, drafts to be verified, and steps in which some sequences bring a chunk and others one
+ * token, over the same pool of pages and under the same rules as the decode step above (the caller's stream and scratch,
+ * nothing allocated or waited for, pointers to the current device's memory, lengths and page numbers held in bounds on the
+ * device). The new tokens of a batch are rows of one array, `rows` of them at most (up to 4194304). */
+
+/* Pages for new tokens, and back: every sequence b goes from len[b] slots to want[b] (both held in [0, max_len]).
+ * First, what is shorter gives its pages back: the table's entries behind the new length's last page go on
+ * the stack free_pages [n_pages] of *n_free numbers (held in [0, n_pages]), in order of sequence and entry, numbers outside the pool
+ * left out (a page that comes back must belong to one sequence only; the stack never holds more than n_pages). Then what
+ * is longer takes pages off the top, in order of sequence. start[b]: the sum of new tokens that the sequences before b ask for,
+ * want - len each (held at 2^31 - 1). A sequence is refused, and keeps its length, where start[b] + its new tokens pass `rows`, or where it
+ * needs pages and the pages needed by all sequences up to it, refused ones too, are more than there are: no later sequence
+ * takes a page that an earlier one did not get. Written: len_out [B] (may be the cache's len), *n_free_out (may be n_free),
+ * start [B], count [B] (new tokens, 0 where refused or none), the new entries of kv->table (which must be writable here;
+ * others stay), and for each of the `rows` rows its sequence and slot, seq [rows] and slot [rows]: row start[b] + i is slot
+ * len[b] + i of b; rows of refused sequences and behind the last have -1 in both. With separate outputs a call repeats itself.
+ * The pool's keys and values are neither read nor written. */
+int mlxr_k_paged_reserve(const mlxr_paged_kv* kv, const int32_t* want, int32_t* free_pages, const int32_t* n_free, int rows,
+                         int32_t* len_out, int32_t* n_free_out, int32_t* start, int32_t* count, int32_t* seq, int32_t* slot,
+                         void* work, size_t work_bytes, void* stream);
+int64_t mlxr_k_paged_reserve_work(const mlxr_paged_kv* kv, int rows);
+
+/* Appends row r's token at slot slot[r] of sequence seq[r]; a row whose sequence is outside [0, B) or whose slot is outside
+ * [0, max_len) is left out whole. Rows of qkv and what happens to them are mlxr_k_paged_append's, with positions [rows] (NULL: the slot),
+ * sines and cosines times rope_scale (1 where the frequencies are not scaled for long contexts), and queries to q_out in
+ * fp32 (q_type 0; may be qkv itself at its stride) or in the cache's type (q_type 1; strides count values). The
+ * lengths are not read. Rows name slots of their own, in pages that belong to one sequence only. Row strides of whole 16
+ * bytes, 16-byte aligned arrays and a rot_dim that is a multiple of 8 are faster than others. */
+int mlxr_k_paged_append_rows(const mlxr_paged_kv* kv, const float* qkv, int row_stride, int rows, const int32_t* seq, const int32_t* slot,
+                             const int32_t* positions, const float* inv_freq, float rope_scale, const float* qn, const float* kn, int nH,
+                             int rot_dim, int traditional, float eps, void* q_out, int q_type, int q_stride, void* stream);
+
+/* Attention from rows to their own sequences' slots: row start[b] + i, i < count[b], is the query at slot len[b] - count[b] + i
+ * (len counts the new tokens) and attends every slot up to its own, or the last `window` of these (0: all). out = sum_j p_j v_j with p =
+ * softmax(scale q k_j). q_type 0: q and out are fp32 and so are the results; q_type 1: both are of the cache's
+ * type, scores, sums and the softmax in fp32, and each p is rounded to the type once (sums are of unrounded ones). A key whose
+ * score is -infinity takes no part; a row that has no slot (count above len), no page of the pool or no score above -infinity gives zeros;
+ * infinities and NaN in keys and values that a row attends count as the formula has them, and others do not reach it. Rows outside
+ * [0, rows) and rows that no sequence names are neither read nor written; sequences name rows of their own. The cache's weights
+ * stay as they are. q, out: 16-byte aligned, strides whole multiples of 16 bytes; out may be q itself at its stride. The same
+ * call gives the same bits; another batch around a row may cut its sums elsewhere. */
+int mlxr_k_paged_attention_rows(const mlxr_paged_kv* kv, const int32_t* start, const int32_t* count, int rows, const void* q, int q_type,
+                                int q_stride, int nH, int window, float scale, void* out, int out_stride, void* work, size_t work_bytes,
+                                void* stream);
+int64_t mlxr_k_paged_attention_rows_work(const mlxr_paged_kv* kv, int nH, int rows, int q_type);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,6 @@
-// A batch's decode step over a pool of KV-cache pages: launchers of paged.hip, evict.hip and sample_rows.hip.
-// They validate nothing: the entry points in capi_batch.cpp check shapes first.
+// A batch's steps over a pool of KV-cache pages: launchers of paged.hip, evict.hip, sample_rows.hip (one new token a
+// sequence), reserve.hip, append_rows.hip and attn_rows.hip (any number). They validate nothing: the entry points in
+// capi_batch.cpp and capi_rows.cpp check shapes first.
 #pragma once
 #include "../../include/mlxr.h"
 #include "common.h"
@@ -7,6 +8,10 @@
 namespace mlxr {
 
 typedef mlxr_paged_kv PagedKV;
+
+// The cache's types: bf16 (0) and f16 (1), rounded to nearest.
+template <int ST> __device__ __forceinline__ uint16_t kv_round(float v) { return ST == 0 ? f32_to_bf16(v) : f32_to_f16(v); }
+template <int ST> __device__ __forceinline__ float kv_float(uint16_t v) { return ST == 0 ? bf16_to_f32(v) : f16_to_f32(v); }
 
 // Lengths and page numbers are read on the device only, so they are held in bounds here.
 __device__ __forceinline__ int paged_len(const PagedKV& kv, int b) {
@@ -84,5 +89,39 @@ struct SampleRowsArgs {
 };
 size_t sample_rows_work(int rows, int V);
 hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s);
+
+struct ReserveArgs {
+    PagedKV kv;                       // table is written through
+    const int* want;
+    int* free_pages; const int* n_free;
+    int rows;
+    int *len_out, *n_free_out, *start, *count, *seq, *slot;
+    void* work;
+};
+size_t paged_reserve_work(const PagedKV& kv, int rows);
+hipError_t launch_paged_reserve(const ReserveArgs& a, hipStream_t s);
+
+struct AppendRowsArgs {
+    PagedKV kv;
+    const float* qkv; int row_stride, rows;
+    const int *seq, *slot, *positions;
+    const float* inv_freq; float rope_scale;
+    const float *qn, *kn;
+    int nH, rot_dim, traditional;
+    float eps;
+    void* q_out; int q_type, q_stride;
+};
+hipError_t launch_paged_append_rows(const AppendRowsArgs& a, hipStream_t s);
+
+struct AttnRowsArgs {
+    PagedKV kv;
+    const int *start, *count; int rows;
+    const void* q; int q_type, q_stride, nH, window;
+    float scale;
+    void* out; int out_stride;
+    void* work;
+};
+size_t paged_attention_rows_work(const PagedKV& kv, int nH, int rows, int q_type);
+hipError_t launch_paged_attention_rows(const AttnRowsArgs& a, hipStream_t s);
 
 }  // namespace mlxr

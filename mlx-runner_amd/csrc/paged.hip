@@ -3,9 +3,6 @@
 
 namespace mlxr {
 
-template <int ST> __device__ __forceinline__ uint16_t kv_round(float v) { return ST == 0 ? f32_to_bf16(v) : f32_to_f16(v); }
-template <int ST> __device__ __forceinline__ float kv_float(uint16_t v) { return ST == 0 ? bf16_to_f32(v) : f16_to_f32(v); }
-
 // ---- append ----
 // One wave per (head, sequence). Lane l holds one pair of a head's dims: of the rotated ones those that rotate
 // into each other (half-split: l and l + rot / 2; neighbours: 2l and 2l + 1), of the rest two neighbours. So the

@@ -125,6 +125,11 @@ def _load():
         "mlxr_k_paged_evict_work": (C.c_int64, [C.POINTER(PagedKV), I]),
         "mlxr_k_sample_rows": (I, [P, I, I, C.c_int64, P, P, P, P, P, P, P, P, C.c_size_t, P]),
         "mlxr_k_sample_rows_work": (C.c_int64, [I, I]),
+        "mlxr_k_paged_reserve": (I, [C.POINTER(PagedKV), P, P, P, I, P, P, P, P, P, P, P, C.c_size_t, P]),
+        "mlxr_k_paged_reserve_work": (C.c_int64, [C.POINTER(PagedKV), I]),
+        "mlxr_k_paged_append_rows": (I, [C.POINTER(PagedKV), P, I, I, P, P, P, P, F, P, P, I, I, I, F, P, I, I, P]),
+        "mlxr_k_paged_attention_rows": (I, [C.POINTER(PagedKV), P, P, I, P, I, I, I, I, F, P, I, P, C.c_size_t, P]),
+        "mlxr_k_paged_attention_rows_work": (C.c_int64, [C.POINTER(PagedKV), I, I, I]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
