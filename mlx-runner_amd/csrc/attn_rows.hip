@@ -1,72 +1,624 @@
 // Attention of any number of new tokens a sequence over a pool of KV-cache pages.
+#include <type_traits>
 #include "batch.h"
 
 namespace mlxr {
 
-__device__ __forceinline__ float at_times(float f, float x) { return __builtin_isinf(x) ? x : f * x; }   // for an f above 0 that may have come out as 0
+// out = sum_j p_j v_j, p = softmax of scale q k_j over the slots up to a row's own: 4 D flops a (row, query head, slot), and
+// 4 D bytes a slot and KV head once. One token a sequence is bound by those reads, a chunk by the matrix cores.
+//
+// Split. The (token, query head of the KV head) pairs of a sequence and KV head, tokens first, are its queries; AR_M of
+// them are an item, so a page is read once for all heads of a group and several tokens. An item walks the pages from the
+// first that its first token attends to its last token's own. All items' pages, laid end to end, are cut into equal runs, one
+// per workgroup, so chunks, prompts and single tokens of one call keep the card evenly busy, and counts and lengths may stay on
+// the device: each workgroup finds its run by a scan over the sequences. How many pages an item has follows from rounding twice,
+// so its length here is a bound that adds up in closed form (at_cum): up to two places of an item hold no
+// page, and AR_GAP more stand for what beginning and ending one costs. An item inside one run is written out at once;
+// one cut by runs leaves partial results (maximum, sum, unnormalised values), which the last workgroup to finish
+// joins in run order: the same bits every time.
+//
+// Inside. Four waves have 32 queries each and read the same page from LDS (copied there straight from the cache, the next
+// one while this one is used; 16-byte pieces XOR-swizzled by the key). 32x32x16 MFMAs:
+//   S^T = K q^T: lane (r = l % 32, h = l / 32) has query r's scores of keys 8 (i / 4) + 4 h + i % 4 of both 32-key halves.
+//   O^T = V^T P^T: a lane's eight scores of 16 keys are what it has to hold of P^T as an operand, if element e of
+//   half h stands for key 8 (e / 4) + 4 h + e % 4. V^T has its keys in that order from the LDS transpose read.
+// So maximum, sum and rescaling of a query stay within two lanes. Queries in the cache's type enter as they are, and
+// p is rounded to it; fp32 ones, and their p, are split into parts that the matrix cores multiply exactly: three bf16 by
+// truncation (24 bits), or two f16 (22 bits, q scaled to at most 2^14 by a power of two). Scores are in powers of two.
+// A query's reference point for p moves only when its maximum is AT_LAZY or more above it: until then p is up to
+// 2^AT_LAZY, and nothing has to be rescaled.
+constexpr int AR_M = 128, AR_WV = 4, AR_TH = 64 * AR_WV;   // queries of an item; waves and threads of a workgroup
+constexpr int AR_MAXW = 512;       // workgroups: two a CU
+constexpr int AR_GAP = 2;          // places behind an item
+constexpr int AR_MINPER = 4;       // places of a run at least
+constexpr float AT_LAZY = 8.0f;
+typedef float at_f16 __attribute__((ext_vector_type(16)));
+typedef __bf16 at_b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 at_b2 __attribute__((ext_vector_type(2)));
+typedef _Float16 at_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 at_h2 __attribute__((ext_vector_type(2)));
+typedef uint32_t at_u4 __attribute__((ext_vector_type(4)));
+typedef short at_s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* at_lptr;
+typedef __attribute__((address_space(3))) at_s4* at_lv4;
 
-// A wave per (row, query head): keys a page at a time, one a lane, then the page's values, two dims a lane.
-template <int ST, bool HQ>
-__global__ __launch_bounds__(256) void attn_rows_kernel(AttnRowsArgs a) {
-    __shared__ float qs[4][128];
+template <int ST> __device__ __forceinline__ at_f16 at_mfma(at_u4 a, at_u4 b, at_f16 c) {
+    if constexpr (ST == 0) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(at_b8, a), __builtin_bit_cast(at_b8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(at_h8, a), __builtin_bit_cast(at_h8, b), c, 0, 0, 0);
+}
+constexpr int at_parts(int ST, bool HQ) { return HQ ? 1 : (ST == 0 ? 3 : 2); }
+// Eight fp32 values as operands: rounded once (HQ), or parts whose sum they are (bf16) or nearly are (f16).
+template <int ST, bool HQ> __device__ __forceinline__ void at_split(const float* x, at_u4* o) {
+    constexpr int NP = at_parts(ST, HQ);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int t = 0; t < NP; t++) {
+            if constexpr (ST == 0 && HQ) o[t][i] = __builtin_bit_cast(uint32_t, at_b2{(__bf16)a, (__bf16)b});
+            else if constexpr (ST == 0) {
+                o[t][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+                a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+                b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+            } else {
+                const at_h2 h = {(_Float16)a, (_Float16)b};
+                o[t][i] = __builtin_bit_cast(uint32_t, h);
+                a -= (float)h[0];
+                b -= (float)h[1];
+            }
+        }
+    }
+}
+__device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float at_safe(float m) { return m == -INFINITY ? 0.0f : m; }   // -inf - -inf would be NaN
+__device__ __forceinline__ float at_times(float f, float x) { return __builtin_isinf(x) ? x : f * x; }   // for an f above 0 that may have come out as 0
+__device__ __forceinline__ void at_store2(float* p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 at_load2(const float* p) {
+    const uint64_t v = __hip_atomic_load(const_cast<uint64_t*>(reinterpret_cast<const uint64_t*>(p)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
+}
+
+struct AtWork {
+    unsigned* count;      // [AR_MAXW] arrivals at the item that starts in a run and goes on behind it; zero between calls
+    float* part;          // [2 W] partial results: [AR_WV][D / 4 + 1][64][2]: a wave's values, then maximum and sum
+    int W;
+};
+__host__ __device__ __forceinline__ constexpr size_t at_part_floats(int D) { return (size_t)AR_WV * (D / 4 + 1) * 128; }
+
+// A sequence's rows: c of them, the first at row `row` and slot `base`; `none` rows in front of these have no slot.
+struct AtSeq { int c, base, row, none; };
+__device__ __forceinline__ AtSeq at_seq(const AttnRowsArgs& a, int b) {
+    const int64_t n = max(0, a.count[b]), s = a.start[b], len = paged_len(a.kv, b);
+    const int64_t i0 = max((int64_t)0, -s), i1 = min(n, (int64_t)a.rows - s);   // tokens whose rows are in the array
+    const int64_t first = min(max(i0, n - len), max(i0, i1));                   // the first of them with a slot
+    return AtSeq{(int)max((int64_t)0, i1 - first), (int)max((int64_t)0, len - n + first), (int)(s + first), (int)max((int64_t)0, first - i0)};
+}
+// Places of items 0 .. n - 1 of a sequence: min(A + floor(2 i / G), cap) + AR_GAP for item i.
+struct AtPlaces {
+    int64_t A, cap, bend;   // from item `bend` on the cap holds
+    int G;
+    __device__ __forceinline__ AtPlaces(const AttnRowsArgs& a, int G_, int base) : G(G_) {
+        const int64_t spread = (AR_M - 1) / G;
+        A = (base + spread) / MLXR_PAGE + 2;
+        cap = a.window > 0 ? (a.window + spread + MLXR_PAGE - 1) / MLXR_PAGE + 1 : (int64_t)1 << 40;
+        bend = cap <= A ? 0 : ((cap - A) * G + 1) / 2;
+    }
+    __device__ __forceinline__ int64_t cum(int64_t n) const {
+        const int64_t m = min(n, bend);
+        const uint32_t u = (uint32_t)m / (uint32_t)G, v = (uint32_t)m % (uint32_t)G;
+        const int64_t steps = (int64_t)G * u * ((int64_t)u - 1) + (int64_t)u * (G / 2) + 2 * (int64_t)u * v + max(0, (int)v - (G + 1) / 2);
+        return n * AR_GAP + m * A + steps + (n - m) * cap;
+    }
+};
+
+template <int ST, int D, bool HQ>
+__global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtWork wk) {
+    constexpr int NP = at_parts(ST, HQ), KS = D / 16, NV = D / 32, TILE = 64 * D * 2, ROW = 2 * D, CH = D / 8;   // CH: 16-byte pieces of a row
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];   // [2 stages][K page, V page]
+    __shared__ uint64_t wave_sum64[2][AR_WV], found_pre;
+    __shared__ int found_b, last, odd_any;
     const PagedKV& kv = a.kv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = kv.D;
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    const int row = (int)(item / a.nH), h = (int)(item % a.nH), kvh = h / (a.nH / kv.nKV);
-    if (row >= a.rows) return;
-    int b = -1;
-    for (int b0 = 0; b0 < kv.B && b < 0; b0 += 64) {
-        const int c = b0 + lane;
-        const bool in = c < kv.B && row >= a.start[c] && row - a.start[c] < a.count[c];
-        const uint64_t m = __ballot(in);
-        if (m) b = b0 + (int)__builtin_ctzll(m);
-    }
-    if (b < 0) return;
-    const int len = paged_len(kv, b), at = len - a.count[b] + (row - a.start[b]);
-    const int first = a.window > 0 ? max(0, at + 1 - a.window) : 0;
-    for (int d = lane; d < D; d += 64) {
-        const int64_t i = (int64_t)row * a.q_stride + h * D + d;
-        qs[wave][d] = a.scale * (HQ ? kv_float<ST>(static_cast<const uint16_t*>(a.q)[i]) : static_cast<const float*>(a.q)[i]);
-    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+    const int G = a.nH / kv.nKV, W = wk.W;
+    // neighbouring runs share keys: those of an XCD (workgroups 8 apart) are neighbours
+    const int w = W % 8 == 0 ? (int)(blockIdx.x % 8) * (W / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
     const uint16_t *K = static_cast<const uint16_t*>(kv.k), *V = static_cast<const uint16_t*>(kv.v);
-    float m = -INFINITY, l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int p = first / MLXR_PAGE; p * MLXR_PAGE <= at; p++) {
-        const int page = paged_page(kv, b, p), key = p * MLXR_PAGE + lane;
-        if (page < 0) continue;
-        const int64_t base = paged_row(kv, page, kvh, 0);
-        float s = -INFINITY;
-        if (key >= first && key <= at) {
-            s = 0.0f;
-            for (int d = 0; d < D; d++) s = fmaf(qs[wave][d], kv_float<ST>(K[base + lane * D + d]), s);
+
+    // this workgroup's run of places
+    auto items_of = [&](const AtSeq& s) { return ((int64_t)s.c * G + AR_M - 1) / AR_M; };
+    auto places_of = [&](const AtSeq& s) -> uint64_t { return s.c ? (uint64_t)(AtPlaces(a, G, s.base).cum(items_of(s)) * kv.nKV) : 0; };
+    auto zero = [&](const AtSeq& s) {   // rows without a slot
+        const int per = a.nH * D * (HQ ? 2 : 4) / 16;
+        for (int64_t i = lane; i < (int64_t)s.none * per; i += 64) {
+            const int64_t row = s.row - s.none + i / per;
+            *reinterpret_cast<at_u4*>(static_cast<uint8_t*>(a.out) + row * a.out_stride * (HQ ? 2 : 4) + i % per * 16) = at_u4{0, 0, 0, 0};
         }
-        const bool odd = s != s;
-        const float mx = fmaxf(m, wave_max(odd ? -INFINITY : s)), ms = mx == -INFINITY ? 0.0f : mx, c = expf(m - ms), e = odd ? s : expf(s - ms);
-        l = l * c + wave_sum(e);
-        for (int i = 0; i < 2; i++) o[i] = m == -INFINITY ? o[i] : at_times(c, o[i]);
-        m = mx;
-        for (int j = 0; j < MLXR_PAGE; j++) {
-            if (__shfl(s, j) == -INFINITY) continue;
-            const float pj = __shfl(e, j);
-            for (int i = 0; i < 2; i++)
-                if (lane + 64 * i < D) o[i] += at_times(pj, kv_float<ST>(V[base + j * D + lane + 64 * i]));
+    };
+    uint64_t total = 0, per, t, t1, pre;
+    int b;
+    AtSeq sq;
+    {
+        uint64_t before = 0, n = 0, chunk = 0;
+        int step = 0;
+        auto scan = [&](int c, bool first) {
+            const AtSeq s = c + tid < kv.B ? at_seq(a, c + tid) : AtSeq{0, 0, 0, 0};
+            n = places_of(s);
+            if (first)
+                for (uint64_t m = __ballot(s.none > 0 && (c + tid) % W == w); m; m &= m - 1) {
+                    const int l = (int)__builtin_ctzll(m);
+                    zero(AtSeq{0, 0, __builtin_amdgcn_readlane(s.row, l), __builtin_amdgcn_readlane(s.none, l)});
+                }
+            const uint64_t v = wave_scan(n);
+            uint64_t* sums = wave_sum64[step++ & 1];
+            if (lane == 63) sums[wave] = v;
+            __syncthreads();
+            before = v - n;
+            chunk = 0;
+#pragma unroll
+            for (int i = 0; i < AR_WV; i++) { before += i < wave ? sums[i] : 0; chunk += sums[i]; }
+        };
+        for (int c = 0; c < kv.B; c += AR_TH) { scan(c, true); total += chunk; }
+        per = max((uint64_t)AR_MINPER, (total + W - 1) / W);
+        t = (uint64_t)w * per;
+        t1 = min(total, t + per);
+        if (t >= total) return;   // fewer runs than workgroups
+        uint64_t run = 0;
+        for (int c = 0; c < kv.B; c += AR_TH) {
+            if (kv.B > AR_TH) scan(c, false);
+            const uint64_t p = run + before;
+            if (p <= t && t < p + n) { found_b = c + tid; found_pre = p; }
+            run += chunk;
+            if (run > t) break;
         }
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(found_b);
+        pre = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)found_pre) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(found_pre >> 32)) << 32;
+        sq = at_seq(a, b);
     }
-    for (int i = 0; i < 2; i++) {
-        if (lane + 64 * i >= D) continue;
-        const float v = l == 0.0f ? 0.0f : o[i] / l;
-        const int64_t to = (int64_t)row * a.out_stride + h * D + lane + 64 * i;
-        if (HQ) static_cast<uint16_t*>(a.out)[to] = kv_round<ST>(v);
-        else static_cast<float*>(a.out)[to] = v;
+    // the item in which the run begins
+    int kvh, item, items;
+    {
+        const AtPlaces pl(a, G, sq.base);
+        items = (int)items_of(sq);
+        const uint64_t each = (uint64_t)pl.cum(items), local = t - pre;
+        kvh = (int)(local / each);
+        pre += kvh * each;
+        const int64_t at = (int64_t)(t - pre);
+        int64_t lo = 0, step = 1;
+        while (step * 64 < items) step *= 64;
+        for (;; step /= 64) {   // the last item that begins at or before the place
+            const int64_t i = lo + lane * step;
+            lo += step * (63 - (int)__builtin_clzll(__ballot(i < items && pl.cum(i) <= at)));
+            if (step == 1) break;
+        }
+        item = __builtin_amdgcn_readfirstlane((int)lo);
+        pre += pl.cum(item);
+    }
+    int slot = 0;   // partial results of this workgroup: its first item's, then its last one's
+    while (true) {
+        // pre: the item's first place
+        const AtPlaces pl(a, G, sq.base);
+        const int f0 = item * AR_M, R = min((int64_t)AR_M, (int64_t)sq.c * G - f0);
+        auto first_of = [&](int tok) { return a.window > 0 ? max(0, sq.base + tok + 1 - a.window) : 0; };
+        const int p0 = first_of(f0 / G) / MLXR_PAGE, pages = (sq.base + (f0 + R - 1) / G) / MLXR_PAGE - p0 + 1;
+        const int tile = (int)(t - pre), tiles = (int)min((int64_t)(pages - tile), (int64_t)(t1 - t));
+        // on to the run's next item
+        auto ahead = [&] {
+            const uint64_t n = (uint64_t)(pl.cum(item + 1) - pl.cum(item));
+            t = pre + n;
+            if (t >= t1) return false;
+            pre = t;
+            if (++item == items) {
+                item = 0;
+                if (++kvh == kv.nKV) {
+                    kvh = 0;
+                    do sq = at_seq(a, ++b);   // t < t1 <= total: another one has rows
+                    while (sq.c == 0);
+                    items = (int)items_of(sq);
+                }
+            }
+            return true;
+        };
+        if (tiles <= 0) {   // the run begins behind an item's pages
+            if (!ahead()) return;
+            slot = 1;            // an item's first part is in the second place unless the run begins with it
+            continue;
+        }
+        // this wave's queries
+        const int mine = min(32, R - 32 * wave);                  // how many, if above 0
+        const bool active = mine > 0;
+        const int f = f0 + (active ? 32 * wave + min(r, mine - 1) : 0), tok = f / G, head = kvh * G + f % G;
+        const int lim = sq.base + tok, low = first_of(tok);       // the slots that this lane's query attends: low .. lim
+        const int lim0 = __builtin_amdgcn_readlane(lim, 0), lim1 = __builtin_amdgcn_readlane(lim, 31), low0 = __builtin_amdgcn_readlane(low, 0), low1 = __builtin_amdgcn_readlane(low, 31);
+        const int64_t q_at = (int64_t)(sq.row + tok) * a.q_stride + (int64_t)head * D;
+        // page numbers, one a lane, 64 at a time
+        int have = 0, ids = paged_page(kv, b, p0 + tile + min(lane, tiles - 1));
+        auto page_of = [&](int i) {
+            if ((i >> 6) != have) {
+                have = i >> 6;
+                ids = paged_page(kv, b, p0 + tile + min(64 * have + lane, tiles - 1));
+            }
+            return __builtin_amdgcn_readlane(ids, i & 63);
+        };
+        auto seek = [&](int i) {   // the next page of the pool
+            while (i < tiles && page_of(i) < 0) i++;
+            return i;
+        };
+        // copies of page i of the run into stage i & 1: waves 0 and 1 the keys, 2 and 3 the values, a KiB at a time
+        auto issue = [&](int i, int stage) {
+            const int page = page_of(i);
+            const uint16_t* from = (wave < 2 ? K : V) + paged_row(kv, page, kvh, 0);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, TILE, 0x00020000);
+            uint8_t* to = lds + stage * 2 * TILE + (wave < 2 ? 0 : TILE);
+#pragma unroll
+            for (int j = 0; j < TILE / 2048; j++) {
+                const int piece = TILE / 2048 * (wave & 1) + j, key = piece * (64 / CH) + lane / CH;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (at_lptr)(to + piece * 1024), 16, key * ROW + 16 * (lane % CH ^ (key & (CH - 1))), 0, 0, 0);
+            }
+        };
+        // queries as operands: dims 16 s + 8 h .. + 7 of query r
+        at_u4 q[KS][NP];
+        float cl = HQ ? fabsf(a.scale) * 1.4426950408889634f : 1.0f;   // scores to powers of two
+        bool nan_q = false, inf_q = false;
+        if (active) {
+            if constexpr (HQ) {
+                // a negative scale turns the signs; 0 leaves 0 or NaN
+                const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+                constexpr uint32_t EXP = ST == 0 ? 0x7f80u : 0x7c00u, MAN = ST == 0 ? 0x7fu : 0x3ffu;
+                uint32_t nan = 0;
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    at_u4 x = gload(reinterpret_cast<const at_u4*>(static_cast<const uint16_t*>(a.q) + q_at + 16 * s + 8 * h));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t y = x[e];
+                        const bool lo = (y & EXP) == EXP, hi = (y >> 16 & EXP) == EXP;
+                        nan |= (uint32_t)(lo && (y & MAN)) | (uint32_t)(hi && (y >> 16 & MAN));
+                        if (cl == 0.0f) { x[e] = (lo ? EXP | MAN : 0u) | (hi ? (EXP | MAN) << 16 : 0u); nan |= (uint32_t)(lo || hi); }
+                        else x[e] ^= flip;
+                    }
+                    q[s][0] = x;
+                }
+                if (cl == 0.0f) cl = 1.0f;
+                nan_q = nan;
+            } else {
+                float x[KS][8], mx = 0.0f;
+                const float* p = static_cast<const float*>(a.q) + q_at + 8 * h;
+                const float by = a.scale * 1.4426950408889634f;
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const float4 u = gload4(p + 16 * s), v = gload4(p + 16 * s + 4);
+                    x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w; x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[s][e] *= by;
+                        mx = fmaxf(mx, fabsf(x[s][e]));
+                        nan_q |= x[s][e] != x[s][e];
+                    }
+                }
+                inf_q = mx == INFINITY;
+                if constexpr (ST == 1) {
+                    mx = xor32_max(mx);
+                    int e2 = 0;
+                    if (mx > 0.0f && mx < INFINITY) { frexpf(mx, &e2); e2 = 14 - e2; e2 = e2 < -126 ? -126 : (e2 > 126 ? 126 : e2); }
+                    const float up = ldexpf(1.0f, e2);
+                    cl = ldexpf(1.0f, -e2);
+#pragma unroll
+                    for (int s = 0; s < KS; s++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[s][e] *= up;
+                }
+#pragma unroll
+                for (int s = 0; s < KS; s++) at_split<ST, HQ>(x[s], q[s]);
+            }
+        }
+        at_f16 o[NV];        // dims 32 n + 8 (i / 4) + 4 h + i % 4 of query r
+        float m, l;          // the point of reference; this lane's keys' sum
+        constexpr float UP = ST == 0 ? 0.0f : 6.0f;   // p times 2^UP: f16 parts end at 2^-24
+        bool careful = false;
+
+        auto tile_of = [&](auto EDGEC, int i, int stage) {
+            constexpr bool EDGE = decltype(EDGEC)::value;
+            const int k0 = (p0 + tile + i) * MLXR_PAGE;
+            int ln = lane;
+            asm volatile("" : "+v"(ln));   // addresses are made here, not kept across pages
+            const uint32_t at = (uint32_t)stage * 2 * TILE, lr = ln & 31, lh = ln >> 5;
+            const uint32_t kaddr = at + lr * ROW + 16 * (lh ^ (lr & (CH - 1)));              // ^ 32 s, + 32 ROW kb
+            const uint32_t j = ln & 15, x = 4 * lh + (j >> 2);
+            const uint32_t vaddr = at + TILE + x * ROW + 16 * ((2 * (ln >> 4 & 1) + ((j & 3) >> 1)) ^ x) + 8 * (j & 1);
+            at_f16 s[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[kb][e] = 0.0f;
+            at_u4 k[2][2];   // the next step's keys are read while this one's products issue
+            auto kread = [&](int ks) {
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) k[ks & 1][kb] = *reinterpret_cast<const at_u4*>(lds + ((kaddr ^ (32u * ks)) + 32u * ROW * kb));
+            };
+            kread(0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (ks + 1 < KS) kread(ks + 1);
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+#pragma unroll
+                    for (int kb = 0; kb < 2; kb++) s[kb] = at_mfma<ST>(k[ks & 1][kb], q[ks][p], s[kb]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    if constexpr (EDGE) {
+                        const int key = k0 + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3);
+                        if (key > lim || key < low) s[kb][e] = -INFINITY;
+                    }
+                    mx = fmaxf(mx, s[kb][e]);
+                }
+            mx = xor32_max(mx);
+            if (HQ || ST == 1) mx *= cl;
+            if (__any(mx > m + AT_LAZY)) {
+                const float mn = fmaxf(m, mx), c = at_exp2(m - at_safe(mn));
+                l *= c;
+                if (__builtin_expect(careful, 0)) {
+#pragma unroll
+                    for (int n = 0; n < NV; n++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[n][e] = at_times(c, o[n][e]);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NV; n++) o[n] *= c;
+                }
+                m = mn;
+            }
+            const float ms = at_safe(m) - UP;
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[kb][e] = at_exp2(HQ || ST == 1 ? fmaf(s[kb][e], cl, -ms) : s[kb][e] - ms);
+                    l += s[kb][e];
+                }
+            // V^T fragments (16 keys st, 32 dims n) f = NV st + n, two ahead of the products
+            uint2 v[3][2];
+            auto vread = [&](int f) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const uint32_t n = f % NV, st = f / NV, ad = (D == 128 ? vaddr ^ (64u * n) ^ (128u * u) : vaddr ^ (64u * n)) + 8u * ROW * u + 16u * ROW * st;
+                    v[f % 3][u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lv4)(lds + ad)));
+                }
+            };
+            vread(0);
+            vread(1);
+#pragma unroll
+            for (int st = 0; st < 4; st++) {
+                float p8[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) p8[e] = s[st >> 1][8 * (st & 1) + e];
+                at_u4 pp[NP];
+                at_split<ST, HQ>(p8, pp);
+                // keys that none of the wave's queries attends may hold anything: their values count as 0 (0 times NaN would not)
+                uint32_t keep[2][2];
+                if constexpr (EDGE)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int key = k0 + 16 * st + 8 * u + 4 * h + 2 * e;
+                            keep[u][e] = (key <= lim1 && key >= low0 ? 0xffffu : 0u) | (key + 1 <= lim1 && key + 1 >= low0 ? 0xffff0000u : 0u);
+                        }
+#pragma unroll
+                for (int n = 0; n < NV; n++) {
+                    const int f = NV * st + n;
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (f + 2 < 4 * NV) vread(f + 2);
+                    if constexpr (EDGE)
+#pragma unroll
+                        for (int u = 0; u < 2; u++) { v[f % 3][u].x &= keep[u][0]; v[f % 3][u].y &= keep[u][1]; }
+                    const at_u4 vt = {v[f % 3][0].x, v[f % 3][0].y, v[f % 3][1].x, v[f % 3][1].y};
+#pragma unroll
+                    for (int p = 0; p < NP; p++) o[n] = at_mfma<ST>(vt, pp[p], o[n]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // Infinities and NaN. A product of 0 and infinity, or of a masked p and NaN, is not what the formula has, nor are parts of an
+        // infinite query or key. Where a result is not finite the item's pages are taken again, with care: a page that holds something
+        // infinite or NaN (keys only matter in parts) key by key in fp32; a score of -infinity is a key that takes no part, an infinite value
+        // stays, however small its p is.
+        bool odd_q = false;
+        auto odd_page = [&](int stage) {
+            uint32_t odd = 0;
+            constexpr uint32_t EXP = ST == 0 ? 0x7f80u : 0x7c00u;
+#pragma unroll 1
+            for (int i = (HQ ? TILE : 0) + lane * 16; i < 2 * TILE; i += 1024) {
+                const at_u4 x = *reinterpret_cast<const at_u4*>(lds + stage * 2 * TILE + i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) odd |= (uint32_t)((x[e] & EXP) == EXP) | (uint32_t)((x[e] >> 16 & EXP) == EXP);
+            }
+            return (bool)__any(odd);
+        };
+        auto slow_page = [&](int i, int stage) {
+            const int k0 = (p0 + tile + i) * MLXR_PAGE;
+            const uint8_t *kt = lds + stage * 2 * TILE, *vt = kt + TILE;
+            const float by = a.scale * 1.4426950408889634f;
+#pragma unroll 1
+            for (int e = 0; e < MLXR_PAGE; e++) {
+                const int key = k0 + e;
+                if (key > lim1 || key < low0) continue;
+                float sc = 0.0f;
+#pragma unroll 1
+                for (int s = 0; s < KS; s++) {
+                    const at_u4 k = *reinterpret_cast<const at_u4*>(kt + e * ROW + 16 * ((2 * s + h) ^ (e & (CH - 1))));
+                    float x[8];
+                    if constexpr (HQ) {
+                        const at_u4 y = gload(reinterpret_cast<const at_u4*>(static_cast<const uint16_t*>(a.q) + q_at + 16 * s + 8 * h));
+#pragma unroll
+                        for (int c = 0; c < 8; c++) x[c] = kv_float<ST>((uint16_t)(y[c / 2] >> 16 * (c & 1)));
+                    } else {
+                        const float4 u = gload4(static_cast<const float*>(a.q) + q_at + 16 * s + 8 * h), v = gload4(static_cast<const float*>(a.q) + q_at + 16 * s + 8 * h + 4);
+                        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 8; c++) sc = fmaf(x[c] * by, kv_float<ST>((uint16_t)(k[c / 2] >> 16 * (c & 1))), sc);
+                }
+                sc = xor32_sum(sc);
+                const bool in = key <= lim && key >= low && sc != -INFINITY;
+                const float mx = in ? fmaxf(m, sc) : m, c = at_exp2(m - at_safe(mx)), p = in ? at_exp2(sc - at_safe(mx) + UP) : 0.0f;
+                m = mx;
+                l = l * c + (h == 0 ? p : 0.0f);   // the two lanes' sums are added in the end
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(vt + e * ROW + 16 * ((4 * n + g) ^ (e & (CH - 1))) + 8 * h);
+                        const float v4[4] = {kv_float<ST>((uint16_t)v.x), kv_float<ST>((uint16_t)(v.x >> 16)), kv_float<ST>((uint16_t)v.y), kv_float<ST>((uint16_t)(v.y >> 16))};
+#pragma unroll
+                        for (int d = 0; d < 4; d++) o[n][4 * g + d] = at_times(c, o[n][4 * g + d]) + (in ? at_times(p, v4[d]) : 0.0f);
+                    }
+            }
+        };
+        while (true) {
+            m = -INFINITY;
+            l = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NV; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[n][e] = 0.0f;
+            int i = seek(0), stage = 0;
+            if (i < tiles) issue(i, 0);
+            while (i < tiles) {
+                const int nxt = seek(i + 1);
+                __builtin_amdgcn_s_waitcnt(0);       // this wave's copies of page i landed ...
+                __builtin_amdgcn_s_barrier();        // ... and every wave's; the other stage is free
+                if (nxt < tiles) issue(nxt, stage ^ 1);
+                const int k0 = (p0 + tile + i) * MLXR_PAGE;
+                if (active && k0 <= lim1 && k0 + MLXR_PAGE > low0) {
+                    if (__builtin_expect(careful, 0) && (odd_q || odd_page(stage))) slow_page(i, stage);
+                    else if (k0 + MLXR_PAGE - 1 <= lim0 && k0 >= low1) tile_of(std::false_type{}, i, stage);
+                    else tile_of(std::true_type{}, i, stage);
+                }
+                i = nxt;
+                stage ^= 1;
+            }
+            if (careful) break;
+            float any = 0.0f * l;   // NaN where one is not finite
+#pragma unroll
+            for (int n = 0; n < NV; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) any = fmaf(0.0f, o[n][e], any);
+            // a query that holds NaN has NaN results, whatever the keys are
+            uint64_t nan_rows = __ballot(nan_q);
+            nan_rows |= nan_rows >> 32;
+            const bool again = active && any != any && !((nan_rows >> r) & 1);
+            __syncthreads();
+            if (tid == 0) odd_any = 0;
+            __syncthreads();
+            if (__any(again) && lane == 0) odd_any = 1;
+            __syncthreads();
+            if (!odd_any) break;
+            careful = true;
+            odd_q = __any(inf_q);
+            have = -1;
+        }
+        l = xor32_sum(l);
+        auto write_out = [&] {
+            if (!active || r >= mine) return;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t to = (int64_t)(sq.row + tok) * a.out_stride + (int64_t)head * D + 4 * h;
+#pragma unroll
+            for (int n = 0; n < NV; n++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    float x[4];
+#pragma unroll
+                    for (int d = 0; d < 4; d++) x[d] = l == 0.0f ? 0.0f : o[n][4 * g + d] * inv;
+                    if constexpr (HQ) {
+                        const uint2 y = {(uint32_t)kv_round<ST>(x[0]) | (uint32_t)kv_round<ST>(x[1]) << 16, (uint32_t)kv_round<ST>(x[2]) | (uint32_t)kv_round<ST>(x[3]) << 16};
+                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + 32 * n + 8 * g) = y;
+                    } else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to + 32 * n + 8 * g) = float4{x[0], x[1], x[2], x[3]};
+                }
+        };
+        if (tiles == pages) write_out();
+        else {
+            // the runs that hold the item, from the first page's to the last one's
+            const uint64_t w0 = pre / per;
+            const int parts = (int)((pre + pages - 1) / per - w0) + 1, first_slot = pre == w0 * per ? 0 : 1;
+            auto part_of = [&](uint64_t run, int s) { return wk.part + (2 * run + s) * at_part_floats(D) + (size_t)wave * (D / 4 + 1) * 128 + 2 * lane; };
+            if (active) {
+                float* to = part_of(w, slot);
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) at_store2(to + (8 * n + e) * 128, o[n][2 * e], o[n][2 * e + 1]);
+                at_store2(to + D / 4 * 128, m, l);
+            }
+            parts_stored();
+            if (tid == 0) last = part_last(wk.count + w0, parts);
+            __syncthreads();
+            if (last) {
+                auto of = [&](int k) { return part_of(w0 + k, k == 0 ? first_slot : 0); };
+                float M = -INFINITY;
+                for (int k = 0; k < parts && active; k++) M = fmaxf(M, at_load2(of(k) + D / 4 * 128).x);
+                M = at_safe(M);
+                l = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[n][e] = 0.0f;
+                for (int k = 0; k < parts && active; k++) {
+                    const float* p = of(k);
+                    const float2 st = at_load2(p + D / 4 * 128);
+                    const float c = at_exp2(st.x - M);   // a part of NaN counts, whatever its maximum: 0 times NaN is NaN
+                    l += c * st.y;
+#pragma unroll
+                    for (int n = 0; n < NV; n++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float2 x = at_load2(p + (8 * n + e) * 128);
+                            o[n][2 * e] += at_times(c, x.x);
+                            o[n][2 * e + 1] += at_times(c, x.y);
+                        }
+                }
+                write_out();
+                if (tid == 0) part_rearm(wk.count + w0);
+            }
+        }
+        slot = 1;
+        if (!ahead()) return;
+        __syncthreads();   // the LDS is written again
     }
 }
 
-size_t paged_attention_rows_work(const PagedKV& kv, int nH, int rows, int q_type) { return 256; }
+static size_t at_layout(const PagedKV& kv, int nH, int rows, void* base, AtWork& wk) {
+    const int64_t G = nH / kv.nKV, items = ((int64_t)rows * G + AR_M - 1) / AR_M + kv.B, places = (kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE + 4 + AR_GAP;
+    const double runs = (double)items * (double)kv.nKV * (double)places / AR_MINPER + 1.0;
+    wk.W = runs < AR_MAXW ? (int)runs : AR_MAXW;
+    uint8_t* p = static_cast<uint8_t*>(base);
+    wk.count = reinterpret_cast<unsigned*>(p);   // first: where it is for every size
+    wk.part = reinterpret_cast<float*>(p + AR_MAXW * sizeof(unsigned));
+    return AR_MAXW * sizeof(unsigned) + (size_t)2 * wk.W * at_part_floats(kv.D) * sizeof(float);
+}
+
+size_t paged_attention_rows_work(const PagedKV& kv, int nH, int rows, int q_type) {
+    AtWork wk;
+    return at_layout(kv, nH, rows, nullptr, wk);
+}
 
 hipError_t launch_paged_attention_rows(const AttnRowsArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)(((int64_t)a.rows * a.nH + 3) / 4));
-#define AT_GO(ST, HQ) hipLaunchKernelGGL((attn_rows_kernel<ST, HQ>), grid, dim3(256), 0, s, a)
-    if (a.kv.st == 0) { if (a.q_type) AT_GO(0, true); else AT_GO(0, false); }
-    else { if (a.q_type) AT_GO(1, true); else AT_GO(1, false); }
+    AtWork wk;
+    at_layout(a.kv, a.nH, a.rows, a.work, wk);
+#define AT_GO(ST, D, HQ) hipLaunchKernelGGL((attn_rows_kernel<ST, D, HQ>), dim3(wk.W), dim3(AR_TH), 0, s, a, wk)
+#define AT_D(ST, HQ) do { if (a.kv.D == 64) AT_GO(ST, 64, HQ); else AT_GO(ST, 128, HQ); } while (0)
+    if (a.kv.st == 0) { if (a.q_type) AT_D(0, true); else AT_D(0, false); }
+    else { if (a.q_type) AT_D(1, true); else AT_D(1, false); }
+#undef AT_D
 #undef AT_GO
     return hipGetLastError();
 }
