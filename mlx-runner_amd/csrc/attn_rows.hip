@@ -12,25 +12,29 @@ namespace mlxr {
 // first that its first token attends to its last token's own. All items' pages, laid end to end, are cut into equal runs, one
 // per workgroup, so chunks, prompts and single tokens of one call keep the card evenly busy, and counts and lengths may stay on
 // the device: each workgroup finds its run by a scan over the sequences. How many pages an item has follows from rounding twice,
-// so its length here is a bound that adds up in closed form (at_cum): up to two places of an item hold no
+// so its length here is a bound that adds up in closed form (AtPlaces): up to two places of an item hold no
 // page, and AR_GAP more stand for what beginning and ending one costs. An item inside one run is written out at once;
 // one cut by runs leaves partial results (maximum, sum, unnormalised values), which the last workgroup to finish
 // joins in run order: the same bits every time.
 //
-// Inside. Four waves have 32 queries each and read the same page from LDS (copied there straight from the cache, the next
-// one while this one is used; 16-byte pieces XOR-swizzled by the key). 32x32x16 MFMAs:
+// Inside. Eight waves have 32 queries each and read the same page from LDS; where an item has 128 queries or fewer, four do, and
+// the other four take every other page, joined through LDS at the end. Pages are copied there straight from the cache, three
+// ahead (or two, in pairs), 16-byte pieces XOR-swizzled by the key. 32x32x16 MFMAs:
 //   S^T = K q^T: lane (r = l % 32, h = l / 32) has query r's scores of keys 8 (i / 4) + 4 h + i % 4 of both 32-key halves.
 //   O^T = V^T P^T: a lane's eight scores of 16 keys are what it has to hold of P^T as an operand, if element e of
 //   half h stands for key 8 (e / 4) + 4 h + e % 4. V^T has its keys in that order from the LDS transpose read.
-// So maximum, sum and rescaling of a query stay within two lanes. Queries in the cache's type enter as they are, and
+// So maximum, sum and rescaling of a query stay within two lanes. Products and softmax take about as long as each other, so
+// the two waves of a SIMD are half a page apart: between two barriers one multiplies (the last page's values, the next one's keys)
+// while the other has its softmax. Queries in the cache's type enter as they are, and
 // p is rounded to it; fp32 ones, and their p, are split into parts that the matrix cores multiply exactly: three bf16 by
 // truncation (24 bits), or two f16 (22 bits, q scaled to at most 2^14 by a power of two). Scores are in powers of two.
 // A query's reference point for p moves only when its maximum is AT_LAZY or more above it: until then p is up to
 // 2^AT_LAZY, and nothing has to be rescaled.
-constexpr int AR_M = 128, AR_WV = 4, AR_TH = 64 * AR_WV;   // queries of an item; waves and threads of a workgroup
-constexpr int AR_MAXW = 512;       // workgroups: two a CU
+constexpr int AR_WV = 8, AR_TH = 64 * AR_WV, AR_M = 32 * AR_WV;   // waves and threads of a workgroup, queries of an item
+constexpr int AR_MAXW = 256;       // workgroups: one a CU
 constexpr int AR_GAP = 2;          // places behind an item
 constexpr int AR_MINPER = 4;       // places of a run at least
+constexpr int AR_RING = 4;         // pages of keys, and of values, in LDS
 constexpr float AT_LAZY = 8.0f;
 typedef float at_f16 __attribute__((ext_vector_type(16)));
 typedef __bf16 at_b8 __attribute__((ext_vector_type(8)));
@@ -83,7 +87,7 @@ __device__ __forceinline__ float2 at_load2(const float* p) {
 
 struct AtWork {
     unsigned* count;      // [AR_MAXW] arrivals at the item that starts in a run and goes on behind it; zero between calls
-    float* part;          // [2 W] partial results: [AR_WV][D / 4 + 1][64][2]: a wave's values, then maximum and sum
+    float* part;          // [2 W] partial results: [AR_WV][D / 4 + 1][64][2]: 32 queries' values, then maximum and sum
     int W;
 };
 __host__ __device__ __forceinline__ constexpr size_t at_part_floats(int D) { return (size_t)AR_WV * (D / 4 + 1) * 128; }
@@ -96,28 +100,40 @@ __device__ __forceinline__ AtSeq at_seq(const AttnRowsArgs& a, int b) {
     const int64_t first = min(max(i0, n - len), max(i0, i1));                   // the first of them with a slot
     return AtSeq{(int)max((int64_t)0, i1 - first), (int)max((int64_t)0, len - n + first), (int)(s + first), (int)max((int64_t)0, first - i0)};
 }
-// Places of items 0 .. n - 1 of a sequence: min(A + floor(2 i / G), cap) + AR_GAP for item i.
+// Places of items 0 .. n - 1 of a sequence: min(A + floor(S i / G), cap) + AR_GAP for item i, S pages of queries (AR_M / 64).
 struct AtPlaces {
+    static constexpr int S = AR_M / MLXR_PAGE;
     int64_t A, cap, bend;   // from item `bend` on the cap holds
     int G;
     __device__ __forceinline__ AtPlaces(const AttnRowsArgs& a, int G_, int base) : G(G_) {
         const int64_t spread = (AR_M - 1) / G;
         A = (base + spread) / MLXR_PAGE + 2;
         cap = a.window > 0 ? (a.window + spread + MLXR_PAGE - 1) / MLXR_PAGE + 1 : (int64_t)1 << 40;
-        bend = cap <= A ? 0 : ((cap - A) * G + 1) / 2;
+        bend = cap <= A ? 0 : ((cap - A) * G + S - 1) / S;
+    }
+    __device__ __forceinline__ int64_t steps(int v) const {   // sum of floor(S i / G) over i < v <= G
+        int64_t n = 0;
+#pragma unroll
+        for (int k = 1; k < S; k++) n += max(0, v - (k * G + S - 1) / S);
+        return n;
     }
     __device__ __forceinline__ int64_t cum(int64_t n) const {
         const int64_t m = min(n, bend);
         const uint32_t u = (uint32_t)m / (uint32_t)G, v = (uint32_t)m % (uint32_t)G;
-        const int64_t steps = (int64_t)G * u * ((int64_t)u - 1) + (int64_t)u * (G / 2) + 2 * (int64_t)u * v + max(0, (int)v - (G + 1) / 2);
-        return n * AR_GAP + m * A + steps + (n - m) * cap;
+        return n * AR_GAP + m * A + (int64_t)S * G * ((int64_t)u * ((int64_t)u - 1) / 2) + u * steps(G) + (int64_t)S * u * v + steps((int)v) + (n - m) * cap;
     }
 };
+
+// Where a key's 16-byte pieces lie in LDS: piece c at c ^ this. Sixteen keys' same piece, and four keys' same four pieces, are in
+// different banks.
+template <int D> __device__ __forceinline__ int at_swz_k(int key) { return D == 128 ? key & 15 : (key >> 1) & 7; }
+template <int D> __device__ __forceinline__ int at_swz_v(int key) { return 4 * (D == 128 ? key & 3 : (key >> 1) & 1) + ((key >> 2) & 3); }
 
 template <int ST, int D, bool HQ>
 __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtWork wk) {
     constexpr int NP = at_parts(ST, HQ), KS = D / 16, NV = D / 32, TILE = 64 * D * 2, ROW = 2 * D, CH = D / 8;   // CH: 16-byte pieces of a row
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TILE];   // [2 stages][K page, V page]
+    constexpr int PW = TILE / 1024 / AR_WV;   // copies a wave and page of keys (or values)
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];   // [AR_RING] pages of keys, then of values; partial results in between
     __shared__ uint64_t wave_sum64[2][AR_WV], found_pre;
     __shared__ int found_b, last, odd_any;
     const PagedKV& kv = a.kv;
@@ -227,36 +243,36 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             slot = 1;            // an item's first part is in the second place unless the run begins with it
             continue;
         }
-        // this wave's queries
-        const int mine = min(32, R - 32 * wave);                  // how many, if above 0
+        // this wave's queries, and the other pages' of few
+        const bool two = R <= AR_M / 2;
+        const int step = two ? 2 : 1, turn = two ? wave >> 2 : 0, block = two ? wave & 3 : wave, blocks = (R + 31) / 32;
+        const int mine = min(32, R - 32 * block);                 // how many, if above 0
         const bool active = mine > 0;
-        const int f = f0 + (active ? 32 * wave + min(r, mine - 1) : 0), tok = f / G, head = kvh * G + f % G;
+        const int f = f0 + (active ? 32 * block + min(r, mine - 1) : 0), tok = f / G, head = kvh * G + f % G;
         const int lim = sq.base + tok, low = first_of(tok);       // the slots that this lane's query attends: low .. lim
         const int lim0 = __builtin_amdgcn_readlane(lim, 0), lim1 = __builtin_amdgcn_readlane(lim, 31), low0 = __builtin_amdgcn_readlane(low, 0), low1 = __builtin_amdgcn_readlane(low, 31);
         const int64_t q_at = (int64_t)(sq.row + tok) * a.q_stride + (int64_t)head * D;
-        // page numbers, one a lane, 64 at a time
+        // page numbers, one a lane, 64 at a time; -1 behind the run and where there is none
         int have = 0, ids = paged_page(kv, b, p0 + tile + min(lane, tiles - 1));
         auto page_of = [&](int i) {
+            if (i >= tiles) return -1;
             if ((i >> 6) != have) {
                 have = i >> 6;
                 ids = paged_page(kv, b, p0 + tile + min(64 * have + lane, tiles - 1));
             }
             return __builtin_amdgcn_readlane(ids, i & 63);
         };
-        auto seek = [&](int i) {   // the next page of the pool
-            while (i < tiles && page_of(i) < 0) i++;
-            return i;
-        };
-        // copies of page i of the run into stage i & 1: waves 0 and 1 the keys, 2 and 3 the values, a KiB at a time
-        auto issue = [&](int i, int stage) {
-            const int page = page_of(i);
-            const uint16_t* from = (wave < 2 ? K : V) + paged_row(kv, page, kvh, 0);
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, TILE, 0x00020000);
-            uint8_t* to = lds + stage * 2 * TILE + (wave < 2 ? 0 : TILE);
+        // this wave's share of a page's copy: its first `rows` rows, and zeros behind them (nothing is read of a page that is not there)
+        auto copy = [&](const uint16_t* pool, bool values, int page, int rows, uint32_t to) {
+            const uint16_t* from = pool + (page < 0 ? 0 : paged_row(kv, page, kvh, 0));
+            const int bytes = page < 0 ? 0 : max(0, min(MLXR_PAGE, rows)) * ROW;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, bytes, 0x00020000);
+            uint8_t* dst = lds + to;
 #pragma unroll
-            for (int j = 0; j < TILE / 2048; j++) {
-                const int piece = TILE / 2048 * (wave & 1) + j, key = piece * (64 / CH) + lane / CH;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (at_lptr)(to + piece * 1024), 16, key * ROW + 16 * (lane % CH ^ (key & (CH - 1))), 0, 0, 0);
+            for (int j = 0; j < PW; j++) {
+                const int piece = wave * PW + j, key = piece * (64 / CH) + lane / CH;
+                const int swz = values ? at_swz_v<D>(key) : at_swz_k<D>(key);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (at_lptr)(dst + piece * 1024), 16, key * ROW + 16 * (lane % CH ^ swz), 0, 0, 0);
             }
         };
         // queries as operands: dims 16 s + 8 h .. + 7 of query r
@@ -318,22 +334,14 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         at_f16 o[NV];        // dims 32 n + 8 (i / 4) + 4 h + i % 4 of query r
         float m, l;          // the point of reference; this lane's keys' sum
         constexpr float UP = ST == 0 ? 0.0f : 6.0f;   // p times 2^UP: f16 parts end at 2^-24
-        bool careful = false;
-
-        auto tile_of = [&](auto EDGEC, int i, int stage) {
-            constexpr bool EDGE = decltype(EDGEC)::value;
-            const int k0 = (p0 + tile + i) * MLXR_PAGE;
+        at_f16 s[2];         // scores of a page, keys 32 kb + 8 (i / 4) + 4 h + i % 4
+        at_u4 pr[HQ ? 4 : 1];   // p of a page, rounded (HQ); s otherwise
+        constexpr uint32_t VALUES = AR_RING * TILE;
+        auto first_key = [&](int i) { return (p0 + tile + i) * MLXR_PAGE; };
+        auto products_k = [&](uint32_t at) {
             int ln = lane;
             asm volatile("" : "+v"(ln));   // addresses are made here, not kept across pages
-            const uint32_t at = (uint32_t)stage * 2 * TILE, lr = ln & 31, lh = ln >> 5;
-            const uint32_t kaddr = at + lr * ROW + 16 * (lh ^ (lr & (CH - 1)));              // ^ 32 s, + 32 ROW kb
-            const uint32_t j = ln & 15, x = 4 * lh + (j >> 2);
-            const uint32_t vaddr = at + TILE + x * ROW + 16 * ((2 * (ln >> 4 & 1) + ((j & 3) >> 1)) ^ x) + 8 * (j & 1);
-            at_f16 s[2];
-#pragma unroll
-            for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[kb][e] = 0.0f;
+            const uint32_t lr = ln & 31, lh = ln >> 5, kaddr = at + lr * ROW + 16 * (lh ^ at_swz_k<D>(lr));   // ^ 32 ks, + 32 ROW kb
             at_u4 k[2][2];   // the next step's keys are read while this one's products issue
             auto kread = [&](int ks) {
 #pragma unroll
@@ -347,34 +355,33 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
 #pragma unroll
                 for (int p = 0; p < NP; p++)
 #pragma unroll
-                    for (int kb = 0; kb < 2; kb++) s[kb] = at_mfma<ST>(k[ks & 1][kb], q[ks][p], s[kb]);
+                    for (int kb = 0; kb < 2; kb++) s[kb] = at_mfma<ST>(k[ks & 1][kb], q[ks][p], ks + p ? s[kb] : at_f16{0.0f});
             }
             __builtin_amdgcn_sched_barrier(0);
+        };
+        auto softmax = [&](auto CARE, int k0) {
+            if (k0 + MLXR_PAGE - 1 > lim0 || k0 < low1)   // some query does not attend all of the page
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int key = k0 + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3);
+                        if (key > lim || key < low) s[kb][e] = -INFINITY;
+                    }
             float mx = -INFINITY;
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    if constexpr (EDGE) {
-                        const int key = k0 + 32 * kb + 8 * (e >> 2) + 4 * h + (e & 3);
-                        if (key > lim || key < low) s[kb][e] = -INFINITY;
-                    }
-                    mx = fmaxf(mx, s[kb][e]);
-                }
+                for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[kb][e]);
             mx = xor32_max(mx);
             if (HQ || ST == 1) mx *= cl;
             if (__any(mx > m + AT_LAZY)) {
                 const float mn = fmaxf(m, mx), c = at_exp2(m - at_safe(mn));
                 l *= c;
-                if (__builtin_expect(careful, 0)) {
 #pragma unroll
-                    for (int n = 0; n < NV; n++)
+                for (int n = 0; n < NV; n++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[n][e] = at_times(c, o[n][e]);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NV; n++) o[n] *= c;
-                }
+                    for (int e = 0; e < 16; e++) o[n][e] = decltype(CARE)::value ? at_times(c, o[n][e]) : c * o[n][e];
                 m = mn;
             }
             const float ms = at_safe(m) - UP;
@@ -385,12 +392,26 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     s[kb][e] = at_exp2(HQ || ST == 1 ? fmaf(s[kb][e], cl, -ms) : s[kb][e] - ms);
                     l += s[kb][e];
                 }
+            if constexpr (HQ)
+#pragma unroll
+                for (int st = 0; st < 4; st++) {
+                    float p8[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) p8[e] = s[st >> 1][8 * (st & 1) + e];
+                    at_split<ST, HQ>(p8, &pr[st]);
+                }
+        };
+        auto products_v = [&](uint32_t at) {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const uint32_t lh = ln >> 5, j = ln & 15;
+            const uint32_t vaddr = at + (4 * lh + (j >> 2)) * ROW + 16 * ((2 * (ln >> 4 & 1) + ((j & 3) >> 1)) ^ (4 * (j >> (D == 128 ? 2 : 3)) + lh)) + 8 * (j & 1);
             // V^T fragments (16 keys st, 32 dims n) f = NV st + n, two ahead of the products
             uint2 v[3][2];
             auto vread = [&](int f) {
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const uint32_t n = f % NV, st = f / NV, ad = (D == 128 ? vaddr ^ (64u * n) ^ (128u * u) : vaddr ^ (64u * n)) + 8u * ROW * u + 16u * ROW * st;
+                    const uint32_t ad = (vaddr ^ (64u * (f % NV)) ^ (32u * u)) + 8u * ROW * u + 16u * ROW * (f / NV);
                     v[f % 3][u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lv4)(lds + ad)));
                 }
             };
@@ -398,29 +419,19 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             vread(1);
 #pragma unroll
             for (int st = 0; st < 4; st++) {
-                float p8[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) p8[e] = s[st >> 1][8 * (st & 1) + e];
                 at_u4 pp[NP];
-                at_split<ST, HQ>(p8, pp);
-                // keys that none of the wave's queries attends may hold anything: their values count as 0 (0 times NaN would not)
-                uint32_t keep[2][2];
-                if constexpr (EDGE)
+                if constexpr (HQ) pp[0] = pr[st];
+                else {
+                    float p8[8];
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const int key = k0 + 16 * st + 8 * u + 4 * h + 2 * e;
-                            keep[u][e] = (key <= lim1 && key >= low0 ? 0xffffu : 0u) | (key + 1 <= lim1 && key + 1 >= low0 ? 0xffff0000u : 0u);
-                        }
+                    for (int e = 0; e < 8; e++) p8[e] = s[st >> 1][8 * (st & 1) + e];
+                    at_split<ST, HQ>(p8, pp);
+                }
 #pragma unroll
                 for (int n = 0; n < NV; n++) {
                     const int f = NV * st + n;
                     __builtin_amdgcn_sched_barrier(0);
                     if (f + 2 < 4 * NV) vread(f + 2);
-                    if constexpr (EDGE)
-#pragma unroll
-                        for (int u = 0; u < 2; u++) { v[f % 3][u].x &= keep[u][0]; v[f % 3][u].y &= keep[u][1]; }
                     const at_u4 vt = {v[f % 3][0].x, v[f % 3][0].y, v[f % 3][1].x, v[f % 3][1].y};
 #pragma unroll
                     for (int p = 0; p < NP; p++) o[n] = at_mfma<ST>(vt, pp[p], o[n]);
@@ -428,25 +439,75 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             }
             __builtin_amdgcn_sched_barrier(0);
         };
+        auto seen = [&](int k0) { return active && k0 <= lim1 && k0 + MLXR_PAGE > low0; };    // some query attends some of the page
+        // The run's pages, `step` of them a turn, two barriers a turn: at the first one waves 0 .. 3 begin the turn's products, at the second one
+        // waves 4 .. 7 do. Turn j's keys are asked for three turns ahead (one, where pages go in pairs), its values a turn later, after
+        // the first barrier: what turn j - 1 read of keys and turn j - 2 of values is free then.
+        const int end = sq.base + sq.c;
+        auto pages_through = [&] {
+            const int turns = (tiles + step - 1) / step, far = two ? 1 : AR_RING - 1;
+            const bool late = wave >= 4;
+            int next[2] = {-1, -1};    // pages whose keys were asked for last: their values are next
+            uint32_t valid = 0;        // of the last 32 pages, by number
+            auto ask = [&](int j) {    // turn j's keys, turn j - 1's values
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    if (g >= step) break;
+                    const int i = j * step + g, page = page_of(i);
+                    copy(K, false, page, MLXR_PAGE, (i & (AR_RING - 1)) * TILE);
+                    if (j) copy(V, true, next[g], end - first_key(i - step), VALUES + ((i - step) & (AR_RING - 1)) * TILE);
+                    next[g] = page;
+                    valid = (valid & ~(1u << (i & 31))) | (uint32_t)(page >= 0) << (i & 31);
+                }
+            };
+            auto first_barrier = [&](int j) {
+                if (two) __builtin_amdgcn_s_waitcnt(0x0F70);                          // vmcnt(0)
+                else __builtin_amdgcn_s_waitcnt(PW == 2 ? 0x0F78 : 0x0F74);           // all but the last two turns' 4 PW copies
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                ask(j + far);
+            };
+            auto second_barrier = [&] {
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            };
+            for (int j = 0; j < far; j++) ask(j);
+            if (late) first_barrier(0), second_barrier();
+            else first_barrier(0);
+            products_k((turn & (AR_RING - 1)) * TILE);   // of a page that is not there: not used
+            for (int j = 0; j < turns; j++) {
+                const int i = j * step + turn, k0 = first_key(i);
+                const bool on = i < tiles && seen(k0) && (valid >> (i & 31) & 1);
+                if (late) first_barrier(j + 1);
+                else second_barrier();
+                if (on) softmax(std::false_type{}, k0);
+                if (late) second_barrier();
+                else first_barrier(j + 1);
+                if (on) products_v(VALUES + (i & (AR_RING - 1)) * TILE);
+                products_k(((i + step) & (AR_RING - 1)) * TILE);
+            }
+            if (!late) second_barrier();
+        };
         // Infinities and NaN. A product of 0 and infinity, or of a masked p and NaN, is not what the formula has, nor are parts of an
         // infinite query or key. Where a result is not finite the item's pages are taken again, with care: a page that holds something
         // infinite or NaN (keys only matter in parts) key by key in fp32; a score of -infinity is a key that takes no part, an infinite value
         // stays, however small its p is.
         bool odd_q = false;
-        auto odd_page = [&](int stage) {
+        auto odd_page = [&] {
             uint32_t odd = 0;
             constexpr uint32_t EXP = ST == 0 ? 0x7f80u : 0x7c00u;
 #pragma unroll 1
-            for (int i = (HQ ? TILE : 0) + lane * 16; i < 2 * TILE; i += 1024) {
-                const at_u4 x = *reinterpret_cast<const at_u4*>(lds + stage * 2 * TILE + i);
+            for (int i = lane * 16; i < TILE; i += 1024)
 #pragma unroll
-                for (int e = 0; e < 4; e++) odd |= (uint32_t)((x[e] & EXP) == EXP) | (uint32_t)((x[e] >> 16 & EXP) == EXP);
-            }
+                for (int u = HQ ? 1 : 0; u < 2; u++) {
+                    const at_u4 x = *reinterpret_cast<const at_u4*>(lds + u * VALUES + i);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) odd |= (uint32_t)((x[e] & EXP) == EXP) | (uint32_t)((x[e] >> 16 & EXP) == EXP);
+                }
             return (bool)__any(odd);
         };
-        auto slow_page = [&](int i, int stage) {
-            const int k0 = (p0 + tile + i) * MLXR_PAGE;
-            const uint8_t *kt = lds + stage * 2 * TILE, *vt = kt + TILE;
+        auto slow_page = [&](int k0) {
             const float by = a.scale * 1.4426950408889634f;
 #pragma unroll 1
             for (int e = 0; e < MLXR_PAGE; e++) {
@@ -454,15 +515,15 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 if (key > lim1 || key < low0) continue;
                 float sc = 0.0f;
 #pragma unroll 1
-                for (int s = 0; s < KS; s++) {
-                    const at_u4 k = *reinterpret_cast<const at_u4*>(kt + e * ROW + 16 * ((2 * s + h) ^ (e & (CH - 1))));
+                for (int ks = 0; ks < KS; ks++) {
+                    const at_u4 k = *reinterpret_cast<const at_u4*>(lds + e * ROW + 16 * ((2 * ks + h) ^ at_swz_k<D>(e)));
                     float x[8];
                     if constexpr (HQ) {
-                        const at_u4 y = gload(reinterpret_cast<const at_u4*>(static_cast<const uint16_t*>(a.q) + q_at + 16 * s + 8 * h));
+                        const at_u4 y = gload(reinterpret_cast<const at_u4*>(static_cast<const uint16_t*>(a.q) + q_at + 16 * ks + 8 * h));
 #pragma unroll
                         for (int c = 0; c < 8; c++) x[c] = kv_float<ST>((uint16_t)(y[c / 2] >> 16 * (c & 1)));
                     } else {
-                        const float4 u = gload4(static_cast<const float*>(a.q) + q_at + 16 * s + 8 * h), v = gload4(static_cast<const float*>(a.q) + q_at + 16 * s + 8 * h + 4);
+                        const float4 u = gload4(static_cast<const float*>(a.q) + q_at + 16 * ks + 8 * h), v = gload4(static_cast<const float*>(a.q) + q_at + 16 * ks + 8 * h + 4);
                         x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
                     }
 #pragma unroll
@@ -477,37 +538,24 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 for (int n = 0; n < NV; n++)
 #pragma unroll
                     for (int g = 0; g < 4; g++) {
-                        const uint2 v = *reinterpret_cast<const uint2*>(vt + e * ROW + 16 * ((4 * n + g) ^ (e & (CH - 1))) + 8 * h);
+                        const uint2 v = *reinterpret_cast<const uint2*>(lds + VALUES + e * ROW + 16 * ((4 * n + g) ^ at_swz_v<D>(e)) + 8 * h);
                         const float v4[4] = {kv_float<ST>((uint16_t)v.x), kv_float<ST>((uint16_t)(v.x >> 16)), kv_float<ST>((uint16_t)v.y), kv_float<ST>((uint16_t)(v.y >> 16))};
 #pragma unroll
                         for (int d = 0; d < 4; d++) o[n][4 * g + d] = at_times(c, o[n][4 * g + d]) + (in ? at_times(p, v4[d]) : 0.0f);
                     }
             }
         };
-        while (true) {
+        auto clear = [&] {
             m = -INFINITY;
             l = 0.0f;
 #pragma unroll
             for (int n = 0; n < NV; n++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[n][e] = 0.0f;
-            int i = seek(0), stage = 0;
-            if (i < tiles) issue(i, 0);
-            while (i < tiles) {
-                const int nxt = seek(i + 1);
-                __builtin_amdgcn_s_waitcnt(0);       // this wave's copies of page i landed ...
-                __builtin_amdgcn_s_barrier();        // ... and every wave's; the other stage is free
-                if (nxt < tiles) issue(nxt, stage ^ 1);
-                const int k0 = (p0 + tile + i) * MLXR_PAGE;
-                if (active && k0 <= lim1 && k0 + MLXR_PAGE > low0) {
-                    if (__builtin_expect(careful, 0) && (odd_q || odd_page(stage))) slow_page(i, stage);
-                    else if (k0 + MLXR_PAGE - 1 <= lim0 && k0 >= low1) tile_of(std::false_type{}, i, stage);
-                    else tile_of(std::true_type{}, i, stage);
-                }
-                i = nxt;
-                stage ^= 1;
-            }
-            if (careful) break;
+        };
+        clear();
+        pages_through();
+        {
             float any = 0.0f * l;   // NaN where one is not finite
 #pragma unroll
             for (int n = 0; n < NV; n++)
@@ -517,42 +565,86 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             uint64_t nan_rows = __ballot(nan_q);
             nan_rows |= nan_rows >> 32;
             const bool again = active && any != any && !((nan_rows >> r) & 1);
-            __syncthreads();
+            __syncthreads();      // also: copies of nothing behind the run are done, and the LDS is free
             if (tid == 0) odd_any = 0;
             __syncthreads();
             if (__any(again) && lane == 0) odd_any = 1;
             __syncthreads();
-            if (!odd_any) break;
-            careful = true;
-            odd_q = __any(inf_q);
-            have = -1;
         }
-        l = xor32_sum(l);
-        auto write_out = [&] {
-            if (!active || r >= mine) return;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int64_t to = (int64_t)(sq.row + tok) * a.out_stride + (int64_t)head * D + 4 * h;
-#pragma unroll
-            for (int n = 0; n < NV; n++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    float x[4];
-#pragma unroll
-                    for (int d = 0; d < 4; d++) x[d] = l == 0.0f ? 0.0f : o[n][4 * g + d] * inv;
-                    if constexpr (HQ) {
-                        const uint2 y = {(uint32_t)kv_round<ST>(x[0]) | (uint32_t)kv_round<ST>(x[1]) << 16, (uint32_t)kv_round<ST>(x[2]) | (uint32_t)kv_round<ST>(x[3]) << 16};
-                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + 32 * n + 8 * g) = y;
-                    } else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to + 32 * n + 8 * g) = float4{x[0], x[1], x[2], x[3]};
+        if (__builtin_expect(odd_any, 0)) {
+            odd_q = __any(inf_q);
+            clear();
+#pragma unroll 1
+            for (int i = 0; i < tiles; i++) {
+                const int page = page_of(i), k0 = first_key(i);
+                if (page < 0) continue;
+                copy(K, false, page, MLXR_PAGE, 0);
+                copy(V, true, page, end - k0, VALUES);
+                __builtin_amdgcn_s_waitcnt(0);
+                __syncthreads();
+                if (i % step == turn && seen(k0)) {
+                    if (odd_q || odd_page()) slow_page(k0);
+                    else {
+                        products_k(0);
+                        softmax(std::true_type{}, k0);
+                        products_v(VALUES);
+                    }
                 }
+                __syncthreads();
+            }
+        }
+        constexpr int NR = 16 * NV;
+        if (two) {   // the other pages' results
+            float* to = reinterpret_cast<float*>(lds) + block * (NR + 2) * 64 + lane;
+            if (turn && active) {
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) to[(16 * n + e) * 64] = o[n][e];
+                to[NR * 64] = m;
+                to[(NR + 1) * 64] = l;
+            }
+            __syncthreads();
+            if (!turn && active) {
+                const float m2 = to[NR * 64], l2 = to[(NR + 1) * 64], M = fmaxf(m, m2), c = at_exp2(m - at_safe(M)), c2 = at_exp2(m2 - at_safe(M));
+                m = M;
+                l = c * l + c2 * l2;
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[n][e] = at_times(c, o[n][e]) + at_times(c2, to[(16 * n + e) * 64]);
+            }
+        }
+        const bool holds = active && !turn;
+        l = xor32_sum(l);
+        // four dims 32 n + 8 g + 4 h .. of query `row` of the item
+        auto put = [&](int row, int n, int g, float inv, const float* x) {
+            const int fq = f0 + row, t = fq / G;
+            const int64_t to = (int64_t)(sq.row + t) * a.out_stride + (int64_t)(kvh * G + fq - t * G) * D + 32 * n + 8 * g + 4 * h;
+            float y[4];
+#pragma unroll
+            for (int d = 0; d < 4; d++) y[d] = inv == 0.0f ? 0.0f : x[d] * inv;
+            if constexpr (HQ) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to) = uint2{(uint32_t)kv_round<ST>(y[0]) | (uint32_t)kv_round<ST>(y[1]) << 16, (uint32_t)kv_round<ST>(y[2]) | (uint32_t)kv_round<ST>(y[3]) << 16};
+            else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to) = float4{y[0], y[1], y[2], y[3]};
         };
-        if (tiles == pages) write_out();
-        else {
+        if (tiles == pages) {
+            if (holds && r < mine) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const float x[4] = {o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]};
+                        put(32 * block + r, n, g, inv, x);
+                    }
+            }
+        } else {
             // the runs that hold the item, from the first page's to the last one's
             const uint64_t w0 = pre / per;
             const int parts = (int)((pre + pages - 1) / per - w0) + 1, first_slot = pre == w0 * per ? 0 : 1;
-            auto part_of = [&](uint64_t run, int s) { return wk.part + (2 * run + s) * at_part_floats(D) + (size_t)wave * (D / 4 + 1) * 128 + 2 * lane; };
-            if (active) {
-                float* to = part_of(w, slot);
+            auto part_of = [&](uint64_t run, int s, int qb) { return wk.part + (2 * run + s) * at_part_floats(D) + (size_t)qb * (D / 4 + 1) * 128 + 2 * lane; };
+            if (holds) {
+                float* to = part_of(w, slot, block);
 #pragma unroll
                 for (int n = 0; n < NV; n++)
 #pragma unroll
@@ -562,31 +654,46 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             parts_stored();
             if (tid == 0) last = part_last(wk.count + w0, parts);
             __syncthreads();
-            if (last) {
-                auto of = [&](int k) { return part_of(w0 + k, k == 0 ? first_slot : 0); };
-                float M = -INFINITY;
-                for (int k = 0; k < parts && active; k++) M = fmaxf(M, at_load2(of(k) + D / 4 * 128).x);
-                M = at_safe(M);
-                l = 0.0f;
+            if (last) {   // all waves: eight of a lane's values of 32 queries at a time, four parts in flight
+#pragma unroll 1
+                for (int id = wave; id < blocks * (D / 16); id += AR_WV) {
+                    const int qb = id % blocks, pc = id / blocks;
+                    auto of = [&](int k) { return part_of(w0 + k, k == 0 ? first_slot : 0, qb); };
+                    float M = -INFINITY, sum = 0.0f, x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                    for (int k = 0; k < parts; k += 8) {
+                        float v[8];
 #pragma unroll
-                for (int n = 0; n < NV; n++)
+                        for (int c = 0; c < 8; c++) v[c] = at_load2(of(min(k + c, parts - 1)) + D / 4 * 128).x;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) o[n][e] = 0.0f;
-                for (int k = 0; k < parts && active; k++) {
-                    const float* p = of(k);
-                    const float2 st = at_load2(p + D / 4 * 128);
-                    const float c = at_exp2(st.x - M);   // a part of NaN counts, whatever its maximum: 0 times NaN is NaN
-                    l += c * st.y;
+                        for (int c = 0; c < 8; c++) M = fmaxf(M, v[c]);
+                    }
+                    M = at_safe(M);
+#pragma unroll 1
+                    for (int k = 0; k < parts; k += 4) {
+                        float2 st[4], v[4][4];
 #pragma unroll
-                    for (int n = 0; n < NV; n++)
+                        for (int c = 0; c < 4; c++) {
+                            const float* p = of(min(k + c, parts - 1));
+                            st[c] = at_load2(p + D / 4 * 128);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const float2 x = at_load2(p + (8 * n + e) * 128);
-                            o[n][2 * e] += at_times(c, x.x);
-                            o[n][2 * e + 1] += at_times(c, x.y);
+                            for (int e = 0; e < 4; e++) v[c][e] = at_load2(p + (4 * pc + e) * 128);
                         }
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            if (k + c >= parts) break;
+                            const float f = at_exp2(st[c].x - M);   // a part of NaN counts, whatever its maximum: 0 times NaN is NaN
+                            sum += f * st[c].y;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) { x[2 * e] += at_times(f, v[c][e].x); x[2 * e + 1] += at_times(f, v[c][e].y); }
+                        }
+                    }
+                    if (32 * qb + r < R) {
+                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                        put(32 * qb + r, pc >> 1, 2 * (pc & 1), inv, x);
+                        put(32 * qb + r, pc >> 1, 2 * (pc & 1) + 1, inv, x + 4);
+                    }
                 }
-                write_out();
                 if (tid == 0) part_rearm(wk.count + w0);
             }
         }
@@ -614,7 +721,12 @@ size_t paged_attention_rows_work(const PagedKV& kv, int nH, int rows, int q_type
 hipError_t launch_paged_attention_rows(const AttnRowsArgs& a, hipStream_t s) {
     AtWork wk;
     at_layout(a.kv, a.nH, a.rows, a.work, wk);
-#define AT_GO(ST, D, HQ) hipLaunchKernelGGL((attn_rows_kernel<ST, D, HQ>), dim3(wk.W), dim3(AR_TH), 0, s, a, wk)
+    // more LDS than a launch has by itself is asked for each time: it holds for the current device only
+#define AT_GO(ST, D, HQ) do { \
+        constexpr int LDS = 2 * AR_RING * 64 * D * 2; \
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_rows_kernel<ST, D, HQ>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS)) return e; \
+        hipLaunchKernelGGL((attn_rows_kernel<ST, D, HQ>), dim3(wk.W), dim3(AR_TH), LDS, s, a, wk); \
+    } while (0)
 #define AT_D(ST, HQ) do { if (a.kv.D == 64) AT_GO(ST, 64, HQ); else AT_GO(ST, 128, HQ); } while (0)
     if (a.kv.st == 0) { if (a.q_type) AT_D(0, true); else AT_D(0, false); }
     else { if (a.q_type) AT_D(1, true); else AT_D(1, false); }
