@@ -36,6 +36,7 @@ constexpr int AR_GAP = 2;          // places behind an item
 constexpr int AR_MINPER = 4;       // places of a run at least
 constexpr int AR_RING = 4;         // pages of keys, and of values, in LDS
 constexpr float AT_LAZY = 8.0f;
+#define AT_IN __attribute__((always_inline))   // what holds the operands' registers has to stay in the kernel
 typedef float at_f16 __attribute__((ext_vector_type(16)));
 typedef __bf16 at_b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 at_b2 __attribute__((ext_vector_type(2)));
@@ -85,6 +86,17 @@ __device__ __forceinline__ float2 at_load2(const float* p) {
     return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
+// Values that are the same in all lanes, for the scalar registers: addresses and loops that are not known to be so cost many times more.
+__device__ __forceinline__ int at_one(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t at_one(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)at_one((int)(uint32_t)v) | (uint64_t)(uint32_t)at_one((int)(v >> 32)) << 32);
+}
+__device__ __forceinline__ uint64_t at_one(uint64_t v) { return (uint64_t)at_one((int64_t)v); }
+
+struct AtShared {
+    uint64_t sums[2][AR_WV], found_pre;
+    int found_b, last, odd_any;
+};
 struct AtWork {
     unsigned* count;      // [AR_MAXW] arrivals at the item that starts in a run and goes on behind it; zero between calls
     float* part;          // [2 W] partial results: [AR_WV][D / 4 + 1][64][2]: 32 queries' values, then maximum and sum
@@ -100,6 +112,7 @@ __device__ __forceinline__ AtSeq at_seq(const AttnRowsArgs& a, int b) {
     const int64_t first = min(max(i0, n - len), max(i0, i1));                   // the first of them with a slot
     return AtSeq{(int)max((int64_t)0, i1 - first), (int)max((int64_t)0, len - n + first), (int)(s + first), (int)max((int64_t)0, first - i0)};
 }
+__device__ __forceinline__ AtSeq at_one(const AtSeq& s) { return AtSeq{at_one(s.c), at_one(s.base), at_one(s.row), at_one(s.none)}; }
 // Places of items 0 .. n - 1 of a sequence: min(A + floor(S i / G), cap) + AR_GAP for item i, S pages of queries (AR_M / 64).
 struct AtPlaces {
     static constexpr int S = AR_M / MLXR_PAGE;
@@ -133,20 +146,19 @@ template <int ST, int D, bool HQ>
 __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtWork wk) {
     constexpr int NP = at_parts(ST, HQ), KS = D / 16, NV = D / 32, TILE = 64 * D * 2, ROW = 2 * D, CH = D / 8;   // CH: 16-byte pieces of a row
     constexpr int PW = TILE / 1024 / AR_WV;   // copies a wave and page of keys (or values)
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];   // [AR_RING] pages of keys, then of values; partial results in between
-    __shared__ uint64_t wave_sum64[2][AR_WV], found_pre;
-    __shared__ int found_b, last, odd_any;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];   // [AR_RING] pages of keys, then of values (partial results in between); AtShared
+    AtShared& sh = *reinterpret_cast<AtShared*>(lds + 2 * AR_RING * TILE);
     const PagedKV& kv = a.kv;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = at_one(tid >> 6), r = lane & 31, h = lane >> 5;
     const int G = a.nH / kv.nKV, W = wk.W;
     // neighbouring runs share keys: those of an XCD (workgroups 8 apart) are neighbours
     const int w = W % 8 == 0 ? (int)(blockIdx.x % 8) * (W / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
-    const uint16_t *K = static_cast<const uint16_t*>(kv.k), *V = static_cast<const uint16_t*>(kv.v);
+    const void *K = kv.k, *V = kv.v;
 
     // this workgroup's run of places
-    auto items_of = [&](const AtSeq& s) { return ((int64_t)s.c * G + AR_M - 1) / AR_M; };
-    auto places_of = [&](const AtSeq& s) -> uint64_t { return s.c ? (uint64_t)(AtPlaces(a, G, s.base).cum(items_of(s)) * kv.nKV) : 0; };
-    auto zero = [&](const AtSeq& s) {   // rows without a slot
+    auto items_of = [&](const AtSeq& s) AT_IN { return ((int64_t)s.c * G + AR_M - 1) / AR_M; };
+    auto places_of = [&](const AtSeq& s) AT_IN -> uint64_t { return s.c ? (uint64_t)(AtPlaces(a, G, s.base).cum(items_of(s)) * kv.nKV) : 0; };
+    auto zero = [&](const AtSeq& s) AT_IN {   // rows without a slot
         const int per = a.nH * D * (HQ ? 2 : 4) / 16;
         for (int64_t i = lane; i < (int64_t)s.none * per; i += 64) {
             const int64_t row = s.row - s.none + i / per;
@@ -159,7 +171,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
     {
         uint64_t before = 0, n = 0, chunk = 0;
         int step = 0;
-        auto scan = [&](int c, bool first) {
+        auto scan = [&](int c, bool first) AT_IN {
             const AtSeq s = c + tid < kv.B ? at_seq(a, c + tid) : AtSeq{0, 0, 0, 0};
             n = places_of(s);
             if (first)
@@ -168,7 +180,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     zero(AtSeq{0, 0, __builtin_amdgcn_readlane(s.row, l), __builtin_amdgcn_readlane(s.none, l)});
                 }
             const uint64_t v = wave_scan(n);
-            uint64_t* sums = wave_sum64[step++ & 1];
+            uint64_t* sums = sh.sums[step++ & 1];
             if (lane == 63) sums[wave] = v;
             __syncthreads();
             before = v - n;
@@ -177,6 +189,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             for (int i = 0; i < AR_WV; i++) { before += i < wave ? sums[i] : 0; chunk += sums[i]; }
         };
         for (int c = 0; c < kv.B; c += AR_TH) { scan(c, true); total += chunk; }
+        total = at_one(total);
         per = max((uint64_t)AR_MINPER, (total + W - 1) / W);
         t = (uint64_t)w * per;
         t1 = min(total, t + per);
@@ -185,22 +198,22 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         for (int c = 0; c < kv.B; c += AR_TH) {
             if (kv.B > AR_TH) scan(c, false);
             const uint64_t p = run + before;
-            if (p <= t && t < p + n) { found_b = c + tid; found_pre = p; }
+            if (p <= t && t < p + n) { sh.found_b = c + tid; sh.found_pre = p; }
             run += chunk;
             if (run > t) break;
         }
         __syncthreads();
-        b = __builtin_amdgcn_readfirstlane(found_b);
-        pre = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)found_pre) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(found_pre >> 32)) << 32;
-        sq = at_seq(a, b);
+        b = at_one(sh.found_b);
+        pre = at_one(sh.found_pre);
+        sq = at_one(at_seq(a, b));
     }
     // the item in which the run begins
     int kvh, item, items;
     {
         const AtPlaces pl(a, G, sq.base);
         items = (int)items_of(sq);
-        const uint64_t each = (uint64_t)pl.cum(items), local = t - pre;
-        kvh = (int)(local / each);
+        const uint64_t each = at_one((uint64_t)pl.cum(items)), local = t - pre;
+        kvh = at_one((int)(local / each));
         pre += kvh * each;
         const int64_t at = (int64_t)(t - pre);
         int64_t lo = 0, step = 1;
@@ -210,20 +223,20 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             lo += step * (63 - (int)__builtin_clzll(__ballot(i < items && pl.cum(i) <= at)));
             if (step == 1) break;
         }
-        item = __builtin_amdgcn_readfirstlane((int)lo);
-        pre += pl.cum(item);
+        item = at_one((int)lo);
+        pre += at_one(pl.cum(item));
     }
     int slot = 0;   // partial results of this workgroup: its first item's, then its last one's
     while (true) {
         // pre: the item's first place
         const AtPlaces pl(a, G, sq.base);
         const int f0 = item * AR_M, R = min((int64_t)AR_M, (int64_t)sq.c * G - f0);
-        auto first_of = [&](int tok) { return a.window > 0 ? max(0, sq.base + tok + 1 - a.window) : 0; };
-        const int p0 = first_of(f0 / G) / MLXR_PAGE, pages = (sq.base + (f0 + R - 1) / G) / MLXR_PAGE - p0 + 1;
+        auto first_of = [&](int tok) AT_IN { return a.window > 0 ? max(0, sq.base + tok + 1 - a.window) : 0; };
+        const int p0 = at_one(first_of(f0 / G) / MLXR_PAGE), pages = at_one((sq.base + (f0 + R - 1) / G) / MLXR_PAGE - p0 + 1);
         const int tile = (int)(t - pre), tiles = (int)min((int64_t)(pages - tile), (int64_t)(t1 - t));
         // on to the run's next item
-        auto ahead = [&] {
-            const uint64_t n = (uint64_t)(pl.cum(item + 1) - pl.cum(item));
+        auto ahead = [&]() AT_IN {
+            const uint64_t n = at_one((uint64_t)(pl.cum(item + 1) - pl.cum(item)));
             t = pre + n;
             if (t >= t1) return false;
             pre = t;
@@ -231,7 +244,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 item = 0;
                 if (++kvh == kv.nKV) {
                     kvh = 0;
-                    do sq = at_seq(a, ++b);   // t < t1 <= total: another one has rows
+                    do sq = at_one(at_seq(a, ++b));   // t < t1 <= total: another one has rows
                     while (sq.c == 0);
                     items = (int)items_of(sq);
                 }
@@ -245,36 +258,38 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         }
         // this wave's queries, and the other pages' of few
         const bool two = R <= AR_M / 2;
-        const int step = two ? 2 : 1, turn = two ? wave >> 2 : 0, block = two ? wave & 3 : wave, blocks = (R + 31) / 32;
+        const int turn = two ? wave >> 2 : 0, block = two ? wave & 3 : wave, blocks = (R + 31) / 32;
         const int mine = min(32, R - 32 * block);                 // how many, if above 0
         const bool active = mine > 0;
         const int f = f0 + (active ? 32 * block + min(r, mine - 1) : 0), tok = f / G, head = kvh * G + f % G;
         const int lim = sq.base + tok, low = first_of(tok);       // the slots that this lane's query attends: low .. lim
         const int lim0 = __builtin_amdgcn_readlane(lim, 0), lim1 = __builtin_amdgcn_readlane(lim, 31), low0 = __builtin_amdgcn_readlane(low, 0), low1 = __builtin_amdgcn_readlane(low, 31);
         const int64_t q_at = (int64_t)(sq.row + tok) * a.q_stride + (int64_t)head * D;
-        // page numbers, one a lane, 64 at a time; -1 behind the run and where there is none
-        int have = 0, ids = paged_page(kv, b, p0 + tile + min(lane, tiles - 1));
-        auto page_of = [&](int i) {
-            if (i >= tiles) return -1;
+        // where pages are in the pools (bytes), one a lane, 64 at a time; below 0 where there is none
+        int have = 0;
+        int64_t offs;
+        auto look = [&]() AT_IN {
+            const int page = paged_page(kv, b, p0 + tile + min(64 * have + lane, tiles - 1));
+            offs = page < 0 ? -1 : ((int64_t)page * kv.nKV + kvh) * TILE;
+        };
+        look();
+        auto page_of = [&](int i) AT_IN -> int64_t {
             if ((i >> 6) != have) {
                 have = i >> 6;
-                ids = paged_page(kv, b, p0 + tile + min(64 * have + lane, tiles - 1));
+                look();
             }
-            return __builtin_amdgcn_readlane(ids, i & 63);
+            return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)offs, i & 63) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(offs >> 32), i & 63) << 32);
         };
-        // this wave's share of a page's copy: its first `rows` rows, and zeros behind them (nothing is read of a page that is not there)
-        auto copy = [&](const uint16_t* pool, bool values, int page, int rows, uint32_t to) {
-            const uint16_t* from = pool + (page < 0 ? 0 : paged_row(kv, page, kvh, 0));
-            const int bytes = page < 0 ? 0 : max(0, min(MLXR_PAGE, rows)) * ROW;
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, bytes, 0x00020000);
+        // a KiB of this wave's share of a page's copy: what lies in its first `bytes`, and zeros behind (nothing is read of a page that is not there)
+        auto copy = [&](const void* pool, bool values, int64_t off, int bytes, uint32_t to, int j) AT_IN {
+            const uint8_t* from = static_cast<const uint8_t*>(pool) + off;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, at_one(off < 0 ? 0 : bytes), 0x00020000);
             uint8_t* dst = lds + to;
-#pragma unroll
-            for (int j = 0; j < PW; j++) {
-                const int piece = wave * PW + j, key = piece * (64 / CH) + lane / CH;
-                const int swz = values ? at_swz_v<D>(key) : at_swz_k<D>(key);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (at_lptr)(dst + piece * 1024), 16, key * ROW + 16 * (lane % CH ^ swz), 0, 0, 0);
-            }
+            const int piece = wave * PW + j, key = piece * (64 / CH) + lane / CH, swz = values ? at_swz_v<D>(key) : at_swz_k<D>(key);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (at_lptr)(dst + piece * 1024), 16, key * ROW + 16 * (lane % CH ^ swz), 0, 0, 0);
         };
+        const int end = sq.base + sq.c;
+        auto rows_of = [&](int i) AT_IN { return max(0, min(MLXR_PAGE, end - (p0 + tile + i) * MLXR_PAGE)) * ROW; };   // bytes of page i in front of the sequence's end
         // queries as operands: dims 16 s + 8 h .. + 7 of query r
         at_u4 q[KS][NP];
         float cl = HQ ? fabsf(a.scale) * 1.4426950408889634f : 1.0f;   // scores to powers of two
@@ -337,30 +352,37 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         at_f16 s[2];         // scores of a page, keys 32 kb + 8 (i / 4) + 4 h + i % 4
         at_u4 pr[HQ ? 4 : 1];   // p of a page, rounded (HQ); s otherwise
         constexpr uint32_t VALUES = AR_RING * TILE;
-        auto first_key = [&](int i) { return (p0 + tile + i) * MLXR_PAGE; };
-        auto products_k = [&](uint32_t at) {
+        auto first_key = [&](int i) AT_IN { return (p0 + tile + i) * MLXR_PAGE; };
+        constexpr int KA = 4, VA = 6;      // fragments in registers: read KA - 1 (VA - 1) steps ahead of their products
+        at_u4 kf[KA][2];
+        uint32_t kaddr;
+        auto kread = [&](int ks) AT_IN {
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++) kf[ks % KA][kb] = *reinterpret_cast<const at_u4*>(lds + ((kaddr ^ (32u * ks)) + 32u * ROW * kb));
+        };
+        auto begin_k = [&](uint32_t at) AT_IN {
             int ln = lane;
             asm volatile("" : "+v"(ln));   // addresses are made here, not kept across pages
-            const uint32_t lr = ln & 31, lh = ln >> 5, kaddr = at + lr * ROW + 16 * (lh ^ at_swz_k<D>(lr));   // ^ 32 ks, + 32 ROW kb
-            at_u4 k[2][2];   // the next step's keys are read while this one's products issue
-            auto kread = [&](int ks) {
+            const uint32_t lr = ln & 31, lh = ln >> 5;
+            kaddr = at + lr * ROW + 16 * (lh ^ at_swz_k<D>(lr));              // ^ 32 ks, + 32 ROW kb
 #pragma unroll
-                for (int kb = 0; kb < 2; kb++) k[ks & 1][kb] = *reinterpret_cast<const at_u4*>(lds + ((kaddr ^ (32u * ks)) + 32u * ROW * kb));
-            };
-            kread(0);
+            for (int ks = 0; ks < KA - 1; ks++) kread(ks);
+        };
+        auto products_k = [&](auto beside) AT_IN {   // beside(ks): what else each step asks for
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 __builtin_amdgcn_sched_barrier(0);
-                if (ks + 1 < KS) kread(ks + 1);
+                if (ks + KA - 1 < KS) kread(ks + KA - 1);
+                beside(ks);
 #pragma unroll
                 for (int p = 0; p < NP; p++)
 #pragma unroll
-                    for (int kb = 0; kb < 2; kb++) s[kb] = at_mfma<ST>(k[ks & 1][kb], q[ks][p], ks + p ? s[kb] : at_f16{0.0f});
+                    for (int kb = 0; kb < 2; kb++) s[kb] = at_mfma<ST>(kf[ks % KA][kb], q[ks][p], ks + p ? s[kb] : at_f16{0.0f});
             }
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto softmax = [&](auto CARE, int k0) {
-            if (k0 + MLXR_PAGE - 1 > lim0 || k0 < low1)   // some query does not attend all of the page
+        auto softmax = [&](auto CARE, int k0) AT_IN {
+            if (__builtin_expect(k0 + MLXR_PAGE - 1 > lim0 || k0 < low1, 0))   // some query does not attend all of the page
 #pragma unroll
                 for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -401,22 +423,21 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     at_split<ST, HQ>(p8, &pr[st]);
                 }
         };
-        auto products_v = [&](uint32_t at) {
+        auto products_v = [&](uint32_t at) AT_IN {
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const uint32_t lh = ln >> 5, j = ln & 15;
             const uint32_t vaddr = at + (4 * lh + (j >> 2)) * ROW + 16 * ((2 * (ln >> 4 & 1) + ((j & 3) >> 1)) ^ (4 * (j >> (D == 128 ? 2 : 3)) + lh)) + 8 * (j & 1);
-            // V^T fragments (16 keys st, 32 dims n) f = NV st + n, two ahead of the products
-            uint2 v[3][2];
-            auto vread = [&](int f) {
+            uint2 v[VA][2];   // V^T fragments (16 keys st, 32 dims n) f = NV st + n
+            auto vread = [&](int f) AT_IN {
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const uint32_t ad = (vaddr ^ (64u * (f % NV)) ^ (32u * u)) + 8u * ROW * u + 16u * ROW * (f / NV);
-                    v[f % 3][u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lv4)(lds + ad)));
+                    v[f % VA][u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lv4)(lds + ad)));
                 }
             };
-            vread(0);
-            vread(1);
+#pragma unroll
+            for (int f = 0; f < VA - 1; f++) vread(f);
 #pragma unroll
             for (int st = 0; st < 4; st++) {
                 at_u4 pp[NP];
@@ -431,70 +452,94 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 for (int n = 0; n < NV; n++) {
                     const int f = NV * st + n;
                     __builtin_amdgcn_sched_barrier(0);
-                    if (f + 2 < 4 * NV) vread(f + 2);
-                    const at_u4 vt = {v[f % 3][0].x, v[f % 3][0].y, v[f % 3][1].x, v[f % 3][1].y};
+                    if (f + VA - 1 < 4 * NV) vread(f + VA - 1);
+                    const at_u4 vt = {v[f % VA][0].x, v[f % VA][0].y, v[f % VA][1].x, v[f % VA][1].y};
 #pragma unroll
                     for (int p = 0; p < NP; p++) o[n] = at_mfma<ST>(vt, pp[p], o[n]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto seen = [&](int k0) { return active && k0 <= lim1 && k0 + MLXR_PAGE > low0; };    // some query attends some of the page
-        // The run's pages, `step` of them a turn, two barriers a turn: at the first one waves 0 .. 3 begin the turn's products, at the second one
-        // waves 4 .. 7 do. Turn j's keys are asked for three turns ahead (one, where pages go in pairs), its values a turn later, after
-        // the first barrier: what turn j - 1 read of keys and turn j - 2 of values is free then.
-        const int end = sq.base + sq.c;
-        auto pages_through = [&] {
-            const int turns = (tiles + step - 1) / step, far = two ? 1 : AR_RING - 1;
+        // pages of the run that some query attends some of: lo .. hi - 1
+        const int lo = active ? low0 / MLXR_PAGE - (p0 + tile) : 0, hi = active ? min(tiles, lim1 / MLXR_PAGE - (p0 + tile) + 1) : 0;
+        // The run's pages, `STEP` of them a turn, two barriers a turn: behind the first one waves 0 .. 3 multiply (the values of the turn before,
+        // then its keys), behind the second one waves 4 .. 7. Among turn j's products a wave asks for turn j + FAR's keys and the values
+        // of the turn in front of that, into what all waves have read before turn j's first barrier.
+        auto pages_through = [&](auto STEPC) AT_IN {
+            constexpr int STEP = decltype(STEPC)::value, FAR = AR_RING / STEP - 1;
+            const int turns = (tiles + STEP - 1) / STEP;
             const bool late = wave >= 4;
-            int next[2] = {-1, -1};    // pages whose keys were asked for last: their values are next
-            uint32_t valid = 0;        // of the last 32 pages, by number
-            auto ask = [&](int j) {    // turn j's keys, turn j - 1's values
+            int64_t keys[STEP], values[STEP];   // the pages of the turn that is asked for, and of the one before
+            int key_at[STEP], value_at[STEP], value_bytes[STEP];
+            uint32_t valid = 0;        // whether the pages asked for are there, the last one's bit lowest
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    if (g >= step) break;
-                    const int i = j * step + g, page = page_of(i);
-                    copy(K, false, page, MLXR_PAGE, (i & (AR_RING - 1)) * TILE);
-                    if (j) copy(V, true, next[g], end - first_key(i - step), VALUES + ((i - step) & (AR_RING - 1)) * TILE);
-                    next[g] = page;
-                    valid = (valid & ~(1u << (i & 31))) | (uint32_t)(page >= 0) << (i & 31);
+            for (int g = 0; g < STEP; g++) keys[g] = -1;
+            auto plan = [&](int j) AT_IN {    // turn j's keys, turn j - 1's values
+#pragma unroll
+                for (int g = 0; g < STEP; g++) {
+                    const int i = j * STEP + g;
+                    values[g] = keys[g];
+                    value_bytes[g] = rows_of(i - STEP);
+                    value_at[g] = VALUES + ((i - STEP) & (AR_RING - 1)) * TILE;
+                    keys[g] = i < tiles ? page_of(i) : -1;
+                    key_at[g] = (i & (AR_RING - 1)) * TILE;
+                    valid = 2 * valid + (keys[g] >= 0);
                 }
             };
-            auto first_barrier = [&](int j) {
-                if (two) __builtin_amdgcn_s_waitcnt(0x0F70);                          // vmcnt(0)
-                else __builtin_amdgcn_s_waitcnt(PW == 2 ? 0x0F78 : 0x0F74);           // all but the last two turns' 4 PW copies
+            constexpr int PIECES = 2 * STEP * PW;
+            auto ask = [&](int n) AT_IN {     // of PIECES
+                const int g = n / (2 * PW), c = n % (2 * PW);
+                if (c < PW) copy(K, false, keys[g], TILE, key_at[g], c);
+                else copy(V, true, values[g], value_bytes[g], value_at[g], c - PW);
+            };
+            auto beside = [&](int ks) AT_IN {
+                if (ks % (KS / PIECES) == 0) ask(ks / (KS / PIECES));
+            };
+            auto first_barrier = [&]() AT_IN {
+                // this wave's copies for the turn landed: all but those of the FAR - 1 turns behind it, PIECES each
+                __builtin_amdgcn_s_waitcnt(STEP == 2 ? 0x0F70 : PW == 2 ? 0x0F78 : 0x0F74);
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                ask(j + far);
             };
-            auto second_barrier = [&] {
+            auto second_barrier = [&]() AT_IN {
                 asm volatile("" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
             };
-            for (int j = 0; j < far; j++) ask(j);
-            if (late) first_barrier(0), second_barrier();
-            else first_barrier(0);
-            products_k((turn & (AR_RING - 1)) * TILE);   // of a page that is not there: not used
+#pragma unroll
+            for (int j = 0; j < FAR; j++) {
+                plan(j);
+#pragma unroll
+                for (int n = 0; n < PIECES; n++) ask(n);
+            }
+            first_barrier();
+            if (late) second_barrier();
+            begin_k(turn * TILE);
+            plan(FAR);
+            products_k(beside);              // of a page that is not there: not used
+#pragma unroll 1
             for (int j = 0; j < turns; j++) {
-                const int i = j * step + turn, k0 = first_key(i);
-                const bool on = i < tiles && seen(k0) && (valid >> (i & 31) & 1);
-                if (late) first_barrier(j + 1);
+                const int i = j * STEP + turn;
+                const bool on = i >= lo && i < hi && (valid >> ((FAR + 1) * STEP - 1 - turn) & 1);
+                if (late) first_barrier();
                 else second_barrier();
-                if (on) softmax(std::false_type{}, k0);
+                if (on) softmax(std::false_type{}, first_key(i));
                 if (late) second_barrier();
-                else first_barrier(j + 1);
+                else first_barrier();
                 if (on) products_v(VALUES + (i & (AR_RING - 1)) * TILE);
-                products_k(((i + step) & (AR_RING - 1)) * TILE);
+                begin_k(((i + STEP) & (AR_RING - 1)) * TILE);
+                plan(j + 1 + FAR);
+                products_k(beside);
             }
             if (!late) second_barrier();
+            __builtin_amdgcn_s_waitcnt(0);   // copies of nothing
         };
         // Infinities and NaN. A product of 0 and infinity, or of a masked p and NaN, is not what the formula has, nor are parts of an
         // infinite query or key. Where a result is not finite the item's pages are taken again, with care: a page that holds something
         // infinite or NaN (keys only matter in parts) key by key in fp32; a score of -infinity is a key that takes no part, an infinite value
         // stays, however small its p is.
         bool odd_q = false;
-        auto odd_page = [&] {
+        auto odd_page = [&]() AT_IN {
             uint32_t odd = 0;
             constexpr uint32_t EXP = ST == 0 ? 0x7f80u : 0x7c00u;
 #pragma unroll 1
@@ -507,7 +552,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 }
             return (bool)__any(odd);
         };
-        auto slow_page = [&](int k0) {
+        auto slow_page = [&](int k0) AT_IN {
             const float by = a.scale * 1.4426950408889634f;
 #pragma unroll 1
             for (int e = 0; e < MLXR_PAGE; e++) {
@@ -545,7 +590,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     }
             }
         };
-        auto clear = [&] {
+        auto clear = [&]() AT_IN {
             m = -INFINITY;
             l = 0.0f;
 #pragma unroll
@@ -554,7 +599,8 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 for (int e = 0; e < 16; e++) o[n][e] = 0.0f;
         };
         clear();
-        pages_through();
+        if (two) pages_through(std::integral_constant<int, 2>{});
+        else pages_through(std::integral_constant<int, 1>{});
         {
             float any = 0.0f * l;   // NaN where one is not finite
 #pragma unroll
@@ -565,27 +611,32 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             uint64_t nan_rows = __ballot(nan_q);
             nan_rows |= nan_rows >> 32;
             const bool again = active && any != any && !((nan_rows >> r) & 1);
-            __syncthreads();      // also: copies of nothing behind the run are done, and the LDS is free
-            if (tid == 0) odd_any = 0;
             __syncthreads();
-            if (__any(again) && lane == 0) odd_any = 1;
+            if (tid == 0) sh.odd_any = 0;
+            __syncthreads();
+            if (__any(again) && lane == 0) sh.odd_any = 1;
             __syncthreads();
         }
-        if (__builtin_expect(odd_any, 0)) {
+        if (__builtin_expect(sh.odd_any, 0)) {
             odd_q = __any(inf_q);
             clear();
 #pragma unroll 1
             for (int i = 0; i < tiles; i++) {
-                const int page = page_of(i), k0 = first_key(i);
+                const int64_t page = page_of(i);
+                const int k0 = first_key(i);
                 if (page < 0) continue;
-                copy(K, false, page, MLXR_PAGE, 0);
-                copy(V, true, page, end - k0, VALUES);
+#pragma unroll
+                for (int n = 0; n < PW; n++) {
+                    copy(K, false, page, TILE, 0, n);
+                    copy(V, true, page, rows_of(i), VALUES, n);
+                }
                 __builtin_amdgcn_s_waitcnt(0);
                 __syncthreads();
-                if (i % step == turn && seen(k0)) {
+                if ((!two || (i & 1) == turn) && i >= lo && i < hi) {
                     if (odd_q || odd_page()) slow_page(k0);
                     else {
-                        products_k(0);
+                        begin_k(0);
+                        products_k([](int) {});
                         softmax(std::true_type{}, k0);
                         products_v(VALUES);
                     }
@@ -618,7 +669,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         const bool holds = active && !turn;
         l = xor32_sum(l);
         // four dims 32 n + 8 g + 4 h .. of query `row` of the item
-        auto put = [&](int row, int n, int g, float inv, const float* x) {
+        auto put = [&](int row, int n, int g, float inv, const float* x) AT_IN {
             const int fq = f0 + row, t = fq / G;
             const int64_t to = (int64_t)(sq.row + t) * a.out_stride + (int64_t)(kvh * G + fq - t * G) * D + 32 * n + 8 * g + 4 * h;
             float y[4];
@@ -642,7 +693,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             // the runs that hold the item, from the first page's to the last one's
             const uint64_t w0 = pre / per;
             const int parts = (int)((pre + pages - 1) / per - w0) + 1, first_slot = pre == w0 * per ? 0 : 1;
-            auto part_of = [&](uint64_t run, int s, int qb) { return wk.part + (2 * run + s) * at_part_floats(D) + (size_t)qb * (D / 4 + 1) * 128 + 2 * lane; };
+            auto part_of = [&](uint64_t run, int s, int qb) AT_IN { return wk.part + (2 * run + s) * at_part_floats(D) + (size_t)qb * (D / 4 + 1) * 128 + 2 * lane; };
             if (holds) {
                 float* to = part_of(w, slot, block);
 #pragma unroll
@@ -652,13 +703,13 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 at_store2(to + D / 4 * 128, m, l);
             }
             parts_stored();
-            if (tid == 0) last = part_last(wk.count + w0, parts);
+            if (tid == 0) sh.last = part_last(wk.count + w0, parts);
             __syncthreads();
-            if (last) {   // all waves: eight of a lane's values of 32 queries at a time, four parts in flight
+            if (sh.last) {   // all waves: eight of a lane's values of 32 queries at a time, four parts in flight
 #pragma unroll 1
                 for (int id = wave; id < blocks * (D / 16); id += AR_WV) {
                     const int qb = id % blocks, pc = id / blocks;
-                    auto of = [&](int k) { return part_of(w0 + k, k == 0 ? first_slot : 0, qb); };
+                    auto of = [&](int k) AT_IN { return part_of(w0 + k, k == 0 ? first_slot : 0, qb); };
                     float M = -INFINITY, sum = 0.0f, x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
                     for (int k = 0; k < parts; k += 8) {
@@ -723,7 +774,7 @@ hipError_t launch_paged_attention_rows(const AttnRowsArgs& a, hipStream_t s) {
     at_layout(a.kv, a.nH, a.rows, a.work, wk);
     // more LDS than a launch has by itself is asked for each time: it holds for the current device only
 #define AT_GO(ST, D, HQ) do { \
-        constexpr int LDS = 2 * AR_RING * 64 * D * 2; \
+        constexpr int LDS = 2 * AR_RING * 64 * D * 2 + (int)sizeof(AtShared); \
         if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_rows_kernel<ST, D, HQ>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS)) return e; \
         hipLaunchKernelGGL((attn_rows_kernel<ST, D, HQ>), dim3(wk.W), dim3(AR_TH), LDS, s, a, wk); \
     } while (0)
