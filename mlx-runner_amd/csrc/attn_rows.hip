@@ -86,6 +86,9 @@ __device__ __forceinline__ float2 at_load2(const float* p) {
     return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
+// The LDS transpose read. Of a pointer of its own (__restrict__): otherwise the compiler, which cannot tell what it reads from what copies write,
+// waits for every copy in flight in front of it.
+__device__ __forceinline__ uint2 at_read_tr(const uint8_t* __restrict__ p) { return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lv4)p)); }
 // Values that are the same in all lanes, for the scalar registers: addresses and loops that are not known to be so cost many times more.
 __device__ __forceinline__ int at_one(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t at_one(int64_t v) {
@@ -353,7 +356,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         at_u4 pr[HQ ? 4 : 1];   // p of a page, rounded (HQ); s otherwise
         constexpr uint32_t VALUES = AR_RING * TILE;
         auto first_key = [&](int i) AT_IN { return (p0 + tile + i) * MLXR_PAGE; };
-        constexpr int KA = 4, VA = 6;      // fragments in registers: read KA - 1 (VA - 1) steps ahead of their products
+        constexpr int KA = HQ ? 3 : 2, VA = HQ ? 5 : 3;      // fragments in registers: read KA - 1 (VA - 1) steps of NP products ahead
         at_u4 kf[KA][2];
         uint32_t kaddr;
         auto kread = [&](int ks) AT_IN {
@@ -433,7 +436,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const uint32_t ad = (vaddr ^ (64u * (f % NV)) ^ (32u * u)) + 8u * ROW * u + 16u * ROW * (f / NV);
-                    v[f % VA][u] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lv4)(lds + ad)));
+                    v[f % VA][u] = at_read_tr(lds + ad);
                 }
             };
 #pragma unroll
@@ -474,6 +477,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             uint32_t valid = 0;        // whether the pages asked for are there, the last one's bit lowest
 #pragma unroll
             for (int g = 0; g < STEP; g++) keys[g] = -1;
+            for (auto& x : pr) x = at_u4{0, 0, 0, 0};   // or an item's would be kept for the next one
             auto plan = [&](int j) AT_IN {    // turn j's keys, turn j - 1's values
 #pragma unroll
                 for (int g = 0; g < STEP; g++) {
