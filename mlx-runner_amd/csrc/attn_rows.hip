@@ -363,11 +363,13 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
 #pragma unroll
             for (int kb = 0; kb < 2; kb++) kf[ks % KA][kb] = *reinterpret_cast<const at_u4*>(lds + ((kaddr ^ (32u * ks)) + 32u * ROW * kb));
         };
-        auto begin_k = [&](uint32_t at) AT_IN {
+        auto find_k = [&](uint32_t at) AT_IN {
             int ln = lane;
             asm volatile("" : "+v"(ln));   // addresses are made here, not kept across pages
             const uint32_t lr = ln & 31, lh = ln >> 5;
             kaddr = at + lr * ROW + 16 * (lh ^ at_swz_k<D>(lr));              // ^ 32 ks, + 32 ROW kb
+        };
+        auto begin_k = [&]() AT_IN {
 #pragma unroll
             for (int ks = 0; ks < KA - 1; ks++) kread(ks);
         };
@@ -426,21 +428,21 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     at_split<ST, HQ>(p8, &pr[st]);
                 }
         };
-        auto products_v = [&](uint32_t at) AT_IN {
+        uint2 vf[VA][2];   // V^T fragments (16 keys st, 32 dims n) f = NV st + n
+        uint32_t vaddr;
+        auto vread = [&](int f) AT_IN {
+#pragma unroll
+            for (int u = 0; u < 2; u++) vf[f % VA][u] = at_read_tr(lds + ((vaddr ^ (64u * (f % NV)) ^ (32u * u)) + 8u * ROW * u + 16u * ROW * (f / NV)));
+        };
+        auto begin_v = [&](uint32_t at) AT_IN {
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const uint32_t lh = ln >> 5, j = ln & 15;
-            const uint32_t vaddr = at + (4 * lh + (j >> 2)) * ROW + 16 * ((2 * (ln >> 4 & 1) + ((j & 3) >> 1)) ^ (4 * (j >> (D == 128 ? 2 : 3)) + lh)) + 8 * (j & 1);
-            uint2 v[VA][2];   // V^T fragments (16 keys st, 32 dims n) f = NV st + n
-            auto vread = [&](int f) AT_IN {
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const uint32_t ad = (vaddr ^ (64u * (f % NV)) ^ (32u * u)) + 8u * ROW * u + 16u * ROW * (f / NV);
-                    v[f % VA][u] = at_read_tr(lds + ad);
-                }
-            };
+            vaddr = at + (4 * lh + (j >> 2)) * ROW + 16 * ((2 * (ln >> 4 & 1) + ((j & 3) >> 1)) ^ (4 * (j >> (D == 128 ? 2 : 3)) + lh)) + 8 * (j & 1);
 #pragma unroll
             for (int f = 0; f < VA - 1; f++) vread(f);
+        };
+        auto products_v = [&](auto beside) AT_IN {   // beside(f): what else each step reads
 #pragma unroll
             for (int st = 0; st < 4; st++) {
                 at_u4 pp[NP];
@@ -456,7 +458,8 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     const int f = NV * st + n;
                     __builtin_amdgcn_sched_barrier(0);
                     if (f + VA - 1 < 4 * NV) vread(f + VA - 1);
-                    const at_u4 vt = {v[f % VA][0].x, v[f % VA][0].y, v[f % VA][1].x, v[f % VA][1].y};
+                    else beside(f);
+                    const at_u4 vt = {vf[f % VA][0].x, vf[f % VA][0].y, vf[f % VA][1].x, vf[f % VA][1].y};
 #pragma unroll
                     for (int p = 0; p < NP; p++) o[n] = at_mfma<ST>(vt, pp[p], o[n]);
                 }
@@ -491,17 +494,20 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 }
             };
             constexpr int PIECES = 2 * STEP * PW;
-            auto ask = [&](int n) AT_IN {     // of PIECES
-                const int g = n / (2 * PW), c = n % (2 * PW);
-                if (c < PW) copy(K, false, keys[g], TILE, key_at[g], c);
-                else copy(V, true, values[g], value_bytes[g], value_at[g], c - PW);
+            auto ask = [&](int n) AT_IN {     // of PIECES, values first
+                const int g = n / PW % STEP, c = n % PW;
+                if (n < PIECES / 2) copy(V, true, values[g], value_bytes[g], value_at[g], c);
+                else copy(K, false, keys[g], TILE, key_at[g], c);
             };
             auto beside = [&](int ks) AT_IN {
                 if (ks % (KS / PIECES) == 0) ask(ks / (KS / PIECES));
             };
             auto first_barrier = [&]() AT_IN {
-                // this wave's copies for the turn landed: all but those of the FAR - 1 turns behind it, PIECES each
-                __builtin_amdgcn_s_waitcnt(STEP == 2 ? 0x0F70 : PW == 2 ? 0x0F78 : 0x0F74);
+                // in front of turn j: this wave's copies of its keys and of the values before landed, and of its values where they are asked for
+                // in time (STEP 1: all but turn j + 1's keys and what turn j + 2 asked for)
+                constexpr int LATER = STEP == 2 ? 0 : PIECES / 2 + PIECES;
+                static_assert(LATER < 16, "the low bits of the count");
+                __builtin_amdgcn_s_waitcnt(0x0F70 | LATER);
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
             };
@@ -514,12 +520,13 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             for (int j = 0; j < FAR; j++) {
                 plan(j);
 #pragma unroll
-                for (int n = 0; n < PIECES; n++) ask(n);
+                for (int n = j ? 0 : PIECES / 2; n < PIECES; n++) ask(n);
             }
+            plan(FAR);
             first_barrier();
             if (late) second_barrier();
-            begin_k(turn * TILE);
-            plan(FAR);
+            find_k(turn * TILE);
+            begin_k();
             products_k(beside);              // of a page that is not there: not used
 #pragma unroll 1
             for (int j = 0; j < turns; j++) {
@@ -527,13 +534,21 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 const bool on = i >= lo && i < hi && (valid >> ((FAR + 1) * STEP - 1 - turn) & 1);
                 if (late) first_barrier();
                 else second_barrier();
-                if (on) softmax(std::false_type{}, first_key(i));
+                plan(j + 1 + FAR);
+                if (on) {
+                    if (STEP == 1) begin_v(VALUES + (i & (AR_RING - 1)) * TILE);
+                    softmax(std::false_type{}, first_key(i));
+                }
                 if (late) second_barrier();
                 else first_barrier();
-                if (on) products_v(VALUES + (i & (AR_RING - 1)) * TILE);
-                begin_k(((i + STEP) & (AR_RING - 1)) * TILE);
-                plan(j + 1 + FAR);
+                __builtin_amdgcn_s_setprio(1);
+                find_k(((i + STEP) & (AR_RING - 1)) * TILE);
+                if (on) {
+                    if (STEP == 2) begin_v(VALUES + (i & (AR_RING - 1)) * TILE);
+                    products_v([&](int f) AT_IN { if (f - 4 * NV + VA - 1 < KA - 1) kread(f - 4 * NV + VA - 1); });
+                } else begin_k();
                 products_k(beside);
+                __builtin_amdgcn_s_setprio(0);
             }
             if (!late) second_barrier();
             __builtin_amdgcn_s_waitcnt(0);   // copies of nothing
@@ -639,10 +654,12 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 if ((!two || (i & 1) == turn) && i >= lo && i < hi) {
                     if (odd_q || odd_page()) slow_page(k0);
                     else {
-                        begin_k(0);
+                        find_k(0);
+                        begin_k();
                         products_k([](int) {});
                         softmax(std::true_type{}, k0);
-                        products_v(VALUES);
+                        begin_v(VALUES);
+                        products_v([](int) {});
                     }
                 }
                 __syncthreads();
