@@ -96,9 +96,17 @@ __device__ __forceinline__ int64_t at_one(int64_t v) {
 }
 __device__ __forceinline__ uint64_t at_one(uint64_t v) { return (uint64_t)at_one((int64_t)v); }
 
+// a / b for a below 2^52: the compiler's own division of 64 bits is a page of code.
+__device__ __forceinline__ uint64_t at_div(uint64_t a, uint64_t b) {
+    uint64_t q = (uint64_t)((double)a / (double)b);
+    if (q * b > a) q--;
+    if (a - q * b >= b) q++;
+    return q;
+}
+
 struct AtShared {
     uint64_t sums[2][AR_WV], found_pre;
-    int found_b, last, odd_any;
+    int found_b, last, odd[AR_WV];
 };
 struct AtWork {
     unsigned* count;      // [AR_MAXW] arrivals at the item that starts in a run and goes on behind it; zero between calls
@@ -133,6 +141,7 @@ struct AtPlaces {
         for (int k = 1; k < S; k++) n += max(0, v - (k * G + S - 1) / S);
         return n;
     }
+    __device__ __forceinline__ int64_t of(int item) const { return min(A + (int64_t)((uint32_t)item * (uint32_t)S / (uint32_t)G), cap) + AR_GAP; }   // items are below 2^23
     __device__ __forceinline__ int64_t cum(int64_t n) const {
         const int64_t m = min(n, bend);
         const uint32_t u = (uint32_t)m / (uint32_t)G, v = (uint32_t)m % (uint32_t)G;
@@ -193,7 +202,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         };
         for (int c = 0; c < kv.B; c += AR_TH) { scan(c, true); total += chunk; }
         total = at_one(total);
-        per = max((uint64_t)AR_MINPER, (total + W - 1) / W);
+        per = max((uint64_t)AR_MINPER, at_one(at_div(total + W - 1, W)));
         t = (uint64_t)w * per;
         t1 = min(total, t + per);
         if (t >= total) return;   // fewer runs than workgroups
@@ -216,7 +225,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         const AtPlaces pl(a, G, sq.base);
         items = (int)items_of(sq);
         const uint64_t each = at_one((uint64_t)pl.cum(items)), local = t - pre;
-        kvh = at_one((int)(local / each));
+        kvh = at_one((int)at_div(local, each));
         pre += kvh * each;
         const int64_t at = (int64_t)(t - pre);
         int64_t lo = 0, step = 1;
@@ -239,7 +248,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         const int tile = (int)(t - pre), tiles = (int)min((int64_t)(pages - tile), (int64_t)(t1 - t));
         // on to the run's next item
         auto ahead = [&]() AT_IN {
-            const uint64_t n = at_one((uint64_t)(pl.cum(item + 1) - pl.cum(item)));
+            const uint64_t n = at_one((uint64_t)pl.of(item));
             t = pre + n;
             if (t >= t1) return false;
             pre = t;
@@ -296,44 +305,31 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         // queries as operands: dims 16 s + 8 h .. + 7 of query r
         at_u4 q[KS][NP];
         float cl = HQ ? fabsf(a.scale) * 1.4426950408889634f : 1.0f;   // scores to powers of two
-        bool nan_q = false, inf_q = false;
-        if (active) {
+        {   // of all waves, those without queries too: what one keeps for the next item costs registers
             if constexpr (HQ) {
-                // a negative scale turns the signs; 0 leaves 0 or NaN
-                const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-                constexpr uint32_t EXP = ST == 0 ? 0x7f80u : 0x7c00u, MAN = ST == 0 ? 0x7fu : 0x3ffu;
-                uint32_t nan = 0;
+                const uint16_t* p = static_cast<const uint16_t*>(a.q) + q_at + 8 * h;
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    at_u4 x = gload(reinterpret_cast<const at_u4*>(static_cast<const uint16_t*>(a.q) + q_at + 16 * s + 8 * h));
+                for (int ks = 0; ks < KS; ks++) q[ks][0] = gload(reinterpret_cast<const at_u4*>(p + 16 * ks));
+                if (a.scale < 0.0f)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const uint32_t y = x[e];
-                        const bool lo = (y & EXP) == EXP, hi = (y >> 16 & EXP) == EXP;
-                        nan |= (uint32_t)(lo && (y & MAN)) | (uint32_t)(hi && (y >> 16 & MAN));
-                        if (cl == 0.0f) { x[e] = (lo ? EXP | MAN : 0u) | (hi ? (EXP | MAN) << 16 : 0u); nan |= (uint32_t)(lo || hi); }
-                        else x[e] ^= flip;
-                    }
-                    q[s][0] = x;
-                }
-                if (cl == 0.0f) cl = 1.0f;
-                nan_q = nan;
+                    for (int ks = 0; ks < KS; ks++) q[ks][0] ^= 0x80008000u;
+                cl = fmaxf(cl, 0x1p-126f);   // a scale of 0: scores of 0, and -infinity stays what it is
             } else {
                 float x[KS][8], mx = 0.0f;
                 const float* p = static_cast<const float*>(a.q) + q_at + 8 * h;
                 const float by = a.scale * 1.4426950408889634f;
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const float4 u = gload4(p + 16 * s), v = gload4(p + 16 * s + 4);
-                    x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w; x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
+                for (int ks = 0; ks < KS; ks++) {
+                    const float4 u = gload4(p + 16 * ks), v = gload4(p + 16 * ks + 4);
+                    x[ks][0] = u.x; x[ks][1] = u.y; x[ks][2] = u.z; x[ks][3] = u.w; x[ks][4] = v.x; x[ks][5] = v.y; x[ks][6] = v.z; x[ks][7] = v.w;
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        x[s][e] *= by;
-                        mx = fmaxf(mx, fabsf(x[s][e]));
-                        nan_q |= x[s][e] != x[s][e];
+                        x[ks][e] *= by;
+                        if (ST == 1) mx = fmaxf(mx, fabsf(x[ks][e]));
                     }
-                }
-                inf_q = mx == INFINITY;
                 if constexpr (ST == 1) {
                     mx = xor32_max(mx);
                     int e2 = 0;
@@ -341,12 +337,12 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     const float up = ldexpf(1.0f, e2);
                     cl = ldexpf(1.0f, -e2);
 #pragma unroll
-                    for (int s = 0; s < KS; s++)
+                    for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[s][e] *= up;
+                        for (int e = 0; e < 8; e++) x[ks][e] *= up;
                 }
 #pragma unroll
-                for (int s = 0; s < KS; s++) at_split<ST, HQ>(x[s], q[s]);
+                for (int ks = 0; ks < KS; ks++) at_split<ST, HQ>(x[ks], q[ks]);
             }
         }
         at_f16 o[NV];        // dims 32 n + 8 (i / 4) + 4 h + i % 4 of query r
@@ -480,7 +476,6 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             uint32_t valid = 0;        // whether the pages asked for are there, the last one's bit lowest
 #pragma unroll
             for (int g = 0; g < STEP; g++) keys[g] = -1;
-            for (auto& x : pr) x = at_u4{0, 0, 0, 0};   // or an item's would be kept for the next one
             auto plan = [&](int j) AT_IN {    // turn j's keys, turn j - 1's values
 #pragma unroll
                 for (int g = 0; g < STEP; g++) {
@@ -502,12 +497,12 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             auto beside = [&](int ks) AT_IN {
                 if (ks % (KS / PIECES) == 0) ask(ks / (KS / PIECES));
             };
-            auto first_barrier = [&]() AT_IN {
+            auto first_barrier = [&](auto MORE) AT_IN {
                 // in front of turn j: this wave's copies of its keys and of the values before landed, and of its values where they are asked for
                 // in time (STEP 1: all but turn j + 1's keys and what turn j + 2 asked for)
                 constexpr int LATER = STEP == 2 ? 0 : PIECES / 2 + PIECES;
-                static_assert(LATER < 16, "the low bits of the count");
-                __builtin_amdgcn_s_waitcnt(0x0F70 | LATER);
+                static_assert(LATER + decltype(MORE)::value < 16, "the low bits of the count");
+                __builtin_amdgcn_s_waitcnt(0x0F70 | (LATER + decltype(MORE)::value));
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
             };
@@ -517,36 +512,39 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 asm volatile("" ::: "memory");
             };
 #pragma unroll
-            for (int j = 0; j < FAR; j++) {
+            for (int j = 0; j <= FAR; j++) {
                 plan(j);
 #pragma unroll
                 for (int n = j ? 0 : PIECES / 2; n < PIECES; n++) ask(n);
             }
-            plan(FAR);
-            first_barrier();
+            first_barrier(std::integral_constant<int, PIECES>{});           // one turn more has been asked for than behind turn 0's products in the loop
             if (late) second_barrier();
             find_k(turn * TILE);
             begin_k();
-            products_k(beside);              // of a page that is not there: not used
+            products_k([](int) {});          // of a page that is not there: not used
 #pragma unroll 1
             for (int j = 0; j < turns; j++) {
                 const int i = j * STEP + turn;
                 const bool on = i >= lo && i < hi && (valid >> ((FAR + 1) * STEP - 1 - turn) & 1);
-                if (late) first_barrier();
+                if (late) first_barrier(std::integral_constant<int, 0>{});
                 else second_barrier();
                 plan(j + 1 + FAR);
+                auto then = [&]() AT_IN {
+                    if (late) second_barrier();
+                    else first_barrier(std::integral_constant<int, 0>{});
+                    __builtin_amdgcn_s_setprio(1);
+                    find_k(((i + STEP) & (AR_RING - 1)) * TILE);
+                };
                 if (on) {
                     if (STEP == 1) begin_v(VALUES + (i & (AR_RING - 1)) * TILE);
                     softmax(std::false_type{}, first_key(i));
-                }
-                if (late) second_barrier();
-                else first_barrier();
-                __builtin_amdgcn_s_setprio(1);
-                find_k(((i + STEP) & (AR_RING - 1)) * TILE);
-                if (on) {
+                    then();
                     if (STEP == 2) begin_v(VALUES + (i & (AR_RING - 1)) * TILE);
                     products_v([&](int f) AT_IN { if (f - 4 * NV + VA - 1 < KA - 1) kread(f - 4 * NV + VA - 1); });
-                } else begin_k();
+                } else {
+                    then();
+                    begin_k();
+                }
                 products_k(beside);
                 __builtin_amdgcn_s_setprio(0);
             }
@@ -620,24 +618,35 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         clear();
         if (two) pages_through(std::integral_constant<int, 2>{});
         else pages_through(std::integral_constant<int, 1>{});
+        bool careful = false;
         {
             float any = 0.0f * l;   // NaN where one is not finite
 #pragma unroll
             for (int n = 0; n < NV; n++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) any = fmaf(0.0f, o[n][e], any);
-            // a query that holds NaN has NaN results, whatever the keys are
-            uint64_t nan_rows = __ballot(nan_q);
-            nan_rows |= nan_rows >> 32;
-            const bool again = active && any != any && !((nan_rows >> r) & 1);
+            bool again = active && any != any;
+            if (__builtin_expect(__any(again), 0)) {   // a query that holds NaN has NaN results, whatever the keys are
+                bool nan_q = false;
+#pragma unroll 1
+                for (int d = 0; d < D / 2; d++) {
+                    const int64_t at = q_at + D / 2 * h + d;
+                    const float x = HQ ? kv_float<ST>(gload(static_cast<const uint16_t*>(a.q) + at)) : gload(static_cast<const float*>(a.q) + at);
+                    nan_q |= x != x;
+                    odd_q |= !HQ && __builtin_isinf(x * a.scale * 1.4426950408889634f);
+                }
+                uint64_t nan_rows = __ballot(nan_q);
+                nan_rows |= nan_rows >> 32;
+                again = again && !((nan_rows >> r) & 1);
+                odd_q = __any(odd_q);
+            }
+            if (lane == 0) sh.odd[wave] = 0;
+            if (__any(again) && lane == 0) sh.odd[wave] = 1;
             __syncthreads();
-            if (tid == 0) sh.odd_any = 0;
-            __syncthreads();
-            if (__any(again) && lane == 0) sh.odd_any = 1;
-            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < AR_WV; i++) careful |= sh.odd[i] != 0;
         }
-        if (__builtin_expect(sh.odd_any, 0)) {
-            odd_q = __any(inf_q);
+        if (__builtin_expect(careful, 0)) {
             clear();
 #pragma unroll 1
             for (int i = 0; i < tiles; i++) {
@@ -665,58 +674,46 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 __syncthreads();
             }
         }
+        // What the waves have of the same queries (the other pages' results; later other runs') is added in the order of `way` through LDS.
         constexpr int NR = 16 * NV;
-        if (two) {   // the other pages' results
-            float* to = reinterpret_cast<float*>(lds) + block * (NR + 2) * 64 + lane;
-            if (turn && active) {
+        int way = turn, ways = two ? 2 : 1, blk = block;
+        bool joined = true;
+#pragma unroll 1
+        for (int pass = 0;; pass++) {
+            const bool here = blk < blocks;
+            if (ways > 1) {
+                const int of = AR_WV / ways;   // blocks' places
+                float* to = reinterpret_cast<float*>(lds) + blk * (NR + 2) * 64 + lane;
+                if (way && here) {
+                    float* mine = to + (way - 1) * of * (NR + 2) * 64;
 #pragma unroll
-                for (int n = 0; n < NV; n++)
+                    for (int n = 0; n < NV; n++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) to[(16 * n + e) * 64] = o[n][e];
-                to[NR * 64] = m;
-                to[(NR + 1) * 64] = l;
-            }
-            __syncthreads();
-            if (!turn && active) {
-                const float m2 = to[NR * 64], l2 = to[(NR + 1) * 64], M = fmaxf(m, m2), c = at_exp2(m - at_safe(M)), c2 = at_exp2(m2 - at_safe(M));
-                m = M;
-                l = c * l + c2 * l2;
+                        for (int e = 0; e < 16; e++) mine[(16 * n + e) * 64] = o[n][e];
+                    mine[NR * 64] = m;
+                    mine[(NR + 1) * 64] = l;
+                }
+                __syncthreads();
+                if (!way && here)
+#pragma unroll 1
+                    for (int k = 1; k < ways; k++, to += of * (NR + 2) * 64) {
+                        const float m2 = to[NR * 64], M = fmaxf(m, m2), c = at_exp2(m - at_safe(M)), c2 = at_exp2(m2 - at_safe(M));
+                        m = M;
+                        l = c * l + c2 * to[(NR + 1) * 64];
 #pragma unroll
-                for (int n = 0; n < NV; n++)
+                        for (int n = 0; n < NV; n++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) o[n][e] = at_times(c, o[n][e]) + at_times(c2, to[(16 * n + e) * 64]);
-            }
-        }
-        const bool holds = active && !turn;
-        l = xor32_sum(l);
-        // four dims 32 n + 8 g + 4 h .. of query `row` of the item
-        auto put = [&](int row, int n, int g, float inv, const float* x) AT_IN {
-            const int fq = f0 + row, t = fq / G;
-            const int64_t to = (int64_t)(sq.row + t) * a.out_stride + (int64_t)(kvh * G + fq - t * G) * D + 32 * n + 8 * g + 4 * h;
-            float y[4];
-#pragma unroll
-            for (int d = 0; d < 4; d++) y[d] = inv == 0.0f ? 0.0f : x[d] * inv;
-            if constexpr (HQ) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to) = uint2{(uint32_t)kv_round<ST>(y[0]) | (uint32_t)kv_round<ST>(y[1]) << 16, (uint32_t)kv_round<ST>(y[2]) | (uint32_t)kv_round<ST>(y[3]) << 16};
-            else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to) = float4{y[0], y[1], y[2], y[3]};
-        };
-        if (tiles == pages) {
-            if (holds && r < mine) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-                for (int n = 0; n < NV; n++)
-#pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        const float x[4] = {o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]};
-                        put(32 * block + r, n, g, inv, x);
+                            for (int e = 0; e < 16; e++) o[n][e] = at_times(c, o[n][e]) + at_times(c2, to[(16 * n + e) * 64]);
                     }
             }
-        } else {
+            if (pass == 0) l = xor32_sum(l);
+            if (pass || tiles == pages) break;
             // the runs that hold the item, from the first page's to the last one's
-            const uint64_t w0 = pre / per;
-            const int parts = (int)((pre + pages - 1) / per - w0) + 1, first_slot = pre == w0 * per ? 0 : 1;
-            auto part_of = [&](uint64_t run, int s, int qb) AT_IN { return wk.part + (2 * run + s) * at_part_floats(D) + (size_t)qb * (D / 4 + 1) * 128 + 2 * lane; };
-            if (holds) {
-                float* to = part_of(w, slot, block);
+            const uint64_t w0 = at_one(at_div(pre, per));
+            const int parts = at_one((int)(at_div(pre + pages - 1, per) - w0)) + 1, first_slot = pre == w0 * per ? 0 : 1;
+            auto part_of = [&](uint64_t run, int sl) AT_IN { return wk.part + (2 * run + sl) * at_part_floats(D) + (size_t)blk * (D / 4 + 1) * 128 + 2 * lane; };
+            if (here && !way) {
+                float* to = part_of(w, slot);
 #pragma unroll
                 for (int n = 0; n < NV; n++)
 #pragma unroll
@@ -726,48 +723,52 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             parts_stored();
             if (tid == 0) sh.last = part_last(wk.count + w0, parts);
             __syncthreads();
-            if (sh.last) {   // all waves: eight of a lane's values of 32 queries at a time, four parts in flight
+            if (!sh.last) { joined = false; break; }
+            // the last one to come joins: a wave per 32 queries and every ways-th part
+            ways = blocks > 4 ? 1 : blocks > 2 ? 2 : blocks > 1 ? 4 : 8;
+            blk = wave % (AR_WV / ways);
+            way = wave / (AR_WV / ways);
+            clear();
 #pragma unroll 1
-                for (int id = wave; id < blocks * (D / 16); id += AR_WV) {
-                    const int qb = id % blocks, pc = id / blocks;
-                    auto of = [&](int k) AT_IN { return part_of(w0 + k, k == 0 ? first_slot : 0, qb); };
-                    float M = -INFINITY, sum = 0.0f, x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-                    for (int k = 0; k < parts; k += 8) {
-                        float v[8];
+            for (int k = way; k < parts && blk < blocks; k += ways) {
+                const float* p = part_of(w0 + k, k == 0 ? first_slot : 0);
+                float2 x[NV][8];
+                const float2 st = at_load2(p + D / 4 * 128);
 #pragma unroll
-                        for (int c = 0; c < 8; c++) v[c] = at_load2(of(min(k + c, parts - 1)) + D / 4 * 128).x;
+                for (int n = 0; n < NV; n++)
 #pragma unroll
-                        for (int c = 0; c < 8; c++) M = fmaxf(M, v[c]);
+                    for (int e = 0; e < 8; e++) x[n][e] = at_load2(p + (8 * n + e) * 128);
+                const float M = fmaxf(m, st.x), c = at_exp2(m - at_safe(M)), c2 = at_exp2(st.x - at_safe(M));   // a part of NaN counts, whatever its maximum: 0 times NaN is NaN
+                m = M;
+                l = c * l + c2 * st.y;
+#pragma unroll
+                for (int n = 0; n < NV; n++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        o[n][2 * e] = at_times(c, o[n][2 * e]) + at_times(c2, x[n][e].x);
+                        o[n][2 * e + 1] = at_times(c, o[n][2 * e + 1]) + at_times(c2, x[n][e].y);
                     }
-                    M = at_safe(M);
-#pragma unroll 1
-                    for (int k = 0; k < parts; k += 4) {
-                        float2 st[4], v[4][4];
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            const float* p = of(min(k + c, parts - 1));
-                            st[c] = at_load2(p + D / 4 * 128);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) v[c][e] = at_load2(p + (4 * pc + e) * 128);
-                        }
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            if (k + c >= parts) break;
-                            const float f = at_exp2(st[c].x - M);   // a part of NaN counts, whatever its maximum: 0 times NaN is NaN
-                            sum += f * st[c].y;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) { x[2 * e] += at_times(f, v[c][e].x); x[2 * e + 1] += at_times(f, v[c][e].y); }
-                        }
-                    }
-                    if (32 * qb + r < R) {
-                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                        put(32 * qb + r, pc >> 1, 2 * (pc & 1), inv, x);
-                        put(32 * qb + r, pc >> 1, 2 * (pc & 1) + 1, inv, x + 4);
-                    }
-                }
-                if (tid == 0) part_rearm(wk.count + w0);
             }
+            if (tid == 0) part_rearm(wk.count + w0);
+        }
+        if (joined && !way && 32 * blk + r < R) {
+            const int fq = f0 + 32 * blk + r, tq = fq / G;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t to = (int64_t)(sq.row + tq) * a.out_stride + (int64_t)(kvh * G + fq - tq * G) * D + 4 * h;
+#pragma unroll
+            for (int n = 0; n < NV; n++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    float y[4];
+#pragma unroll
+                    for (int d = 0; d < 4; d++) y[d] = inv == 0.0f ? 0.0f : o[n][4 * g + d] * inv;
+                    if constexpr (HQ) {
+                        at_u4 y4[1];
+                        float y8[8] = {y[0], y[1], y[2], y[3], 0.0f, 0.0f, 0.0f, 0.0f};
+                        at_split<ST, true>(y8, y4);
+                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + 32 * n + 8 * g) = uint2{y4[0][0], y4[0][1]};
+                    } else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to + 32 * n + 8 * g) = float4{y[0], y[1], y[2], y[3]};
+                }
         }
         slot = 1;
         if (!ahead()) return;
