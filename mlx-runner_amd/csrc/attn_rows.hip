@@ -349,7 +349,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         float m, l;          // the point of reference; this lane's keys' sum
         constexpr float UP = ST == 0 ? 0.0f : 6.0f;   // p times 2^UP: f16 parts end at 2^-24
         at_f16 s[2];         // scores of a page, keys 32 kb + 8 (i / 4) + 4 h + i % 4
-        at_u4 pr[HQ ? 4 : 1];   // p of a page, rounded (HQ); s otherwise
+        at_u4 pr[4];         // p of a page, rounded (HQ; s otherwise)
         constexpr uint32_t VALUES = AR_RING * TILE;
         auto first_key = [&](int i) AT_IN { return (p0 + tile + i) * MLXR_PAGE; };
         constexpr int KA = HQ ? 3 : 2, VA = HQ ? 5 : 3;      // fragments in registers: read KA - 1 (VA - 1) steps of NP products ahead
@@ -538,6 +538,9 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 if (on) {
                     if (STEP == 1) begin_v(VALUES + (i & (AR_RING - 1)) * TILE);
                     softmax(std::false_type{}, first_key(i));
+                    // all of it in front of the barrier: a computation in registers may be moved behind one
+                    if constexpr (HQ) asm volatile("" : "+v"(pr[0]), "+v"(pr[1]), "+v"(pr[2]), "+v"(pr[3]), "+v"(l));
+                    else asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(l));
                     then();
                     if (STEP == 2) begin_v(VALUES + (i & (AR_RING - 1)) * TILE);
                     products_v([&](int f) AT_IN { if (f - 4 * NV + VA - 1 < KA - 1) kread(f - 4 * NV + VA - 1); });
