@@ -107,6 +107,7 @@ __device__ __forceinline__ uint64_t at_div(uint64_t a, uint64_t b) {
 struct AtShared {
     uint64_t sums[2][AR_WV], found_pre;
     int found_b, last, odd[AR_WV];
+    float m[AR_WV][64], l[AR_WV][64];
 };
 struct AtWork {
     unsigned* count;      // [AR_MAXW] arrivals at the item that starts in a run and goes on behind it; zero between calls
@@ -180,17 +181,35 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
     uint64_t total = 0, per, t, t1, pre;
     int b;
     AtSeq sq;
-    {
+    auto zeros = [&](const AtSeq& s, int first) AT_IN {   // of the sequences first + lane, each by one workgroup
+        for (uint64_t idle = __ballot(s.none > 0 && (first + lane) % W == w); idle; idle &= idle - 1) {
+            const int i = (int)__builtin_ctzll(idle);
+            zero(AtSeq{0, 0, __builtin_amdgcn_readlane(s.row, i), __builtin_amdgcn_readlane(s.none, i)});
+        }
+    };
+    auto run_of = [&]() AT_IN {   // false: there are fewer runs than workgroups
+        per = max((uint64_t)AR_MINPER, at_one(at_div(total + W - 1, W)));
+        t = (uint64_t)w * per;
+        t1 = min(total, t + per);
+        return t < total;
+    };
+    if (kv.B <= 64) {   // each wave by itself
+        const AtSeq s = lane < kv.B ? at_seq(a, lane) : AtSeq{0, 0, 0, 0};
+        const uint64_t n = places_of(s), upto = wave_scan(n);
+        if (wave == 0) zeros(s, 0);
+        total = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)upto, 63) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(upto >> 32), 63) << 32;
+        if (!run_of()) return;
+        b = (int)__builtin_ctzll(__ballot(upto - n <= t && t < upto));
+        const uint64_t before = upto - n;
+        pre = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)before, b) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(before >> 32), b) << 32;
+        sq = AtSeq{__builtin_amdgcn_readlane(s.c, b), __builtin_amdgcn_readlane(s.base, b), __builtin_amdgcn_readlane(s.row, b), 0};
+    } else {
         uint64_t before = 0, n = 0, chunk = 0;
         int step = 0;
         auto scan = [&](int c, bool first) AT_IN {
             const AtSeq s = c + tid < kv.B ? at_seq(a, c + tid) : AtSeq{0, 0, 0, 0};
             n = places_of(s);
-            if (first)
-                for (uint64_t m = __ballot(s.none > 0 && (c + tid) % W == w); m; m &= m - 1) {
-                    const int l = (int)__builtin_ctzll(m);
-                    zero(AtSeq{0, 0, __builtin_amdgcn_readlane(s.row, l), __builtin_amdgcn_readlane(s.none, l)});
-                }
+            if (first) zeros(s, c + 64 * wave);
             const uint64_t v = wave_scan(n);
             uint64_t* sums = sh.sums[step++ & 1];
             if (lane == 63) sums[wave] = v;
@@ -200,15 +219,14 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
 #pragma unroll
             for (int i = 0; i < AR_WV; i++) { before += i < wave ? sums[i] : 0; chunk += sums[i]; }
         };
+#pragma unroll 1
         for (int c = 0; c < kv.B; c += AR_TH) { scan(c, true); total += chunk; }
         total = at_one(total);
-        per = max((uint64_t)AR_MINPER, at_one(at_div(total + W - 1, W)));
-        t = (uint64_t)w * per;
-        t1 = min(total, t + per);
-        if (t >= total) return;   // fewer runs than workgroups
+        if (!run_of()) return;
         uint64_t run = 0;
+#pragma unroll 1
         for (int c = 0; c < kv.B; c += AR_TH) {
-            if (kv.B > AR_TH) scan(c, false);
+            scan(c, false);
             const uint64_t p = run + before;
             if (p <= t && t < p + n) { sh.found_b = c + tid; sh.found_pre = p; }
             run += chunk;
@@ -623,11 +641,12 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         else pages_through(std::integral_constant<int, 1>{});
         bool careful = false;
         {
-            float any = 0.0f * l;   // NaN where one is not finite
+            float odd4[4] = {0.0f * l, 0.0f, 0.0f, 0.0f};   // NaN where one is not finite
 #pragma unroll
             for (int n = 0; n < NV; n++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) any = fmaf(0.0f, o[n][e], any);
+                for (int e = 0; e < 16; e++) odd4[e & 3] = fmaf(0.0f, o[n][e], odd4[e & 3]);
+            const float any = (odd4[0] + odd4[1]) + (odd4[2] + odd4[3]);
             bool again = active && any != any;
             if (__builtin_expect(__any(again), 0)) {   // a query that holds NaN has NaN results, whatever the keys are
                 bool nan_q = false;
@@ -677,56 +696,99 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 __syncthreads();
             }
         }
-        // What the waves have of the same queries (the other pages' results; later other runs') is added in the order of `way` through LDS.
+        // Where several waves have the same queries (each other's pages; later other runs'), all eight lay down what they have and take eight of a lane's
+        // values of 32 queries at a time, added in the order of `way`.
         constexpr int NR = 16 * NV;
         int way = turn, ways = two ? 2 : 1, blk = block;
-        bool joined = true;
+        l = xor32_sum(l);
+        // four dims 32 n + 8 g + 4 h .. of the queries 32 qb + r
+        auto place = [&](int qb) AT_IN {
+            const int fq = f0 + min(32 * qb + r, R - 1), tq = fq / G;
+            return (int64_t)(sq.row + tq) * a.out_stride + (int64_t)(kvh * G + fq - tq * G) * D + 4 * h;
+        };
+        auto put = [&](int64_t to, int n, int g, float inv, float x0, float x1, float x2, float x3) AT_IN {
+            float y[8] = {x0 * inv, x1 * inv, x2 * inv, x3 * inv, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (inv == 0.0f)   // no key: nothing times 0
+#pragma unroll
+                for (int d = 0; d < 4; d++) y[d] = 0.0f;
+            if constexpr (HQ) {
+                at_u4 y4[1];
+                at_split<ST, true>(y, y4);
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + 32 * n + 8 * g) = uint2{y4[0][0], y4[0][1]};
+            } else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to + 32 * n + 8 * g) = float4{y[0], y[1], y[2], y[3]};
+        };
+        // the runs that hold the item, from the first page's to the last one's
+        const bool whole = tiles == pages;
+        const uint64_t w0 = whole ? 0 : at_one(at_div(pre, per));
+        const int parts = whole ? 1 : at_one((int)(at_div(pre + pages - 1, per) - w0)) + 1, first_slot = pre == w0 * per ? 0 : 1;
+        auto part_of = [&](uint64_t run, int sl, int qb) AT_IN { return wk.part + (2 * run + sl) * at_part_floats(D) + (size_t)qb * (D / 4 + 1) * 128 + 2 * lane; };
 #pragma unroll 1
         for (int pass = 0;; pass++) {
-            const bool here = blk < blocks;
+            const bool out = pass || whole, here = blk < blocks;
             if (ways > 1) {
                 const int of = AR_WV / ways;   // blocks' places
-                float* to = reinterpret_cast<float*>(lds) + blk * (NR + 2) * 64 + lane;
-                if (way && here) {
-                    float* mine = to + (way - 1) * of * (NR + 2) * 64;
+                float* all = reinterpret_cast<float*>(lds) + lane;
+                if (here) {
+                    float* mine = all + (way * of + blk) * NR * 64;
 #pragma unroll
                     for (int n = 0; n < NV; n++)
 #pragma unroll
                         for (int e = 0; e < 16; e++) mine[(16 * n + e) * 64] = o[n][e];
-                    mine[NR * 64] = m;
-                    mine[(NR + 1) * 64] = l;
+                    sh.m[way * of + blk][lane] = m;
+                    sh.l[way * of + blk][lane] = l;
                 }
                 __syncthreads();
-                if (!way && here)
 #pragma unroll 1
-                    for (int k = 1; k < ways; k++, to += of * (NR + 2) * 64) {
-                        const float m2 = to[NR * 64], M = fmaxf(m, m2), c = at_exp2(m - at_safe(M)), c2 = at_exp2(m2 - at_safe(M));
-                        m = M;
-                        l = c * l + c2 * to[(NR + 1) * 64];
+                for (int id = wave; id < blocks * (NR / 8); id += AR_WV) {
+                    const int qb = id % blocks, pc = id / blocks;
+                    float M = -INFINITY, L = 0.0f, x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int k = 0; k < ways; k++) M = fmaxf(M, sh.m[k * of + qb][lane]);
+#pragma unroll 2
+                    for (int k = 0; k < ways; k++) {
+                        const float c = at_exp2(sh.m[k * of + qb][lane] - at_safe(M));   // a part of NaN counts, whatever its maximum: 0 times NaN is NaN
+                        const float* v = all + ((k * of + qb) * NR + 8 * pc) * 64;
+                        L += c * sh.l[k * of + qb][lane];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] += at_times(c, v[e * 64]);
+                    }
+                    if (out) {
+                        if (32 * qb + r < R) {
+                            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                            const int64_t to = place(qb);
+                            put(to, pc >> 1, 2 * (pc & 1), inv, x[0], x[1], x[2], x[3]);
+                            put(to, pc >> 1, 2 * (pc & 1) + 1, inv, x[4], x[5], x[6], x[7]);
+                        }
+                    } else {
+                        float* to = part_of(w, slot, qb);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) at_store2(to + (4 * pc + e) * 128, x[2 * e], x[2 * e + 1]);
+                        if (pc == 0) at_store2(to + D / 4 * 128, M, L);
+                    }
+                }
+            } else if (here) {
+                if (out) {
+                    if (32 * blk + r < R) {
+                        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                        const int64_t to = place(blk);
 #pragma unroll
                         for (int n = 0; n < NV; n++)
 #pragma unroll
-                            for (int e = 0; e < 16; e++) o[n][e] = at_times(c, o[n][e]) + at_times(c2, to[(16 * n + e) * 64]);
+                            for (int g = 0; g < 4; g++) put(to, n, g, inv, o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]);
                     }
-            }
-            if (pass == 0) l = xor32_sum(l);
-            if (pass || tiles == pages) break;
-            // the runs that hold the item, from the first page's to the last one's
-            const uint64_t w0 = at_one(at_div(pre, per));
-            const int parts = at_one((int)(at_div(pre + pages - 1, per) - w0)) + 1, first_slot = pre == w0 * per ? 0 : 1;
-            auto part_of = [&](uint64_t run, int sl) AT_IN { return wk.part + (2 * run + sl) * at_part_floats(D) + (size_t)blk * (D / 4 + 1) * 128 + 2 * lane; };
-            if (here && !way) {
-                float* to = part_of(w, slot);
+                } else {
+                    float* to = part_of(w, slot, blk);
 #pragma unroll
-                for (int n = 0; n < NV; n++)
+                    for (int n = 0; n < NV; n++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) at_store2(to + (8 * n + e) * 128, o[n][2 * e], o[n][2 * e + 1]);
-                at_store2(to + D / 4 * 128, m, l);
+                        for (int e = 0; e < 8; e++) at_store2(to + (8 * n + e) * 128, o[n][2 * e], o[n][2 * e + 1]);
+                    at_store2(to + D / 4 * 128, m, l);
+                }
             }
+            if (out) break;
             parts_stored();
             if (tid == 0) sh.last = part_last(wk.count + w0, parts);
             __syncthreads();
-            if (!sh.last) { joined = false; break; }
+            if (!sh.last) break;
             // the last one to come joins: a wave per 32 queries and every ways-th part
             ways = blocks > 4 ? 1 : blocks > 2 ? 2 : blocks > 1 ? 4 : 8;
             blk = wave % (AR_WV / ways);
@@ -734,14 +796,14 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             clear();
 #pragma unroll 1
             for (int k = way; k < parts && blk < blocks; k += ways) {
-                const float* p = part_of(w0 + k, k == 0 ? first_slot : 0);
+                const float* p = part_of(w0 + k, k == 0 ? first_slot : 0, blk);
                 float2 x[NV][8];
                 const float2 st = at_load2(p + D / 4 * 128);
 #pragma unroll
                 for (int n = 0; n < NV; n++)
 #pragma unroll
                     for (int e = 0; e < 8; e++) x[n][e] = at_load2(p + (8 * n + e) * 128);
-                const float M = fmaxf(m, st.x), c = at_exp2(m - at_safe(M)), c2 = at_exp2(st.x - at_safe(M));   // a part of NaN counts, whatever its maximum: 0 times NaN is NaN
+                const float M = fmaxf(m, st.x), c = at_exp2(m - at_safe(M)), c2 = at_exp2(st.x - at_safe(M));
                 m = M;
                 l = c * l + c2 * st.y;
 #pragma unroll
@@ -754,28 +816,9 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             }
             if (tid == 0) part_rearm(wk.count + w0);
         }
-        if (joined && !way && 32 * blk + r < R) {
-            const int fq = f0 + 32 * blk + r, tq = fq / G;
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int64_t to = (int64_t)(sq.row + tq) * a.out_stride + (int64_t)(kvh * G + fq - tq * G) * D + 4 * h;
-#pragma unroll
-            for (int n = 0; n < NV; n++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    float y[4];
-#pragma unroll
-                    for (int d = 0; d < 4; d++) y[d] = inv == 0.0f ? 0.0f : o[n][4 * g + d] * inv;
-                    if constexpr (HQ) {
-                        at_u4 y4[1];
-                        float y8[8] = {y[0], y[1], y[2], y[3], 0.0f, 0.0f, 0.0f, 0.0f};
-                        at_split<ST, true>(y8, y4);
-                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + 32 * n + 8 * g) = uint2{y4[0][0], y4[0][1]};
-                    } else *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to + 32 * n + 8 * g) = float4{y[0], y[1], y[2], y[3]};
-                }
-        }
         slot = 1;
         if (!ahead()) return;
-        __syncthreads();   // the LDS is written again
+        lds_barrier();     // the LDS is written again; results may still be on their way
     }
 }
 
