@@ -9,7 +9,7 @@ namespace mlxr {
 //
 // Split. The (token, query head of the KV head) pairs of a sequence and KV head, tokens first, are its queries; AR_M of
 // them are an item, so a page is read once for all heads of a group and several tokens. An item walks the pages from the
-// first that its first token attends to its last token's own. All items' pages, laid end to end, are cut into equal runs, one
+// first that its first token attends to its last token's own. All items' pages (pairs of pages, see below), laid end to end, are cut into equal runs, one
 // per workgroup, so chunks, prompts and single tokens of one call keep the card evenly busy, and counts and lengths may stay on
 // the device: each workgroup finds its run by a scan over the sequences. How many pages an item has follows from rounding twice,
 // so its length here is a bound that adds up in closed form (AtPlaces): up to two places of an item hold no
@@ -32,8 +32,8 @@ namespace mlxr {
 // 2^AT_LAZY, and nothing has to be rescaled.
 constexpr int AR_WV = 8, AR_TH = 64 * AR_WV, AR_M = 32 * AR_WV;   // waves and threads of a workgroup, queries of an item
 constexpr int AR_MAXW = 256;       // workgroups: one a CU
-constexpr int AR_GAP = 2;          // places behind an item
-constexpr int AR_MINPER = 4;       // places of a run at least
+constexpr int AR_GAP = 5;          // places behind an item
+constexpr int AR_MINPER = 2;       // places of a run at least
 constexpr int AR_RING = 4;         // pages of keys, and of values, in LDS
 constexpr float AT_LAZY = 8.0f;
 #define AT_IN __attribute__((always_inline))   // what holds the operands' registers has to stay in the kernel
@@ -125,29 +125,35 @@ __device__ __forceinline__ AtSeq at_seq(const AttnRowsArgs& a, int b) {
     return AtSeq{(int)max((int64_t)0, i1 - first), (int)max((int64_t)0, len - n + first), (int)(s + first), (int)max((int64_t)0, first - i0)};
 }
 __device__ __forceinline__ AtSeq at_one(const AtSeq& s) { return AtSeq{at_one(s.c), at_one(s.base), at_one(s.row), at_one(s.none)}; }
-// Places of items 0 .. n - 1 of a sequence: min(A + floor(S i / G), cap) + AR_GAP for item i, S pages of queries (AR_M / 64).
+// How many items a sequence has, and their places: min(A + floor(S i / G), cap) + AR_GAP for item i, S pages of queries (AR_M / 64); half as many
+// pages for a last item of AR_M / 2 queries or fewer, whose pages go in pairs.
 struct AtPlaces {
     static constexpr int S = AR_M / MLXR_PAGE;
     int64_t A, cap, bend;   // from item `bend` on the cap holds
-    int G;
-    __device__ __forceinline__ AtPlaces(const AttnRowsArgs& a, int G_, int base) : G(G_) {
-        const int64_t spread = (AR_M - 1) / G;
-        A = (base + spread) / MLXR_PAGE + 2;
+    int G, items;
+    bool few;
+    __device__ __forceinline__ AtPlaces(const AttnRowsArgs& a, int G_, const AtSeq& s) : G(G_) {
+        const int64_t spread = (AR_M - 1) / G, queries = (int64_t)s.c * G;
+        items = (int)((queries + AR_M - 1) / AR_M);
+        few = queries - (int64_t)(items - 1) * AR_M <= AR_M / 2;
+        A = (s.base + spread) / MLXR_PAGE + 2;
         cap = a.window > 0 ? (a.window + spread + MLXR_PAGE - 1) / MLXR_PAGE + 1 : (int64_t)1 << 40;
         bend = cap <= A ? 0 : ((cap - A) * G + S - 1) / S;
     }
+    __device__ __forceinline__ int64_t pages(int item) const { return min(A + (int64_t)((uint32_t)item * (uint32_t)S / (uint32_t)G), cap); }   // items are below 2^23
+    __device__ __forceinline__ int64_t of(int item) const { return (few && item == items - 1 ? (pages(item) + 1) / 2 : pages(item)) + AR_GAP; }
     __device__ __forceinline__ int64_t steps(int v) const {   // sum of floor(S i / G) over i < v <= G
         int64_t n = 0;
 #pragma unroll
         for (int k = 1; k < S; k++) n += max(0, v - (k * G + S - 1) / S);
         return n;
     }
-    __device__ __forceinline__ int64_t of(int item) const { return min(A + (int64_t)((uint32_t)item * (uint32_t)S / (uint32_t)G), cap) + AR_GAP; }   // items are below 2^23
-    __device__ __forceinline__ int64_t cum(int64_t n) const {
-        const int64_t m = min(n, bend);
+    __device__ __forceinline__ int64_t cum(int n) const {     // of items 0 .. n - 1, n < items or the last of them counted whole
+        const int64_t m = min((int64_t)n, bend);
         const uint32_t u = (uint32_t)m / (uint32_t)G, v = (uint32_t)m % (uint32_t)G;
-        return n * AR_GAP + m * A + (int64_t)S * G * ((int64_t)u * ((int64_t)u - 1) / 2) + u * steps(G) + (int64_t)S * u * v + steps((int)v) + (n - m) * cap;
+        return (int64_t)n * AR_GAP + m * A + (int64_t)S * G * ((int64_t)u * ((int64_t)u - 1) / 2) + u * steps(G) + (int64_t)S * u * v + steps((int)v) + (n - m) * cap;
     }
+    __device__ __forceinline__ int64_t all() const { return cum(items - 1) + of(items - 1); }
 };
 
 // Where a key's 16-byte pieces lie in LDS: piece c at c ^ this. Sixteen keys' same piece, and four keys' same four pieces, are in
@@ -169,8 +175,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
     const void *K = kv.k, *V = kv.v;
 
     // this workgroup's run of places
-    auto items_of = [&](const AtSeq& s) AT_IN { return ((int64_t)s.c * G + AR_M - 1) / AR_M; };
-    auto places_of = [&](const AtSeq& s) AT_IN -> uint64_t { return s.c ? (uint64_t)(AtPlaces(a, G, s.base).cum(items_of(s)) * kv.nKV) : 0; };
+    auto places_of = [&](const AtSeq& s) AT_IN -> uint64_t { return s.c ? (uint64_t)(AtPlaces(a, G, s).all() * kv.nKV) : 0; };
     auto zero = [&](const AtSeq& s) AT_IN {   // rows without a slot
         const int per = a.nH * D * (HQ ? 2 : 4) / 16;
         for (int64_t i = lane; i < (int64_t)s.none * per; i += 64) {
@@ -240,30 +245,32 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
     // the item in which the run begins
     int kvh, item, items;
     {
-        const AtPlaces pl(a, G, sq.base);
-        items = (int)items_of(sq);
-        const uint64_t each = at_one((uint64_t)pl.cum(items)), local = t - pre;
+        const AtPlaces pl(a, G, sq);
+        items = at_one(pl.items);
+        const uint64_t each = at_one((uint64_t)pl.all()), local = t - pre;
         kvh = at_one((int)at_div(local, each));
         pre += kvh * each;
         const int64_t at = (int64_t)(t - pre);
-        int64_t lo = 0, step = 1;
+        int lo = 0, step = 1;
         while (step * 64 < items) step *= 64;
         for (;; step /= 64) {   // the last item that begins at or before the place
-            const int64_t i = lo + lane * step;
-            lo += step * (63 - (int)__builtin_clzll(__ballot(i < items && pl.cum(i) <= at)));
+            const int i = lo + lane * step;
+            lo += step * (63 - (int)__builtin_clzll(__ballot(i < items && i >= lo && pl.cum(i) <= at)));
             if (step == 1) break;
         }
-        item = at_one((int)lo);
+        item = at_one(lo);
         pre += at_one(pl.cum(item));
     }
     int slot = 0;   // partial results of this workgroup: its first item's, then its last one's
     while (true) {
         // pre: the item's first place
-        const AtPlaces pl(a, G, sq.base);
+        const AtPlaces pl(a, G, sq);
         const int f0 = item * AR_M, R = min((int64_t)AR_M, (int64_t)sq.c * G - f0);
         auto first_of = [&](int tok) AT_IN { return a.window > 0 ? max(0, sq.base + tok + 1 - a.window) : 0; };
         const int p0 = at_one(first_of(f0 / G) / MLXR_PAGE), pages = at_one((sq.base + (f0 + R - 1) / G) / MLXR_PAGE - p0 + 1);
-        const int tile = (int)(t - pre), tiles = (int)min((int64_t)(pages - tile), (int64_t)(t1 - t));
+        const bool two = R <= AR_M / 2;   // pages go in pairs
+        const int pair = two ? 2 : 1, place = (int)(t - pre), places = (pages + pair - 1) / pair, tile = place * pair;   // the run's first page of the item
+        const int tiles = (int)min((int64_t)(pages - tile), (int64_t)(t1 - t) * pair);
         // on to the run's next item
         auto ahead = [&]() AT_IN {
             const uint64_t n = at_one((uint64_t)pl.of(item));
@@ -276,7 +283,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     kvh = 0;
                     do sq = at_one(at_seq(a, ++b));   // t < t1 <= total: another one has rows
                     while (sq.c == 0);
-                    items = (int)items_of(sq);
+                    items = at_one(AtPlaces(a, G, sq).items);
                 }
             }
             return true;
@@ -287,7 +294,6 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             continue;
         }
         // this wave's queries, and the other pages' of few
-        const bool two = R <= AR_M / 2;
         const int turn = two ? wave >> 2 : 0, block = two ? wave & 3 : wave, blocks = (R + 31) / 32;
         const int mine = min(32, R - 32 * block);                 // how many, if above 0
         const bool active = mine > 0;
@@ -702,7 +708,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         int way = turn, ways = two ? 2 : 1, blk = block;
         l = xor32_sum(l);
         // four dims 32 n + 8 g + 4 h .. of the queries 32 qb + r
-        auto place = [&](int qb) AT_IN {
+        auto result_of = [&](int qb) AT_IN {
             const int fq = f0 + min(32 * qb + r, R - 1), tq = fq / G;
             return (int64_t)(sq.row + tq) * a.out_stride + (int64_t)(kvh * G + fq - tq * G) * D + 4 * h;
         };
@@ -720,7 +726,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         // the runs that hold the item, from the first page's to the last one's
         const bool whole = tiles == pages;
         const uint64_t w0 = whole ? 0 : at_one(at_div(pre, per));
-        const int parts = whole ? 1 : at_one((int)(at_div(pre + pages - 1, per) - w0)) + 1, first_slot = pre == w0 * per ? 0 : 1;
+        const int parts = whole ? 1 : at_one((int)(at_div(pre + places - 1, per) - w0)) + 1, first_slot = pre == w0 * per ? 0 : 1;
         auto part_of = [&](uint64_t run, int sl, int qb) AT_IN { return wk.part + (2 * run + sl) * at_part_floats(D) + (size_t)qb * (D / 4 + 1) * 128 + 2 * lane; };
 #pragma unroll 1
         for (int pass = 0;; pass++) {
@@ -754,7 +760,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     if (out) {
                         if (32 * qb + r < R) {
                             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                            const int64_t to = place(qb);
+                            const int64_t to = result_of(qb);
                             put(to, pc >> 1, 2 * (pc & 1), inv, x[0], x[1], x[2], x[3]);
                             put(to, pc >> 1, 2 * (pc & 1) + 1, inv, x[4], x[5], x[6], x[7]);
                         }
@@ -769,7 +775,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 if (out) {
                     if (32 * blk + r < R) {
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                        const int64_t to = place(blk);
+                        const int64_t to = result_of(blk);
 #pragma unroll
                         for (int n = 0; n < NV; n++)
 #pragma unroll
