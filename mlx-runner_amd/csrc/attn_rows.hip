@@ -52,27 +52,26 @@ template <int ST> __device__ __forceinline__ at_f16 at_mfma(at_u4 a, at_u4 b, at
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(at_h8, a), __builtin_bit_cast(at_h8, b), c, 0, 0, 0);
 }
 constexpr int at_parts(int ST, bool HQ) { return HQ ? 1 : (ST == 0 ? 3 : 2); }
-// Eight fp32 values as operands: rounded once (HQ), or parts whose sum they are (bf16) or nearly are (f16).
-template <int ST, bool HQ> __device__ __forceinline__ void at_split(const float* x, at_u4* o) {
-    constexpr int NP = at_parts(ST, HQ);
+// Two fp32 values as dword i of operands: rounded once (HQ), or parts whose sum they are (bf16) or nearly are (f16).
+template <int ST, bool HQ> __device__ __forceinline__ void at_split2(float a, float b, int i, at_u4* o) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float a = x[2 * i], b = x[2 * i + 1];
-#pragma unroll
-        for (int t = 0; t < NP; t++) {
-            if constexpr (ST == 0 && HQ) o[t][i] = __builtin_bit_cast(uint32_t, at_b2{(__bf16)a, (__bf16)b});
-            else if constexpr (ST == 0) {
-                o[t][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-                a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-                b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-            } else {
-                const at_h2 h = {(_Float16)a, (_Float16)b};
-                o[t][i] = __builtin_bit_cast(uint32_t, h);
-                a -= (float)h[0];
-                b -= (float)h[1];
-            }
+    for (int t = 0; t < at_parts(ST, HQ); t++) {
+        if constexpr (ST == 0 && HQ) o[t][i] = __builtin_bit_cast(uint32_t, at_b2{(__bf16)a, (__bf16)b});
+        else if constexpr (ST == 0) {
+            o[t][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+            a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+            b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+        } else {
+            const at_h2 h = {(_Float16)a, (_Float16)b};
+            o[t][i] = __builtin_bit_cast(uint32_t, h);
+            a -= (float)h[0];
+            b -= (float)h[1];
         }
     }
+}
+template <int ST, bool HQ> __device__ __forceinline__ void at_split(const float* x, at_u4* o) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) at_split2<ST, HQ>(x[2 * i], x[2 * i + 1], i, o);
 }
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float at_safe(float m) { return m == -INFINITY ? 0.0f : m; }   // -inf - -inf would be NaN
@@ -462,26 +461,26 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
 #pragma unroll
             for (int f = 0; f < VA - 1; f++) vread(f);
         };
-        auto products_v = [&](auto beside) AT_IN {   // beside(f): what else each step reads
+        auto products_v = [&](auto beside) AT_IN {   // beside(f): what else each step asks for or reads
+            at_u4 pp[2][NP];   // p of 16 keys; the next ones' are split among these ones' products
+            auto split = [&](int st, int i) AT_IN { at_split2<ST, HQ>(s[st >> 1][8 * (st & 1) + 2 * i], s[st >> 1][8 * (st & 1) + 2 * i + 1], i, pp[st & 1]); };
+            if constexpr (!HQ)
 #pragma unroll
-            for (int st = 0; st < 4; st++) {
-                at_u4 pp[NP];
-                if constexpr (HQ) pp[0] = pr[st];
+                for (int i = 0; i < 4; i++) split(0, i);
+#pragma unroll
+            for (int f = 0; f < 4 * NV; f++) {
+                const int st = f / NV, n = f % NV;
+                __builtin_amdgcn_sched_barrier(0);
+                if (f + VA - 1 < 4 * NV) vread(f + VA - 1);
+                beside(f);
+                const at_u4 vt = {vf[f % VA][0].x, vf[f % VA][0].y, vf[f % VA][1].x, vf[f % VA][1].y};
+                if constexpr (HQ) o[n] = at_mfma<ST>(vt, pr[st], o[n]);
                 else {
-                    float p8[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) p8[e] = s[st >> 1][8 * (st & 1) + e];
-                    at_split<ST, HQ>(p8, pp);
-                }
+                    for (int p = 0; p < NP; p++) o[n] = at_mfma<ST>(vt, pp[st & 1][p], o[n]);
+                    if (st < 3)
 #pragma unroll
-                for (int n = 0; n < NV; n++) {
-                    const int f = NV * st + n;
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (f + VA - 1 < 4 * NV) vread(f + VA - 1);
-                    else beside(f);
-                    const at_u4 vt = {vf[f % VA][0].x, vf[f % VA][0].y, vf[f % VA][1].x, vf[f % VA][1].y};
-#pragma unroll
-                    for (int p = 0; p < NP; p++) o[n] = at_mfma<ST>(vt, pp[p], o[n]);
+                        for (int i = 0; i < 4 / NV; i++) split(st + 1, 4 / NV * n + i);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -518,8 +517,15 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 if (n < PIECES / 2) copy(V, true, values[g], value_bytes[g], value_at[g], c);
                 else copy(K, false, keys[g], TILE, key_at[g], c);
             };
-            auto beside = [&](int ks) AT_IN {
-                if (ks % (KS / PIECES) == 0) ask(ks / (KS / PIECES));
+            // a turn's copies among its products, evenly: values beside the values' products, keys beside the keys'
+            auto beside_v = [&](int f) AT_IN {
+                constexpr int EACH = 8 * NV / PIECES;
+                if (f % EACH == EACH / 2) ask(f / EACH);
+                if (f >= 4 * NV - KA + 1) kread(f - (4 * NV - KA + 1));
+            };
+            auto beside_k = [&](int ks) AT_IN {
+                constexpr int EACH = 2 * KS / PIECES;
+                if (ks % EACH == EACH / 2) ask(PIECES / 2 + ks / EACH);
             };
             auto first_barrier = [&](auto MORE) AT_IN {
                 // in front of turn j: this wave's copies of its keys and of the values before landed, and of its values where they are asked for
@@ -567,12 +573,14 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     else asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(l));
                     then();
                     if (STEP == 2) begin_v(VALUES + (i & (AR_RING - 1)) * TILE);
-                    products_v([&](int f) AT_IN { if (f - 4 * NV + VA - 1 < KA - 1) kread(f - 4 * NV + VA - 1); });
+                    products_v(beside_v);
                 } else {
                     then();
+#pragma unroll
+                    for (int n = 0; n < PIECES / 2; n++) ask(n);
                     begin_k();
                 }
-                products_k(beside);
+                products_k(beside_k);
                 __builtin_amdgcn_s_setprio(0);
             }
             if (!late) second_barrier();
