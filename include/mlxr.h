@@ -391,7 +391,7 @@ int64_t mlxr_k_sample_rows_work(int rows, int V);
  * start [B], count [B] (new tokens, 0 where refused or none), the new entries of kv->table (which must be writable here;
  * others stay), and for each of the `rows` rows its sequence and slot, seq [rows] and slot [rows]: row start[b] + i is slot
  * len[b] + i of b; rows of refused sequences and behind the last have -1 in both. With separate outputs a call repeats itself.
- * The pool's keys and values are neither read nor written. */
+ * The pool's keys and values are neither read nor written. MLXR_E_UNSUPPORTED: B sequences of max_len slots have 2^30 pages or more. */
 int mlxr_k_paged_reserve(const mlxr_paged_kv* kv, const int32_t* want, int32_t* free_pages, const int32_t* n_free, int rows,
                          int32_t* len_out, int32_t* n_free_out, int32_t* start, int32_t* count, int32_t* seq, int32_t* slot,
                          void* work, size_t work_bytes, void* stream);

@@ -19,7 +19,7 @@ int check_rows(int rows) { return rows < 1 || rows > MAX_ROWS ? bad("rows: 1 .. 
 int check_reserve(const mlxr_paged_kv* kv, int rows) {
     if (int rc = check_kv(kv)) return rc;
     if (rows < 0 || rows > MAX_ROWS) return bad("paged_reserve: 0 .. 4194304 rows");
-    if ((int64_t)kv->B * ((kv->max_len + MLXR_PAGE - 1) / MLXR_PAGE) >= (int64_t)1 << 31) return set_error(MLXR_E_UNSUPPORTED, "paged_reserve: the batch could hold 2^31 pages");
+    if ((int64_t)kv->B * ((kv->max_len + MLXR_PAGE - 1) / MLXR_PAGE) >= (int64_t)1 << 30) return set_error(MLXR_E_UNSUPPORTED, "paged_reserve: the batch could hold 2^30 pages");
     return MLXR_OK;
 }
 int check_attention(const mlxr_paged_kv* kv, int nH, int rows, int q_type) {

@@ -81,6 +81,9 @@ def test_sizes_past_32_bits():
     big = kv(B=65535, max_len=1 << 24, table_stride=1 << 18, slot_stride=1 << 24)
     assert reserve(kv(table=10 * P, B=65535, max_len=1 << 24, table_stride=1 << 18)) == UNSUPPORTED
     assert lib.mlxr_k_paged_reserve_work(ctypes.byref(big), 1) < 0
+    for B in (4095, 4096):   # 2^30 pages
+        c = kv(table=10 * P, B=B, max_len=1 << 24, table_stride=1 << 18)
+        assert (lib.mlxr_k_paged_reserve_work(ctypes.byref(c), 1) < 0) == (B == 4096)
     assert lib.mlxr_k_paged_reserve_work(ctypes.byref(kv(B=65535)), 1 << 22) >= 65536 * 16
     assert attention(kv(nKV=1), nH=4096, q_stride=4096 * 128, out_stride=4096 * 128, rows=1 << 22) == UNSUPPORTED
     assert lib.mlxr_k_paged_attention_rows_work(ctypes.byref(kv(nKV=1)), 4096, 1 << 22, 0) < 0
