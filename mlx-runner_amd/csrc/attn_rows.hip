@@ -13,7 +13,7 @@ namespace mlxr {
 // per workgroup, so chunks, prompts and single tokens of one call keep the card evenly busy, and counts and lengths may stay on
 // the device: each workgroup finds its run by a scan over the sequences. How many pages an item has follows from rounding twice,
 // so its length here is a bound that adds up in closed form (AtPlaces): up to two places of an item hold no
-// page, and AR_GAP more stand for what beginning and ending one costs. An item inside one run is written out at once;
+// page, and at_gap more stand for what beginning and ending one costs. An item inside one run is written out at once;
 // one cut by runs leaves partial results (maximum, sum, unnormalised values), which the last workgroup to finish
 // joins in run order: the same bits every time.
 //
@@ -32,7 +32,9 @@ namespace mlxr {
 // 2^AT_LAZY, and nothing has to be rescaled.
 constexpr int AR_WV = 8, AR_TH = 64 * AR_WV, AR_M = 32 * AR_WV;   // waves and threads of a workgroup, queries of an item
 constexpr int AR_MAXW = 256;       // workgroups: one a CU
-constexpr int AR_GAP = 5;          // places behind an item
+// Places behind an item: a page of 64 dims is passed in less time (24 windows of 1024: 58.2 us with 5, 55.2 with 7, 56.0 with 9; of
+// 128 dims 4 to 6 are alike).
+__host__ __device__ __forceinline__ constexpr int at_gap(int D) { return D == 64 ? 7 : 5; }
 constexpr int AR_MINPER = 2;       // places of a run at least
 constexpr int AR_RING = 4;         // pages of keys, and of values, in LDS
 constexpr float AT_LAZY = 8.0f;
@@ -124,10 +126,10 @@ __device__ __forceinline__ AtSeq at_seq(const AttnRowsArgs& a, int b) {
     return AtSeq{(int)max((int64_t)0, i1 - first), (int)max((int64_t)0, len - n + first), (int)(s + first), (int)max((int64_t)0, first - i0)};
 }
 __device__ __forceinline__ AtSeq at_one(const AtSeq& s) { return AtSeq{at_one(s.c), at_one(s.base), at_one(s.row), at_one(s.none)}; }
-// How many items a sequence has, and their places: min(A + floor(S i / G), cap) + AR_GAP for item i, S pages of queries (AR_M / 64); half as many
+// How many items a sequence has, and their places: min(A + floor(S i / G), cap) + GAP for item i, S pages of queries (AR_M / 64); half as many
 // pages for a last item of AR_M / 2 queries or fewer, whose pages go in pairs.
-struct AtPlaces {
-    static constexpr int S = AR_M / MLXR_PAGE;
+template <int D> struct AtPlaces {
+    static constexpr int S = AR_M / MLXR_PAGE, GAP = at_gap(D);
     int64_t A, cap, bend;   // from item `bend` on the cap holds
     int G, items;
     bool few;
@@ -140,7 +142,7 @@ struct AtPlaces {
         bend = cap <= A ? 0 : ((cap - A) * G + S - 1) / S;
     }
     __device__ __forceinline__ int64_t pages(int item) const { return min(A + (int64_t)((uint32_t)item * (uint32_t)S / (uint32_t)G), cap); }   // items are below 2^23
-    __device__ __forceinline__ int64_t of(int item) const { return (few && item == items - 1 ? (pages(item) + 1) / 2 : pages(item)) + AR_GAP; }
+    __device__ __forceinline__ int64_t of(int item) const { return (few && item == items - 1 ? (pages(item) + 1) / 2 : pages(item)) + GAP; }
     __device__ __forceinline__ int64_t steps(int v) const {   // sum of floor(S i / G) over i < v <= G
         int64_t n = 0;
 #pragma unroll
@@ -150,7 +152,7 @@ struct AtPlaces {
     __device__ __forceinline__ int64_t cum(int n) const {     // of items 0 .. n - 1, n < items or the last of them counted whole
         const int64_t m = min((int64_t)n, bend);
         const uint32_t u = (uint32_t)m / (uint32_t)G, v = (uint32_t)m % (uint32_t)G;
-        return (int64_t)n * AR_GAP + m * A + (int64_t)S * G * ((int64_t)u * ((int64_t)u - 1) / 2) + u * steps(G) + (int64_t)S * u * v + steps((int)v) + (n - m) * cap;
+        return (int64_t)n * GAP + m * A + (int64_t)S * G * ((int64_t)u * ((int64_t)u - 1) / 2) + u * steps(G) + (int64_t)S * u * v + steps((int)v) + (n - m) * cap;
     }
     __device__ __forceinline__ int64_t all() const { return cum(items - 1) + of(items - 1); }
 };
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
     const void *K = kv.k, *V = kv.v;
 
     // this workgroup's run of places
-    auto places_of = [&](const AtSeq& s) AT_IN -> uint64_t { return s.c ? (uint64_t)(AtPlaces(a, G, s).all() * kv.nKV) : 0; };
+    auto places_of = [&](const AtSeq& s) AT_IN -> uint64_t { return s.c ? (uint64_t)(AtPlaces<D>(a, G, s).all() * kv.nKV) : 0; };
     auto zero = [&](const AtSeq& s) AT_IN {   // rows without a slot
         const int per = a.nH * D * (HQ ? 2 : 4) / 16;
         for (int64_t i = lane; i < (int64_t)s.none * per; i += 64) {
@@ -244,7 +246,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
     // the item in which the run begins
     int kvh, item, items;
     {
-        const AtPlaces pl(a, G, sq);
+        const AtPlaces<D> pl(a, G, sq);
         items = at_one(pl.items);
         const uint64_t each = at_one((uint64_t)pl.all()), local = t - pre;
         kvh = at_one((int)at_div(local, each));
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
     int slot = 0;   // partial results of this workgroup: its first item's, then its last one's
     while (true) {
         // pre: the item's first place
-        const AtPlaces pl(a, G, sq);
+        const AtPlaces<D> pl(a, G, sq);
         const int f0 = item * AR_M, R = min((int64_t)AR_M, (int64_t)sq.c * G - f0);
         auto first_of = [&](int tok) AT_IN { return a.window > 0 ? max(0, sq.base + tok + 1 - a.window) : 0; };
         const int p0 = at_one(first_of(f0 / G) / MLXR_PAGE), pages = at_one((sq.base + (f0 + R - 1) / G) / MLXR_PAGE - p0 + 1);
@@ -282,7 +284,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                     kvh = 0;
                     do sq = at_one(at_seq(a, ++b));   // t < t1 <= total: another one has rows
                     while (sq.c == 0);
-                    items = at_one(AtPlaces(a, G, sq).items);
+                    items = at_one(AtPlaces<D>(a, G, sq).items);
                 }
             }
             return true;
@@ -837,7 +839,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
 }
 
 static size_t at_layout(const PagedKV& kv, int nH, int rows, void* base, AtWork& wk) {
-    const int64_t G = nH / kv.nKV, items = ((int64_t)rows * G + AR_M - 1) / AR_M + kv.B, places = (kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE + 4 + AR_GAP;
+    const int64_t G = nH / kv.nKV, items = ((int64_t)rows * G + AR_M - 1) / AR_M + kv.B, places = (kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE + 4 + at_gap(kv.D);
     const double runs = (double)items * (double)kv.nKV * (double)places / AR_MINPER + 1.0;
     wk.W = runs < AR_MAXW ? (int)runs : AR_MAXW;
     uint8_t* p = static_cast<uint8_t*>(base);
