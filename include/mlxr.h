@@ -414,8 +414,9 @@ int mlxr_k_paged_append_rows(const mlxr_paged_kv* kv, const float* qkv, int row_
  * score is -infinity takes no part; a row that has no slot (count above len), no page of the pool or no score above -infinity gives zeros;
  * infinities and NaN in keys and values that a row attends count as the formula has them, and others do not reach it. Rows outside
  * [0, rows) and rows that no sequence names are neither read nor written; sequences name rows of their own. The cache's weights
- * stay as they are. q, out: 16-byte aligned, strides whole multiples of 16 bytes; out may be q itself at its stride. The same
- * call gives the same bits; another batch around a row may cut its sums elsewhere. */
+ * stay as they are. q, out: 16-byte aligned, strides whole multiples of 16 bytes; out may be q itself at its stride. work: zero
+ * before its first use and this entry point's alone, one call at a time (sizes may differ from call to call). The same call gives
+ * the same bits; another batch around a row may cut its sums elsewhere. */
 int mlxr_k_paged_attention_rows(const mlxr_paged_kv* kv, const int32_t* start, const int32_t* count, int rows, const void* q, int q_type,
                                 int q_stride, int nH, int window, float scale, void* out, int out_stride, void* work, size_t work_bytes,
                                 void* stream);

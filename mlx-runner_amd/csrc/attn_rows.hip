@@ -7,15 +7,15 @@ namespace mlxr {
 // out = sum_j p_j v_j, p = softmax of scale q k_j over the slots up to a row's own: 4 D flops a (row, query head, slot), and
 // 4 D bytes a slot and KV head once. One token a sequence is bound by those reads, a chunk by the matrix cores.
 //
-// Split. The (token, query head of the KV head) pairs of a sequence and KV head, tokens first, are its queries; AR_M of
-// them are an item, so a page is read once for all heads of a group and several tokens. An item walks the pages from the
-// first that its first token attends to its last token's own. All items' pages (pairs of pages, see below), laid end to end, are cut into equal runs, one
-// per workgroup, so chunks, prompts and single tokens of one call keep the card evenly busy, and counts and lengths may stay on
-// the device: each workgroup finds its run by a scan over the sequences. How many pages an item has follows from rounding twice,
-// so its length here is a bound that adds up in closed form (AtPlaces): up to two places of an item hold no
-// page, and at_gap more stand for what beginning and ending one costs. An item inside one run is written out at once;
-// one cut by runs leaves partial results (maximum, sum, unnormalised values), which the last workgroup to finish
-// joins in run order: the same bits every time.
+// Split. The (token, query head of the KV head) pairs of a sequence and KV head, tokens first, are its queries; AR_M of them
+// are an item, so a page is read once for all heads of a group and several tokens. An item walks the pages from the first
+// that its first token attends to its last token's own. All items' pages (pairs of pages, see below), laid end to end, are
+// cut into equal runs, one per workgroup, so chunks, prompts and single tokens of one call keep the card evenly busy, and
+// counts and lengths may stay on the device: each workgroup finds its run by a scan over the sequences. How many pages an
+// item has follows from rounding twice, so its length here is a bound that adds up in closed form (AtPlaces): up to two
+// places of an item hold no page, and at_gap more stand for what beginning and ending one costs. An item inside one run is
+// written out at once; one cut by runs leaves partial results (maximum, sum, unnormalised values), which the last workgroup
+// to finish joins in run order: the same bits every time.
 //
 // Inside. Eight waves have 32 queries each and read the same page from LDS; where an item has 128 queries or fewer, four do, and
 // the other four take every other page, joined through LDS at the end. Pages are copied there straight from the cache, three
@@ -30,6 +30,24 @@ namespace mlxr {
 // truncation (24 bits), or two f16 (22 bits, q scaled to at most 2^14 by a power of two). Scores are in powers of two.
 // A query's reference point for p moves only when its maximum is AT_LAZY or more above it: until then p is up to
 // 2^AT_LAZY, and nothing has to be rescaled.
+//
+// Roundings. Scores, sums and values are fp32. Queries of the cache's type and p rounded to it (half a step, 2^-8 of p in
+// bf16; the sum is of the unrounded p) cost one product a key and dim each; fp32 ones three (bf16) or two (f16), and are
+// right to 24 and 22 bits.
+//
+// Measured, and what bounds it. 2048 tokens after 30000, 40 heads of 128, 8 KV heads, bf16: 1.24 ms, 1.05 PF/s: the matrix
+// cores are busy for 57% of the cycles, at the 1.8 to 1.85 GHz that the power limit leaves (1.10 ms without the copies, 1.04
+// without the softmax), and a page's turn is 2.05 us: 0.6 for the keys' products, 0.35 to 0.45 for the values', 0.75 to 0.9
+// for the softmax, 0.2 for what the copies need, 0.1 for barriers. 2048 after 0: 62 us, 0.55 PF/s: 2.4 items a run, whose
+// beginnings and ends (10 us each) are most of what is missing. 32 sequences, 24 with one new token and 8 with up to 400,
+// after up to 7000: 207 us, matrix cores busy for 37% of the cycles, half of it as before and the rest for beginnings, ends
+// and joins. Five tokens of fp32 after 7000: 34 us, of which 5 are the launch, 2.6 the search for the run, 5 the queries, 13
+// two turns behind each other, 4 partial results and 3 to 5 the join: one round trip after another; its reads alone would be
+// 6.
+// Both sides of the choices. Pages in pairs where an item has AR_M / 2 queries or fewer: 33.6 us against 36.8 for the five
+// tokens, 207 against 223 for the 32 sequences, 55 against 61 for 24 windows of 1024. Each wave looks for its run by itself
+// (up to 64 sequences): 33.6 against 34.8 and 55 against 57. Items of AR_M queries rather than of half as many read a page
+// for twice as many products.
 constexpr int AR_WV = 8, AR_TH = 64 * AR_WV, AR_M = 32 * AR_WV;   // waves and threads of a workgroup, queries of an item
 constexpr int AR_MAXW = 256;       // workgroups: one a CU
 // Places behind an item: a page of 64 dims is passed in less time (24 windows of 1024: 58.2 us with 5, 55.2 with 7, 56.0 with 9; of
@@ -87,8 +105,8 @@ __device__ __forceinline__ float2 at_load2(const float* p) {
     return float2{__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
-// The LDS transpose read. Of a pointer of its own (__restrict__): otherwise the compiler, which cannot tell what it reads from what copies write,
-// waits for every copy in flight in front of it.
+// The LDS transpose read. Of a pointer of its own (__restrict__): otherwise the compiler, which cannot tell what it reads from
+// what copies write, waits for every copy in flight in front of it.
 __device__ __forceinline__ uint2 at_read_tr(const uint8_t* __restrict__ p) { return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lv4)p)); }
 // Values that are the same in all lanes, for the scalar registers: addresses and loops that are not known to be so cost many times more.
 __device__ __forceinline__ int at_one(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -126,8 +144,8 @@ __device__ __forceinline__ AtSeq at_seq(const AttnRowsArgs& a, int b) {
     return AtSeq{(int)max((int64_t)0, i1 - first), (int)max((int64_t)0, len - n + first), (int)(s + first), (int)max((int64_t)0, first - i0)};
 }
 __device__ __forceinline__ AtSeq at_one(const AtSeq& s) { return AtSeq{at_one(s.c), at_one(s.base), at_one(s.row), at_one(s.none)}; }
-// How many items a sequence has, and their places: min(A + floor(S i / G), cap) + GAP for item i, S pages of queries (AR_M / 64); half as many
-// pages for a last item of AR_M / 2 queries or fewer, whose pages go in pairs.
+// How many items a sequence has, and their places: min(A + floor(S i / G), cap) + GAP for item i, S pages of queries (AR_M / 64);
+// half as many pages for a last item of AR_M / 2 queries or fewer, whose pages go in pairs.
 template <int D> struct AtPlaces {
     static constexpr int S = AR_M / MLXR_PAGE, GAP = at_gap(D);
     int64_t A, cap, bend;   // from item `bend` on the cap holds
@@ -317,7 +335,8 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             }
             return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)offs, i & 63) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(offs >> 32), i & 63) << 32);
         };
-        // a KiB of this wave's share of a page's copy: what lies in its first `bytes`, and zeros behind (nothing is read of a page that is not there)
+        // a KiB of this wave's share of a page's copy: what lies in its first `bytes`, and zeros behind (nothing is read of a page
+        // that is not there)
         auto copy = [&](const void* pool, bool values, int64_t off, int bytes, uint32_t to, int j) AT_IN {
             const uint8_t* from = static_cast<const uint8_t*>(pool) + off;
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, at_one(off < 0 ? 0 : bytes), 0x00020000);
