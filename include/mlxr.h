@@ -409,7 +409,7 @@ int mlxr_k_paged_append_rows(const mlxr_paged_kv* kv, const float* qkv, int row_
 
 /* Attention from rows to their own sequences' slots: row start[b] + i, i < count[b], is the query at slot len[b] - count[b] + i
  * (len counts the new tokens) and attends every slot up to its own, or the last `window` of these (0: all). out = sum_j p_j v_j with p =
- * softmax(scale q k_j). q_type 0: q and out are fp32 and so are the results; q_type 1: both are of the cache's
+ * softmax(scale q k_j), |scale| at most 2^126. q_type 0: q and out are fp32 and so are the results; q_type 1: both are of the cache's
  * type, scores, sums and the softmax in fp32, and each p is rounded to the type once (sums are of unrounded ones). A key whose
  * score is -infinity takes no part; a row that has no slot (count above len), no page of the pool or no score above -infinity gives zeros;
  * infinities and NaN in keys and values that a row attends count as the formula has them, and others do not reach it. Rows outside

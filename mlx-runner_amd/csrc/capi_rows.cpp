@@ -97,7 +97,7 @@ int mlxr_k_paged_attention_rows(const mlxr_paged_kv* kv, const int32_t* start, c
             return bad("paged_attention_rows: q and out 16-byte aligned, strides whole multiples of 16 bytes and at least nH * D values");
         if (out == q && out_stride != q_stride) return bad("paged_attention_rows: out over q needs its stride");
         if (window < 0) return bad("paged_attention_rows: window");
-        if (!std::isfinite(scale)) return bad("paged_attention_rows: scale is not finite");
+        if (!(std::fabs(scale) <= 0x1p126f)) return bad("paged_attention_rows: scale is NaN or above 2^126");
         if (!aligned(start, 4) || !aligned(count, 4)) return bad("paged_attention_rows: alignment");
         if (int rc = check_work(work, work_bytes, (int64_t)paged_attention_rows_work(*kv, nH, rows, q_type))) return rc;
         hipStream_t s = static_cast<hipStream_t>(stream);

@@ -64,7 +64,7 @@ def test_append_refuses(over):
 
 
 @pytest.mark.parametrize("over", [dict(start=None), dict(count=None), dict(q=None), dict(out=None), dict(nH=0), dict(nH=5), dict(window=-1), dict(scale=float("nan")),
-                                  dict(scale=float("inf")), dict(q_stride=508), dict(q_stride=514), dict(out_stride=510), dict(q=P + 4), dict(out=P + 8),
+                                  dict(scale=float("inf")), dict(scale=2.0 ** 127), dict(scale=-(2.0 ** 127)), dict(q_stride=508), dict(q_stride=514), dict(out_stride=510), dict(q=P + 4), dict(out=P + 8),
                                   dict(work=None), dict(work=P + 16), dict(work_bytes=16), dict(out_stride=516), dict(rows=0), dict(rows=(1 << 22) + 1),
                                   dict(q_type=2), dict(q_type=1, q_stride=516, out_stride=516), dict(start=P + 2), dict(count=P + 1)])
 def test_attention_refuses(over):

@@ -12,6 +12,7 @@ import numpy as np
 import pytest
 
 from qfix import bf16_round, bf16_to_f32
+from test_batch_cpu import INVALID
 from test_batch_gpu import PAGE, U, Cache, Hip, from_half, same, to_half, within, workspace
 
 pytestmark = pytest.mark.gpu
@@ -706,6 +707,66 @@ def test_steps_captured(gpu):
             assert same(x, y), i
     hip("hipGraphExecDestroy", graph)
     hip("hipStreamDestroy", st)
+
+
+def test_steps_captured_in_the_strictest_mode(gpu):
+    """Nothing that the calls ask of the runtime is forbidden in a capture of mode 'global', and the first run of buffers may be a replay."""
+    hip = Hip(gpu)
+    a, b, st, graph, ex = Server(gpu), Server(gpu), hip.stream(), ctypes.c_void_p(), ctypes.c_void_p()
+    hip("hipStreamBeginCapture", st, 0)
+    b.run(st)
+    hip("hipStreamEndCapture", st, ctypes.byref(graph))
+    hip("hipGraphInstantiate", ctypes.byref(ex), graph, None, None, ctypes.c_size_t(0))
+    for i, (change, new) in enumerate(steps(np.random.default_rng(20), a.B, a.width, 4)):
+        lens = a.len.numpy()
+        for s in (a, b):
+            s.inputs([0 if x is None else lens[j] + x for j, x in enumerate(change)], np.concatenate(new))
+        a.run(st)
+        hip("hipGraphLaunch", ex, st)
+        hip.wait(st)
+        for x, y in zip(a.state(), b.state()):
+            assert same(x, y), i
+    hip("hipGraphExecDestroy", ex)
+    hip("hipStreamDestroy", st)
+
+
+def test_host_memory_is_refused(gpu):
+    """Every pointer that a kernel would follow, at memory that the device does not have: an error, and nothing written."""
+    s, host = Server(gpu), np.zeros(1 << 16, np.uint8)
+    at = -(-host.ctypes.data // 256) * 256
+    names = {"mlxr_k_paged_reserve": (1, 2, 3, 5, 6, 7, 8, 9, 10, 11), "mlxr_k_paged_append_rows": (1, 4, 5, 7, 15), "mlxr_k_paged_attention_rows": (1, 2, 4, 10, 12)}
+    real = {n: getattr(gpu.lib, n) for n in names}
+
+    class Lib:   # the server's calls, with argument `bad` of `name` replaced
+        name = bad = None
+
+        def __getattr__(self, n):
+            if n not in real:
+                return getattr(gpu.lib, n)
+            return lambda *x: real[n](*(at if n == self.name and i == self.bad else y for i, y in enumerate(x)))
+
+    class Gpu:
+        lib, check = Lib(), staticmethod(lambda rc: seen.append(rc))
+    s.inputs([3, 1, 0, 2, 70], np.ones((76, s.width), np.float32))
+    s.gpu = Gpu
+    for Lib.name, places in names.items():
+        for Lib.bad in places:
+            seen = []
+            print(f"[case] {Lib.name} {Lib.bad}", flush=True)
+            s.run()
+            assert seen == [INVALID if n == Lib.name else 0 for n in names], (Lib.name, Lib.bad)
+    gpu.synchronize()
+    assert not host.any()
+
+
+def test_one_workspace_for_all_sizes(gpu):
+    """Calls of other batches, types and sizes take turns on a workspace of the largest one's size."""
+    big, small = Cache(gpu, [3000, 700], 2, 128, 0, seed=31).up(), Cache(gpu, [90], 1, 64, 0, seed=32).up()
+    runs = [Rows(big, [300, 1], 8, 1, seed=31), Rows(small, [3], 3, 0, seed=32), Rows(big, [5, 2], 8, 0, seed=33), Rows(small, [80], 1, 1, seed=34)]
+    alone = [attend(gpu, r) for r in runs]
+    work = workspace(gpu, max(gpu.lib.mlxr_k_paged_attention_rows_work(ctypes.byref(r.c.desc()), r.nH, r.rows, r.io) for r in runs))
+    for r, want in list(zip(runs, alone)) * 2:
+        assert same(attend(gpu, r, work=work), want)
 
 
 def test_two_streams_at_once(gpu):
