@@ -15,7 +15,9 @@ namespace mlxr {
 // item has follows from rounding twice, so its length here is a bound that adds up in closed form (AtPlaces): up to two
 // places of an item hold no page, and at_gap more stand for what beginning and ending one costs. An item inside one run is
 // written out at once; one cut by runs leaves partial results (maximum, sum, unnormalised values), which the last workgroup
-// to finish joins in run order: the same bits every time.
+// to finish joins in run order: the same bits every time. A part is 2.5 us of a join by one workgroup, so where a wave would
+// have more than AR_GROUP of them they are joined in groups, and then the groups (180 tokens after 594 and 52 after 11387,
+// five heads of one KV head: 63 us, 185 with one join).
 //
 // Inside. Eight waves have 32 queries each and read the same page from LDS; where an item has 128 queries or fewer, four do, and
 // the other four take every other page, joined through LDS at the end. Pages are copied there straight from the cache, three
@@ -53,6 +55,8 @@ constexpr int AR_MAXW = 256;       // workgroups: one a CU
 // Places behind an item: a page of 64 dims is passed in less time (24 windows of 1024: 58.2 us with 5, 55.2 with 7, 56.0 with 9; of
 // 128 dims 4 to 6 are alike).
 __host__ __device__ __forceinline__ constexpr int at_gap(int D) { return D == 64 ? 7 : 5; }
+constexpr int AR_COUNTS = 4 * AR_MAXW;
+constexpr int AR_GROUP = 8;        // parts that a wave joins one after another
 constexpr int AR_MINPER = 2;       // places of a run at least
 constexpr int AR_RING = 4;         // pages of keys, and of values, in LDS
 constexpr float AT_LAZY = 8.0f;
@@ -129,7 +133,8 @@ struct AtShared {
     float m[AR_WV][64], l[AR_WV][64];
 };
 struct AtWork {
-    unsigned* count;      // [AR_MAXW] arrivals at the item that starts in a run and goes on behind it; zero between calls
+    unsigned* count;      // [AR_COUNTS] arrivals; zero between calls. [w0]: at the item that starts in run w0 and goes on behind it;
+                          // [AR_MAXW + w0], [2 AR_MAXW + run]: at its first group of parts, at the group that starts with the run
     float* part;          // [2 W] partial results: [AR_WV][D / 4 + 1][64][2]: 32 queries' values, then maximum and sum
     int W;
 };
@@ -280,7 +285,6 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         item = at_one(lo);
         pre += at_one(pl.cum(item));
     }
-    int slot = 0;   // partial results of this workgroup: its first item's, then its last one's
     while (true) {
         // pre: the item's first place
         const AtPlaces<D> pl(a, G, sq);
@@ -309,7 +313,6 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         };
         if (tiles <= 0) {   // the run begins behind an item's pages
             if (!ahead()) return;
-            slot = 1;            // an item's first part is in the second place unless the run begins with it
             continue;
         }
         // this wave's queries, and the other pages' of few
@@ -754,12 +757,21 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         };
         // the runs that hold the item, from the first page's to the last one's
         const bool whole = tiles == pages;
-        const uint64_t w0 = whole ? 0 : at_one(at_div(pre, per));
-        const int parts = whole ? 1 : at_one((int)(at_div(pre + places - 1, per) - w0)) + 1, first_slot = pre == w0 * per ? 0 : 1;
-        auto part_of = [&](uint64_t run, int sl, int qb) AT_IN { return wk.part + (2 * run + sl) * at_part_floats(D) + (size_t)qb * (D / 4 + 1) * 128 + 2 * lane; };
+        const int w0 = whole ? 0 : at_one((int)at_div(pre, per));
+        const int parts = whole ? 1 : at_one((int)at_div(pre + places - 1, per)) - w0 + 1, first_slot = pre == (uint64_t)w0 * per ? 0 : 1;
+        // a run has two parts at most: of what it begins with, and of an item that starts behind that
+        auto part_of = [&](int run, int qb) AT_IN {
+            return wk.part + (size_t)(2 * run + (run == w0 ? first_slot : 0)) * at_part_floats(D) + (size_t)qb * (D / 4 + 1) * 128 + 2 * lane;
+        };
+        // How parts are joined: a wave has 32 queries and every ways-th part. Above AR_GROUP a wave, the last workgroup of each
+        // group of parts joins these where the group's first part was, and the last of those the groups.
+        const int join_ways = blocks > 4 ? 1 : blocks > 2 ? 2 : blocks > 1 ? 4 : 8, group = AR_GROUP * join_ways;
+        const bool grouped = parts > group;
+        const int g0 = grouped ? w0 + (w - w0) / group * group : w0;   // the first run of this one's group
+        int to_run = w;
 #pragma unroll 1
         for (int pass = 0;; pass++) {
-            const bool out = pass || whole, here = blk < blocks;
+            const bool out = whole || pass == (grouped ? 2 : 1), here = blk < blocks;
             if (ways > 1) {
                 const int of = AR_WV / ways;   // blocks' places
                 float* all = reinterpret_cast<float*>(lds) + lane;
@@ -794,7 +806,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                             put(to, pc >> 1, 2 * (pc & 1) + 1, inv, x[4], x[5], x[6], x[7]);
                         }
                     } else {
-                        float* to = part_of(w, slot, qb);
+                        float* to = part_of(to_run, qb);
 #pragma unroll
                         for (int e = 0; e < 4; e++) at_store2(to + (4 * pc + e) * 128, x[2 * e], x[2 * e + 1]);
                         if (pc == 0) at_store2(to + D / 4 * 128, M, L);
@@ -811,7 +823,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                             for (int g = 0; g < 4; g++) put(to, n, g, inv, o[n][4 * g], o[n][4 * g + 1], o[n][4 * g + 2], o[n][4 * g + 3]);
                     }
                 } else {
-                    float* to = part_of(w, slot, blk);
+                    float* to = part_of(to_run, blk);
 #pragma unroll
                     for (int n = 0; n < NV; n++)
 #pragma unroll
@@ -821,17 +833,20 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             }
             if (out) break;
             parts_stored();
-            if (tid == 0) sh.last = part_last(wk.count + w0, parts);
+            const bool last_join = pass == 1 || !grouped;   // of groups, or of all parts
+            unsigned* count = wk.count + (last_join ? w0 : g0 == w0 ? AR_MAXW + w0 : 2 * AR_MAXW + g0);
+            const int n = !grouped ? parts : pass ? (parts + group - 1) / group : min(group, parts - (g0 - w0));
+            if (tid == 0) sh.last = part_last(count, n);
             __syncthreads();
             if (!sh.last) break;
-            // the last one to come joins: a wave per 32 queries and every ways-th part
-            ways = blocks > 4 ? 1 : blocks > 2 ? 2 : blocks > 1 ? 4 : 8;
+            const int from = last_join ? w0 : g0, stride = pass ? group : 1;
+            ways = join_ways;
             blk = wave % (AR_WV / ways);
             way = wave / (AR_WV / ways);
             clear();
 #pragma unroll 1
-            for (int k = way; k < parts && blk < blocks; k += ways) {
-                const float* p = part_of(w0 + k, k == 0 ? first_slot : 0, blk);
+            for (int k = way; k < n && blk < blocks; k += ways) {
+                const float* p = part_of(from + k * stride, blk);
                 float2 x[NV][8];
                 const float2 st = at_load2(p + D / 4 * 128);
 #pragma unroll
@@ -849,9 +864,9 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                         o[n][2 * e + 1] = at_times(c, o[n][2 * e + 1]) + at_times(c2, x[n][e].y);
                     }
             }
-            if (tid == 0) part_rearm(wk.count + w0);
+            if (tid == 0) part_rearm(count);
+            to_run = g0;
         }
-        slot = 1;
         if (!ahead()) return;
         lds_barrier();     // the LDS is written again; results may still be on their way
     }
@@ -863,8 +878,8 @@ static size_t at_layout(const PagedKV& kv, int nH, int rows, void* base, AtWork&
     wk.W = runs < AR_MAXW ? (int)runs : AR_MAXW;
     uint8_t* p = static_cast<uint8_t*>(base);
     wk.count = reinterpret_cast<unsigned*>(p);   // first: where it is for every size
-    wk.part = reinterpret_cast<float*>(p + AR_MAXW * sizeof(unsigned));
-    return AR_MAXW * sizeof(unsigned) + (size_t)2 * wk.W * at_part_floats(kv.D) * sizeof(float);
+    wk.part = reinterpret_cast<float*>(p + AR_COUNTS * sizeof(unsigned));
+    return AR_COUNTS * sizeof(unsigned) + (size_t)2 * wk.W * at_part_floats(kv.D) * sizeof(float);
 }
 
 size_t paged_attention_rows_work(const PagedKV& kv, int nH, int rows, int q_type) {

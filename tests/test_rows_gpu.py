@@ -144,6 +144,18 @@ def test_attention_sizes(gpu, count, length, nKV, G, D, st, io):
     check(attend(gpu, r), r, *reference(r, 0, 0.09))
 
 
+@pytest.mark.parametrize("counts,lengths,G,D,st,io", [([60], [9000], 5, 128, 0, 1), ([180, 60], [1500, 9000], 5, 128, 0, 0), ([20], [5000], 4, 64, 1, 1),
+                                                      ([30], [14000], 2, 64, 0, 0), ([1], [40000], 1, 128, 0, 1), ([40, 3], [33000, 100], 1, 128, 1, 0)])
+def test_attention_of_many_parts(gpu, counts, lengths, G, D, st, io):
+    """Few queries and many pages: an item is cut into so many runs that its parts are joined in groups, and twice the same."""
+    c = Cache(gpu, lengths, 1, D, st, seed=77).up()
+    r = Rows(c, counts, G, io, seed=77)
+    work = workspace(gpu, gpu.lib.mlxr_k_paged_attention_rows_work(ctypes.byref(c.desc()), r.nH, r.rows, io))
+    got = attend(gpu, r, work=work)
+    check(got, r, *reference(r, 0, 0.09))
+    assert same(attend(gpu, r, work=work), got)
+
+
 @pytest.mark.parametrize("window", [1, 2, 31, 63, 64, 65, 128, 1000, 1 << 30])
 @pytest.mark.parametrize("D,st,io,G", [(128, 0, 1, 4), (64, 1, 0, 3)])
 def test_attention_window(gpu, window, D, st, io, G):
