@@ -38,12 +38,12 @@ namespace mlxr {
 // right to 24 and 22 bits.
 //
 // Measured, and what bounds it. 2048 tokens after 30000, 40 heads of 128, 8 KV heads, bf16: 1.24 ms, 1.05 PF/s: the matrix
-// cores are busy for 57% of the cycles, at the 1.8 to 1.85 GHz that the power limit leaves (1.10 ms without the copies, 1.04
+// cores are busy for 58% of the cycles, at the 1.8 to 1.85 GHz that the power limit leaves (1.10 ms without the copies, 1.04
 // without the softmax), and a page's turn is 2.05 us: 0.6 for the keys' products, 0.35 to 0.45 for the values', 0.75 to 0.9
 // for the softmax, 0.2 for what the copies need, 0.1 for barriers. 2048 after 0: 62 us, 0.55 PF/s: 2.4 items a run, whose
 // beginnings and ends (10 us each) are most of what is missing. 32 sequences, 24 with one new token and 8 with up to 400,
 // after up to 7000: 207 us, matrix cores busy for 37% of the cycles, half of it as before and the rest for beginnings, ends
-// and joins. Five tokens of fp32 after 7000: 34 us, of which 5 are the launch, 2.6 the search for the run, 5 the queries, 13
+// and joins. Five tokens of fp32 after 7000: 33 us, of which 5 are the launch, 2.6 the search for the run, 5 the queries, 13
 // two turns behind each other, 4 partial results and 3 to 5 the join: one round trip after another; its reads alone would be
 // 6.
 // Both sides of the choices. Pages in pairs where an item has AR_M / 2 queries or fewer: 33.6 us against 36.8 for the five
