@@ -35,7 +35,8 @@ namespace mlxr {
 //
 // Roundings. Scores, sums and values are fp32. Queries of the cache's type and p rounded to it (half a step, 2^-8 of p in
 // bf16; the sum is of the unrounded p) cost one product a key and dim each; fp32 ones three (bf16) or two (f16), and are
-// right to 24 and 22 bits.
+// right to 24 and 22 bits. A lane sums p page by page and adds the pages' sums: 131072 equal keys that weigh as much as one key in
+// front of them are 1e-4 off, 2e-3 with one addition a key, in the same time.
 //
 // Measured, and what bounds it. 2048 tokens after 30000, 40 heads of 128, 8 KV heads, bf16: 1.24 ms, 1.05 PF/s: the matrix
 // cores are busy for 58% of the cycles, at the 1.8 to 1.85 GHz that the power limit leaves (1.10 ms without the copies, 1.04
@@ -455,13 +456,15 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 m = mn;
             }
             const float ms = at_safe(m) - UP;
+            float sum[4];        // of the page: many small p would lose bits one after another beside a large one in l
 #pragma unroll
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     s[kb][e] = at_exp2(HQ || ST == 1 ? fmaf(s[kb][e], cl, -ms) : s[kb][e] - ms);
-                    l += s[kb][e];
+                    sum[e & 3] = kb == 0 && e < 4 ? s[kb][e] : sum[e & 3] + s[kb][e];
                 }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             if constexpr (HQ)
 #pragma unroll
                 for (int st = 0; st < 4; st++) {

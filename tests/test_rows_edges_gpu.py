@@ -1,0 +1,55 @@
+"""Attention of rows where the tests of its sizes do not look.
+
+Tolerances as in test_rows_gpu, with u = 2^-24; terms that are all alike are rounded alike, so their common error counts in full."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from test_batch_gpu import PAGE, U, from_half, to_half, workspace
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------- long tails
+def tail_attention(gpu, n, nKV, G, D, st, io, sink, rows=64):
+    """One key of a large score at slot `sink`, and about n of score 0. Rows and heads differ in what the n weigh together against
+    the one: from a 64th to four times as much. Values: 0 and -1 in turn for the one, 1 and 0 for the others. All pages but the
+    one key's are the same one, so a long sequence needs no memory; 256 KV heads, so a run is long too."""
+    d, nH, length, rs = gpu.DeviceArray.from_numpy, nKV * G, n + rows, np.random.default_rng(n)
+    kv = np.zeros((2, 2, nKV, PAGE, D), np.float32)
+    kv[1, ..., ::2] = 1.0
+    kv[0, 0, :, sink % PAGE, 0] = 8.0
+    kv[1, 0, :, sink % PAGE, ::2], kv[1, 0, :, sink % PAGE, 1::2] = 0.0, -1.0
+    k, v = (d(to_half(x, st).reshape(x.shape)) for x in kv)
+    table = np.full((1, -(-length // PAGE)), 1, np.int32)
+    table[0, sink // PAGE] = 0
+    q = np.zeros((rows, nH, D), np.float32)
+    q[..., 0] = np.log(n / 2.0 ** rs.uniform(-6, 2, (rows, nH)))      # times 8 and a scale of 1/8: the large score
+    bits = to_half(q, st).reshape(q.shape) if io else q
+    score = (from_half(bits, st) if io else q)[..., :1].astype(np.float64)
+    w, others = np.exp(score), (n + np.arange(rows))[:, None, None].astype(np.float64)
+    want = np.where(np.arange(D) % 2 == 0, others / (w + others), -w / (w + others))
+    dt, dl, ds, dc, dq, out = d(table), d(np.array([length], np.int32)), d(np.zeros(1, np.int32)), d(np.array([rows], np.int32)), d(bits), d(np.zeros_like(bits))
+    desc = gpu.PagedKV(k=k.ptr, v=v.ptr, table=dt.ptr, len=dl.ptr, weight=None, position=None, n_pages=2, table_stride=table.shape[1], slot_stride=0,
+                       max_len=length, B=1, nKV=nKV, D=D, st=st)
+    ref = ctypes.byref(desc)
+    work = workspace(gpu, gpu.lib.mlxr_k_paged_attention_rows_work(ref, nH, rows, io))
+    gpu.check(gpu.lib.mlxr_k_paged_attention_rows(ref, ds.ptr, dc.ptr, rows, dq.ptr, io, nH * D, nH, 0, 0.125, out.ptr, nH * D, work.ptr, work.nbytes, None))
+    gpu.synchronize()
+    return (from_half(out.numpy(), st) if io else out.numpy()), want, score
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("place", ["first", "middle", "last"])
+def test_sum_of_equal_keys(gpu, D, place):
+    """Keys that are each far less than the last bits of the sum that holds a large one still add up."""
+    n = 131072
+    got, want, score = tail_attention(gpu, n, 256, 1, D, 0, 0, {"first": 5, "middle": n // 2, "last": n - 70}[place])
+    # a wave has every other page. The sum rounds once a page (u of itself, all alike), the values twelve times: four steps of 16
+    # keys in three parts. A score: the query's parts, scaling, the exponential's argument (2^-24 and 6 u); a dozen roundings besides
+    pages = n / PAGE / 2 + 1
+    times = np.where(np.arange(D) % 2 == 0, 13, 1)
+    tol = np.abs(want) * (times * pages * U + score * 7 * U + 14 * U)
+    worst = (np.abs(got - want) / tol).max()
+    assert worst <= 1, worst
