@@ -30,8 +30,12 @@ namespace mlxr {
 // while the other has its softmax. Queries in the cache's type enter as they are, and
 // p is rounded to it; fp32 ones, and their p, are split into parts that the matrix cores multiply exactly: three bf16 by
 // truncation (24 bits), or two f16 (22 bits, q scaled to at most 2^14 by a power of two). Scores are in powers of two.
-// A query's reference point for p moves only when its maximum is AT_LAZY or more above it: until then p is up to
-// 2^AT_LAZY, and nothing has to be rescaled.
+// A query's reference point for p moves only when a page's maximum is LAZY or more above it: until then p is up to
+// 2^LAZY, and nothing has to be rescaled. f16 ends 2^-24 below one, so that a long tail of small p would lose its bits, and with
+// one sign where keys are alike (131072 equal ones that weigh as much as one in front of them: 2^-12 of the result): with such a
+// cache the point moves down to a page's maximum as well when that is LAZY or more below, so that what ends is 2^-24 (2^-28 of
+// fp32 queries) of the largest p of its own page, whatever the length. That costs nothing at D 128 and 3% at D 64 (24 windows
+// in fp32 67 -> 69 us); LAZY of 5, 6 and 7 are alike.
 //
 // Roundings. Scores, sums and values are fp32. Queries of the cache's type and p rounded to it (half a step, 2^-8 of p in
 // bf16; the sum is of the unrounded p) cost one product a key and dim each; fp32 ones three (bf16) or two (f16), and are
@@ -60,7 +64,6 @@ constexpr int AR_COUNTS = 4 * AR_MAXW;
 constexpr int AR_GROUP = 8;        // parts that a wave joins one after another
 constexpr int AR_MINPER = 2;       // places of a run at least
 constexpr int AR_RING = 4;         // pages of keys, and of values, in LDS
-constexpr float AT_LAZY = 8.0f;
 #define AT_IN __attribute__((always_inline))   // what holds the operands' registers has to stay in the kernel
 typedef float at_f16 __attribute__((ext_vector_type(16)));
 typedef __bf16 at_b8 __attribute__((ext_vector_type(8)));
@@ -395,7 +398,8 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
         }
         at_f16 o[NV];        // dims 32 n + 8 (i / 4) + 4 h + i % 4 of query r
         float m, l;          // the point of reference; this lane's keys' sum
-        constexpr float UP = ST == 0 ? 0.0f : 6.0f;   // p times 2^UP: f16 parts end at 2^-24
+        constexpr float LAZY = ST == 1 && !HQ ? 6.0f : 8.0f;   // how far p's point of reference may be from a page's maximum
+        constexpr float UP = ST == 0 ? 0.0f : 15.0f - LAZY;         // p times 2^UP: up to 2^15
         at_f16 s[2];         // scores of a page, keys 32 kb + 8 (i / 4) + 4 h + i % 4
         at_u4 pr[4];         // p of a page, rounded (HQ; s otherwise)
         constexpr uint32_t VALUES = AR_RING * TILE;
@@ -446,8 +450,12 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
                 for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[kb][e]);
             mx = xor32_max(mx);
             if (HQ || ST == 1) mx *= cl;
-            if (__any(mx > m + AT_LAZY)) {
-                const float mn = fmaxf(m, mx), c = at_exp2(m - at_safe(mn));
+            bool move = mx > m + LAZY;
+            if (ST == 1) move |= mx < m - LAZY && mx > -INFINITY;
+            if (__any(move)) {
+                float mn = fmaxf(m, mx);
+                if (ST == 1 && mx < m && mx > -INFINITY && xor32_max(l) * at_exp2(m - mx) < 0x1p64f) mn = mx;   // what goes before stays far from overflow
+                const float c = at_exp2(m - at_safe(mn));
                 l *= c;
 #pragma unroll
                 for (int n = 0; n < NV; n++)

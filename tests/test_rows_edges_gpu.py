@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 from test_batch_gpu import PAGE, U, from_half, to_half, workspace
+from test_rows_gpu import half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -51,5 +52,20 @@ def test_sum_of_equal_keys(gpu, D, place):
     pages = n / PAGE / 2 + 1
     times = np.where(np.arange(D) % 2 == 0, 13, 1)
     tol = np.abs(want) * (times * pages * U + score * 7 * U + 14 * U)
+    worst = (np.abs(got - want) / tol).max()
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("n,G,D,io", [(32768, 4, 128, 0), (131072, 4, 64, 0), (131072, 1, 128, 0), (131072, 4, 128, 1), (3000000, 1, 64, 1)])
+@pytest.mark.parametrize("place", ["first", "middle", "last"])
+def test_long_tail_in_f16(gpu, n, G, D, io, place):
+    """The numbers of f16 end 2^-24 below one, and a long tail's p end further below the largest: they keep their bits."""
+    print(f"[case] {n} {G} {D} {io} {place}", flush=True)
+    got, want, score = tail_attention(gpu, n, 256, G, D, 1, io, {"first": 5, "middle": n // 2, "last": n - 70}[place])
+    # a score: the query's parts (2^-22), scaling, the exponential's argument (6 u); a p: its rounding, all alike. A tail's p is a power of two
+    # of its own page's largest, so that their sums, page by page, are exact: the large one is less than 2^28 of them. 63 of them beside the
+    # large one end 2^-34 of it away, half of that off at most: 2^-29 together, 2^-23 of a tail that weighs a 64th. A dozen roundings of sums and results
+    e = half_step(1) if io else 2.0 ** -22
+    tol = np.abs(want) * (score * ((0 if io else e) + 6 * U) + 2 * e + 12 * U + half_step(1) * io) + 2.0 ** -25 * io
     worst = (np.abs(got - want) / tol).max()
     assert worst <= 1, worst
