@@ -2,12 +2,13 @@
 
 Tolerances as in test_rows_gpu, with u = 2^-24; terms that are all alike are rounded alike, so their common error counts in full."""
 import ctypes
+import time
 
 import numpy as np
 import pytest
 
-from test_batch_gpu import PAGE, U, from_half, to_half, workspace
-from test_rows_gpu import half_step
+from test_batch_gpu import PAGE, U, Cache, from_half, to_half, workspace
+from test_rows_gpu import Rows, attend, check, half_step, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,39 @@ def test_long_tail_in_f16(gpu, n, G, D, io, place):
     tol = np.abs(want) * (score * ((0 if io else e) + 6 * U) + 2 * e + 12 * U + half_step(1) * io) + 2.0 ** -25 * io
     worst = (np.abs(got - want) / tol).max()
     assert worst <= 1, worst
+
+
+# ------------------------------------------------------------------------------------------- many sequences
+def scattered(gpu, at, B=60000):
+    """Chunks of eight sequences of a batch whose other ones are idle, and a function that runs the call."""
+    lens, counts = np.zeros(B, int), np.zeros(B, int)
+    lens[at], counts[at] = 700 + 37 * np.arange(8), 100
+    c = Cache(gpu, lens, 1, 64, 0, seed=5).up()
+    r = Rows(c, counts, 1, 1, seed=6, gap=0)
+    d, kv = gpu.DeviceArray.from_numpy, c.desc()
+    ds, dc, dq, do = d(r.start), d(r.count), d(r.bits), d(np.full(r.bits.shape, 7, r.bits.dtype))
+    work = workspace(gpu, gpu.lib.mlxr_k_paged_attention_rows_work(ctypes.byref(kv), 1, r.rows, 1))
+
+    def run():
+        gpu.check(gpu.lib.mlxr_k_paged_attention_rows(ctypes.byref(kv), ds.ptr, dc.ptr, r.rows, dq.ptr, 1, r.width, 1, 0, 0.09, do.ptr, r.width, work.ptr, work.nbytes, None))
+        gpu.synchronize()
+        return do.numpy
+    return c, r, run
+
+
+def test_idle_sequences_between(gpu):
+    """Thousands of idle sequences between those with rows: the same results, and they cost about what they cost behind them."""
+    times = []
+    for at in (np.arange(8), np.arange(8) * 7500 + 3000):
+        c, r, run = scattered(gpu, at)
+        check(run()(), r, *reference(r, 0, 0.09))
+        best = np.inf
+        for _ in range(20):
+            t = time.perf_counter()
+            run()
+            best = min(best, time.perf_counter() - t)
+        times.append(best)
+    print(times)
+    # the batch is looked over twice either way, 120 steps each; between two chunks lie 7500 more sequences, 30 steps. One by one they
+    # would be 7500 steps
+    assert times[1] < 3 * times[0], times
