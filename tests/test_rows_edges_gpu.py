@@ -7,8 +7,8 @@ import time
 import numpy as np
 import pytest
 
-from test_batch_gpu import PAGE, U, Cache, from_half, to_half, workspace
-from test_rows_gpu import Rows, attend, check, half_step, reference
+from test_batch_gpu import PAGE, U, Cache, from_half, same, to_half, within, workspace
+from test_rows_gpu import INF, Rows, attend, check, half_step, one_half, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,98 @@ def test_idle_sequences_between(gpu):
     # the batch is looked over twice either way, 120 steps each; between two chunks lie 7500 more sequences, 30 steps. One by one they
     # would be 7500 steps
     assert times[1] < 3 * times[0], times
+
+
+@pytest.mark.parametrize("B,nKV,G,D,st,io,window,idle", [(65, 2, 2, 128, 0, 0, 0, 0.1), (65, 1, 3, 64, 1, 1, 50, 0.5), (600, 1, 2, 128, 0, 0, 70, 0.9), (600, 2, 1, 64, 0, 1, 0, 0.2),
+                                                         (1100, 1, 1, 128, 1, 0, 0, 0.95)])
+def test_bounds_of_many_sequences(gpu, B, nKV, G, D, st, io, window, idle):
+    """What only the device sees of a batch of more sequences than a wave looks over at once: lengths and counts of no use, counts
+    above lengths, pages that are not there, rows in front of the array and behind it."""
+    print(f"[case] {B} {nKV} {G} {D} {st} {io} {window} {idle}", flush=True)
+    rs = np.random.default_rng(B + D)
+    lens = rs.integers(0, 260, B)
+    lens[-2:] = 259, 200
+    c = Cache(gpu, lens, nKV, D, st, seed=B)
+    bad = rs.permutation(np.arange(2, B - 2))[:12]
+    c.lens[bad[:4]] = [-7, 5000, -2 ** 31, 2 ** 31 - 1]
+    for b in bad[1], bad[3]:                                     # held at max_len: pages for that
+        c.table[b, :-(-c.max_len // PAGE)] = c.table[B - 2, :-(-c.max_len // PAGE)]
+    c.table[bad[4], 0], c.table[bad[5], :3] = c.k.shape[0], [-1, -2 ** 31, 2 ** 31 - 1]
+    c.up()
+    counts = np.where(rs.random(B) < idle, 0, np.minimum(rs.integers(1, 60, B), lens))
+    counts[bad] = [5, 9, 4, 30, 20, 20, -4, -2 ** 31, lens[bad[8]] + 3, lens[bad[9]] + 70, 6, 8]
+    r = Rows(c, counts, nKV * G, io, seed=B)
+    r.set(np.where(np.isnan(r.q), np.float32(0.25), r.q))        # rows of no sequence have one here
+    want = reference(r, window, 0.09)
+    got = attend(gpu, r, window=window)
+    check(got, r, *want)
+    over = r.start[bad[9]] + np.arange(70)
+    assert not got[over, :nKV * G * D].any()
+    start = r.start.copy()
+    start[bad[10]], start[bad[11]], start[bad[8]], start[bad[9]] = -5, r.rows - 1, r.rows + 1, 2 ** 31 - 2
+    check(attend(gpu, r, window=window, start=start), r, *reference(r, window, 0.09, start=start.astype(np.int64)))
+
+
+@pytest.mark.parametrize("B", [3, 64, 65, 700])
+@pytest.mark.parametrize("D,st,io", [(128, 0, 0), (64, 1, 1)])
+def test_no_sequence_has_a_slot(gpu, B, D, st, io):
+    """Rows of sequences without any slot, and nothing else to do: zeros, and the workspace serves the next call."""
+    c, full = Cache(gpu, [0] * B, 1, D, st, seed=1, max_len=64).up(), Cache(gpu, [40] * B, 1, D, st, seed=2).up()
+    r, other = Rows(c, np.arange(B) % 4, 2, io, seed=3), Rows(full, np.arange(B) % 4, 2, io, seed=4)
+    work = workspace(gpu, gpu.lib.mlxr_k_paged_attention_rows_work(ctypes.byref(full.desc()), 2, max(r.rows, other.rows), io))
+    check(attend(gpu, r, work=work), r, *reference(r, 0, 0.09))
+    check(attend(gpu, other, work=work), other, *reference(other, 0, 0.09))
+
+
+# ------------------------------------------------------------------------------------------- infinities
+@pytest.mark.parametrize("st,io", [(0, 0), (0, 1), (1, 0), (1, 1)])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("odd", [INF, -INF])
+@pytest.mark.parametrize("window", [0, 90])
+def test_infinities_in_sight(gpu, st, io, D, odd, window):
+    """Rows that attend an infinite key or value get what the formula gives, others what they get without: a key is left out where its
+    score is -infinity, its infinite values too, and makes NaN where it is +infinity; an infinite value stays where it is attended."""
+    lens, counts, G = [300, 128, 70], [150, 128, 1], 3
+    c = Cache(gpu, lens, 1, D, st, seed=52)
+    r = Rows(c, counts, G, io, seed=52)
+    key, value = {0: 222, 1: 64, 2: 3}, {0: 180, 1: 30, 2: 60}
+    q = r.q.copy()
+    sign = np.zeros(r.rows)
+    for b in range(3):
+        mine = r.start[b] + np.arange(counts[b])
+        sign[mine] = np.where(np.arange(counts[b]) % 3 == 1, 1, -1)    # a third of the rows have +infinity
+        for g in range(G):
+            q[mine, g * D + 5] = (np.abs(q[mine, g * D + 5]) + 0.25) * sign[mine] * np.sign(odd)
+    r.set(q)
+
+    class Gone:   # without the infinite keys, and with zeros for infinite values
+        def __getattr__(self, name):
+            return getattr(c, name)
+
+        def rows(self, pool, b, h, m):
+            x, there = c.rows(pool, b, h, m)
+            gone = np.arange(m) == key[b]
+            x = np.where(gone[:, None], 0, x)
+            if pool is c.v:
+                x[value[b], 7] = 0
+            return x, there & ~gone
+    spot = lambda b, j: (c.table[b, j // PAGE], 0, j % PAGE)  # noqa: E731
+    for b in range(3):
+        c.k[spot(b, key[b])][5], c.v[spot(b, key[b])][:], c.v[spot(b, value[b])][7] = (one_half(odd, st) for _ in range(3))
+    c.up()
+    got = attend(gpu, r, window=window)
+    r.c = Gone()
+    want, tol, named = reference(r, window, 0.09)
+    r.c = c
+    want, n = want.reshape(r.rows, G, D), G * D
+    for b in range(3):
+        rows, slot = r.start[b] + np.arange(counts[b]), lens[b] - counts[b] + np.arange(counts[b])
+        sees = lambda j: (slot >= j) & ((slot - window < j) | (window == 0))  # noqa: E731
+        want[rows[sees(value[b])], :, 7] = odd
+        want[rows[sees(key[b]) & (sign[rows] > 0)]] = np.nan
+    want = want.reshape(r.rows, n)
+    x = (from_half(got, st) if io else got)[:, :n]
+    finite, odd_ones = named[:, None] & np.isfinite(want), named[:, None] & ~np.isfinite(want)
+    assert np.array_equal(x[odd_ones], want[odd_ones].astype(np.float32), equal_nan=True)
+    assert within(np.abs(x[finite] - want[finite]), tol[finite]) <= 1
+    assert same(got[~named], np.full_like(got[~named], 7))
