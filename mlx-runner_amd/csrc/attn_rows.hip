@@ -13,7 +13,7 @@ namespace mlxr {
 // cut into equal runs, one per workgroup, so chunks, prompts and single tokens of one call keep the card evenly busy, and
 // counts and lengths may stay on the device: each workgroup finds its run by a scan over the sequences. How many pages an
 // item has follows from rounding twice, so its length here is a bound that adds up in closed form (AtPlaces): up to two
-// places of an item hold no page, and at_gap more stand for what beginning and ending one costs. An item inside one run is
+// places of an item hold no page, and AR_GAP more stand for what beginning and ending one costs. An item inside one run is
 // written out at once; one cut by runs leaves partial results (maximum, sum, unnormalised values), which the last workgroup
 // to finish joins in run order: the same bits every time. A part is 2.5 us of a join by one workgroup, so where a wave would
 // have more than AR_GROUP of them they are joined in groups, and then the groups (180 tokens after 594 and 52 after 11387,
@@ -57,9 +57,9 @@ namespace mlxr {
 // for twice as many products.
 constexpr int AR_WV = 8, AR_TH = 64 * AR_WV, AR_M = 32 * AR_WV;   // waves and threads of a workgroup, queries of an item
 constexpr int AR_MAXW = 256;       // workgroups: one a CU
-// Places behind an item: a page of 64 dims is passed in less time (24 windows of 1024: 58.2 us with 5, 55.2 with 7, 56.0 with 9; of
-// 128 dims 4 to 6 are alike).
-__host__ __device__ __forceinline__ constexpr int at_gap(int D) { return D == 64 ? 7 : 5; }
+// Places behind an item. Of 128 dims 4 to 6 are alike; of 64 dims 5 is 1 to 5% faster than 7 in six of nine batches (2048 tokens
+// after 0: 48 us against 50, with 9 52; 10 chunks with a window of 300: 40 against 42) and 2% slower in one (24 windows of 1024).
+constexpr int AR_GAP = 5;
 constexpr int AR_COUNTS = 4 * AR_MAXW;
 constexpr int AR_GROUP = 8;        // parts that a wave joins one after another
 constexpr int AR_MINPER = 2;       // places of a run at least
@@ -156,7 +156,7 @@ __device__ __forceinline__ AtSeq at_one(const AtSeq& s) { return AtSeq{at_one(s.
 // How many items a sequence has, and their places: min(A + floor(S i / G), cap) + GAP for item i, S pages of queries (AR_M / 64);
 // half as many pages for a last item of AR_M / 2 queries or fewer, whose pages go in pairs.
 template <int D> struct AtPlaces {
-    static constexpr int S = AR_M / MLXR_PAGE, GAP = at_gap(D);
+    static constexpr int S = AR_M / MLXR_PAGE, GAP = AR_GAP;
     int64_t A, cap, bend;   // from item `bend` on the cap holds
     int G, items;
     bool few;
@@ -902,7 +902,7 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
 }
 
 static size_t at_layout(const PagedKV& kv, int nH, int rows, void* base, AtWork& wk) {
-    const int64_t G = nH / kv.nKV, items = ((int64_t)rows * G + AR_M - 1) / AR_M + kv.B, places = (kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE + 4 + at_gap(kv.D);
+    const int64_t G = nH / kv.nKV, items = ((int64_t)rows * G + AR_M - 1) / AR_M + kv.B, places = (kv.max_len + MLXR_PAGE - 1) / MLXR_PAGE + 4 + AR_GAP;
     const double runs = (double)items * (double)kv.nKV * (double)places / AR_MINPER + 1.0;
     wk.W = runs < AR_MAXW ? (int)runs : AR_MAXW;
     uint8_t* p = static_cast<uint8_t*>(base);
