@@ -409,10 +409,14 @@ int mlxr_k_paged_append_rows(const mlxr_paged_kv* kv, const float* qkv, int row_
 
 /* Attention from rows to their own sequences' slots: row start[b] + i, i < count[b], is the query at slot len[b] - count[b] + i
  * (len counts the new tokens) and attends every slot up to its own, or the last `window` of these (0: all). out = sum_j p_j v_j with p =
- * softmax(scale q k_j), |scale| at most 2^126. q_type 0: q and out are fp32 and so are the results; q_type 1: both are of the cache's
- * type, scores, sums and the softmax in fp32, and each p is rounded to the type once (sums are of unrounded ones). A key whose
+ * softmax(scale q k_j), |scale| at most 2^126. q_type 0: q and out are fp32, and so are the results, q and p being right to 24 bits over
+ * bf16 and to 22 over f16 (of a query's largest value, of a page's largest p, where they are far smaller); q_type 1: both are of the cache's
+ * type, scores, sums and the softmax in fp32, and each p is rounded to the type once (sums are of unrounded ones). Sums of many
+ * slots have fp32's roundings. scale q (q_type 0) or q k_j (q_type 1) is computed as it stands: beyond fp32's range it is infinite; with q_type 1
+ * a |scale| below 2^-126 / log2(e), 0 too, counts as that. A key whose
  * score is -infinity takes no part; a row that has no slot (count above len), no page of the pool or no score above -infinity gives zeros;
- * infinities and NaN in keys and values that a row attends count as the formula has them, and others do not reach it. Rows outside
+ * infinities and NaN in keys and values that a row attends count as the formula has them, and others do not reach it (where some
+ * are met, attended or not, the call is several times slower). Rows outside
  * [0, rows) and rows that no sequence names are neither read nor written; sequences name rows of their own. The cache's weights
  * stay as they are. q, out: 16-byte aligned, strides whole multiples of 16 bytes; out may be q itself at its stride. work: zero
  * before its first use and this entry point's alone, one call at a time (sizes may differ from call to call). The same call gives

@@ -25,7 +25,7 @@ __device__ __forceinline__ void ar_mark(const PagedKV& kv, const ArRow& r, int k
     if (kv.position) kv.position[paged_slot(kv, r.b, kvh, r.slot)] = r.pos;
 }
 
-// A workgroup per row (and, for few rows, per AR_T / (D / 8) of its heads: 4 rows of 512 + 2 * 128 heads take 4.9 us, 22
+// A workgroup per row (and, where that makes no more than four workgroups a CU, per AR_T / (D / 8) of its heads: 4 rows of 512 + 2 * 128 heads take 4.9 us, 22
 // without; one of 4096 + 2 * 1024 5.1 and 240; 2048 rows 14.9 and 13.8). Eight lanes (D 64) or sixteen have a head, eight
 // dims each: of the rotated ones four and those that they rotate into, of the rest neighbours. So a wave asks for eight or
 // four heads with two 16-byte loads a lane, the norm is a sum over a row of lanes, and a lane's four sines and cosines, which

@@ -43,17 +43,26 @@ namespace mlxr {
 // front of them are 1e-4 off, 2e-3 with one addition a key, in the same time.
 //
 // Measured, and what bounds it. 2048 tokens after 30000, 40 heads of 128, 8 KV heads, bf16: 1.24 ms, 1.05 PF/s: the matrix
-// cores are busy for 58% of the cycles, at the 1.8 to 1.85 GHz that the power limit leaves (1.10 ms without the copies, 1.04
+// cores are busy for 57% of the cycles, at the 1.8 to 1.85 GHz that the power limit leaves (1.10 ms without the copies, 1.04
 // without the softmax), and a page's turn is 2.05 us: 0.6 for the keys' products, 0.35 to 0.45 for the values', 0.75 to 0.9
-// for the softmax, 0.2 for what the copies need, 0.1 for barriers. 2048 after 0: 62 us, 0.55 PF/s: 2.4 items a run, whose
-// beginnings and ends (10 us each) are most of what is missing. 32 sequences, 24 with one new token and 8 with up to 400,
-// after up to 7000: 207 us, matrix cores busy for 37% of the cycles, half of it as before and the rest for beginnings, ends
-// and joins. Five tokens of fp32 after 7000: 33 us, of which 5 are the launch, 2.6 the search for the run, 5 the queries, 13
-// two turns behind each other, 4 partial results and 3 to 5 the join: one round trip after another; its reads alone would be
-// 6.
-// Both sides of the choices. Pages in pairs where an item has AR_M / 2 queries or fewer: 33.6 us against 36.8 for the five
-// tokens, 207 against 223 for the 32 sequences, 55 against 61 for 24 windows of 1024. Each wave looks for its run by itself
-// (up to 64 sequences): 33.6 against 34.8 and 55 against 57. Items of AR_M queries rather than of half as many read a page
+// for the softmax, 0.2 for what the copies need, 0.1 for barriers. 2048 after 0: 62 us, 0.55 PF/s: 1.7 parts of items a run, of
+// 10 pages each. A part costs 10 us beside its pages: 4 until the first ones are there, 1.3 for the queries, 1.3 for the look
+// for what is not finite, 3.5 to hand its results over (2.2 to write a whole item's); a join, in 159 of the 251 runs, 6.7 more.
+// 32 sequences, 24 with one new token and 8 with up to 400, after up to 7000: 207 us, matrix cores busy for 37% of the cycles: a
+// run has 2.7 parts and 103 pages, half of them in pairs for four queries; 53 at 2.05 us, 25 pairs at 2.5, 11 until first pages are
+// there, 18 for beginnings and ends, 5 for joins. 24 windows of 1024, 64 dims, f16: 58 us, two parts of 12 pages a run, 1.55 us a page, a
+// quarter of the places without one. fp32 queries over bf16: a page 4.5 us, a part 16 beside its pages (8 for the
+// queries, 2.6 for the look, 5.2 to hand over), a join 7.5. Five tokens of fp32 after 7000: 33 us, of which 5 are the launch, 2.6 the
+// search for the run, 5 the queries, 13 two turns behind each other, 4 partial results and 3 to 5 the join: one round trip after
+// another; its reads alone would be 6.
+// What is not finite sends its run's part of the item through the pages again: one infinite value in 2048 tokens after 0 makes 62 us 370
+// (fp32 queries 117 and 1270), 2048 after 30000 1.24 ms 4.2, five tokens 33 us 145. The fp32 kernels of 128 dims spill
+// registers on that way (580 bytes a lane over bf16, 332 over f16); in the page loops two are read back, where a page is masked.
+// More than 64 sequences are scanned by the workgroup, twice: 32 single tokens of up to 8192 slots take as long among 512 sequences as
+// alone, among 32768 90 to 100 us longer.
+// Both sides of the choices. Pages in pairs where an item has AR_M / 2 queries or fewer: 34.4 us against 38.5 for the five
+// tokens, 208 against 227 for the 32 sequences, 58 against 62 for the windows. Each wave looks for its run by itself
+// (up to 64 sequences): 34.4 against 35.6 and 58 against 59. Items of AR_M queries rather than of half as many read a page
 // for twice as many products.
 constexpr int AR_WV = 8, AR_TH = 64 * AR_WV, AR_M = 32 * AR_WV;   // waves and threads of a workgroup, queries of an item
 constexpr int AR_MAXW = 256;       // workgroups: one a CU
