@@ -34,7 +34,7 @@ namespace mlxr {
 // 2^LAZY, and nothing has to be rescaled. f16 ends 2^-24 below one, so that a long tail of small p would lose its bits, and with
 // one sign where keys are alike (131072 equal ones that weigh as much as one in front of them: 2^-12 of the result): with such a
 // cache the point moves down to a page's maximum as well when that is LAZY or more below, so that what ends is 2^-24 (2^-28 of
-// fp32 queries) of the largest p of its own page, whatever the length. That costs nothing at D 128 and 3% at D 64 (24 windows
+// fp32 queries) of the largest p of its own page, whatever the length (fp32 queries: by whole powers of two, so that moves round nothing). That costs nothing at D 128 and 3% at D 64 (24 windows
 // in fp32 67 -> 69 us); LAZY of 5, 6 and 7 are alike.
 //
 // Roundings. Scores, sums and values are fp32. Queries of the cache's type and p rounded to it (half a step, 2^-8 of p in
@@ -480,8 +480,9 @@ __global__ __launch_bounds__(AR_TH, 2) void attn_rows_kernel(AttnRowsArgs a, AtW
             bool move = mx > m + LAZY;
             if (ST == 1) move |= mx < m - LAZY && mx > -INFINITY;
             if (__any(move)) {
-                float mn = fmaxf(m, mx);
-                if (ST == 1 && mx < m && mx > -INFINITY && xor32_max(l) * at_exp2(m - mx) < 0x1p64f) mn = mx;   // what goes before stays far from overflow
+                const float to = ST == 1 && !HQ ? rintf(mx) : mx;   // whole: any number of moves up and down rounds nothing
+                float mn = fmaxf(m, to);
+                if (ST == 1 && to < m && to > -INFINITY && xor32_max(l) * at_exp2(m - to) < 0x1p64f) mn = to;   // what goes before stays far from overflow
                 const float c = at_exp2(m - at_safe(mn));
                 l *= c;
 #pragma unroll

@@ -72,6 +72,39 @@ def test_long_tail_in_f16(gpu, n, G, D, io, place):
     assert worst <= 1, worst
 
 
+@pytest.mark.parametrize("G,D,io", [(4, 128, 0), (1, 64, 0), (4, 64, 1), (1, 128, 1)])
+def test_pages_of_two_scores_in_f16(gpu, G, D, io):
+    """Pages whose scores are 6 to 29 powers of two apart, in turn: either kind keeps its bits, however often the larger comes back."""
+    d, n, rows, nKV, rs = gpu.DeviceArray.from_numpy, 32768, 64, 256, np.random.default_rng(D)
+    nH, length = nKV * G, n + 64
+    kv = np.zeros((2, 2, nKV, PAGE, D), np.float32)
+    kv[0, 1, ..., 0] = 8.0
+    kv[1, 0, ..., ::2], kv[1, 1, ..., 1::2] = 1.0, -1.0
+    k, v = (d(to_half(x, 1).reshape(x.shape)) for x in kv)
+    table = (np.arange(length // PAGE) % 2).astype(np.int32)[None]
+    q = np.zeros((rows, nH, D), np.float32)
+    q[..., 0] = rs.uniform(4.3, 20.0, (rows, nH))
+    bits = to_half(q, 1).reshape(q.shape) if io else q
+    score = (from_half(bits, 1) if io else q)[..., :1].astype(np.float64)
+    large = np.cumsum(np.arange(length) // PAGE % 2)[n:][:, None, None] * np.exp(score)
+    small = np.cumsum(1 - np.arange(length) // PAGE % 2)[n:][:, None, None]
+    want = np.where(np.arange(D) % 2 == 0, small, -large) / (large + small)
+    dt, dl, ds, dc, dq, out = d(table), d(np.array([length], np.int32)), d(np.zeros(1, np.int32)), d(np.array([rows], np.int32)), d(bits), d(np.zeros_like(bits))
+    desc = gpu.PagedKV(k=k.ptr, v=v.ptr, table=dt.ptr, len=dl.ptr, weight=None, position=None, n_pages=2, table_stride=table.shape[1], slot_stride=0,
+                       max_len=length, B=1, nKV=nKV, D=D, st=1)
+    ref = ctypes.byref(desc)
+    work = workspace(gpu, gpu.lib.mlxr_k_paged_attention_rows_work(ref, nH, rows, io))
+    gpu.check(gpu.lib.mlxr_k_paged_attention_rows(ref, ds.ptr, dc.ptr, rows, dq.ptr, io, nH * D, nH, 0, 0.125, out.ptr, nH * D, work.ptr, work.nbytes, None))
+    gpu.synchronize()
+    got = from_half(out.numpy(), 1) if io else out.numpy()
+    # roundings all alike: one of the sum and eight of the values a page (four steps of 16 keys, two parts), two of each where the point
+    # of reference moves by a power that is no whole number (queries in f16); those of a score and a p as above
+    e, pages = half_step(1) if io else 2.0 ** -22, length / PAGE
+    tol = np.abs(want) * (score * ((0 if io else e) + 6 * U) + 2 * e + (13 if io else 9) * pages * U + 12 * U + half_step(1) * io) + 2.0 ** -25 * io
+    worst = (np.abs(got - want) / tol).max()
+    assert worst <= 1, worst
+
+
 # ------------------------------------------------------------------------------------------- many sequences
 def scattered(gpu, at, B=60000):
     """Chunks of eight sequences of a batch whose other ones are idle, and a function that runs the call."""
